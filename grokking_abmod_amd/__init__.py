@@ -29,7 +29,13 @@ EXPORTS = (
     "mg_tokenizer_from_text", "mg_tokenizer_encode", "mg_tokenizer_decode", "mg_sample_logits", "mg_sample_logits_noalloc", "mg_expf",
     "mg_adamw_default", "mg_cross_entropy", "mg_loss_and_gradient", "mg_train_batch",
     "mg_equation_split", "mg_equation_batch", "mg_text_batch",
+    "mg_kv8_sizes", "mg_kv8_append", "mg_kv8_read", "mg_kv8_attention_workspace", "mg_kv8_attention",
+    "mg_token_logprobs_workspace", "mg_token_logprobs_noalloc", "mg_token_logprobs_backward_noalloc",
+    "mg_token_logprobs",
 )
+
+MG_F32, MG_F16, MG_BF16 = range(3)  # element types of the device operators
+TOP_MAX = 32  # MG_TOP_MAX
 
 IGNORE_TARGET = 0xFFFFFFFF  # MG_IGNORE_TARGET (src/gpt/mod.rs:26)
 
@@ -76,6 +82,13 @@ class GptConfig(ctypes.Structure):
         return isinstance(other, GptConfig) and self.as_dict() == other.as_dict()
 
 
+class Kv8(ctypes.Structure):
+    """mg_kv8: an 8-bit KV cache in the caller's device buffers (pointers as ints)."""
+
+    _fields_ = [(name, ctypes.c_uint32) for name in ("batch", "kv_heads", "head_width", "capacity")] + [
+        (name, ctypes.c_void_p) for name in ("k", "v", "k_scale", "v_scale")]
+
+
 class MeshGptError(RuntimeError):
     def __init__(self, status, message):
         super().__init__(message)
@@ -87,6 +100,8 @@ _u32p = ctypes.POINTER(ctypes.c_uint32)
 _f32p = ctypes.POINTER(ctypes.c_float)
 _szp = ctypes.POINTER(ctypes.c_size_t)
 _cfgp = ctypes.POINTER(GptConfig)
+_kv8p = ctypes.POINTER(Kv8)
+_strides = ctypes.c_int64 * 3
 _lib = None
 
 
@@ -149,6 +164,15 @@ def lib():
         "mg_equation_batch": (i, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_double, u64, i, _szp, sz, _u32p,
                                   _u32p]),
         "mg_text_batch": (i, [_u32p, sz, _cfgp, i, sz, sz, u64, _u32p, _u32p]),
+        "mg_kv8_sizes": (i, [_kv8p, _szp, _szp]),
+        "mg_kv8_append": (i, [i, _kv8p, i, sz, vp, _strides, vp, _strides, vp, vp, vp]),
+        "mg_kv8_read": (i, [i, _kv8p, i, sz, sz, vp, _strides, vp, _strides, vp, vp]),
+        "mg_kv8_attention_workspace": (i, [_kv8p, sz, sz, _szp]),
+        "mg_kv8_attention": (i, [i, _kv8p, i, sz, sz, vp, _strides, vp, _strides, vp, vp, f, vp, sz, vp]),
+        "mg_token_logprobs_workspace": (i, [sz, sz, sz, _szp]),
+        "mg_token_logprobs_noalloc": (i, [i, i, vp, sz, sz, sz, vp, f, vp, vp, vp, sz, vp, vp, vp, sz, vp]),
+        "mg_token_logprobs_backward_noalloc": (i, [i, i, vp, sz, sz, sz, vp, f, vp, vp, vp, vp, vp, sz, vp]),
+        "mg_token_logprobs": (i, [i, _f32p, sz, sz, _u32p, f, _f32p, _f32p, sz, _u32p, _f32p]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)
@@ -229,6 +253,77 @@ def sample_logits_noalloc(logits_ptr, rows, vocab, temperature, rng_ptr, tokens_
     """mg_sample_logits_noalloc on device pointers (ints); enqueued on `stream`."""
     _check(lib().mg_sample_logits_noalloc(device, logits_ptr, rows, vocab, temperature, rng_ptr, tokens_ptr,
                                           nonfinite_ptr, stream))
+
+
+def kv8_sizes(cache):
+    """mg_kv8_sizes: bytes of k (and of v), bytes of k_scale (and of v_scale)."""
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    _check(lib().mg_kv8_sizes(cache, ctypes.byref(codes), ctypes.byref(scales)))
+    return codes.value, scales.value
+
+
+def kv8_append(cache, type, count, k, k_strides, v, v_strides, lengths, counts=None, stream=None, device=0):
+    """mg_kv8_append on device pointers (ints); strides are (sequence, token,
+    head) in elements; enqueued on `stream`."""
+    _check(lib().mg_kv8_append(device, cache, type, count, k, _strides(*k_strides), v, _strides(*v_strides), lengths,
+                               counts, stream))
+
+
+def kv8_read(cache, type, first, count, k, k_strides, v, v_strides, lengths=None, stream=None, device=0):
+    """mg_kv8_read on device pointers (ints); enqueued on `stream`."""
+    _check(lib().mg_kv8_read(device, cache, type, first, count, k, _strides(*k_strides), v, _strides(*v_strides),
+                             lengths, stream))
+
+
+def kv8_attention_workspace(cache, heads, count):
+    """mg_kv8_attention_workspace: bytes of scratch that a call needs."""
+    n = ctypes.c_size_t()
+    _check(lib().mg_kv8_attention_workspace(cache, heads, count, ctypes.byref(n)))
+    return n.value
+
+
+def kv8_attention(cache, type, heads, count, q, q_strides, out, out_strides, lengths, counts, scale, workspace=None,
+                  workspace_bytes=0, stream=None, device=0):
+    """mg_kv8_attention on device pointers (ints); enqueued on `stream`."""
+    _check(lib().mg_kv8_attention(device, cache, type, heads, count, q, _strides(*q_strides), out,
+                                  _strides(*out_strides), lengths, counts, scale, workspace, workspace_bytes, stream))
+
+
+def token_logprobs_workspace(rows, vocab, top):
+    """mg_token_logprobs_workspace: bytes of scratch that a call needs."""
+    n = ctypes.c_size_t()
+    _check(lib().mg_token_logprobs_workspace(rows, vocab, top, ctypes.byref(n)))
+    return n.value
+
+
+def token_logprobs_noalloc(type, logits, rows, vocab, stride, tokens, temperature, logprob, entropy=None, stats=None,
+                           top=0, top_tokens=None, top_logprobs=None, workspace=None, workspace_bytes=0, stream=None,
+                           device=0):
+    """mg_token_logprobs_noalloc on device pointers (ints); enqueued on `stream`."""
+    _check(lib().mg_token_logprobs_noalloc(device, type, logits, rows, vocab, stride, tokens, temperature, logprob,
+                                           entropy, stats, top, top_tokens, top_logprobs, workspace, workspace_bytes,
+                                           stream))
+
+
+def token_logprobs_backward_noalloc(type, logits, rows, vocab, stride, tokens, temperature, stats, entropy, d_logprob,
+                                    d_entropy, d_logits, d_stride, stream=None, device=0):
+    """mg_token_logprobs_backward_noalloc on device pointers (ints); enqueued on `stream`."""
+    _check(lib().mg_token_logprobs_backward_noalloc(device, type, logits, rows, vocab, stride, tokens, temperature,
+                                                    stats, entropy, d_logprob, d_entropy, d_logits, d_stride, stream))
+
+
+def token_logprobs(logits, tokens, temperature=1.0, top=0, device=0):
+    """Log probabilities of `tokens` under rows of f32 logits (mg_token_logprobs):
+    (logprobs, entropies, alternatives, their logprobs), the last two rows x top."""
+    logits, tokens = _f32(np.atleast_2d(logits)), _u32(tokens).reshape(-1)
+    rows, vocab = logits.shape
+    if tokens.size != rows:
+        raise MeshGptError(MG_INVALID_ARGUMENT, "logits and tokens must have equal rows")
+    logprob, entropy = np.empty(rows, dtype=np.float32), np.empty(rows, dtype=np.float32)
+    ids, best = np.empty((rows, top), dtype=np.uint32), np.empty((rows, top), dtype=np.float32)
+    _check(lib().mg_token_logprobs(device, _p(logits, _f32p), rows, vocab, _p(tokens, _u32p), temperature,
+                                   _p(logprob, _f32p), _p(entropy, _f32p), top, _p(ids, _u32p), _p(best, _f32p)))
+    return logprob, entropy, ids, best
 
 
 def device_expf(x, device=0):

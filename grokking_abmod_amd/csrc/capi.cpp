@@ -7,6 +7,7 @@
 
 #include "meshgpt_types.hpp"
 #include "model.hpp"
+#include "operators.hpp"
 
 using namespace meshgpt;
 
@@ -116,6 +117,20 @@ MeshGpt &model_of(mg_model *m) {
 void copy_out(const std::vector<float> &v, float *out, size_t n) {
     require(out != nullptr && n >= v.size(), "output buffer is too small");
     std::memcpy(out, v.data(), v.size() * sizeof(float));
+}
+
+Kv8 to_cache(const mg_kv8 *c) {
+    require(c != nullptr, "cache must not be null");
+    require(c->batch <= 1u << 24 && c->kv_heads <= 1u << 24 && c->head_width <= 1u << 24 && c->capacity <= 1u << 30,
+            "cache dimensions are out of range");
+    Kv8 k{int(c->batch), int(c->kv_heads), int(c->head_width), kv8_pad(int(c->head_width)), int(c->capacity),
+          c->k,          c->v,             c->k_scale,         c->v_scale};
+    return k;
+}
+
+Strides to_strides(const int64_t *s) {
+    require(s != nullptr, "strides must not be null");
+    return Strides{{s[0], s[1], s[2]}};
 }
 
 }  // namespace
@@ -372,6 +387,92 @@ int mg_sample_logits_noalloc(int device, const float *logits, size_t rows, size_
                 "logits, states and tokens must not be null");
         sample_logits_noalloc(device, logits, rows, vocab, temperature, rng_states, tokens, nonfinite,
                               static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_kv8_sizes(const mg_kv8 *cache, size_t *codes, size_t *scales) {
+    return guarded([&] {
+        require(codes != nullptr && scales != nullptr, "outputs must not be null");
+        Kv8 c = to_cache(cache);
+        c.k = c.v = c.ks = c.vs = reinterpret_cast<uint8_t *>(256);  // the buffers may come after
+        kv8_check(c);
+        *codes = kv8_code_bytes(c);
+        *scales = kv8_scale_bytes(c);
+    });
+}
+
+int mg_kv8_append(int device, const mg_kv8 *cache, int type, size_t count, const void *k, const int64_t k_strides[3],
+                  const void *v, const int64_t v_strides[3], const int32_t *lengths, const int32_t *counts,
+                  void *stream) {
+    return guarded([&] {
+        kv8_append(device, to_cache(cache), Type(type), count, k, to_strides(k_strides), v, to_strides(v_strides),
+                   lengths, counts, static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_kv8_read(int device, const mg_kv8 *cache, int type, size_t first, size_t count, void *k,
+                const int64_t k_strides[3], void *v, const int64_t v_strides[3], const int32_t *lengths, void *stream) {
+    return guarded([&] {
+        kv8_read(device, to_cache(cache), Type(type), first, count, k, to_strides(k_strides), v, to_strides(v_strides),
+                 lengths, static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_kv8_attention_workspace(const mg_kv8 *cache, size_t heads, size_t count, size_t *bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "output must not be null");
+        Kv8 c = to_cache(cache);
+        c.k = c.v = c.ks = c.vs = reinterpret_cast<uint8_t *>(256);
+        kv8_check(c);
+        *bytes = kv8_attention_workspace(c, heads, count);
+    });
+}
+
+int mg_kv8_attention(int device, const mg_kv8 *cache, int type, size_t heads, size_t count, const void *q,
+                     const int64_t q_strides[3], void *out, const int64_t out_strides[3], const int32_t *lengths,
+                     const int32_t *counts, float scale, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        kv8_attention(device, to_cache(cache), Type(type), heads, count, q, to_strides(q_strides), out,
+                      to_strides(out_strides), lengths, counts, scale, workspace, workspace_bytes,
+                      static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_token_logprobs_workspace(size_t rows, size_t vocab, size_t top, size_t *bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "output must not be null");
+        *bytes = token_logprobs_workspace(rows, vocab, top);
+    });
+}
+
+int mg_token_logprobs_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab, size_t stride,
+                              const uint32_t *tokens, float temperature, float *logprob, float *entropy, float *stats,
+                              size_t top, uint32_t *top_tokens, float *top_logprobs, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        token_logprobs_noalloc(device, Type(type), logits, rows, vocab, stride, tokens, temperature, logprob, entropy,
+                               stats, top, top_tokens, top_logprobs, workspace, workspace_bytes,
+                               static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_token_logprobs_backward_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab,
+                                       size_t stride, const uint32_t *tokens, float temperature, const float *stats,
+                                       const float *entropy, const float *d_logprob, const float *d_entropy,
+                                       void *d_logits, size_t d_stride, void *stream) {
+    return guarded([&] {
+        token_logprobs_backward_noalloc(device, Type(type), logits, rows, vocab, stride, tokens, temperature, stats,
+                                        entropy, d_logprob, d_entropy, d_logits, d_stride,
+                                        static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_token_logprobs(int device, const float *logits, size_t rows, size_t vocab, const uint32_t *tokens,
+                      float temperature, float *logprob, float *entropy, size_t top, uint32_t *top_tokens,
+                      float *top_logprobs) {
+    return guarded([&] {
+        token_logprobs(device, logits, rows, vocab, tokens, temperature, logprob, entropy, top, top_tokens,
+                       top_logprobs);
     });
 }
 

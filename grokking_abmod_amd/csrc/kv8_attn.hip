@@ -1,0 +1,544 @@
+// Causal attention over the 8-bit KV cache: o_i = sum_j softmax_j(scale q_i.k_j) v_j
+// over the keys j at or before query i's position.
+//
+// Every product runs on the BF16 matrix cores.  An E4M3 code is exact in BF16,
+// so keys and values go there as codes, two an instruction, and their scales
+// meet the scores and the probabilities in FP32.  Queries and probabilities go
+// there as one BF16 (BF16 calls: half a step, 2^-9, of each probability, of
+// random sign and of the size of the result's own rounding), as two (F16 calls:
+// 16 bits of the probabilities, queries exact) or as three (F32 calls: 24 bits,
+// exact), each piece a product of its own.  Scores, maxima, sums and outputs are
+// FP32.
+//
+// A wave takes tiles of 64 keys for 16 query rows at a time; query heads that
+// share a cached head are rows of the same tile.  The scores are computed
+// transposed, S^T = K Q^T: a lane then holds 16 keys of one row, all of them in
+// one block of 16 tokens when the rows of K are taken in the order
+// 16 (m / 4) + 4 t + m % 4 for matrix row m of product t.  So one scale of the
+// keys and one of the values serve a lane, the maximum and the sum need two lane
+// exchanges, and the probabilities are where the second product, O^T = V^T P^T,
+// takes them: nothing moves between lanes.  Its values come in 16-byte loads
+// because the cache holds them transposed.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "operators.hpp"
+#include "types.hpp"
+
+namespace meshgpt::kern {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+
+// Pieces of a query or probability in BF16.
+template <class T>
+constexpr int kPieces = sizeof(typename T::Raw) == 4 ? 3 : 1;
+template <>
+constexpr int kPieces<F16> = 2;
+
+__device__ __forceinline__ float bits(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+__device__ __forceinline__ float power(int byte) { return bits(uint32_t(byte) << 23); }
+
+// Two codes of a word as BF16.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+}
+__device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(bf16x8, u32x4{codes2<false>(a), codes2<true>(a), codes2<false>(b), codes2<true>(b)});
+}
+
+// x as a sum of NP BF16 values: all but the last cut off, the last rounded
+// (and exact, for the third of an f32).
+template <int NP>
+__device__ __forceinline__ void pieces8(const float (&x)[8], bf16x8 (&out)[NP]) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+    for (int p = 0; p + 1 < NP; ++p) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_perm(bits(r[2 * i + 1]), bits(r[2 * i]), 0x07060302);  // the two high halves
+            r[2 * i] -= bits(bits(r[2 * i]) & 0xffff0000u);
+            r[2 * i + 1] -= bits(bits(r[2 * i + 1]) & 0xffff0000u);
+        }
+        out[p] = __builtin_bit_cast(bf16x8, w);
+    }
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{r[2 * i], r[2 * i + 1]}, bf16x2));
+    out[NP - 1] = __builtin_bit_cast(bf16x8, w);
+}
+
+// The larger (sum) of the four lanes that hold a row.
+__device__ __forceinline__ float row_max(float v) {
+    const auto s = __builtin_amdgcn_permlane16_swap(int(bits(v)), int(bits(v)), false, false);
+    v = fmaxf(bits(uint32_t(s[0])), bits(uint32_t(s[1])));
+    const auto t = __builtin_amdgcn_permlane32_swap(int(bits(v)), int(bits(v)), false, false);
+    return fmaxf(bits(uint32_t(t[0])), bits(uint32_t(t[1])));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    const auto s = __builtin_amdgcn_permlane16_swap(int(bits(v)), int(bits(v)), false, false);
+    v = bits(uint32_t(s[0])) + bits(uint32_t(s[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(int(bits(v)), int(bits(v)), false, false);
+    return bits(uint32_t(t[0])) + bits(uint32_t(t[1]));
+}
+
+// The sequence of a pair (sequence, cached head), and whether its length and
+// count are possible.
+struct Sequence {
+    int seq, head, length, count;
+    bool valid;
+    __device__ __forceinline__ Sequence(const Kv8AttnArgs &a, int pair) {
+        seq = pair / a.cache.heads;
+        head = pair - seq * a.cache.heads;
+        length = a.lengths[seq];
+        count = a.counts ? a.counts[seq] : a.count;
+        valid = length >= 0 && length <= a.cache.capacity && count >= 0 && count <= a.count && count <= length;
+        if (!valid) count = a.count;
+    }
+};
+
+template <class T>
+__device__ __forceinline__ typename T::Raw *out_row(const Kv8AttnArgs &a, const Sequence &s, int r) {
+    const int i = r / a.group;
+    return static_cast<typename T::Raw *>(a.out) + s.seq * a.os.s[0] + i * a.os.s[1] +
+           (s.head * a.group + r - i * a.group) * a.os.s[2];
+}
+
+// NT tiles of 16 rows a wave.  WIDE: every wave has rows of its own and walks
+// all their keys; else the workgroup's waves share 16 NT rows, take the key tiles
+// in turn and join their states at the end.
+template <class T, int PAD, int NT, bool WIDE>
+__global__ void __launch_bounds__(64 * kWaves) kv8_attn_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
+    constexpr int NP = kPieces<T>, STEPS = PAD / 32, DT = PAD / 16;
+    constexpr int WORDS = PAD >= 64 ? PAD / 16 : 2;  // 4-byte words of a key that a lane holds
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    // Workgroups of a pair lie 8 apart, on one XCD and its L2; long rows first.
+    const int id = int(blockIdx.x), pair = id % pairs8;
+    if (pair >= pairs) return;
+    const int split = id / pairs8 % a.splits, tile0 = row_tiles - 1 - id / pairs8 / a.splits;
+    const Sequence s(a, pair);
+    const int row0 = (WIDE ? tile0 * kWaves + wave : tile0) * 16 * NT, rows = s.count * a.group;
+    if (row0 >= rows) return;
+    const int row_end = min(row0 + 16 * NT, rows);
+    if (!s.valid) {
+        if (a.out && a.splits == 1)
+            for (int r = row0; r < row_end; ++r)
+                for (int d = WIDE ? lane : int(threadIdx.x); d < a.cache.width; d += WIDE ? 64 : 64 * kWaves)
+                    out_row<T>(a, s, r)[d] = T::from_float(__builtin_nanf(""));
+        return;
+    }
+    const int begin = s.length - s.count;  // the first query's position
+    const int seen = begin + row0 / a.group, keys = begin + (row_end - 1) / a.group + 1;
+    int t0, t1;
+    if (a.chunk) {
+        t0 = split * (a.chunk / 64);
+        t1 = min((keys + 63) / 64, (split + 1) * (a.chunk / 64));
+        if (t0 >= t1 && a.out) return;  // the join does not read it
+    } else {
+        const int tiles = (keys + 63) / 64, each = (tiles + a.splits - 1) / a.splits;
+        t0 = split * each;
+        t1 = min(tiles, t0 + each);
+    }
+
+    bf16x8 qf[NT][NP][STEPS];
+    int place[NT];  // the row's position, -1 behind the last row
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + n, i = r / a.group;
+        place[t] = r < rows ? begin + i : -1;
+        const auto *q = static_cast<const typename T::Raw *>(a.q) + s.seq * a.qs.s[0] + i * a.qs.s[1] +
+                        (s.head * a.group + r - i * a.group) * a.qs.s[2];
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            const int d = PAD >= 64 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 8 * g;
+            float x[8];
+            if (a.q_aligned && r < rows && d + 8 <= a.cache.width) {
+#pragma unroll
+                for (int j = 0; j < 8 / T::kGroup; ++j) {
+                    float y[T::kGroup];
+                    T::unpack(reinterpret_cast<const uint4 *>(q + d)[j], y);
+#pragma unroll
+                    for (int e = 0; e < T::kGroup; ++e) x[j * T::kGroup + e] = y[e];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = r < rows && d + j < a.cache.width ? T::to_float(q[d + j]) : 0.0f;
+            }
+            bf16x8 piece[NP];
+            pieces8<NP>(x, piece);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) qf[t][p][k] = piece[p];
+        }
+    }
+
+    const uint8_t *const kbase = a.cache.k + size_t(pair) * a.cache.capacity * PAD +
+                                 (16 * (n >> 2) + (n & 3)) * PAD + (PAD >= 64 ? 16 : 8) * g;
+    const uint8_t *const vbase = a.cache.v + size_t(pair) * a.cache.capacity * PAD + n * 64 + 16 * g;
+    const uint8_t *const ksbase = a.cache.ks + size_t(pair) * (a.cache.capacity / 16) + g;
+    const uint8_t *const vsbase = a.cache.vs + size_t(pair) * (a.cache.capacity / 16) + g;
+    auto load_keys = [&](int tile, uint32_t (&k)[4][WORDS]) {
+        const uint8_t *p = kbase + size_t(tile) * 64 * PAD;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if constexpr (PAD >= 64) {
+#pragma unroll
+                for (int c = 0; c < PAD / 64; ++c) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(p + 4 * t * PAD + 64 * c);
+                    k[t][4 * c] = w.x;
+                    k[t][4 * c + 1] = w.y;
+                    k[t][4 * c + 2] = w.z;
+                    k[t][4 * c + 3] = w.w;
+                }
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2 *>(p + 4 * t * PAD);
+                k[t][0] = w.x;
+                k[t][1] = w.y;
+            }
+        }
+    };
+
+    float m[NT], l[NT];
+    f32x4 acc[NT][DT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    constexpr int STRIDE = WIDE ? 1 : kWaves;
+    int tile = WIDE ? t0 : t0 + wave;
+    uint32_t kw[4][WORDS];
+    int kbyte = 0, vbyte = 0;
+    if (tile < t1) {
+        load_keys(tile, kw);
+        kbyte = ksbase[4 * tile];
+        vbyte = vsbase[4 * tile];
+    }
+    for (; tile < t1; tile += STRIDE) {
+        uint4 vw[DT];
+        const uint8_t *const vt = vbase + size_t(tile) * 64 * PAD;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const uint4 *>(vt + d * 16 * 64);
+        // The next tile's keys are under way during this one's products.
+        const int next = min(tile + STRIDE, t1 - 1);
+        uint32_t kn[4][WORDS];
+        load_keys(next, kn);
+        const int kbyte_next = ksbase[4 * next], vbyte_next = vsbase[4 * next];
+
+        f32x4 st[NT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int r = 0; r < NT; ++r) st[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const bf16x8 kf = codes8(kw[t][2 * k], kw[t][2 * k + 1]);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                    for (int r = 0; r < NT; ++r)
+                        st[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[r][p][k], st[r][t], 0, 0, 0);
+            }
+        }
+        const float kscale = power(kbyte) * a.scale_log2, vscale = power(vbyte);
+        const bool masked = tile * 64 + 63 > seen;  // some row does not see all of the tile
+        bf16x8 pf[NT][NP][2];
+#pragma unroll
+        for (int r = 0; r < NT; ++r) {
+            float x[16], top = -INFINITY;
+            const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[j] = st[r][j / 4][j % 4] * kscale;
+                if (masked && key0 + j > place[r]) x[j] = -INFINITY;
+                top = fmaxf(top, x[j]);
+            }
+            top = fmaxf(row_max(top), m[r]);
+            // A row that has seen no key yet keeps -inf; 0 stands for it below.
+            const float base = top == -INFINITY ? 0.0f : top, drop = __builtin_amdgcn_exp2f(m[r] - base);
+            m[r] = top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                float p = __builtin_amdgcn_exp2f(x[j] - base);
+                // What lies behind a row may be anything: it takes no part.
+                if (masked && key0 + j > place[r]) p = 0.0f;
+                sum += p;
+                x[j] = p * vscale;
+                if (masked && key0 + j > place[r]) x[j] = 0.0f;
+            }
+            l[r] = l[r] * drop + sum;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[r][d] *= drop;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = x[8 * h + j];
+                bf16x8 piece[NP];
+                pieces8<NP>(y, piece);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) pf[r][p][h] = piece[p];
+            }
+        }
+        // NaN codes times a probability of 0 would reach rows that do not see
+        // them: in a masked tile they are taken out, and make NaN what sees them.
+        bool special = false;
+        if (masked) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    any |= ((&vw[d].x)[e] & 0x7f7f7f7fu) + 0x01010101u;
+            special = __any((any & 0x80808080u) != 0);
+        }
+        if (special) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                f32x4 hit[NT];
+#pragma unroll
+                for (int r = 0; r < NT; ++r) hit[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                u32x4 w{vw[d].x, vw[d].y, vw[d].z, vw[d].w}, nan;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    nan[e] = (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in each such byte
+                    w[e] &= ~(nan[e] * 0xffu);
+                    nan[e] *= 0x38u;  // the code of 1
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bf16x8 nf = codes8(nan[2 * h], nan[2 * h + 1]);
+#pragma unroll
+                    for (int r = 0; r < NT; ++r) {
+                        u32x4 see;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = tile * 64 + 16 * g + 8 * h + 2 * e;
+                            see[e] = (key <= place[r] ? 0x3f80u : 0u) | (key + 1 <= place[r] ? 0x3f800000u : 0u);
+                        }
+                        hit[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(nf, __builtin_bit_cast(bf16x8, see), hit[r], 0,
+                                                                         0, 0);
+                    }
+                }
+                vw[d] = uint4{w[0], w[1], w[2], w[3]};
+#pragma unroll
+                for (int r = 0; r < NT; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (hit[r][e] > 0.0f) acc[r][d][e] = __builtin_nanf("");
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bf16x8 vf = h ? codes8(vw[d].z, vw[d].w) : codes8(vw[d].x, vw[d].y);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                    for (int r = 0; r < NT; ++r)
+                        acc[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][p][h], acc[r][d], 0, 0, 0);
+            }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) kw[t][w] = kn[t][w];
+        kbyte = kbyte_next;
+        vbyte = vbyte_next;
+    }
+
+    const bool direct = a.out && a.splits == 1;
+    auto part_row = [&](int r) { return a.part + ((size_t(pair) * a.rows + r) * a.splits + split) * a.stride; };
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float sum = row_sum(l[t]);
+            const int r = row0 + 16 * t + n;
+            if (r >= rows) continue;
+            if (direct) {
+                auto *o = out_row<T>(a, s, r);
+                const float inverse = 1.0f / sum;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int at = 16 * d + 4 * g + e;
+                        if (at < a.cache.width) o[at] = T::from_float(acc[t][d][e] * inverse);
+                    }
+            } else {
+                float *o = part_row(r);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int at = 16 * d + 4 * g + e;
+                        if (at < a.stride - 2) o[at] = acc[t][d][e];
+                    }
+                if (g == 0) {
+                    o[a.stride - 2] = m[t];
+                    o[a.stride - 1] = sum;
+                }
+            }
+        }
+    } else {
+        static_assert(NT == 1, "shared rows: one tile");
+        constexpr int PART = PAD < 128 ? PAD : 128;  // channels joined at a time
+        __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
+        __shared__ __align__(16) float wave_o[kWaves][16][PART + 4];
+        const float sum = row_sum(l[0]);
+        if (g == 0) {
+            wave_m[wave][n] = m[0];
+            wave_l[wave][n] = sum;
+        }
+        __syncthreads();
+        float top = wave_m[0][n];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wave_m[w][n]);
+        const float base = top == -INFINITY ? 0.0f : top, mine = __builtin_amdgcn_exp2f(m[0] - base);
+        const int real = row_end - row0;
+#pragma unroll
+        for (int c = 0; c < PAD / PART; ++c) {
+            if (c) __syncthreads();
+#pragma unroll
+            for (int d = 0; d < PART / 16; ++d) {
+                const f32x4 v = acc[0][c * (PART / 16) + d] * mine;
+                *reinterpret_cast<f32x4 *>(&wave_o[wave][n][16 * d + 4 * g]) = v;
+            }
+            __syncthreads();
+            for (int i = int(threadIdx.x); i < real * PART; i += 64 * kWaves) {
+                const int r = i / PART, d = i % PART, at = c * PART + d;
+                float v = 0.0f, total = 0.0f, high = wave_m[0][r];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) high = fmaxf(high, wave_m[w][r]);
+                const float from = high == -INFINITY ? 0.0f : high;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    v += wave_o[w][r][d];
+                    total += wave_l[w][r] * __builtin_amdgcn_exp2f(wave_m[w][r] - from);
+                }
+                if (direct) {
+                    if (at < a.cache.width) out_row<T>(a, s, row0 + r)[at] = T::from_float(v / total);
+                } else {
+                    float *o = part_row(row0 + r);
+                    if (at < a.stride - 2) o[at] = v;
+                    if (at == 0) {
+                        o[a.stride - 2] = high;
+                        o[a.stride - 1] = total;
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Joins the shares of a row: a wave a row.
+template <class T>
+__global__ void __launch_bounds__(256) kv8_join_kernel(Kv8AttnArgs a, int pairs) {
+    const int64_t u = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (u >= int64_t(pairs) * a.rows) return;
+    const int pair = int(u / a.rows), r = int(u - int64_t(pair) * a.rows);
+    const Sequence s(a, pair);
+    if (r >= s.count * a.group) return;
+    auto *o = out_row<T>(a, s, r);
+    if (!s.valid) {
+        for (int d = lane; d < a.cache.width; d += 64) o[d] = T::from_float(__builtin_nanf(""));
+        return;
+    }
+    // The shares that this row's tile of rows wrote reach to the tile's last
+    // row; those past this row's own keys hold nothing of it.
+    const int keys = s.length - s.count + r / a.group + 1, used = (keys + a.chunk - 1) / a.chunk;
+    const float *p = a.part + size_t(u) * a.splits * a.stride;
+    float top = -INFINITY;
+    for (int k = 0; k < used; ++k) top = fmaxf(top, p[size_t(k) * a.stride + a.stride - 2]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < used; ++k) {
+        const float *q = p + size_t(k) * a.stride;
+        const float f = __builtin_amdgcn_exp2f(q[a.stride - 2] - base);
+        total += f * q[a.stride - 1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (lane + 64 * e < a.cache.width) acc[e] += f * q[lane + 64 * e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < a.cache.width) o[lane + 64 * e] = T::from_float(acc[e] / total);
+}
+
+// Tiles of 16 rows that a wave with rows of its own takes: as many as its
+// registers hold.
+template <class T>
+constexpr int wide_tiles(int pad) {
+    return pad <= 64 ? 2 : pad == 128 ? (kPieces<T> == 3 ? 1 : 2) : 1;
+}
+
+template <class T, int PAD>
+void launch_attn(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) {
+    const int pairs = a.cache.batch * a.cache.heads;
+    const int pairs8 = plan.wide ? (pairs + 7) / 8 * 8 : pairs;
+    const dim3 grid(uint32_t(pairs8) * uint32_t(a.splits) * uint32_t(plan.row_tiles));
+    if (plan.wide)
+        hipLaunchKernelGGL((kv8_attn_kernel<T, PAD, wide_tiles<T>(PAD), true>), grid, dim3(64 * kWaves), 0, stream, a,
+                           pairs, pairs8, plan.row_tiles);
+    else
+        hipLaunchKernelGGL((kv8_attn_kernel<T, PAD, 1, false>), grid, dim3(64 * kWaves), 0, stream, a, pairs, pairs8,
+                           plan.row_tiles);
+    if (a.out && a.splits > 1)
+        hipLaunchKernelGGL((kv8_join_kernel<T>), dim3(uint32_t((int64_t(pairs) * a.rows + 3) / 4)), dim3(256), 0,
+                           stream, a, pairs);
+}
+
+template <class T>
+void attn_of(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) {
+    switch (a.cache.pad) {
+    case 32: return launch_attn<T, 32>(a, plan, stream);
+    case 64: return launch_attn<T, 64>(a, plan, stream);
+    case 128: return launch_attn<T, 128>(a, plan, stream);
+    default: return launch_attn<T, 256>(a, plan, stream);
+    }
+}
+
+}  // namespace
+
+Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count) {
+    Kv8Plan p{};
+    const int64_t rows = int64_t(count) * group;
+    const int pairs = std::max(1, cache.batch * cache.heads);
+    const int tiles = type == Type::F32 ? wide_tiles<F32>(cache.pad) : type == Type::F16 ? wide_tiles<F16>(cache.pad)
+                                                                                         : wide_tiles<BF16>(cache.pad);
+    p.wide = rows > 16;
+    const int each = p.wide ? 16 * kWaves * tiles : 16;
+    p.row_tiles = int((rows + each - 1) / each);
+    // Shares of the keys: about 2048 workgroups, of 256 keys or more.
+    const int64_t groups = int64_t(pairs) * p.row_tiles, most = std::max(1, cache.capacity / 256);
+    const int64_t want = std::min<int64_t>(std::min<int64_t>(most, 256), (2048 + groups - 1) / groups);
+    p.chunk = int((cache.capacity + want - 1) / want + 63) / 64 * 64;
+    p.splits = (cache.capacity + p.chunk - 1) / p.chunk;
+    p.part_floats = p.splits > 1 ? size_t(pairs) * size_t(rows) * size_t(p.splits) * size_t(cache.pad + 2) : 0;
+    return p;
+}
+
+void kv8_attention(const Kv8AttnArgs &a, Type type, const Kv8Plan &plan, hipStream_t stream) {
+    switch (type) {
+    case Type::F32: return attn_of<F32>(a, plan, stream);
+    case Type::F16: return attn_of<F16>(a, plan, stream);
+    default: return attn_of<BF16>(a, plan, stream);
+    }
+}
+
+}  // namespace meshgpt::kern

@@ -1,0 +1,526 @@
+// Log probabilities of given tokens under rows of logits z at a temperature T,
+// with the entropy and the best alternatives, and their gradient.
+//
+//   d_v = (z_v - max z) / T,  S = sum_v exp(d_v),  log p_v = d_v - ln S
+//   entropy H = ln S - sum_v exp(d_v) d_v / S
+//   dz_v = [g (1[v = token] - p_v) - h p_v (log p_v + H)] / T
+//
+// The forward pass reads a row once: each thread keeps its running maximum, the
+// sum and the sum of exp(d) d against it, in FP32, and they join at the end.
+// The alternatives come out of the same pass.  The k-th largest of the threads'
+// maxima bounds the k-th largest logit from below, so only the threads whose
+// maximum reaches it hold any of the best k; those look at their logits again
+// (from the cache) and a few more than k of them are sorted by counting.
+// Reading the logits is what bounds it.  Rows are cut into chunks of at most
+// 128 logits a thread, so that the logits over the bound always fit the list,
+// and shorter ones where there are few rows; a wave then joins a row's chunks.
+// Rows of up to 1024 logits stay in a wave's registers.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+
+#include "operators.hpp"
+#include "types.hpp"
+
+namespace meshgpt::kern {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kSmall = 1024;           // logits of a row that one wave holds
+constexpr int kThreadMost = 128;       // logits of a thread's share of a chunk
+constexpr int kList = 4096;            // candidates of a chunk: over kTopMax - 1 threads' shares
+constexpr uint32_t kIgnore = 0xffffffffu;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A thread's share of a chunk is its groups and at most one logit before and
+// behind them.
+constexpr int kChunkMost = kBlock * (kThreadMost - 16);
+static_assert((kTopMax - 1) * kThreadMost <= kList, "the logits over the bound fit the list");
+
+// Orders as the floats do, -0 with 0; NaN is not asked for.
+__device__ __forceinline__ uint32_t order(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unorder(uint32_t k) {
+    return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// Larger logits first, of equal ones the lower token.
+__device__ __forceinline__ uint64_t candidate(uint32_t k, uint32_t token) { return (uint64_t(k) << 32) | uint32_t(~token); }
+
+// Maximum, sum and sum of exp(d) d of some logits.  `m` starts at -inf; sums
+// are against max(m, -FLT_MAX), so that -inf logits add 0 to both.
+struct Sums {
+    float m = -INFINITY, s = 0.0f, a = 0.0f;
+    // The sums against a maximum of at least `top`.
+    __device__ __forceinline__ void raise(float top, float c) {
+        const float to = fmaxf(m, top), step = fmaxf((fmaxf(m, -FLT_MAX) - fmaxf(to, -FLT_MAX)) * c, -1e20f);
+        const float f = __builtin_amdgcn_exp2f(step);
+        a = f * fmaf(step, s, a);
+        s *= f;
+        m = to;
+    }
+    __device__ __forceinline__ void join(float m2, float s2, float a2, float c) {
+        Sums o;
+        o.m = m2;
+        o.s = s2;
+        o.a = a2;
+        raise(m2, c);
+        o.raise(m, c);
+        s += o.s;
+        a += o.a;
+    }
+};
+
+// d in log2 units against base; exp(d) d of -inf is 0.
+__device__ __forceinline__ void add(float x, float base, float c, float &s, float &a) {
+    const float d = __builtin_elementwise_maximum((x - base) * c, -1000.0f), e = __builtin_amdgcn_exp2f(d);
+    s += e;
+    a = fmaf(e, d, a);
+}
+
+__device__ __forceinline__ void wave_join(Sums &t, float c) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const float m = __shfl_xor(t.m, k, 64), s = __shfl_xor(t.s, k, 64), a = __shfl_xor(t.a, k, 64);
+        t.join(m, s, a, c);
+    }
+}
+
+__device__ __forceinline__ uint64_t wave_best(uint64_t v) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const uint64_t o = __shfl_xor(v, k, 64);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+// A row's results from its sums (a in log2 units); one thread.
+template <class T>
+__device__ __forceinline__ void write_row(const LogprobArgs &a, size_t row, const Sums &t, float &log_sum) {
+    const auto *z = static_cast<const typename T::Raw *>(a.logits) + row * a.stride;
+    const bool empty = t.s == 0.0f;  // no token is allowed: log probabilities are -inf
+    log_sum = empty ? -INFINITY : logf(t.s);
+    if (a.logprob) {
+        const uint32_t token = a.tokens[row];
+        float v = 0.0f;
+        if (token != kIgnore) {
+            if (token >= a.vocab)
+                v = __builtin_nanf("");
+            else
+                v = empty ? -INFINITY : (T::to_float(z[token]) - t.m) * a.inv_temperature - log_sum;
+        }
+        a.logprob[row] = v;
+    }
+    if (a.entropy) a.entropy[row] = empty ? 0.0f : log_sum - t.a / (t.s * kLog2e);
+    if (a.stats) {
+        a.stats[2 * row] = t.s == t.s ? t.m : __builtin_nanf("");
+        a.stats[2 * row + 1] = log_sum;
+    }
+}
+
+// Alternative i of a row.  A row with a NaN or +inf has no probabilities (s is
+// NaN): its alternatives are its first tokens, at NaN.
+__device__ __forceinline__ void write_top(const LogprobArgs &a, size_t row, int i, uint64_t best, const Sums &t,
+                                          float log_sum) {
+    const bool none = !(t.s == t.s);
+    const uint32_t token = none ? uint32_t(i) : ~uint32_t(best);
+    a.top_tokens[row * a.top + i] = token;
+    if (a.top_logprobs)
+        a.top_logprobs[row * a.top + i] =
+            none ? __builtin_nanf("")
+                 : t.s == 0.0f ? -INFINITY : (unorder(uint32_t(best >> 32)) - t.m) * a.inv_temperature - log_sum;
+}
+
+// Rows of up to 64 N logits, a wave a row.
+template <class T, int N>
+__global__ void __launch_bounds__(kBlock) logprob_small_kernel(LogprobArgs a) {
+    const size_t row = size_t(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= a.rows) return;
+    const auto *z = static_cast<const typename T::Raw *>(a.logits) + row * a.stride;
+    const float c = a.inv_temperature * kLog2e;
+    float x[N];
+    Sums t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t v = lane + 64 * i;
+        x[i] = v < a.vocab ? T::to_float(z[v]) : -INFINITY;
+        t.m = fmaxf(t.m, x[i]);
+    }
+    const float base = fmaxf(t.m, -FLT_MAX);
+#pragma unroll
+    for (int i = 0; i < N; ++i) add(x[i], base, c, t.s, t.a);
+    wave_join(t, c);
+    float log_sum = 0.0f;
+    if (lane == 0) write_row<T>(a, row, t, log_sum);
+    if (!a.top) return;
+    log_sum = __shfl(log_sum, 0, 64);
+    uint32_t taken = 0;
+    for (int k = 0; k < a.top; ++k) {
+        uint64_t best = 0;
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t v = lane + 64 * i;
+            const uint64_t o = v < a.vocab && !(taken >> i & 1) ? candidate(order(x[i]), v) : 0;
+            if (o > best) {
+                best = o;
+                at = i;
+            }
+        }
+        const uint64_t first = wave_best(best);
+        if (best == first) {  // candidates differ, so one lane has it
+            taken |= 1u << at;
+            write_top(a, row, k, first, t, log_sum);
+        }
+    }
+}
+
+// One chunk of a row.
+template <class T>
+__global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
+    using Raw = typename T::Raw;
+    constexpr int G = T::kGroup;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t row = blockIdx.x / uint32_t(a.chunks);
+    const int chunk = int(blockIdx.x - uint32_t(row) * uint32_t(a.chunks));
+    const auto *z = static_cast<const Raw *>(a.logits) + row * a.stride;
+    const float c = a.inv_temperature * kLog2e;
+    const uint32_t lo = uint32_t(chunk) * uint32_t(a.chunk);
+    const uint32_t hi = uint32_t(min(size_t(lo) + size_t(a.chunk), a.vocab));
+    // [lo, body) and [tail, hi) lie outside whole 16-byte groups.
+    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(z + lo) % 16 / sizeof(Raw));
+    const uint32_t body = min(hi, lo + (G - off) % G), groups = (hi - body) / G, tail = body + groups * G;
+    const uint4 *const zg = reinterpret_cast<const uint4 *>(z + body);
+
+    Sums t;
+    auto one = [&](float x) {
+        if (x > t.m) t.raise(x, c);
+        add(x, fmaxf(t.m, -FLT_MAX), c, t.s, t.a);
+    };
+    auto group = [&](uint4 w) {
+        float x[G];
+        T::unpack(w, x);
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < G; ++j) top = fmaxf(top, x[j]);
+        if (top > t.m) t.raise(top, c);
+        const float base = fmaxf(t.m, -FLT_MAX);
+        float s = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int j = 0; j < G; ++j) add(x[j], base, c, s, q);
+        t.s += s;
+        t.a += q;
+    };
+    if (uint32_t(tid) < body - lo) one(T::to_float(z[lo + tid]));
+    if (uint32_t(tid) < hi - tail) one(T::to_float(z[tail + tid]));
+    uint32_t i = tid;
+    for (; i + 3 * kBlock < groups; i += 4 * kBlock) {
+        uint4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = zg[i + u * kBlock];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) group(w[u]);
+    }
+    for (; i < groups; i += kBlock) group(zg[i]);
+
+    __shared__ float joined[kBlock / 64][3];
+    __shared__ uint32_t tops[kBlock];
+    __shared__ uint32_t bound, found, over;
+    __shared__ uint64_t list[kList];
+    const bool any = uint32_t(tid) < body - lo || uint32_t(tid) < hi - tail || uint32_t(tid) < groups;
+    const uint32_t mine = any ? order(t.m) : 0;
+    if (a.top) tops[tid] = mine;
+    wave_join(t, c);
+    if (lane == 0) {
+        joined[wave][0] = t.m;
+        joined[wave][1] = t.s;
+        joined[wave][2] = t.a;
+    }
+    if (tid == 0) found = over = 0;
+    __syncthreads();
+    t.m = joined[0][0];
+    t.s = joined[0][1];
+    t.a = joined[0][2];
+#pragma unroll
+    for (int w = 1; w < kBlock / 64; ++w) t.join(joined[w][0], joined[w][1], joined[w][2], c);
+    float log_sum = 0.0f;
+    if (a.chunks > 1) {
+        if (tid == 0) {
+            float *p = a.part_stats + (row * a.chunks + chunk) * 3;
+            p[0] = t.m;
+            p[1] = t.s;
+            p[2] = t.a;
+        }
+    } else {
+        if (tid == 0) write_row<T>(a, row, t, log_sum);
+        log_sum = t.s == 0.0f ? -INFINITY : logf(t.s);
+    }
+    if (!a.top) return;
+    uint64_t *const part = a.part_top + (row * a.chunks + chunk) * a.top;
+    const int top = a.top, have = int(min(uint32_t(top), hi - lo));  // the chunk may hold fewer
+    if (!(t.s == t.s)) {  // a NaN: any tokens do, they are not used
+        if (tid < top) {
+            if (a.chunks > 1)
+                part[tid] = 0;
+            else
+                write_top(a, row, tid, 0, t, log_sum);
+        }
+        return;
+    }
+    // The have-th largest of the threads' maxima, bit by bit, where so many
+    // threads hold any; with fewer (a short chunk) every logit is looked at.
+    if (wave == 0) {
+        uint32_t k[kBlock / 64], at = 0;
+#pragma unroll
+        for (int w = 0; w < kBlock / 64; ++w) k[w] = tops[lane + 64 * w];
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < kBlock / 64; ++w) n += __popcll(__ballot(k[w] >= (at | bit)));
+            if (n >= have) at |= bit;
+        }
+        if (lane == 0) bound = at;
+    }
+    __syncthreads();
+    const uint32_t least = bound;
+    auto offer = [&](float x, uint32_t v, bool equal_too) {
+        const uint32_t k = order(x);
+        if (k < least || (k == least && !equal_too)) return;
+        const uint32_t at = atomicAdd(&found, 1u);
+        if (at < uint32_t(kList))
+            list[at] = candidate(k, v);
+        else
+            over = 1;
+    };
+    auto share = [&](bool equal_too) {
+        if (uint32_t(tid) < body - lo) offer(T::to_float(z[lo + tid]), lo + tid, equal_too);
+        if (uint32_t(tid) < hi - tail) offer(T::to_float(z[tail + tid]), tail + tid, equal_too);
+        for (uint32_t j = tid; j < groups; j += kBlock) {
+            float x[G];
+            T::unpack(zg[j], x);
+#pragma unroll
+            for (int e = 0; e < G; ++e) offer(x[e], body + j * G + e, equal_too);
+        }
+    };
+    if (mine >= least && any) share(true);
+    __syncthreads();
+    if (over) {
+        // Many logits equal the bound (most of a masked row, say): the ones
+        // over it, which fit, then equal ones in the order of their tokens
+        // until there are enough.
+        __syncthreads();
+        if (tid == 0) found = 0;
+        __syncthreads();
+        if (mine > least && any) share(false);
+        for (uint32_t from = lo; from < hi; from += kBlock) {
+            __syncthreads();
+            if (found >= uint32_t(have)) break;
+            __syncthreads();
+            const uint32_t v = from + tid;
+            if (v < hi && order(T::to_float(z[v])) == least) {
+                const uint32_t at = atomicAdd(&found, 1u);
+                list[min(at, uint32_t(kList - 1))] = candidate(least, v);
+            }
+        }
+        __syncthreads();
+    }
+    // A candidate's place is the number of those before it.
+    const int n = min(int(found), kList);
+    for (int j = tid; j < n; j += kBlock) {
+        const uint64_t v = list[j];
+        int before = 0;
+        for (int o = 0; o < n; ++o) before += list[o] > v;
+        if (before < top) {
+            if (a.chunks > 1)
+                part[before] = v;
+            else
+                write_top(a, row, before, v, t, log_sum);
+        }
+    }
+    if (a.chunks > 1 && tid >= have && tid < top) part[tid] = 0;
+}
+
+// Joins a row's chunks: one wave.  Lane c holds chunks c, c + 64, ... by the
+// first of their candidates that is not taken.
+template <class T>
+__global__ void __launch_bounds__(64) logprob_join_kernel(LogprobArgs a) {
+    const size_t row = blockIdx.x;
+    const int lane = threadIdx.x;
+    const float c = a.inv_temperature * kLog2e;
+    Sums t;
+    for (int k = lane; k < a.chunks; k += 64) {
+        const float *p = a.part_stats + (row * a.chunks + k) * 3;
+        t.join(p[0], p[1], p[2], c);
+    }
+    wave_join(t, c);
+    float log_sum = 0.0f;
+    if (lane == 0) write_row<T>(a, row, t, log_sum);
+    if (!a.top) return;
+    log_sum = t.s == 0.0f ? -INFINITY : logf(t.s);
+    constexpr int HELD = ((1 << 24) / kChunkMost + 64) / 64;  // chunks of a lane at most
+    uint64_t head[HELD];
+    uint32_t taken[HELD];
+    const uint64_t *const lists = a.part_top + row * a.chunks * a.top;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int k = lane + 64 * i;
+        taken[i] = 0;
+        head[i] = k < a.chunks ? lists[size_t(k) * a.top] : 0;
+    }
+    for (int k = 0; k < a.top; ++k) {
+        uint64_t best = head[0];
+#pragma unroll
+        for (int i = 1; i < HELD; ++i) best = head[i] > best ? head[i] : best;
+        const uint64_t first = wave_best(best);
+        if (lane == 0) write_top(a, row, k, first, t, log_sum);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (head[i] == first && first) {
+                const int chunk = lane + 64 * i;
+                head[i] = int(++taken[i]) < a.top ? lists[size_t(chunk) * a.top + taken[i]] : 0;
+            }
+    }
+}
+
+// Groups of logits a thread takes at a time, and of a row's share a workgroup.
+constexpr int kGradChunk = 16;  // 16-byte groups of a thread
+
+template <class T>
+__device__ __forceinline__ float grad_of(float x, uint32_t v, const LogprobBackwardArgs &a, uint32_t token, float m,
+                                         float log_sum, float g, float h, float entropy) {
+    // log p in natural units; a row without any allowed token has m = -inf.
+    const float lp = (x - m) * a.inv_temperature - log_sum, p = __builtin_amdgcn_exp2f(lp * kLog2e);
+    const float of_p = h == 0.0f ? g : fmaf(h, (p > 0.0f ? lp : 0.0f) + entropy, g);
+    float d = -p * of_p;
+    if (v == token) d += g;
+    return d * a.inv_temperature;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwardArgs a, uint32_t chunks) {
+    using Raw = typename T::Raw;
+    constexpr int G = T::kGroup;
+    const int tid = threadIdx.x;
+    const size_t row = blockIdx.x / chunks;
+    const uint32_t chunk = blockIdx.x - uint32_t(row) * chunks;
+    const auto *z = static_cast<const Raw *>(a.logits) + row * a.stride;
+    auto *out = static_cast<Raw *>(a.d_logits) + row * a.d_stride;
+    const uint32_t token = a.tokens ? a.tokens[row] : kIgnore;
+    const float m = a.stats[2 * row], log_sum = a.stats[2 * row + 1];
+    float g = a.d_logprob && token != kIgnore ? a.d_logprob[row] : 0.0f;
+    if (token != kIgnore && token >= a.vocab) g = __builtin_nanf("");
+    const float h = a.d_entropy ? a.d_entropy[row] : 0.0f, entropy = a.d_entropy ? a.entropy[row] : 0.0f;
+    const bool none = m == -INFINITY;  // no token is allowed: nothing depends on the logits
+    auto grad = [&](float x, uint32_t v) {
+        return none ? 0.0f : grad_of<T>(x, v, a, token, m, log_sum, g, h, entropy);
+    };
+    const uint32_t size = kBlock * kGradChunk * G, lo = chunk * size;
+    const uint32_t hi = uint32_t(min(size_t(lo) + size, a.vocab));
+    const uint32_t in_off = uint32_t(reinterpret_cast<uintptr_t>(z + lo) % 16);
+    if (in_off != uint32_t(reinterpret_cast<uintptr_t>(out + lo) % 16)) {  // no common 16-byte groups
+        for (uint32_t v = lo + tid; v < hi; v += kBlock) out[v] = T::from_float(grad(T::to_float(z[v]), v));
+        return;
+    }
+    const uint32_t body = min(hi, lo + (G - in_off / uint32_t(sizeof(Raw))) % G), groups = (hi - body) / G,
+                   tail = body + groups * G;
+    if (uint32_t(tid) < body - lo) out[lo + tid] = T::from_float(grad(T::to_float(z[lo + tid]), lo + tid));
+    if (uint32_t(tid) < hi - tail) out[tail + tid] = T::from_float(grad(T::to_float(z[tail + tid]), tail + tid));
+    const uint4 *const zg = reinterpret_cast<const uint4 *>(z + body);
+    uint4 *const og = reinterpret_cast<uint4 *>(out + body);
+    auto one = [&](uint4 w, uint32_t i) {
+        float x[G];
+        T::unpack(w, x);
+#pragma unroll
+        for (int j = 0; j < G; ++j) x[j] = grad(x[j], body + i * G + j);
+        og[i] = T::pack(x);
+    };
+    uint32_t i = tid;
+    for (; i + 3 * kBlock < groups; i += 4 * kBlock) {
+        uint4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = zg[i + u * kBlock];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) one(w[u], i + u * kBlock);
+    }
+    for (; i < groups; i += kBlock) one(zg[i], i);
+}
+
+// Short rows: a wave a row.
+template <class T>
+__global__ void __launch_bounds__(kBlock) logprob_backward_small_kernel(LogprobBackwardArgs a) {
+    const size_t row = size_t(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    const auto *z = static_cast<const typename T::Raw *>(a.logits) + row * a.stride;
+    auto *out = static_cast<typename T::Raw *>(a.d_logits) + row * a.d_stride;
+    const uint32_t token = a.tokens ? a.tokens[row] : kIgnore;
+    const float m = a.stats[2 * row], log_sum = a.stats[2 * row + 1];
+    float g = a.d_logprob && token != kIgnore ? a.d_logprob[row] : 0.0f;
+    if (token != kIgnore && token >= a.vocab) g = __builtin_nanf("");
+    const float h = a.d_entropy ? a.d_entropy[row] : 0.0f, entropy = a.d_entropy ? a.entropy[row] : 0.0f;
+    for (uint32_t v = threadIdx.x & 63; v < a.vocab; v += 64)
+        out[v] = T::from_float(m == -INFINITY ? 0.0f
+                                              : grad_of<T>(T::to_float(z[v]), v, a, token, m, log_sum, g, h, entropy));
+}
+
+template <class T>
+void forward_of(const LogprobArgs &a, hipStream_t stream) {
+    if (a.vocab <= size_t(kSmall)) {
+        const dim3 grid(uint32_t((a.rows + kBlock / 64 - 1) / (kBlock / 64)));
+        if (a.vocab <= 256)
+            hipLaunchKernelGGL((logprob_small_kernel<T, 4>), grid, dim3(kBlock), 0, stream, a);
+        else
+            hipLaunchKernelGGL((logprob_small_kernel<T, kSmall / 64>), grid, dim3(kBlock), 0, stream, a);
+        return;
+    }
+    hipLaunchKernelGGL((logprob_kernel<T>), dim3(uint32_t(a.rows * size_t(a.chunks))), dim3(kBlock), 0, stream, a);
+    if (a.chunks > 1)
+        hipLaunchKernelGGL((logprob_join_kernel<T>), dim3(uint32_t(a.rows)), dim3(64), 0, stream, a);
+}
+
+template <class T>
+void backward_of(const LogprobBackwardArgs &a, hipStream_t stream) {
+    if (a.vocab <= size_t(kSmall)) {
+        hipLaunchKernelGGL((logprob_backward_small_kernel<T>), dim3(uint32_t((a.rows + kBlock / 64 - 1) / (kBlock / 64))),
+                           dim3(kBlock), 0, stream, a);
+        return;
+    }
+    const size_t size = size_t(kBlock) * kGradChunk * T::kGroup, chunks = (a.vocab + size - 1) / size;
+    hipLaunchKernelGGL((logprob_backward_kernel<T>), dim3(uint32_t(a.rows * chunks)), dim3(kBlock), 0, stream, a,
+                       uint32_t(chunks));
+}
+
+}  // namespace
+
+void logprob_chunks(size_t rows, size_t vocab, int &chunks, int &chunk) {
+    chunks = 1;
+    chunk = int(vocab);
+    if (vocab <= size_t(kSmall)) return;
+    // About 1024 workgroups, each of 2048 logits or more.
+    const size_t want = std::min<size_t>((1024 + rows - 1) / std::max<size_t>(rows, 1), (vocab + 2047) / 2048);
+    size_t size = (vocab + want - 1) / want;
+    size = std::min<size_t>((size + 63) / 64 * 64, size_t(kChunkMost));
+    chunk = int(size);
+    chunks = int((vocab + size - 1) / size);
+}
+
+void token_logprobs(const LogprobArgs &a, Type type, hipStream_t stream) {
+    switch (type) {
+    case Type::F32: return forward_of<F32>(a, stream);
+    case Type::F16: return forward_of<F16>(a, stream);
+    default: return forward_of<BF16>(a, stream);
+    }
+}
+
+void token_logprobs_backward(const LogprobBackwardArgs &a, Type type, hipStream_t stream) {
+    switch (type) {
+    case Type::F32: return backward_of<F32>(a, stream);
+    case Type::F16: return backward_of<F16>(a, stream);
+    default: return backward_of<BF16>(a, stream);
+    }
+}
+
+}  // namespace meshgpt::kern

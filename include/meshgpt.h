@@ -237,6 +237,102 @@ int mg_sample_logits(int device, const float *logits, size_t rows, size_t vocab,
 int mg_sample_logits_noalloc(int device, const float *logits, size_t rows, size_t vocab, float temperature,
                              uint64_t *rng_states, uint32_t *tokens, int *nonfinite, void *stream);
 
+/* Operators on device buffers that the caller owns.  No counterpart in the
+ * reference: its cache-free FP32 program has none of them.
+ *
+ * Each enqueues its work on `stream` (a hipStream_t of `device`; NULL is the
+ * default stream) and returns without waiting, allocates nothing, and can be
+ * captured into a HIP graph.  Pointers are device pointers; lengths, counts,
+ * tokens and scratch are read and written by the enqueued work, so they have to
+ * stay until it is done.  Calls that may overlap need workspaces of their own, as
+ * do captured graphs that may.  The calling thread's current device is the same
+ * on return as on entry. */
+enum { MG_F32 = 0, MG_F16 = 1, MG_BF16 = 2 };
+
+/* An 8-bit KV cache of `batch` sequences, in buffers of the caller:
+ *   k        [batch][kv_heads][capacity][P]            E4M3 codes
+ *   v        [batch][kv_heads][capacity / 64][P][64]   E4M3 codes, transposed
+ *   k_scale  [batch][kv_heads][capacity / 16]          one byte b for 16 tokens
+ *   v_scale  the same                                  of a head: scale 2^(b - 127)
+ * P is the head width (1..256) padded to 32, 64, 128 or 256; padded channels of
+ * written tokens hold 0.  capacity is a multiple of 64; k and v are aligned to
+ * 16 bytes.  The buffers need no clearing: positions behind a sequence's length
+ * are never used, whatever they hold. */
+typedef struct {
+    uint32_t batch, kv_heads, head_width, capacity;
+    uint8_t *k, *v, *k_scale, *v_scale;
+} mg_kv8;
+/* Bytes of k (and of v), and of k_scale (and of v_scale). */
+int mg_kv8_sizes(const mg_kv8 *cache, size_t *codes, size_t *scales);
+
+/* Writes the last tokens of each sequence to its cache, quantised.  lengths
+ * (batch ints) are the sequences' tokens with the new ones; counts (batch ints,
+ * or NULL: `count` each) how many of them are new, at most `count`.  New token i
+ * of sequence s, head h is at k + s * k_strides[0] + i * k_strides[1] + h *
+ * k_strides[2] (in elements of `type`), head_width elements in a row; v alike.
+ * The scale of 16 tokens is the smallest power of two from 2^-117 to 2^120 with
+ * which their largest magnitude is at most 448, and the codes are the nearest,
+ * ties to even (with 2^120, to at most 240).  A 16-token block that was begun by
+ * an earlier call keeps its scale or, where the new tokens need it, takes a
+ * larger one: then its older codes are rounded once more.  NaN and infinities
+ * become NaN.  A sequence whose length is negative or over the capacity, or
+ * whose count is negative or over its length or over `count`, is left as it is. */
+int mg_kv8_append(int device, const mg_kv8 *cache, int type, size_t count, const void *k, const int64_t k_strides[3],
+                  const void *v, const int64_t v_strides[3], const int32_t *lengths, const int32_t *counts,
+                  void *stream);
+/* Reads positions first..first + count - 1 of every sequence back, as values of
+ * `type` (strides as in mg_kv8_append, for the outputs); with `lengths` (NULL:
+ * none) only those inside each sequence, and the outputs behind stay as they are. */
+int mg_kv8_read(int device, const mg_kv8 *cache, int type, size_t first, size_t count, void *k,
+                const int64_t k_strides[3], void *v, const int64_t v_strides[3], const int32_t *lengths, void *stream);
+/* Causal attention of each sequence's last tokens over its cache: query i of the
+ * counts[s] (or `count`) last tokens sees the keys up to its own position, with
+ * weights softmax(scale q.k).  `heads` is a multiple of kv_heads; query head h
+ * reads cached head h / (heads / kv_heads).  q and out are laid out as the inputs
+ * of mg_kv8_append, with `heads` heads; out may be q.  Rows behind a sequence's
+ * count stay as they are.  A NaN or infinity that a row sees makes what depends
+ * on it NaN; what it does not see has no effect.  The rows of a sequence whose
+ * length or count is impossible (as above) are filled with NaN, all `count` of
+ * them.  F32 calls keep 24 bits of the queries and probabilities, F16 and BF16
+ * calls 16 and 8 of the probabilities; sums are FP32.  The workspace holds
+ * mg_kv8_attention_workspace bytes, aligned to 4 (NULL where that is 0). */
+int mg_kv8_attention_workspace(const mg_kv8 *cache, size_t heads, size_t count, size_t *bytes);
+int mg_kv8_attention(int device, const mg_kv8 *cache, int type, size_t heads, size_t count, const void *q,
+                     const int64_t q_strides[3], void *out, const int64_t out_strides[3], const int32_t *lengths,
+                     const int32_t *counts, float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Log probabilities of given tokens: for each row of `vocab` logits (rows
+ * `stride` elements of `type` apart) at `temperature`, the log probability of
+ * tokens[r], the entropy of the row's distribution, and the `top` (at most
+ * MG_TOP_MAX) most probable tokens, of equal ones the lowest first, with their
+ * log probabilities (rows x top each).  stats, two floats a row, receives what
+ * the gradient needs: the largest logit and the log of the sum of
+ * exp((logit - largest) / temperature).  logprob, entropy, stats and
+ * top_logprobs may be NULL.  A token of MG_IGNORE_TARGET has log probability 0,
+ * one outside the vocabulary NaN.  Logits of -inf are tokens that are not
+ * allowed; a row without any other has log probabilities of -inf and entropy 0.
+ * A NaN or +inf makes its row NaN, and its alternatives the tokens 0..top-1. */
+#define MG_TOP_MAX 32
+int mg_token_logprobs_workspace(size_t rows, size_t vocab, size_t top, size_t *bytes);
+int mg_token_logprobs_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab, size_t stride,
+                              const uint32_t *tokens, float temperature, float *logprob, float *entropy, float *stats,
+                              size_t top, uint32_t *top_tokens, float *top_logprobs, void *workspace,
+                              size_t workspace_bytes, void *stream);
+/* The gradient of the logits, written in their type, from the gradients of the
+ * log probabilities and of the entropies (rows floats each; either may be NULL)
+ * and the forward call's stats and entropies.  Rows of MG_IGNORE_TARGET take
+ * nothing from d_logprob; a row without an allowed token has gradient 0.
+ * d_logits may be the logits, with the same stride. */
+int mg_token_logprobs_backward_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab,
+                                       size_t stride, const uint32_t *tokens, float temperature, const float *stats,
+                                       const float *entropy, const float *d_logprob, const float *d_entropy,
+                                       void *d_logits, size_t d_stride, void *stream);
+/* mg_token_logprobs_noalloc on host arrays of f32 logits (mg_logits,
+ * mg_last_logits); it allocates, waits, and refuses tokens outside the vocabulary. */
+int mg_token_logprobs(int device, const float *logits, size_t rows, size_t vocab, const uint32_t *tokens,
+                      float temperature, float *logprob, float *entropy, size_t top, uint32_t *top_tokens,
+                      float *top_logprobs);
+
 /* out[i] = the f32 exp the sampler of mg_generate uses (the reference's
  * f32::exp, i.e. the C library's expf), evaluated on `device`.  No separate
  * reference call: it lets tests compare the device exp with the host's. */
