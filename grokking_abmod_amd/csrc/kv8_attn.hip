@@ -23,6 +23,7 @@
 
 #include <algorithm>
 
+#include "lds_dma.hpp"
 #include "operators.hpp"
 #include "types.hpp"
 
@@ -93,6 +94,106 @@ __device__ __forceinline__ float row_sum(float v) {
     return bits(uint32_t(t[0])) + bits(uint32_t(t[1]));
 }
 
+// Rows keep a maximum that their scores may pass by up to 2^kSlack before sums
+// and outputs are brought to a new one: nearly no tile after the first does, and
+// nothing is lost, for probabilities are floating point.  Values past 2^80 take
+// no slack: it would bring sums over 2^24 of them near the end of FP32's range.
+constexpr float kSlack = 8.0f;
+constexpr int kSlackByte = 127 + 80;
+
+// The probabilities of a row's 16 scores in this lane against the row's maximum
+// m (log2 units), times the values' scale, as pieces; l gains their sum.  Returns
+// the factor that earlier sums and outputs take.  MASK: only keys at or before
+// `place` count, the others may be anything.
+template <bool MASK, int NP>
+__device__ __forceinline__ float soften(const f32x4 (&st)[4], int kbyte, int vbyte, float scale_log2, int key0, int place,
+                                        float &m, float &l, bf16x8 (&pf)[NP][2]) {
+    const float kscale = power(kbyte) * scale_log2;
+    float x[16], top;
+    if constexpr (MASK) {
+        top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            x[j] = key0 + j <= place ? st[j / 4][j % 4] * kscale : -INFINITY;
+            top = fmaxf(top, x[j]);
+        }
+    } else {
+        top = st[0][0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, st[j / 4][j % 4]);
+        top *= kscale;
+    }
+    top = row_max(top);
+    float drop = 1.0f;
+    if (__any(top > m + (vbyte > kSlackByte ? 0.0f : kSlack))) {
+        const float next = fmaxf(m, top);
+        drop = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
+        m = next;
+        l *= drop;
+    }
+    // A row that has seen no key yet keeps -inf; 0 stands for it.
+    const float base = m == -INFINITY ? 0.0f : m;
+    const float vscale = power(vbyte);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        float p = __builtin_amdgcn_exp2f(MASK ? x[j] - base : fmaf(st[j / 4][j % 4], kscale, -base));
+        if (MASK && key0 + j > place) p = 0.0f;
+        sum += p;
+        x[j] = MASK && key0 + j > place ? 0.0f : p * vscale;
+    }
+    l += sum;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = x[8 * h + j];
+        bf16x8 piece[NP];
+        pieces8<NP>(y, piece);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) pf[p][h] = piece[p];
+    }
+    return drop;
+}
+
+// Bytes of a word that are NaN codes, as 1 each.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
+    return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+}
+
+// NaN codes times a probability of 0 would reach rows that do not see them: in a
+// masked tile they are taken out of the 16 values w of a channel, and make NaN of
+// the outputs (channel d of each row tile) whose rows see them.
+template <int NT>
+__device__ __forceinline__ void take_out(uint4 &v, int key0, const int (&place)[NT], f32x4 (&out)[NT]) {
+    u32x4 w{v.x, v.y, v.z, v.w}, one;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        one[e] = nan_codes(w[e]);
+        w[e] &= ~(one[e] * 0xffu);
+        one[e] *= 0x38u;  // the code of 1
+    }
+    v = uint4{w[0], w[1], w[2], w[3]};
+#pragma unroll
+    for (int r = 0; r < NT; ++r) {
+        f32x4 hit{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 see;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = key0 + 8 * h + 2 * e;
+                see[e] = (key <= place[r] ? 0x3f80u : 0u) | (key + 1 <= place[r] ? 0x3f800000u : 0u);
+            }
+            hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8(one[2 * h], one[2 * h + 1]),
+                                                          __builtin_bit_cast(bf16x8, see), hit, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (hit[e] > 0.0f) out[r][e] = __builtin_nanf("");
+    }
+}
+
 // The sequence of a pair (sequence, cached head), and whether its length and
 // count are possible.
 struct Sequence {
@@ -115,52 +216,20 @@ __device__ __forceinline__ typename T::Raw *out_row(const Kv8AttnArgs &a, const 
            (s.head * a.group + r - i * a.group) * a.os.s[2];
 }
 
-// NT tiles of 16 rows a wave.  WIDE: every wave has rows of its own and walks
-// all their keys; else the workgroup's waves share 16 NT rows, take the key tiles
-// in turn and join their states at the end.
-template <class T, int PAD, int NT, bool WIDE>
-__global__ void __launch_bounds__(64 * kWaves) kv8_attn_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
-    constexpr int NP = kPieces<T>, STEPS = PAD / 32, DT = PAD / 16;
-    constexpr int WORDS = PAD >= 64 ? PAD / 16 : 2;  // 4-byte words of a key that a lane holds
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    // Workgroups of a pair lie 8 apart, on one XCD and its L2; long rows first.
-    const int id = int(blockIdx.x), pair = id % pairs8;
-    if (pair >= pairs) return;
-    const int split = id / pairs8 % a.splits, tile0 = row_tiles - 1 - id / pairs8 / a.splits;
-    const Sequence s(a, pair);
-    const int row0 = (WIDE ? tile0 * kWaves + wave : tile0) * 16 * NT, rows = s.count * a.group;
-    if (row0 >= rows) return;
-    const int row_end = min(row0 + 16 * NT, rows);
-    if (!s.valid) {
-        if (a.out && a.splits == 1)
-            for (int r = row0; r < row_end; ++r)
-                for (int d = WIDE ? lane : int(threadIdx.x); d < a.cache.width; d += WIDE ? 64 : 64 * kWaves)
-                    out_row<T>(a, s, r)[d] = T::from_float(__builtin_nanf(""));
-        return;
-    }
-    const int begin = s.length - s.count;  // the first query's position
-    const int seen = begin + row0 / a.group, keys = begin + (row_end - 1) / a.group + 1;
-    int t0, t1;
-    if (a.chunk) {
-        t0 = split * (a.chunk / 64);
-        t1 = min((keys + 63) / 64, (split + 1) * (a.chunk / 64));
-        if (t0 >= t1 && a.out) return;  // the join does not read it
-    } else {
-        const int tiles = (keys + 63) / 64, each = (tiles + a.splits - 1) / a.splits;
-        t0 = split * each;
-        t1 = min(tiles, t0 + each);
-    }
-
-    bf16x8 qf[NT][NP][STEPS];
-    int place[NT];  // the row's position, -1 behind the last row
+// Queries of a wave's NT tiles of 16 rows from row0, as pieces in the order of
+// the score product, and the rows' positions (-1 behind the last row).
+template <class T, int PAD, int NT>
+__device__ __forceinline__ void load_queries(const Kv8AttnArgs &a, const Sequence &s, int row0, int rows, int lane,
+                                             bf16x8 (&qf)[NT][kPieces<T>][PAD / 32], int (&place)[NT]) {
+    const int n = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int r = row0 + 16 * t + n, i = r / a.group;
-        place[t] = r < rows ? begin + i : -1;
+        place[t] = r < rows ? s.length - s.count + i : -1;
         const auto *q = static_cast<const typename T::Raw *>(a.q) + s.seq * a.qs.s[0] + i * a.qs.s[1] +
                         (s.head * a.group + r - i * a.group) * a.qs.s[2];
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
+        for (int k = 0; k < PAD / 32; ++k) {
             const int d = PAD >= 64 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 8 * g;
             float x[8];
             if (a.q_aligned && r < rows && d + 8 <= a.cache.width) {
@@ -175,12 +244,57 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_attn_kernel(Kv8AttnArgs a, in
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = r < rows && d + j < a.cache.width ? T::to_float(q[d + j]) : 0.0f;
             }
-            bf16x8 piece[NP];
-            pieces8<NP>(x, piece);
+            bf16x8 piece[kPieces<T>];
+            pieces8<kPieces<T>>(x, piece);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) qf[t][p][k] = piece[p];
+            for (int p = 0; p < kPieces<T>; ++p) qf[t][p][k] = piece[p];
         }
     }
+}
+
+// The key tiles of a share for rows that see `keys` keys.
+struct Tiles {
+    int first, last;
+    __device__ __forceinline__ Tiles(const Kv8AttnArgs &a, int split, int keys) {
+        const int tiles = (keys + 63) / 64;
+        const int each = a.chunk ? a.chunk / 64 : (tiles + a.splits - 1) / a.splits;
+        first = split * each;
+        last = min(tiles, first + each);
+    }
+};
+
+template <class T>
+__device__ __forceinline__ void fill_nan(const Kv8AttnArgs &a, const Sequence &s, int row0, int row_end, int from,
+                                         int step) {
+    for (int r = row0; r < row_end; ++r)
+        for (int d = from; d < a.cache.width; d += step) out_row<T>(a, s, r)[d] = T::from_float(__builtin_nanf(""));
+}
+
+// Up to 16 rows of a pair a workgroup, as in single tokens: its waves take the
+// key tiles in turn, straight from memory into operands, and join their states at
+// the end.  The bytes of the cache bound it.
+template <class T, int PAD>
+__global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, int pairs, int row_tiles) {
+    constexpr int NP = kPieces<T>, STEPS = PAD / 32, DT = PAD / 16;
+    constexpr int WORDS = PAD >= 64 ? PAD / 16 : 2;  // 4-byte words of a key that a lane holds
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int id = int(blockIdx.x), pair = id % pairs, split = id / pairs % a.splits;
+    const int row0 = id / pairs / a.splits * 16;
+    const Sequence s(a, pair);
+    const int rows = s.count * a.group, row_end = min(row0 + 16, rows);
+    if (row0 >= rows) return;
+    if (!s.valid) {
+        if (a.out && a.splits == 1) fill_nan<T>(a, s, row0, row_end, int(threadIdx.x), 64 * kWaves);
+        return;
+    }
+    const int begin = s.length - s.count;  // the first query's position
+    const int seen = begin + row0 / a.group;
+    const Tiles tiles(a, split, begin + (row_end - 1) / a.group + 1);
+    if (tiles.first >= tiles.last && a.out) return;  // the join does not read it
+
+    bf16x8 qf[1][NP][STEPS];
+    int place[1];
+    load_queries<T, PAD, 1>(a, s, row0, rows, lane, qf, place);
 
     const uint8_t *const kbase = a.cache.k + size_t(pair) * a.cache.capacity * PAD +
                                  (16 * (n >> 2) + (n & 3)) * PAD + (PAD >= 64 ? 16 : 8) * g;
@@ -208,138 +322,63 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_attn_kernel(Kv8AttnArgs a, in
         }
     };
 
-    float m[NT], l[NT];
-    f32x4 acc[NT][DT];
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc[DT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    constexpr int STRIDE = WIDE ? 1 : kWaves;
-    int tile = WIDE ? t0 : t0 + wave;
+    int tile = tiles.first + wave;
     uint32_t kw[4][WORDS];
     int kbyte = 0, vbyte = 0;
-    if (tile < t1) {
+    if (tile < tiles.last) {
         load_keys(tile, kw);
         kbyte = ksbase[4 * tile];
         vbyte = vsbase[4 * tile];
     }
-    for (; tile < t1; tile += STRIDE) {
+    for (; tile < tiles.last; tile += kWaves) {
         uint4 vw[DT];
         const uint8_t *const vt = vbase + size_t(tile) * 64 * PAD;
 #pragma unroll
         for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const uint4 *>(vt + d * 16 * 64);
         // The next tile's keys are under way during this one's products.
-        const int next = min(tile + STRIDE, t1 - 1);
+        const int next = min(tile + kWaves, tiles.last - 1);
         uint32_t kn[4][WORDS];
         load_keys(next, kn);
         const int kbyte_next = ksbase[4 * next], vbyte_next = vsbase[4 * next];
 
-        f32x4 st[NT][4];
+        f32x4 st[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int r = 0; r < NT; ++r) st[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            st[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int k = 0; k < STEPS; ++k) {
                 const bf16x8 kf = codes8(kw[t][2 * k], kw[t][2 * k + 1]);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                    for (int r = 0; r < NT; ++r)
-                        st[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[r][p][k], st[r][t], 0, 0, 0);
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[0][p][k], st[t], 0, 0, 0);
             }
         }
-        const float kscale = power(kbyte) * a.scale_log2, vscale = power(vbyte);
+        const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
         const bool masked = tile * 64 + 63 > seen;  // some row does not see all of the tile
-        bf16x8 pf[NT][NP][2];
+        bf16x8 pf[NP][2];
+        const float drop = masked ? soften<true, NP>(st, kbyte, vbyte, a.scale_log2, key0, place[0], m, l, pf)
+                                  : soften<false, NP>(st, kbyte, vbyte, a.scale_log2, key0, place[0], m, l, pf);
+        if (__any(drop != 1.0f)) {
 #pragma unroll
-        for (int r = 0; r < NT; ++r) {
-            float x[16], top = -INFINITY;
-            const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[j] = st[r][j / 4][j % 4] * kscale;
-                if (masked && key0 + j > place[r]) x[j] = -INFINITY;
-                top = fmaxf(top, x[j]);
-            }
-            top = fmaxf(row_max(top), m[r]);
-            // A row that has seen no key yet keeps -inf; 0 stands for it below.
-            const float base = top == -INFINITY ? 0.0f : top, drop = __builtin_amdgcn_exp2f(m[r] - base);
-            m[r] = top;
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                float p = __builtin_amdgcn_exp2f(x[j] - base);
-                // What lies behind a row may be anything: it takes no part.
-                if (masked && key0 + j > place[r]) p = 0.0f;
-                sum += p;
-                x[j] = p * vscale;
-                if (masked && key0 + j > place[r]) x[j] = 0.0f;
-            }
-            l[r] = l[r] * drop + sum;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) acc[r][d] *= drop;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float y[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = x[8 * h + j];
-                bf16x8 piece[NP];
-                pieces8<NP>(y, piece);
-#pragma unroll
-                for (int p = 0; p < NP; ++p) pf[r][p][h] = piece[p];
-            }
+            for (int d = 0; d < DT; ++d) acc[d] *= drop;
         }
-        // NaN codes times a probability of 0 would reach rows that do not see
-        // them: in a masked tile they are taken out, and make NaN what sees them.
-        bool special = false;
         if (masked) {
             uint32_t any = 0;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
+                any |= nan_codes(vw[d].x) | nan_codes(vw[d].y) | nan_codes(vw[d].z) | nan_codes(vw[d].w);
+            if (__any(any != 0)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    any |= ((&vw[d].x)[e] & 0x7f7f7f7fu) + 0x01010101u;
-            special = __any((any & 0x80808080u) != 0);
-        }
-        if (special) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                f32x4 hit[NT];
-#pragma unroll
-                for (int r = 0; r < NT; ++r) hit[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                u32x4 w{vw[d].x, vw[d].y, vw[d].z, vw[d].w}, nan;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    nan[e] = (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in each such byte
-                    w[e] &= ~(nan[e] * 0xffu);
-                    nan[e] *= 0x38u;  // the code of 1
+                for (int d = 0; d < DT; ++d) {
+                    f32x4 out[1] = {acc[d]};
+                    take_out<1>(vw[d], key0, place, out);
+                    acc[d] = out[0];
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bf16x8 nf = codes8(nan[2 * h], nan[2 * h + 1]);
-#pragma unroll
-                    for (int r = 0; r < NT; ++r) {
-                        u32x4 see;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int key = tile * 64 + 16 * g + 8 * h + 2 * e;
-                            see[e] = (key <= place[r] ? 0x3f80u : 0u) | (key + 1 <= place[r] ? 0x3f800000u : 0u);
-                        }
-                        hit[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(nf, __builtin_bit_cast(bf16x8, see), hit[r], 0,
-                                                                         0, 0);
-                    }
-                }
-                vw[d] = uint4{w[0], w[1], w[2], w[3]};
-#pragma unroll
-                for (int r = 0; r < NT; ++r)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (hit[r][e] > 0.0f) acc[r][d][e] = __builtin_nanf("");
             }
         }
 #pragma unroll
@@ -349,9 +388,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_attn_kernel(Kv8AttnArgs a, in
                 const bf16x8 vf = h ? codes8(vw[d].z, vw[d].w) : codes8(vw[d].x, vw[d].y);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                    for (int r = 0; r < NT; ++r)
-                        acc[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][p][h], acc[r][d], 0, 0, 0);
+                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[p][h], acc[d], 0, 0, 0);
             }
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -361,85 +398,239 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_attn_kernel(Kv8AttnArgs a, in
         vbyte = vbyte_next;
     }
 
-    const bool direct = a.out && a.splits == 1;
-    auto part_row = [&](int r) { return a.part + ((size_t(pair) * a.rows + r) * a.splits + split) * a.stride; };
-    if constexpr (WIDE) {
+    constexpr int PART = PAD < 128 ? PAD : 128;  // channels joined at a time
+    __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
+    __shared__ __align__(16) float wave_o[kWaves][16][PART + 4];
+    const float sum = row_sum(l);
+    if (g == 0) {
+        wave_m[wave][n] = m;
+        wave_l[wave][n] = sum;
+    }
+    __syncthreads();
+    float top = wave_m[0][n];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const float sum = row_sum(l[t]);
-            const int r = row0 + 16 * t + n;
-            if (r >= rows) continue;
-            if (direct) {
-                auto *o = out_row<T>(a, s, r);
-                const float inverse = 1.0f / sum;
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wave_m[w][n]);
+    const float base = top == -INFINITY ? 0.0f : top, mine = __builtin_amdgcn_exp2f(m - base);
+    const int real = row_end - row0;
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+    for (int c = 0; c < PAD / PART; ++c) {
+        if (c) __syncthreads();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int at = 16 * d + 4 * g + e;
-                        if (at < a.cache.width) o[at] = T::from_float(acc[t][d][e] * inverse);
-                    }
-            } else {
-                float *o = part_row(r);
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int at = 16 * d + 4 * g + e;
-                        if (at < a.stride - 2) o[at] = acc[t][d][e];
-                    }
-                if (g == 0) {
-                    o[a.stride - 2] = m[t];
-                    o[a.stride - 1] = sum;
-                }
-            }
-        }
-    } else {
-        static_assert(NT == 1, "shared rows: one tile");
-        constexpr int PART = PAD < 128 ? PAD : 128;  // channels joined at a time
-        __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
-        __shared__ __align__(16) float wave_o[kWaves][16][PART + 4];
-        const float sum = row_sum(l[0]);
-        if (g == 0) {
-            wave_m[wave][n] = m[0];
-            wave_l[wave][n] = sum;
-        }
+        for (int d = 0; d < PART / 16; ++d)
+            *reinterpret_cast<f32x4 *>(&wave_o[wave][n][16 * d + 4 * g]) = acc[c * (PART / 16) + d] * mine;
         __syncthreads();
-        float top = wave_m[0][n];
+        for (int i = int(threadIdx.x); i < real * PART; i += 64 * kWaves) {
+            const int r = i / PART, d = i % PART, at = c * PART + d;
+            float v = 0.0f, total = 0.0f, high = wave_m[0][r];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wave_m[w][n]);
-        const float base = top == -INFINITY ? 0.0f : top, mine = __builtin_amdgcn_exp2f(m[0] - base);
-        const int real = row_end - row0;
+            for (int w = 1; w < kWaves; ++w) high = fmaxf(high, wave_m[w][r]);
+            const float from = high == -INFINITY ? 0.0f : high;
 #pragma unroll
-        for (int c = 0; c < PAD / PART; ++c) {
-            if (c) __syncthreads();
-#pragma unroll
-            for (int d = 0; d < PART / 16; ++d) {
-                const f32x4 v = acc[0][c * (PART / 16) + d] * mine;
-                *reinterpret_cast<f32x4 *>(&wave_o[wave][n][16 * d + 4 * g]) = v;
+            for (int w = 0; w < kWaves; ++w) {
+                v += wave_o[w][r][d];
+                total += wave_l[w][r] * __builtin_amdgcn_exp2f(wave_m[w][r] - from);
             }
-            __syncthreads();
-            for (int i = int(threadIdx.x); i < real * PART; i += 64 * kWaves) {
-                const int r = i / PART, d = i % PART, at = c * PART + d;
-                float v = 0.0f, total = 0.0f, high = wave_m[0][r];
-#pragma unroll
-                for (int w = 1; w < kWaves; ++w) high = fmaxf(high, wave_m[w][r]);
-                const float from = high == -INFINITY ? 0.0f : high;
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    v += wave_o[w][r][d];
-                    total += wave_l[w][r] * __builtin_amdgcn_exp2f(wave_m[w][r] - from);
+            if (a.out && a.splits == 1) {
+                if (at < a.cache.width) out_row<T>(a, s, row0 + r)[at] = T::from_float(v / total);
+            } else {
+                float *o = a.part + ((size_t(pair) * a.rows + row0 + r) * a.splits + split) * a.stride;
+                if (at < a.stride - 2) o[at] = v;
+                if (at == 0) {
+                    o[a.stride - 2] = high;
+                    o[a.stride - 1] = total;
                 }
-                if (direct) {
-                    if (at < a.cache.width) out_row<T>(a, s, row0 + r)[at] = T::from_float(v / total);
+            }
+        }
+    }
+}
+
+// Many rows of a pair a workgroup, as in prompts: every wave has NT tiles of 16
+// rows of its own, and the waves share the key tiles through LDS.  A tile is
+// loaded straight into LDS in the order in which the products read it, so that a
+// wave's reads are consecutive, two tiles ahead (one at a width of 256, where two
+// fill the LDS of two workgroups), with one barrier a tile.  Two waves share a
+// SIMD: one's exponentials run beside the other's products.
+template <class T, int PAD, int NT>
+__global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
+    constexpr int NP = kPieces<T>, DT = PAD / 16;
+    constexpr int STAGES = PAD <= 128 ? 3 : 2, HALF = 64 * PAD, STAGE = 2 * HALF;  // keys, then values
+    constexpr int LOADS = STAGE / 1024 / kWaves;                                    // of a wave, a tile
+    static_assert(LOADS * kWaves * 1024 == STAGE, "each wave loads as much");
+    __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    // Workgroups of a pair lie 8 apart, on one XCD and its L2; long rows first.
+    const int id = int(blockIdx.x), pair = id % pairs8;
+    if (pair >= pairs) return;
+    const int split = id / pairs8 % a.splits, tile0 = row_tiles - 1 - id / pairs8 / a.splits;
+    const Sequence s(a, pair);
+    constexpr int ROWS = 16 * NT * kWaves;
+    const int rows = s.count * a.group, block0 = tile0 * ROWS, block_end = min(block0 + ROWS, rows);
+    if (block0 >= rows) return;
+    if (!s.valid) {
+        if (a.out && a.splits == 1) fill_nan<T>(a, s, block0, block_end, int(threadIdx.x), 64 * kWaves);
+        return;
+    }
+    const int begin = s.length - s.count;  // the first query's position
+    const Tiles tiles(a, split, begin + (block_end - 1) / a.group + 1);
+    if (tiles.first >= tiles.last) return;  // the join does not read it
+    const int row0 = block0 + 16 * NT * wave, row_end = min(row0 + 16 * NT, rows);
+    const int seen = begin + row0 / a.group;
+    // The wave's own keys end earlier than the workgroup's.
+    const int mine = row0 < rows ? (begin + (row_end - 1) / a.group + 64) / 64 : 0;
+
+    const uint8_t *const kpair = a.cache.k + size_t(pair) * a.cache.capacity * PAD;
+    const uint8_t *const vpair = a.cache.v + size_t(pair) * a.cache.capacity * PAD;
+    // Load i of a tile: 64 pieces of 16 bytes, in the order of their readers.
+    auto load_tile = [&](int tile, int stage) {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int i = wave * LOADS + u;
+            uint8_t *const to = lds + stage * STAGE + i * 1024;
+            if (i < HALF / 1024) {  // keys
+                int key, at;
+                if constexpr (PAD >= 64) {
+                    const int t = i / (PAD / 64), c = i % (PAD / 64);
+                    key = 16 * (n >> 2) + 4 * t + (n & 3);
+                    at = 64 * c + 16 * g;
                 } else {
-                    float *o = part_row(row0 + r);
-                    if (at < a.stride - 2) o[at] = v;
-                    if (at == 0) {
-                        o[a.stride - 2] = high;
-                        o[a.stride - 1] = total;
-                    }
+                    key = 16 * (n >> 2) + 4 * (2 * i + (lane >> 5)) + (n & 3);
+                    at = 16 * (lane >> 4 & 1);
                 }
+                dma16(kpair + (size_t(tile) * 64 + key) * PAD + at, to);
+            } else {
+                const int d = i - HALF / 1024;
+                dma16(vpair + size_t(tile) * 64 * PAD + (16 * d + n) * 64 + 16 * g, to);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+        if (tiles.first + i < tiles.last) load_tile(tiles.first + i, i);
+
+    bf16x8 qf[NT][NP][PAD / 32];
+    int place[NT];
+    load_queries<T, PAD, NT>(a, s, row0, rows, lane, qf, place);
+    float m[NT], l[NT];
+    f32x4 acc[NT][DT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // Four scales of a tile are a word that all lanes read.
+    typedef const __attribute__((address_space(4))) uint32_t *Words;
+    const Words kscales = (Words)(a.cache.ks + size_t(pair) * (a.cache.capacity / 16));
+    const Words vscales = (Words)(a.cache.vs + size_t(pair) * (a.cache.capacity / 16));
+
+    int stage = 0;
+    for (int tile = tiles.first; tile < tiles.last; ++tile) {
+        if (STAGES > 2 && tile + 1 < tiles.last)
+            wait_vm<(STAGES - 2) * LOADS>();
+        else
+            wait_vm<0>();
+        barrier_lds();  // everyone's loads of this tile, and everyone past the one before
+        if (tile + STAGES - 1 < tiles.last) load_tile(tile + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        const uint8_t *const now = lds + stage * STAGE;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        if (tile >= mine) continue;
+        const int kbyte = kscales[tile] >> (8 * g) & 0xff, vbyte = vscales[tile] >> (8 * g) & 0xff;
+
+        f32x4 st[NT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int r = 0; r < NT; ++r) st[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < (PAD + 63) / 64; ++c) {
+                uint4 w{};
+                if constexpr (PAD >= 64)
+                    w = *reinterpret_cast<const uint4 *>(now + ((t * (PAD / 64) + c) * 64 + lane) * 16);
+                else
+                    *reinterpret_cast<uint2 *>(&w) =
+                        *reinterpret_cast<const uint2 *>(now + ((t * 2 + (g >> 1)) * 16 + n) * 16 + 8 * (g & 1));
+#pragma unroll
+                for (int k = 0; k < (PAD >= 64 ? 2 : 1); ++k) {
+                    const bf16x8 kf = k ? codes8(w.z, w.w) : codes8(w.x, w.y);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                        for (int r = 0; r < NT; ++r)
+                            st[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[r][p][2 * c + k], st[r][t], 0, 0, 0);
+                }
+            }
+        }
+        const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
+        const bool masked = tile * 64 + 63 > seen;
+        bf16x8 pf[NT][NP][2];
+#pragma unroll
+        for (int r = 0; r < NT; ++r) {
+            const float drop = masked ? soften<true, NP>(st[r], kbyte, vbyte, a.scale_log2, key0, place[r], m[r], l[r], pf[r])
+                                      : soften<false, NP>(st[r], kbyte, vbyte, a.scale_log2, key0, place[r], m[r], l[r], pf[r]);
+            if (__any(drop != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[r][d] *= drop;
+            }
+        }
+        const uint8_t *const vt = now + HALF + lane * 16;
+        bool special = false;
+        if (masked) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(vt + d * 1024);
+                any |= nan_codes(w.x) | nan_codes(w.y) | nan_codes(w.z) | nan_codes(w.w);
+            }
+            special = __any(any != 0);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            uint4 w = *reinterpret_cast<const uint4 *>(vt + d * 1024);
+            if (special) {
+                f32x4 out[NT];
+#pragma unroll
+                for (int r = 0; r < NT; ++r) out[r] = acc[r][d];
+                take_out<NT>(w, key0, place, out);
+#pragma unroll
+                for (int r = 0; r < NT; ++r) acc[r][d] = out[r];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bf16x8 vf = h ? codes8(w.z, w.w) : codes8(w.x, w.y);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                    for (int r = 0; r < NT; ++r)
+                        acc[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][p][h], acc[r][d], 0, 0, 0);
+            }
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float sum = row_sum(l[t]);
+        const int r = row0 + 16 * t + n;
+        if (r >= rows) continue;
+        if (a.splits == 1) {
+            auto *o = out_row<T>(a, s, r);
+            const float inverse = 1.0f / sum;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = 16 * d + 4 * g + e;
+                    if (at < a.cache.width) o[at] = T::from_float(acc[t][d][e] * inverse);
+                }
+        } else {
+            float *o = a.part + ((size_t(pair) * a.rows + r) * a.splits + split) * a.stride;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[16 * d + 4 * g + e] = acc[t][d][e];
+            if (g == 0) {
+                o[a.stride - 2] = m[t];
+                o[a.stride - 1] = sum;
             }
         }
     }
@@ -490,14 +681,15 @@ constexpr int wide_tiles(int pad) {
 template <class T, int PAD>
 void launch_attn(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) {
     const int pairs = a.cache.batch * a.cache.heads;
-    const int pairs8 = plan.wide ? (pairs + 7) / 8 * 8 : pairs;
-    const dim3 grid(uint32_t(pairs8) * uint32_t(a.splits) * uint32_t(plan.row_tiles));
-    if (plan.wide)
-        hipLaunchKernelGGL((kv8_attn_kernel<T, PAD, wide_tiles<T>(PAD), true>), grid, dim3(64 * kWaves), 0, stream, a,
-                           pairs, pairs8, plan.row_tiles);
-    else
-        hipLaunchKernelGGL((kv8_attn_kernel<T, PAD, 1, false>), grid, dim3(64 * kWaves), 0, stream, a, pairs, pairs8,
-                           plan.row_tiles);
+    if (plan.wide) {
+        const int pairs8 = (pairs + 7) / 8 * 8;
+        hipLaunchKernelGGL((kv8_tiles_kernel<T, PAD, wide_tiles<T>(PAD)>),
+                           dim3(uint32_t(pairs8) * uint32_t(a.splits) * uint32_t(plan.row_tiles)), dim3(64 * kWaves), 0,
+                           stream, a, pairs, pairs8, plan.row_tiles);
+    } else {
+        hipLaunchKernelGGL((kv8_rows_kernel<T, PAD>), dim3(uint32_t(pairs) * uint32_t(a.splits) * uint32_t(plan.row_tiles)),
+                           dim3(64 * kWaves), 0, stream, a, pairs, plan.row_tiles);
+    }
     if (a.out && a.splits > 1)
         hipLaunchKernelGGL((kv8_join_kernel<T>), dim3(uint32_t((int64_t(pairs) * a.rows + 3) / 4)), dim3(256), 0,
                            stream, a, pairs);
