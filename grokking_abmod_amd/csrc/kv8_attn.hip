@@ -46,13 +46,14 @@ __device__ __forceinline__ float bits(uint32_t u) { return __builtin_bit_cast(fl
 __device__ __forceinline__ uint32_t bits(float f) { return __builtin_bit_cast(uint32_t, f); }
 __device__ __forceinline__ float power(int byte) { return bits(uint32_t(byte) << 23); }
 
-// Two codes of a word as BF16.
+// Codes times a power of two as BF16.
 template <bool HIGH>
-__device__ __forceinline__ uint32_t codes2(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+__device__ __forceinline__ uint32_t codes2(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HIGH));
 }
-__device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
-    return __builtin_bit_cast(bf16x8, u32x4{codes2<false>(a), codes2<true>(a), codes2<false>(b), codes2<true>(b)});
+__device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b, float scale = 1.0f) {
+    return __builtin_bit_cast(bf16x8, u32x4{codes2<false>(a, scale), codes2<true>(a, scale), codes2<false>(b, scale),
+                                            codes2<true>(b, scale)});
 }
 
 // x as a sum of NP BF16 values: all but the last cut off, the last rounded
@@ -80,18 +81,12 @@ __device__ __forceinline__ void pieces8(const float (&x)[8], bf16x8 (&out)[NP]) 
     out[NP - 1] = __builtin_bit_cast(bf16x8, w);
 }
 
-// The larger (sum) of the four lanes that hold a row.
+// The largest of the four lanes that hold a row.
 __device__ __forceinline__ float row_max(float v) {
     const auto s = __builtin_amdgcn_permlane16_swap(int(bits(v)), int(bits(v)), false, false);
     v = fmaxf(bits(uint32_t(s[0])), bits(uint32_t(s[1])));
     const auto t = __builtin_amdgcn_permlane32_swap(int(bits(v)), int(bits(v)), false, false);
     return fmaxf(bits(uint32_t(t[0])), bits(uint32_t(t[1])));
-}
-__device__ __forceinline__ float row_sum(float v) {
-    const auto s = __builtin_amdgcn_permlane16_swap(int(bits(v)), int(bits(v)), false, false);
-    v = bits(uint32_t(s[0])) + bits(uint32_t(s[1]));
-    const auto t = __builtin_amdgcn_permlane32_swap(int(bits(v)), int(bits(v)), false, false);
-    return bits(uint32_t(t[0])) + bits(uint32_t(t[1]));
 }
 
 // Rows keep a maximum that their scores may pass by up to 2^kSlack before sums
@@ -102,95 +97,114 @@ constexpr float kSlack = 8.0f;
 constexpr int kSlackByte = 127 + 80;
 
 // The probabilities of a row's 16 scores in this lane against the row's maximum
-// m (log2 units), times the values' scale, as pieces; l gains their sum.  Returns
-// the factor that earlier sums and outputs take.  MASK: only keys at or before
-// `place` count, the others may be anything.
-template <bool MASK, int NP>
-__device__ __forceinline__ float soften(const f32x4 (&st)[4], int kbyte, int vbyte, float scale_log2, int key0, int place,
-                                        float &m, float &l, bf16x8 (&pf)[NP][2]) {
-    const float kscale = power(kbyte) * scale_log2;
-    float x[16], top;
-    if constexpr (MASK) {
-        top = -INFINITY;
+// m (log2 units), as pieces.  Returns the factor that earlier sums and outputs
+// take.  With `masked` only keys at or before `place` count, and the scores of
+// the others may be anything.
+template <int NP>
+__device__ __forceinline__ float soften(f32x4 (&st)[4], bool masked, float kscale, float slack, int key0, int place,
+                                        float &m, bf16x8 (&pf)[NP][2]) {
+    if (masked) {
+        __builtin_amdgcn_sched_barrier(0);  // a branch: few tiles are masked
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            x[j] = key0 + j <= place ? st[j / 4][j % 4] * kscale : -INFINITY;
-            top = fmaxf(top, x[j]);
-        }
-    } else {
-        top = st[0][0];
-#pragma unroll
-        for (int j = 1; j < 16; ++j) top = fmaxf(top, st[j / 4][j % 4]);
-        top *= kscale;
+        for (int j = 0; j < 16; ++j)
+            if (key0 + j > place) st[j / 4][j % 4] = -INFINITY;
+        if (key0 > place) kscale = 1.0f;  // the scale may be anything too
     }
-    top = row_max(top);
+    float top = st[0][0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, st[j / 4][j % 4]);
+    top = row_max(top * kscale);
     float drop = 1.0f;
-    if (__any(top > m + (vbyte > kSlackByte ? 0.0f : kSlack))) {
+    if (__any(top > m + slack)) {
         const float next = fmaxf(m, top);
         drop = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
         m = next;
-        l *= drop;
     }
     // A row that has seen no key yet keeps -inf; 0 stands for it.
     const float base = m == -INFINITY ? 0.0f : m;
-    const float vscale = power(vbyte);
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        float p = __builtin_amdgcn_exp2f(MASK ? x[j] - base : fmaf(st[j / 4][j % 4], kscale, -base));
-        if (MASK && key0 + j > place) p = 0.0f;
-        sum += p;
-        x[j] = MASK && key0 + j > place ? 0.0f : p * vscale;
-    }
-    l += sum;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        float y[8];
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[8 * h + j];
+        for (int j = 0; j < 8; ++j)
+            x[j] = __builtin_amdgcn_exp2f(fmaf(st[2 * h + j / 4][j % 4], kscale, -base));
         bf16x8 piece[NP];
-        pieces8<NP>(y, piece);
+        pieces8<NP>(x, piece);
 #pragma unroll
         for (int p = 0; p < NP; ++p) pf[p][h] = piece[p];
     }
     return drop;
 }
 
+// A block's scale of the values, 1 behind the sequence, where the byte may be
+// anything; and what scores may pass the maximum by with it.
+__device__ __forceinline__ float value_scale(int byte, int key0, int length) {
+    return key0 < length ? power(byte) : 1.0f;
+}
+__device__ __forceinline__ float slack_of(int byte) { return byte > kSlackByte ? 0.0f : kSlack; }
+
+// The sums of the probabilities are a product with ones: row n's lands in every
+// element of its lanes.
+template <int NP>
+__device__ __forceinline__ f32x4 add_sums(const bf16x8 (&pf)[NP][2], f32x4 l) {
+    const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+#pragma unroll
+    for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[p][h], l, 0, 0, 0);
+    return l;
+}
+
+// A NaN value times a probability of 0 would reach rows that do not see its
+// token.  So tiles that some row does not see whole are weighed with their NaN
+// codes taken out (what lies behind a sequence may hold any), and where there
+// were some, the outputs of the rows that see them are made NaN at the end.
+
 // Bytes of a word that are NaN codes, as 1 each.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
     return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
 }
-
-// NaN codes times a probability of 0 would reach rows that do not see them: in a
-// masked tile they are taken out of the 16 values w of a channel, and make NaN of
-// the outputs (channel d of each row tile) whose rows see them.
-template <int NT>
-__device__ __forceinline__ void take_out(uint4 &v, int key0, const int (&place)[NT], f32x4 (&out)[NT]) {
-    u32x4 w{v.x, v.y, v.z, v.w}, one;
+// Takes them out; the words in which there were some.
+__device__ __forceinline__ uint32_t clean(uint4 &v) {
+    const uint32_t x = nan_codes(v.x), y = nan_codes(v.y), z = nan_codes(v.z), w = nan_codes(v.w);
+    v.x &= ~(x * 0xffu);
+    v.y &= ~(y * 0xffu);
+    v.z &= ~(z * 0xffu);
+    v.w &= ~(w * 0xffu);
+    return x | y | z | w;
+}
+// acc = NaN where a row sees a NaN of tiles [from, to): a product of the places
+// of the NaN codes with those that a row sees counts them.
+template <int PAD, int NT>
+__device__ __forceinline__ void mark_nan(const uint8_t *vpair, int from, int to, int lane, const int (&place)[NT],
+                                         f32x4 (&acc)[NT][PAD / 16]) {
+    const int n = lane & 15, g = lane >> 4;
+    for (int tile = from; tile < to; ++tile) {
+        const uint8_t *const vt = vpair + size_t(tile) * 64 * PAD + n * 64 + 16 * g;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        one[e] = nan_codes(w[e]);
-        w[e] &= ~(one[e] * 0xffu);
-        one[e] *= 0x38u;  // the code of 1
-    }
-    v = uint4{w[0], w[1], w[2], w[3]};
+        for (int d = 0; d < PAD / 16; ++d) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(vt + d * 16 * 64);
+            // 0x38 is the code of 1.
+            const u32x4 one{nan_codes(v.x) * 0x38u, nan_codes(v.y) * 0x38u, nan_codes(v.z) * 0x38u, nan_codes(v.w) * 0x38u};
 #pragma unroll
-    for (int r = 0; r < NT; ++r) {
-        f32x4 hit{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = 0; r < NT; ++r) {
+                f32x4 hits{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4 see;
+                for (int h = 0; h < 2; ++h) {
+                    u32x4 see;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int key = key0 + 8 * h + 2 * e;
-                see[e] = (key <= place[r] ? 0x3f80u : 0u) | (key + 1 <= place[r] ? 0x3f800000u : 0u);
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = tile * 64 + 16 * g + 8 * h + 2 * e;
+                        see[e] = (key <= place[r] ? 0x3f80u : 0u) | (key + 1 <= place[r] ? 0x3f800000u : 0u);
+                    }
+                    hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8(one[2 * h], one[2 * h + 1]),
+                                                                   __builtin_bit_cast(bf16x8, see), hits, 0, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (hits[e] > 0.0f) acc[r][d][e] = __builtin_nanf("");
             }
-            hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8(one[2 * h], one[2 * h + 1]),
-                                                          __builtin_bit_cast(bf16x8, see), hit, 0, 0, 0);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (hit[e] > 0.0f) out[r][e] = __builtin_nanf("");
     }
 }
 
@@ -322,10 +336,11 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
         }
     };
 
-    float m = -INFINITY, l = 0.0f;
-    f32x4 acc[DT];
+    float m = -INFINITY;
+    f32x4 acc[1][DT], l{0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t nans = 0;  // NaN codes were taken out
 #pragma unroll
-    for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int d = 0; d < DT; ++d) acc[0][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     int tile = tiles.first + wave;
     uint32_t kw[4][WORDS];
@@ -361,34 +376,26 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
         const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
         const bool masked = tile * 64 + 63 > seen;  // some row does not see all of the tile
         bf16x8 pf[NP][2];
-        const float drop = masked ? soften<true, NP>(st, kbyte, vbyte, a.scale_log2, key0, place[0], m, l, pf)
-                                  : soften<false, NP>(st, kbyte, vbyte, a.scale_log2, key0, place[0], m, l, pf);
+        const float kscale = power(kbyte) * a.scale_log2, vscale = value_scale(vbyte, key0, s.length);
+        const float drop = soften<NP>(st, masked, kscale, slack_of(vbyte), key0, place[0], m, pf);
         if (__any(drop != 1.0f)) {
+            l *= drop;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) acc[d] *= drop;
+            for (int d = 0; d < DT; ++d) acc[0][d] *= drop;
         }
+        l = add_sums<NP>(pf, l);
         if (masked) {
-            uint32_t any = 0;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-                any |= nan_codes(vw[d].x) | nan_codes(vw[d].y) | nan_codes(vw[d].z) | nan_codes(vw[d].w);
-            if (__any(any != 0)) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    f32x4 out[1] = {acc[d]};
-                    take_out<1>(vw[d], key0, place, out);
-                    acc[d] = out[0];
-                }
-            }
+            for (int d = 0; d < DT; ++d) nans |= clean(vw[d]);
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const bf16x8 vf = h ? codes8(vw[d].z, vw[d].w) : codes8(vw[d].x, vw[d].y);
+                const bf16x8 vf = h ? codes8(vw[d].z, vw[d].w, vscale) : codes8(vw[d].x, vw[d].y, vscale);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
-                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[p][h], acc[d], 0, 0, 0);
+                    acc[0][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[p][h], acc[0][d], 0, 0, 0);
             }
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -398,13 +405,20 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
         vbyte = vbyte_next;
     }
 
+    if (__any(nans != 0)) {
+        // This wave's tiles from the first one masked.
+        int from = tiles.first + wave;
+        if (seen / 64 > from) from += (seen / 64 - from + kWaves - 1) / kWaves * kWaves;
+        for (int t = from; t < tiles.last; t += kWaves)
+            mark_nan<PAD, 1>(a.cache.v + size_t(pair) * a.cache.capacity * PAD, t, t + 1, lane, place, acc);
+    }
+
     constexpr int PART = PAD < 128 ? PAD : 128;  // channels joined at a time
     __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
     __shared__ __align__(16) float wave_o[kWaves][16][PART + 4];
-    const float sum = row_sum(l);
     if (g == 0) {
         wave_m[wave][n] = m;
-        wave_l[wave][n] = sum;
+        wave_l[wave][n] = l[0];
     }
     __syncthreads();
     float top = wave_m[0][n];
@@ -417,7 +431,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
         if (c) __syncthreads();
 #pragma unroll
         for (int d = 0; d < PART / 16; ++d)
-            *reinterpret_cast<f32x4 *>(&wave_o[wave][n][16 * d + 4 * g]) = acc[c * (PART / 16) + d] * mine;
+            *reinterpret_cast<f32x4 *>(&wave_o[wave][n][16 * d + 4 * g]) = acc[0][c * (PART / 16) + d] * mine;
         __syncthreads();
         for (int i = int(threadIdx.x); i < real * PART; i += 64 * kWaves) {
             const int r = i / PART, d = i % PART, at = c * PART + d;
@@ -457,6 +471,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
     constexpr int LOADS = STAGE / 1024 / kWaves;                                    // of a wave, a tile
     static_assert(LOADS * kWaves * 1024 == STAGE, "each wave loads as much");
     __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
+    __shared__ uint32_t nans;  // NaN codes were taken out
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     // Workgroups of a pair lie 8 apart, on one XCD and its L2; long rows first.
     const int id = int(blockIdx.x), pair = id % pairs8;
@@ -475,6 +490,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
     if (tiles.first >= tiles.last) return;  // the join does not read it
     const int row0 = block0 + 16 * NT * wave, row_end = min(row0 + 16 * NT, rows);
     const int seen = begin + row0 / a.group;
+    const int cleaned = (begin + block0 / a.group) / 64;  // the first tile that some row may not see whole
+    if (threadIdx.x == 0) nans = 0;
     // The wave's own keys end earlier than the workgroup's.
     const int mine = row0 < rows ? (begin + (row_end - 1) / a.group + 64) / 64 : 0;
 
@@ -510,12 +527,12 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
     bf16x8 qf[NT][NP][PAD / 32];
     int place[NT];
     load_queries<T, PAD, NT>(a, s, row0, rows, lane, qf, place);
-    float m[NT], l[NT];
-    f32x4 acc[NT][DT];
+    float m[NT];
+    f32x4 acc[NT][DT], l[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         m[t] = -INFINITY;
-        l[t] = 0.0f;
+        l[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -525,6 +542,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
     const Words vscales = (Words)(a.cache.vs + size_t(pair) * (a.cache.capacity / 16));
 
     int stage = 0;
+    uint32_t kword = kscales[tiles.first], vword = vscales[tiles.first];
     for (int tile = tiles.first; tile < tiles.last; ++tile) {
         if (STAGES > 2 && tile + 1 < tiles.last)
             wait_vm<(STAGES - 2) * LOADS>();
@@ -532,10 +550,23 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
             wait_vm<0>();
         barrier_lds();  // everyone's loads of this tile, and everyone past the one before
         if (tile + STAGES - 1 < tiles.last) load_tile(tile + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-        const uint8_t *const now = lds + stage * STAGE;
+        uint8_t *const now = lds + stage * STAGE;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
+        if (tile >= cleaned) {
+            uint32_t any = 0;
+            for (int i = int(threadIdx.x); i < HALF / 16; i += 64 * kWaves) {
+                uint4 *const w = reinterpret_cast<uint4 *>(now + HALF) + i;
+                uint4 v = *w;
+                any |= clean(v);
+                *w = v;
+            }
+            if (any) nans = 1;
+            barrier_lds();
+        }
+        const int kbyte = kword >> (8 * g) & 0xff, vbyte = vword >> (8 * g) & 0xff, next = min(tile + 1, tiles.last - 1);
+        kword = kscales[next];
+        vword = vscales[next];
         if (tile >= mine) continue;
-        const int kbyte = kscales[tile] >> (8 * g) & 0xff, vbyte = vscales[tile] >> (8 * g) & 0xff;
 
         f32x4 st[NT][4];
 #pragma unroll
@@ -563,41 +594,25 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
         }
         const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
         const bool masked = tile * 64 + 63 > seen;
+        const float kscale = power(kbyte) * a.scale_log2, vscale = value_scale(vbyte, key0, s.length);
         bf16x8 pf[NT][NP][2];
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
-            const float drop = masked ? soften<true, NP>(st[r], kbyte, vbyte, a.scale_log2, key0, place[r], m[r], l[r], pf[r])
-                                      : soften<false, NP>(st[r], kbyte, vbyte, a.scale_log2, key0, place[r], m[r], l[r], pf[r]);
+            const float drop = soften<NP>(st[r], masked, kscale, slack_of(vbyte), key0, place[r], m[r], pf[r]);
             if (__any(drop != 1.0f)) {
+                l[r] *= drop;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[r][d] *= drop;
             }
+            l[r] = add_sums<NP>(pf[r], l[r]);
         }
         const uint8_t *const vt = now + HALF + lane * 16;
-        bool special = false;
-        if (masked) {
-            uint32_t any = 0;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(vt + d * 1024);
-                any |= nan_codes(w.x) | nan_codes(w.y) | nan_codes(w.z) | nan_codes(w.w);
-            }
-            special = __any(any != 0);
-        }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            uint4 w = *reinterpret_cast<const uint4 *>(vt + d * 1024);
-            if (special) {
-                f32x4 out[NT];
-#pragma unroll
-                for (int r = 0; r < NT; ++r) out[r] = acc[r][d];
-                take_out<NT>(w, key0, place, out);
-#pragma unroll
-                for (int r = 0; r < NT; ++r) acc[r][d] = out[r];
-            }
+            const uint4 w = *reinterpret_cast<const uint4 *>(vt + d * 1024);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const bf16x8 vf = h ? codes8(w.z, w.w) : codes8(w.x, w.y);
+                const bf16x8 vf = h ? codes8(w.z, w.w, vscale) : codes8(w.x, w.y, vscale);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
@@ -606,10 +621,11 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
             }
         }
     }
+    if (tiles.last > cleaned && nans) mark_nan<PAD, NT>(vpair, max(tiles.first, cleaned), min(tiles.last, mine), lane, place, acc);
 
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const float sum = row_sum(l[t]);
+        const float sum = l[t][0];
         const int r = row0 + 16 * t + n;
         if (r >= rows) continue;
         if (a.splits == 1) {
