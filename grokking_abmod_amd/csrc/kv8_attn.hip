@@ -32,6 +32,7 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
@@ -173,38 +174,32 @@ __device__ __forceinline__ uint32_t clean(uint4 &v) {
     v.w &= ~(w * 0xffu);
     return x | y | z | w;
 }
-// acc = NaN where a row sees a NaN of tiles [from, to): a product of the places
+// acc = NaN where a row sees a NaN of the tile: a product of the places
 // of the NaN codes with those that a row sees counts them.
-template <int PAD, int NT>
-__device__ __forceinline__ void mark_nan(const uint8_t *vpair, int from, int to, int lane, const int (&place)[NT],
-                                         f32x4 (&acc)[NT][PAD / 16]) {
+template <int PAD>
+__device__ __forceinline__ void mark_nan(const uint8_t *vpair, int tile, int lane, int place, f32x4 (&acc)[PAD / 16]) {
     const int n = lane & 15, g = lane >> 4;
-    for (int tile = from; tile < to; ++tile) {
-        const uint8_t *const vt = vpair + size_t(tile) * 64 * PAD + n * 64 + 16 * g;
+    const uint8_t *const vt = vpair + size_t(tile) * 64 * PAD + n * 64 + 16 * g;
 #pragma unroll
-        for (int d = 0; d < PAD / 16; ++d) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(vt + d * 16 * 64);
-            // 0x38 is the code of 1.
-            const u32x4 one{nan_codes(v.x) * 0x38u, nan_codes(v.y) * 0x38u, nan_codes(v.z) * 0x38u, nan_codes(v.w) * 0x38u};
+    for (int d = 0; d < PAD / 16; ++d) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(vt + d * 16 * 64);
+        // 0x38 is the code of 1.
+        const u32x4 one{nan_codes(v.x) * 0x38u, nan_codes(v.y) * 0x38u, nan_codes(v.z) * 0x38u, nan_codes(v.w) * 0x38u};
+        f32x4 hits{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int r = 0; r < NT; ++r) {
-                f32x4 hits{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h = 0; h < 2; ++h) {
+            u32x4 see;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    u32x4 see;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = tile * 64 + 16 * g + 8 * h + 2 * e;
-                        see[e] = (key <= place[r] ? 0x3f80u : 0u) | (key + 1 <= place[r] ? 0x3f800000u : 0u);
-                    }
-                    hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8(one[2 * h], one[2 * h + 1]),
-                                                                   __builtin_bit_cast(bf16x8, see), hits, 0, 0, 0);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (hits[e] > 0.0f) acc[r][d][e] = __builtin_nanf("");
+            for (int e = 0; e < 4; ++e) {
+                const int key = tile * 64 + 16 * g + 8 * h + 2 * e;
+                see[e] = (key <= place ? 0x3f80u : 0u) | (key + 1 <= place ? 0x3f800000u : 0u);
             }
+            hits = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8(one[2 * h], one[2 * h + 1]),
+                                                           __builtin_bit_cast(bf16x8, see), hits, 0, 0, 0);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (hits[e] > 0.0f) acc[d][e] = __builtin_nanf("");
     }
 }
 
@@ -230,40 +225,24 @@ __device__ __forceinline__ typename T::Raw *out_row(const Kv8AttnArgs &a, const 
            (s.head * a.group + r - i * a.group) * a.os.s[2];
 }
 
-// Queries of a wave's NT tiles of 16 rows from row0, as pieces in the order of
-// the score product, and the rows' positions (-1 behind the last row).
-template <class T, int PAD, int NT>
-__device__ __forceinline__ void load_queries(const Kv8AttnArgs &a, const Sequence &s, int row0, int rows, int lane,
-                                             bf16x8 (&qf)[NT][kPieces<T>][PAD / 32], int (&place)[NT]) {
-    const int n = lane & 15, g = lane >> 4;
+// Eight elements of a query from d as pieces, zeros where there are none.
+template <class T>
+__device__ __forceinline__ void query8(const Kv8AttnArgs &a, const typename T::Raw *q, bool real, int d,
+                                       bf16x8 (&piece)[kPieces<T>]) {
+    float x[8];
+    if (a.q_aligned && real && d + 8 <= a.cache.width) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = row0 + 16 * t + n, i = r / a.group;
-        place[t] = r < rows ? s.length - s.count + i : -1;
-        const auto *q = static_cast<const typename T::Raw *>(a.q) + s.seq * a.qs.s[0] + i * a.qs.s[1] +
-                        (s.head * a.group + r - i * a.group) * a.qs.s[2];
+        for (int j = 0; j < 8 / T::kGroup; ++j) {
+            float y[T::kGroup];
+            T::unpack(reinterpret_cast<const uint4 *>(q + d)[j], y);
 #pragma unroll
-        for (int k = 0; k < PAD / 32; ++k) {
-            const int d = PAD >= 64 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 8 * g;
-            float x[8];
-            if (a.q_aligned && r < rows && d + 8 <= a.cache.width) {
-#pragma unroll
-                for (int j = 0; j < 8 / T::kGroup; ++j) {
-                    float y[T::kGroup];
-                    T::unpack(reinterpret_cast<const uint4 *>(q + d)[j], y);
-#pragma unroll
-                    for (int e = 0; e < T::kGroup; ++e) x[j * T::kGroup + e] = y[e];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = r < rows && d + j < a.cache.width ? T::to_float(q[d + j]) : 0.0f;
-            }
-            bf16x8 piece[kPieces<T>];
-            pieces8<kPieces<T>>(x, piece);
-#pragma unroll
-            for (int p = 0; p < kPieces<T>; ++p) qf[t][p][k] = piece[p];
+            for (int e = 0; e < T::kGroup; ++e) x[j * T::kGroup + e] = y[e];
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = real && d + j < a.cache.width ? T::to_float(q[d + j]) : 0.0f;
     }
+    pieces8<kPieces<T>>(x, piece);
 }
 
 // The key tiles of a share for rows that see `keys` keys.
@@ -306,9 +285,20 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
     const Tiles tiles(a, split, begin + (row_end - 1) / a.group + 1);
     if (tiles.first >= tiles.last && a.out) return;  // the join does not read it
 
-    bf16x8 qf[1][NP][STEPS];
-    int place[1];
-    load_queries<T, PAD, 1>(a, s, row0, rows, lane, qf, place);
+    bf16x8 qf[NP][STEPS];
+    const int row = row0 + n, place = row < rows ? begin + row / a.group : -1;
+    {
+        const int i = row / a.group;
+        const auto *q = static_cast<const typename T::Raw *>(a.q) + s.seq * a.qs.s[0] + i * a.qs.s[1] +
+                        (s.head * a.group + row - i * a.group) * a.qs.s[2];
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            bf16x8 piece[NP];
+            query8<T>(a, q, row < rows, PAD >= 64 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 8 * g, piece);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) qf[p][k] = piece[p];
+        }
+    }
 
     const uint8_t *const kbase = a.cache.k + size_t(pair) * a.cache.capacity * PAD +
                                  (16 * (n >> 2) + (n & 3)) * PAD + (PAD >= 64 ? 16 : 8) * g;
@@ -337,10 +327,10 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
     };
 
     float m = -INFINITY;
-    f32x4 acc[1][DT], l{0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 acc[DT], l{0.0f, 0.0f, 0.0f, 0.0f};
     uint32_t nans = 0;  // NaN codes were taken out
 #pragma unroll
-    for (int d = 0; d < DT; ++d) acc[0][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     int tile = tiles.first + wave;
     uint32_t kw[4][WORDS];
@@ -370,18 +360,18 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
                 const bf16x8 kf = codes8(kw[t][2 * k], kw[t][2 * k + 1]);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
-                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[0][p][k], st[t], 0, 0, 0);
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[p][k], st[t], 0, 0, 0);
             }
         }
         const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
         const bool masked = tile * 64 + 63 > seen;  // some row does not see all of the tile
         bf16x8 pf[NP][2];
         const float kscale = power(kbyte) * a.scale_log2, vscale = value_scale(vbyte, key0, s.length);
-        const float drop = soften<NP>(st, masked, kscale, slack_of(vbyte), key0, place[0], m, pf);
+        const float drop = soften<NP>(st, masked, kscale, slack_of(vbyte), key0, place, m, pf);
         if (__any(drop != 1.0f)) {
             l *= drop;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) acc[0][d] *= drop;
+            for (int d = 0; d < DT; ++d) acc[d] *= drop;
         }
         l = add_sums<NP>(pf, l);
         if (masked) {
@@ -395,7 +385,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
                 const bf16x8 vf = h ? codes8(vw[d].z, vw[d].w, vscale) : codes8(vw[d].x, vw[d].y, vscale);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
-                    acc[0][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[p][h], acc[0][d], 0, 0, 0);
+                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[p][h], acc[d], 0, 0, 0);
             }
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -410,7 +400,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
         int from = tiles.first + wave;
         if (seen / 64 > from) from += (seen / 64 - from + kWaves - 1) / kWaves * kWaves;
         for (int t = from; t < tiles.last; t += kWaves)
-            mark_nan<PAD, 1>(a.cache.v + size_t(pair) * a.cache.capacity * PAD, t, t + 1, lane, place, acc);
+            mark_nan<PAD>(a.cache.v + size_t(pair) * a.cache.capacity * PAD, t, lane, place, acc);
     }
 
     constexpr int PART = PAD < 128 ? PAD : 128;  // channels joined at a time
@@ -431,7 +421,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
         if (c) __syncthreads();
 #pragma unroll
         for (int d = 0; d < PART / 16; ++d)
-            *reinterpret_cast<f32x4 *>(&wave_o[wave][n][16 * d + 4 * g]) = acc[0][c * (PART / 16) + d] * mine;
+            *reinterpret_cast<f32x4 *>(&wave_o[wave][n][16 * d + 4 * g]) = acc[c * (PART / 16) + d] * mine;
         __syncthreads();
         for (int i = int(threadIdx.x); i < real * PART; i += 64 * kWaves) {
             const int r = i / PART, d = i % PART, at = c * PART + d;
@@ -458,27 +448,124 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
     }
 }
 
-// Many rows of a pair a workgroup, as in prompts: every wave has NT tiles of 16
-// rows of its own, and the waves share the key tiles through LDS.  A tile is
-// loaded straight into LDS in the order in which the products read it, so that a
-// wave's reads are consecutive, two tiles ahead (one at a width of 256, where two
-// fill the LDS of two workgroups), with one barrier a tile.  Two waves share a
-// SIMD: one's exponentials run beside the other's products.
-template <class T, int PAD, int NT>
-__global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
-    constexpr int NP = kPieces<T>, DT = PAD / 16;
-    constexpr int STAGES = PAD <= 128 ? 3 : 2, HALF = 64 * PAD, STAGE = 2 * HALF;  // keys, then values
-    constexpr int LOADS = STAGE / 1024 / kWaves;                                    // of a wave, a tile
-    static_assert(LOADS * kWaves * 1024 == STAGE, "each wave loads as much");
-    __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
+// The schedule of N operands read from LDS with NP products each: a few reads
+// ahead of the products.
+template <int N, int NP>
+__device__ __forceinline__ void paced() {
+    constexpr int AHEAD = N < 6 ? N : 6;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NP, 0);
+        if (i + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
+// As soften(), mark_nan() and load_queries() for the products of 32 x 32: a lane
+// holds 16 keys of a row in each 32, one block of 16 tokens, and a row is two lanes.
+template <int NP, int SUB>
+__device__ __forceinline__ float soften32(f32x16 (&st)[SUB], bool masked, float (&kscale)[SUB], float slack,
+                                          const int (&key0)[SUB], int place, float &m, float &l, bf16x8 (&pf)[SUB][NP][2]) {
+    if (masked) {
+        __builtin_amdgcn_sched_barrier(0);  // a branch: few tiles are masked
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (key0[u] + j > place) st[u][j] = -INFINITY;
+            if (key0[u] > place) kscale[u] = 1.0f;  // the scale may be anything too
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+        float t = st[u][0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) t = fmaxf(t, st[u][j]);
+        top = fmaxf(top, t * kscale[u]);
+    }
+    const auto both = __builtin_amdgcn_permlane32_swap(int(bits(top)), int(bits(top)), false, false);
+    top = fmaxf(bits(uint32_t(both[0])), bits(uint32_t(both[1])));
+    float drop = 1.0f;
+    if (__any(top > m + slack)) {
+        const float next = fmaxf(m, top);
+        drop = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.0f : next));
+        m = next;
+        l *= drop;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(fmaf(st[u][8 * h + j], kscale[u], -base));
+            l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            bf16x8 piece[NP];
+            pieces8<NP>(x, piece);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) pf[u][p][h] = piece[p];
+        }
+    return drop;
+}
+
+template <int PAD>
+__device__ __forceinline__ void mark_nan32(const uint8_t *vpair, int from, int to, int lane, int place,
+                                           f32x16 (&acc)[PAD / 32]) {
+    for (int tile = from; tile < to; ++tile)
+        for (int u = 0; u < 2; ++u) {
+            const int key0 = tile * 64 + 32 * u + 16 * (lane >> 5);
+            const uint8_t *const vt = vpair + size_t(tile) * 64 * PAD + (lane & 31) * 64 + 32 * u + 16 * (lane >> 5);
+#pragma unroll
+            for (int d = 0; d < PAD / 32; ++d) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(vt + d * 32 * 64);
+                // 0x38 is the code of 1.
+                const u32x4 one{nan_codes(v.x) * 0x38u, nan_codes(v.y) * 0x38u, nan_codes(v.z) * 0x38u,
+                                nan_codes(v.w) * 0x38u};
+                f32x16 hits{};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    u32x4 see;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + 8 * h + 2 * e;
+                        see[e] = (key <= place ? 0x3f80u : 0u) | (key + 1 <= place ? 0x3f800000u : 0u);
+                    }
+                    hits = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes8(one[2 * h], one[2 * h + 1]),
+                                                                   __builtin_bit_cast(bf16x8, see), hits, 0, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (hits[e] > 0.0f) acc[d][e] = __builtin_nanf("");
+            }
+        }
+}
+
+// Many rows of a pair a workgroup, as in prompts: every wave has 32 rows of its
+// own, and the waves share the key tiles as BF16 in LDS.  Each converts its part of
+// the next tile, which it has in registers since the tile before, into the other
+// half of the LDS while the products run, so a code is converted once for 128 rows,
+// with one barrier a tile; operands lie in LDS in the order of their readers, 16
+// bytes a lane.  The products are of 32 x 32: the vector unit waits less for them
+// than for 16 x 16 (beside as many exponentials a product of the same size took 12.9
+// cycles against 22).  SUB times 32 keys are softened together, as the registers
+// allow.
+template <class T, int PAD, int SUB>
+__global__ void __launch_bounds__(64 * kWaves, PAD == 256 ? 1 : 2)
+kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
+    constexpr int NP = kPieces<T>, DT = PAD / 32, ROWS = 32 * kWaves;
+    // A tile's groups: 64 lanes' 16 codes of the keys (32 u + ..., 32 c + ...), then
+    // of the values; in LDS two operands of 8 elements for each lane.
+    static_assert(kWaves == 4, "two waves take the keys, two the values");
+    __shared__ bf16x8 lds[2][4 * DT][2][64];
     __shared__ uint32_t nans;  // NaN codes were taken out
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
     // Workgroups of a pair lie 8 apart, on one XCD and its L2; long rows first.
     const int id = int(blockIdx.x), pair = id % pairs8;
     if (pair >= pairs) return;
     const int split = id / pairs8 % a.splits, tile0 = row_tiles - 1 - id / pairs8 / a.splits;
     const Sequence s(a, pair);
-    constexpr int ROWS = 16 * NT * kWaves;
     const int rows = s.count * a.group, block0 = tile0 * ROWS, block_end = min(block0 + ROWS, rows);
     if (block0 >= rows) return;
     if (!s.valid) {
@@ -488,7 +575,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
     const int begin = s.length - s.count;  // the first query's position
     const Tiles tiles(a, split, begin + (block_end - 1) / a.group + 1);
     if (tiles.first >= tiles.last) return;  // the join does not read it
-    const int row0 = block0 + 16 * NT * wave, row_end = min(row0 + 16 * NT, rows);
+    const int row0 = block0 + 32 * wave, row_end = min(row0 + 32, rows);
     const int seen = begin + row0 / a.group;
     const int cleaned = (begin + block0 / a.group) / 64;  // the first tile that some row may not see whole
     if (threadIdx.x == 0) nans = 0;
@@ -497,157 +584,153 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv8_tiles_kernel(Kv8AttnArgs a
 
     const uint8_t *const kpair = a.cache.k + size_t(pair) * a.cache.capacity * PAD;
     const uint8_t *const vpair = a.cache.v + size_t(pair) * a.cache.capacity * PAD;
-    // Load i of a tile: 64 pieces of 16 bytes, in the order of their readers.
-    auto load_tile = [&](int tile, int stage) {
+    // A wave takes the keys or the values of 32 tokens.
+    const bool values = wave >= 2;
+    const int half = wave & 1;
+    const uint8_t *const from = values ? vpair + n * 64 + 32 * half + 16 * g
+                                       : kpair + (32 * half + 16 * (n >> 2 & 1) + 4 * (n >> 3) + (n & 3)) * PAD + 16 * g;
+    const int apart = values ? 32 * 64 : 32;
+    uint4 raw[DT];
+    auto load_tile = [&](int tile) {
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int i = wave * LOADS + u;
-            uint8_t *const to = lds + stage * STAGE + i * 1024;
-            if (i < HALF / 1024) {  // keys
-                int key, at;
-                if constexpr (PAD >= 64) {
-                    const int t = i / (PAD / 64), c = i % (PAD / 64);
-                    key = 16 * (n >> 2) + 4 * t + (n & 3);
-                    at = 64 * c + 16 * g;
-                } else {
-                    key = 16 * (n >> 2) + 4 * (2 * i + (lane >> 5)) + (n & 3);
-                    at = 16 * (lane >> 4 & 1);
-                }
-                dma16(kpair + (size_t(tile) * 64 + key) * PAD + at, to);
-            } else {
-                const int d = i - HALF / 1024;
-                dma16(vpair + size_t(tile) * 64 * PAD + (16 * d + n) * 64 + 16 * g, to);
+        for (int v = 0; v < DT; ++v) raw[v] = *reinterpret_cast<const uint4 *>(from + size_t(tile) * 64 * PAD + v * apart);
+    };
+    auto convert_tile = [&](int tile, uint32_t vword) {
+        float scale = 1.0f;
+        if (values) {
+            const int block = 2 * half + g;
+            scale = value_scale(vword >> (8 * block) & 0xff, tile * 64 + 16 * block, s.length);
+            if (tile >= cleaned) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int v = 0; v < DT; ++v) any |= clean(raw[v]);
+                if (any) nans = 1;
             }
         }
+#pragma unroll
+        for (int v = 0; v < DT; ++v) {
+            lds[tile & 1][wave * DT + v][0][lane] = codes8(raw[v].x, raw[v].y, scale);
+            lds[tile & 1][wave * DT + v][1][lane] = codes8(raw[v].z, raw[v].w, scale);
+        }
     };
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i)
-        if (tiles.first + i < tiles.last) load_tile(tiles.first + i, i);
+    load_tile(tiles.first);
 
-    bf16x8 qf[NT][NP][PAD / 32];
-    int place[NT];
-    load_queries<T, PAD, NT>(a, s, row0, rows, lane, qf, place);
-    float m[NT];
-    f32x4 acc[NT][DT], l[NT];
+    bf16x8 qf[NP][DT][2];
+    const int r = row0 + n, place = r < rows ? begin + r / a.group : -1;
+    {
+        const int i = r / a.group;
+        const auto *q = static_cast<const typename T::Raw *>(a.q) + s.seq * a.qs.s[0] + i * a.qs.s[1] +
+                        (s.head * a.group + r - i * a.group) * a.qs.s[2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < DT; ++c)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k = 0; k < 2; ++k) {
+                bf16x8 piece[NP];
+                query8<T>(a, q, r < rows, 32 * c + 16 * g + 8 * k, piece);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) qf[p][c][k] = piece[p];
+            }
     }
+    float m = -INFINITY, l = 0.0f;
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
     // Four scales of a tile are a word that all lanes read.
     typedef const __attribute__((address_space(4))) uint32_t *Words;
     const Words kscales = (Words)(a.cache.ks + size_t(pair) * (a.cache.capacity / 16));
     const Words vscales = (Words)(a.cache.vs + size_t(pair) * (a.cache.capacity / 16));
 
-    int stage = 0;
     uint32_t kword = kscales[tiles.first], vword = vscales[tiles.first];
+    __syncthreads();  // nans is cleared
+    convert_tile(tiles.first, vword);
+    if (tiles.first + 1 < tiles.last) load_tile(tiles.first + 1);
+    vword = vscales[min(tiles.first + 1, tiles.last - 1)];
     for (int tile = tiles.first; tile < tiles.last; ++tile) {
-        if (STAGES > 2 && tile + 1 < tiles.last)
-            wait_vm<(STAGES - 2) * LOADS>();
-        else
-            wait_vm<0>();
-        barrier_lds();  // everyone's loads of this tile, and everyone past the one before
-        if (tile + STAGES - 1 < tiles.last) load_tile(tile + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-        uint8_t *const now = lds + stage * STAGE;
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
-        if (tile >= cleaned) {
-            uint32_t any = 0;
-            for (int i = int(threadIdx.x); i < HALF / 16; i += 64 * kWaves) {
-                uint4 *const w = reinterpret_cast<uint4 *>(now + HALF) + i;
-                uint4 v = *w;
-                any |= clean(v);
-                *w = v;
+        barrier_lds();  // this tile is there, and everyone past the one before
+        const uint32_t kbytes = kword, vbytes = vscales[tile];
+        if (tile + 1 < tiles.last) {
+            convert_tile(tile + 1, vword);
+            kword = kscales[tile + 1];
+            if (tile + 2 < tiles.last) {
+                load_tile(tile + 2);
+                vword = vscales[tile + 2];
             }
-            if (any) nans = 1;
-            barrier_lds();
         }
-        const int kbyte = kword >> (8 * g) & 0xff, vbyte = vword >> (8 * g) & 0xff, next = min(tile + 1, tiles.last - 1);
-        kword = kscales[next];
-        vword = vscales[next];
+        const auto &now = lds[tile & 1];
         if (tile >= mine) continue;
-
-        f32x4 st[NT][4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int r = 0; r < NT; ++r) st[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < (PAD + 63) / 64; ++c) {
-                uint4 w{};
-                if constexpr (PAD >= 64)
-                    w = *reinterpret_cast<const uint4 *>(now + ((t * (PAD / 64) + c) * 64 + lane) * 16);
-                else
-                    *reinterpret_cast<uint2 *>(&w) =
-                        *reinterpret_cast<const uint2 *>(now + ((t * 2 + (g >> 1)) * 16 + n) * 16 + 8 * (g & 1));
-#pragma unroll
-                for (int k = 0; k < (PAD >= 64 ? 2 : 1); ++k) {
-                    const bf16x8 kf = k ? codes8(w.z, w.w) : codes8(w.x, w.y);
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                        for (int r = 0; r < NT; ++r)
-                            st[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[r][p][2 * c + k], st[r][t], 0, 0, 0);
-                }
-            }
-        }
-        const int key0 = tile * 64 + 16 * g;  // of the lane's 16 keys
         const bool masked = tile * 64 + 63 > seen;
-        const float kscale = power(kbyte) * a.scale_log2, vscale = value_scale(vbyte, key0, s.length);
-        bf16x8 pf[NT][NP][2];
 #pragma unroll
-        for (int r = 0; r < NT; ++r) {
-            const float drop = soften<NP>(st[r], masked, kscale, slack_of(vbyte), key0, place[r], m[r], pf[r]);
+        for (int step = 0; step < 2; step += SUB) {
+            f32x16 st[SUB];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) st[u] = f32x16{};
+#pragma unroll
+            for (int c = 0; c < DT; ++c)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) {
+                        const bf16x8 kf = now[(step + u) * DT + c][k][lane];
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; --p)
+                            st[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[p][c][k], st[u], 0, 0, 0);
+                    }
+            paced<2 * DT * SUB, NP>();
+            int key0[SUB];  // of the lane's 16 keys
+            float kscale[SUB], slack = kSlack;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                const int at = 8 * (2 * (step + u) + g), vbyte = vbytes >> at & 0xff;
+                key0[u] = tile * 64 + 32 * (step + u) + 16 * g;
+                kscale[u] = power(kbytes >> at & 0xff) * a.scale_log2;
+                slack = fminf(slack, slack_of(vbyte));
+            }
+            bf16x8 pf[SUB][NP][2];
+            const float drop = soften32<NP, SUB>(st, masked, kscale, slack, key0, place, m, l, pf);
             if (__any(drop != 1.0f)) {
-                l[r] *= drop;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[r][d] *= drop;
+                for (int d = 0; d < DT; ++d) acc[d] *= drop;
             }
-            l[r] = add_sums<NP>(pf[r], l[r]);
-        }
-        const uint8_t *const vt = now + HALF + lane * 16;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(vt + d * 1024);
+            for (int u = 0; u < SUB; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bf16x8 vf = h ? codes8(w.z, w.w, vscale) : codes8(w.x, w.y, vscale);
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
+                    for (int d = 0; d < DT; ++d) {
+                        const bf16x8 vf = now[2 * DT + (step + u) * DT + d][h][lane];
 #pragma unroll
-                    for (int r = 0; r < NT; ++r)
-                        acc[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][p][h], acc[r][d], 0, 0, 0);
-            }
+                        for (int p = NP - 1; p >= 0; --p)
+                            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][p][h], acc[d], 0, 0, 0);
+                    }
+            paced<2 * DT * SUB, NP>();
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if (tiles.last > cleaned && nans) mark_nan<PAD, NT>(vpair, max(tiles.first, cleaned), min(tiles.last, mine), lane, place, acc);
-
+    if (tiles.last > cleaned && nans)
+        mark_nan32<PAD>(vpair, max(tiles.first, cleaned), min(tiles.last, mine), lane, place, acc);
+    const auto both = __builtin_amdgcn_permlane32_swap(int(bits(l)), int(bits(l)), false, false);
+    const float sum = bits(uint32_t(both[0])) + bits(uint32_t(both[1]));
+    if (r >= rows) return;
+    if (a.splits == 1) {
+        auto *o = out_row<T>(a, s, r);
+        const float inverse = 1.0f / sum;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const float sum = l[t][0];
-        const int r = row0 + 16 * t + n;
-        if (r >= rows) continue;
-        if (a.splits == 1) {
-            auto *o = out_row<T>(a, s, r);
-            const float inverse = 1.0f / sum;
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int at = 16 * d + 4 * g + e;
-                    if (at < a.cache.width) o[at] = T::from_float(acc[t][d][e] * inverse);
-                }
-        } else {
-            float *o = a.part + ((size_t(pair) * a.rows + r) * a.splits + split) * a.stride;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[16 * d + 4 * g + e] = acc[t][d][e];
-            if (g == 0) {
-                o[a.stride - 2] = m[t];
-                o[a.stride - 1] = sum;
+            for (int e = 0; e < 16; ++e) {
+                const int at = 32 * d + 8 * (e / 4) + 4 * g + e % 4;
+                if (at < a.cache.width) o[at] = T::from_float(acc[d][e] * inverse);
             }
+    } else {
+        float *o = a.part + ((size_t(pair) * a.rows + r) * a.splits + split) * a.stride;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[32 * d + 8 * (e / 4) + 4 * g + e % 4] = acc[d][e];
+        if (g == 0) {
+            o[a.stride - 2] = m;
+            o[a.stride - 1] = sum;
         }
     }
 }
@@ -687,19 +770,13 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8AttnArgs a, int pairs)
         if (lane + 64 * e < a.cache.width) o[lane + 64 * e] = T::from_float(acc[e] / total);
 }
 
-// Tiles of 16 rows that a wave with rows of its own takes: as many as its
-// registers hold.
-template <class T>
-constexpr int wide_tiles(int pad) {
-    return pad <= 64 ? 2 : pad == 128 ? (kPieces<T> == 3 ? 1 : 2) : 1;
-}
-
 template <class T, int PAD>
 void launch_attn(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) {
     const int pairs = a.cache.batch * a.cache.heads;
     if (plan.wide) {
+        constexpr int SUB = PAD <= 64 || (PAD == 128 && kPieces<T> == 1) ? 2 : 1;
         const int pairs8 = (pairs + 7) / 8 * 8;
-        hipLaunchKernelGGL((kv8_tiles_kernel<T, PAD, wide_tiles<T>(PAD)>),
+        hipLaunchKernelGGL((kv8_tiles_kernel<T, PAD, SUB>),
                            dim3(uint32_t(pairs8) * uint32_t(a.splits) * uint32_t(plan.row_tiles)), dim3(64 * kWaves), 0,
                            stream, a, pairs, pairs8, plan.row_tiles);
     } else {
@@ -723,14 +800,12 @@ void attn_of(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) {
 
 }  // namespace
 
-Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count) {
+Kv8Plan kv8_plan(const Kv8 &cache, int group, int count) {
     Kv8Plan p{};
     const int64_t rows = int64_t(count) * group;
     const int pairs = std::max(1, cache.batch * cache.heads);
-    const int tiles = type == Type::F32 ? wide_tiles<F32>(cache.pad) : type == Type::F16 ? wide_tiles<F16>(cache.pad)
-                                                                                         : wide_tiles<BF16>(cache.pad);
     p.wide = rows > 16;
-    const int each = p.wide ? 16 * kWaves * tiles : 16;
+    const int each = p.wide ? 32 * kWaves : 16;
     p.row_tiles = int((rows + each - 1) / each);
     // Shares of the keys: about 2048 workgroups, of 256 keys or more.
     const int64_t groups = int64_t(pairs) * p.row_tiles, most = std::max(1, cache.capacity / 256);
