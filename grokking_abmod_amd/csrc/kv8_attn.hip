@@ -225,6 +225,24 @@ __device__ __forceinline__ typename T::Raw *out_row(const Kv8AttnArgs &a, const 
            (s.head * a.group + r - i * a.group) * a.os.s[2];
 }
 
+// Four outputs of a row from `at`, those inside the width.
+template <class T>
+__device__ __forceinline__ void store4(const Kv8AttnArgs &a, typename T::Raw *o, int at, f32x4 v) {
+    if (a.o_aligned && at + 4 <= a.cache.width) {
+        if constexpr (T::kGroup == 4) {
+            *reinterpret_cast<f32x4 *>(o + at) = v;
+        } else {
+            const float x[8] = {v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f};
+            const uint4 w = T::pack(x);
+            *reinterpret_cast<uint2 *>(o + at) = uint2{w.x, w.y};
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (at + e < a.cache.width) o[at + e] = T::from_float(v[e]);
+}
+
 // Eight elements of a query from d as pieces, zeros where there are none.
 template <class T>
 __device__ __forceinline__ void query8(const Kv8AttnArgs &a, const typename T::Raw *q, bool real, int d,
@@ -712,22 +730,20 @@ kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
     const auto both = __builtin_amdgcn_permlane32_swap(int(bits(l)), int(bits(l)), false, false);
     const float sum = bits(uint32_t(both[0])) + bits(uint32_t(both[1]));
     if (r >= rows) return;
+    auto four = [&](int d, int e) { return f32x4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]}; };
     if (a.splits == 1) {
         auto *o = out_row<T>(a, s, r);
         const float inverse = 1.0f / sum;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int at = 32 * d + 8 * (e / 4) + 4 * g + e % 4;
-                if (at < a.cache.width) o[at] = T::from_float(acc[d][e] * inverse);
-            }
+            for (int e = 0; e < 4; ++e) store4<T>(a, o, 32 * d + 8 * e + 4 * g, four(d, e) * inverse);
     } else {
         float *o = a.part + ((size_t(pair) * a.rows + r) * a.splits + split) * a.stride;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[32 * d + 8 * (e / 4) + 4 * g + e % 4] = acc[d][e];
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<f32x4 *>(o + 32 * d + 8 * e + 4 * g) = four(d, e);
         if (g == 0) {
             o[a.stride - 2] = m;
             o[a.stride - 1] = sum;
@@ -735,39 +751,40 @@ kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
     }
 }
 
-// Joins the shares of a row: a wave a row.
-template <class T>
-__global__ void __launch_bounds__(256) kv8_join_kernel(Kv8AttnArgs a, int pairs) {
-    const int64_t u = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (u >= int64_t(pairs) * a.rows) return;
+// Joins the shares of a row: a lane takes four of its channels.
+template <class T, int PAD>
+__global__ void __launch_bounds__(256) kv8_join_kernel(Kv8AttnArgs a, int64_t total) {
+    constexpr int LANES = PAD / 4;
+    const int64_t u = int64_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    const int d = 4 * (threadIdx.x % LANES);
+    if (u >= total) return;
     const int pair = int(u / a.rows), r = int(u - int64_t(pair) * a.rows);
     const Sequence s(a, pair);
     if (r >= s.count * a.group) return;
     auto *o = out_row<T>(a, s, r);
-    if (!s.valid) {
-        for (int d = lane; d < a.cache.width; d += 64) o[d] = T::from_float(__builtin_nanf(""));
-        return;
+    f32x4 out;
+    if (s.valid) {
+        // The shares of this row's tile of rows reach to the tile's last row;
+        // those past this row's own keys hold nothing of it.
+        const int keys = s.length - s.count + r / a.group + 1, used = (keys + a.chunk - 1) / a.chunk;
+        const float *p = a.part + size_t(u) * a.splits * a.stride;
+        float m = -INFINITY, l = 0.0f;
+        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int k = 0; k < used; ++k, p += a.stride) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(p + d);
+            const float mk = p[a.stride - 2], lk = p[a.stride - 1], top = fmaxf(m, mk);
+            const float base = top == -INFINITY ? 0.0f : top;
+            const float old = __builtin_amdgcn_exp2f(m - base), now = __builtin_amdgcn_exp2f(mk - base);
+            acc = acc * old + v * now;
+            l = l * old + lk * now;
+            m = top;
+        }
+        out = acc * (1.0f / l);
+    } else {
+        out = f32x4{} + __builtin_nanf("");
     }
-    // The shares that this row's tile of rows wrote reach to the tile's last
-    // row; those past this row's own keys hold nothing of it.
-    const int keys = s.length - s.count + r / a.group + 1, used = (keys + a.chunk - 1) / a.chunk;
-    const float *p = a.part + size_t(u) * a.splits * a.stride;
-    float top = -INFINITY;
-    for (int k = 0; k < used; ++k) top = fmaxf(top, p[size_t(k) * a.stride + a.stride - 2]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < used; ++k) {
-        const float *q = p + size_t(k) * a.stride;
-        const float f = __builtin_amdgcn_exp2f(q[a.stride - 2] - base);
-        total += f * q[a.stride - 1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < a.cache.width) acc[e] += f * q[lane + 64 * e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < a.cache.width) o[lane + 64 * e] = T::from_float(acc[e] / total);
+    store4<T>(a, o, d, out);
 }
 
 template <class T, int PAD>
@@ -784,8 +801,8 @@ void launch_attn(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) 
                            dim3(64 * kWaves), 0, stream, a, pairs, plan.row_tiles);
     }
     if (a.out && a.splits > 1)
-        hipLaunchKernelGGL((kv8_join_kernel<T>), dim3(uint32_t((int64_t(pairs) * a.rows + 3) / 4)), dim3(256), 0,
-                           stream, a, pairs);
+        hipLaunchKernelGGL((kv8_join_kernel<T, PAD>), dim3(uint32_t((int64_t(pairs) * a.rows * (PAD / 4) + 255) / 256)),
+                           dim3(256), 0, stream, a, int64_t(pairs) * a.rows);
 }
 
 template <class T>
@@ -807,12 +824,17 @@ Kv8Plan kv8_plan(const Kv8 &cache, int group, int count) {
     p.wide = rows > 16;
     const int each = p.wide ? 32 * kWaves : 16;
     p.row_tiles = int((rows + each - 1) / each);
-    // Shares of the keys: about 2048 workgroups, of 256 keys or more.
-    const int64_t groups = int64_t(pairs) * p.row_tiles, most = std::max(1, cache.capacity / 256);
-    const int64_t want = std::min<int64_t>(std::min<int64_t>(most, 256), (2048 + groups - 1) / groups);
+    // Shares of the keys, for enough workgroups (two or more a CU are resident)
+    // of like length.  Their join is a launch of its own, some 6 us with what it
+    // waits for, so single tokens take 1024 keys or more a share (32 x 8 heads, up
+    // to 576 keys: 10.7 us in one share, 18.8 in shares of 256), prompts, which
+    // work longer on a key, 512 (3 x 8 heads, 1001 rows, up to 1501 keys: 49.6 us in
+    // four shares, 56.3 in three, 66.0 in two).
+    const int64_t groups = int64_t(pairs) * p.row_tiles, least = p.wide ? 512 : 1024, aim = p.wide ? 1024 : 2048;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>({cache.capacity / least, 256, (aim + groups - 1) / groups}));
     p.chunk = int((cache.capacity + want - 1) / want + 63) / 64 * 64;
     p.splits = (cache.capacity + p.chunk - 1) / p.chunk;
-    p.part_floats = p.splits > 1 ? size_t(pairs) * size_t(rows) * size_t(p.splits) * size_t(cache.pad + 2) : 0;
+    p.part_floats = p.splits > 1 ? size_t(pairs) * size_t(rows) * size_t(p.splits) * size_t(kv8_part_stride(cache.pad)) : 0;
     return p;
 }
 

@@ -189,10 +189,10 @@ void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t
     const kern::Kv8Plan plan = kern::kv8_plan(cache, group, int(count));
     require(plan.part_floats == 0 || (workspace && workspace_bytes >= plan.part_floats * 4),
             "the workspace is too small: mg_kv8_attention_workspace gives its size");
-    require(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "the workspace must be aligned to 4 bytes");
+    require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
     const double pairs = double(cache.batch) * cache.heads;
     check_grid((pairs + 7) * plan.splits * plan.row_tiles);
-    check_grid(pairs * double(count) * group / 4 + 1);
+    check_grid(pairs * double(count) * group + 1);
     const OnDevice on(device);
     kern::Kv8AttnArgs a{};
     a.cache = cache;
@@ -209,7 +209,7 @@ void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t
     a.splits = plan.splits;
     a.chunk = plan.chunk;
     a.part = static_cast<float *>(workspace);
-    a.stride = cache.pad + 2;
+    a.stride = kern::kv8_part_stride(cache.pad);
     a.q_aligned = aligned16(q, qs, type);
     a.o_aligned = aligned16(out, os, type);
     kern::kv8_attention(a, type, plan, stream);

@@ -75,6 +75,9 @@ struct Kv8AttnArgs {
     int stride;
     int q_aligned, o_aligned;
 };
+// Floats of a share's state: 16-byte groups, the last two elements the maximum
+// and the sum.
+inline int kv8_part_stride(int pad) { return pad + 4; }
 // How a call is cut: the rows of a workgroup and the shares of the keys.
 struct Kv8Plan {
     bool wide;  // a wave has rows of its own; else the waves share a workgroup's rows and split its keys

@@ -295,7 +295,7 @@ int mg_kv8_read(int device, const mg_kv8 *cache, int type, size_t first, size_t 
  * length or count is impossible (as above) are filled with NaN, all `count` of
  * them.  F32 calls keep 24 bits of the queries and probabilities, F16 and BF16
  * calls 16 and 8 of the probabilities; sums are FP32.  The workspace holds
- * mg_kv8_attention_workspace bytes, aligned to 4 (NULL where that is 0). */
+ * mg_kv8_attention_workspace bytes, aligned to 16 (NULL where that is 0). */
 int mg_kv8_attention_workspace(const mg_kv8 *cache, size_t heads, size_t count, size_t *bytes);
 int mg_kv8_attention(int device, const mg_kv8 *cache, int type, size_t heads, size_t count, const void *q,
                      const int64_t q_strides[3], void *out, const int64_t out_strides[3], const int32_t *lengths,

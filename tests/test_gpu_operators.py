@@ -481,7 +481,7 @@ def test_a_serving_step_as_a_graph(kind):
     projection; captured once on a stream of its own and replayed with new inputs,
     each replay against the plain forms on the cache it left."""
     rng = np.random.default_rng(9)
-    batch, heads, kv_heads, width, capacity, vocab, prompt = 3, 4, 2, 64, 512, 300, 21
+    batch, heads, kv_heads, width, capacity, vocab, prompt = 3, 4, 2, 64, 2048, 300, 21
     cache = L.Cache(batch, kv_heads, width, capacity, rng)
     lengths = np.array([21, 5, 14], np.int32)
     scale = 0.125

@@ -82,7 +82,7 @@ def test_attention_refusals():
     assert room > 0
     refused("workspace is too small", call, cache=long)
     refused("workspace is too small", call, cache=long, workspace=256, workspace_bytes=15)
-    refused("aligned to 4", call, cache=long, workspace=257, workspace_bytes=room)
+    refused("aligned to 16", call, cache=long, workspace=264, workspace_bytes=room)
     refused("capacity", G.kv8_attention_workspace, c, 4, 129)
     refused("multiple of the cache's heads", G.kv8_attention_workspace, c, 3, 1)
 
