@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <cfloat>
 
+#include "dpp.hpp"
 #include "operators.hpp"
 #include "types.hpp"
 
@@ -28,15 +29,16 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kSmall = 1024;           // logits of a row that one wave holds
-constexpr int kThreadMost = 128;       // logits of a thread's share of a chunk
-constexpr int kList = 4096;            // candidates of a chunk: over kTopMax - 1 threads' shares
+constexpr int kThreadMost = 64;        // logits of a thread's share of a chunk, at most
+constexpr int kList = 2048;            // candidates of a chunk: kTopMax threads' shares
+constexpr int kStaged = 2048;          // candidates that a join holds in LDS
 constexpr uint32_t kIgnore = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A thread's share of a chunk is its groups and at most one logit before and
 // behind them.
 constexpr int kChunkMost = kBlock * (kThreadMost - 16);
-static_assert((kTopMax - 1) * kThreadMost <= kList, "the logits over the bound fit the list");
+static_assert(kTopMax * kThreadMost <= kList, "the logits over the bound fit the list");
 
 // Orders as the floats do, -0 with 0; NaN is not asked for.
 __device__ __forceinline__ uint32_t order(float x) {
@@ -80,21 +82,38 @@ __device__ __forceinline__ void add(float x, float base, float c, float &s, floa
     a = fmaf(e, d, a);
 }
 
-__device__ __forceinline__ void wave_join(Sums &t, float c) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const float m = __shfl_xor(t.m, k, 64), s = __shfl_xor(t.s, k, 64), a = __shfl_xor(t.a, k, 64);
-        t.join(m, s, a, c);
-    }
+__device__ __forceinline__ float wave_top(float v) {
+    v = fmaxf(v, dpp_move<0xB1>(v, v));
+    v = fmaxf(v, dpp_move<0x4E>(v, v));
+    v = fmaxf(v, dpp_move<0x141>(v, v));
+    v = fmaxf(v, dpp_move<0x140>(v, v));
+    v = fmaxf(v, dpp_move<0x142, 0xa>(v, v));
+    v = fmaxf(v, dpp_move<0x143, 0xc>(v, v));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+__device__ __forceinline__ void wave_join(Sums &t, float c) {
+    t.raise(wave_top(t.m), c);
+    t.s = wave_sum(t.s);
+    t.a = wave_sum(t.a);
+}
+
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ uint32_t largest_of(uint32_t v) {
+    return max(v, uint32_t(__builtin_amdgcn_update_dpp(int(v), int(v), CTRL, ROW_MASK, 0xf, false)));
+}
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+    v = largest_of<0xB1>(v);
+    v = largest_of<0x4E>(v);
+    v = largest_of<0x141>(v);
+    v = largest_of<0x140>(v);
+    v = largest_of<0x142, 0xa>(v);
+    v = largest_of<0x143, 0xc>(v);
+    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
+}
 __device__ __forceinline__ uint64_t wave_best(uint64_t v) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const uint64_t o = __shfl_xor(v, k, 64);
-        v = o > v ? o : v;
-    }
-    return v;
+    const uint32_t high = wave_largest(uint32_t(v >> 32));
+    return (uint64_t(high) << 32) | wave_largest(uint32_t(v >> 32) == high ? uint32_t(v) : 0);
 }
 
 // A row's results from its sums (a in log2 units); one thread.
@@ -158,24 +177,20 @@ __global__ void __launch_bounds__(kBlock) logprob_small_kernel(LogprobArgs a) {
     if (lane == 0) write_row<T>(a, row, t, log_sum);
     if (!a.top) return;
     log_sum = __shfl(log_sum, 0, 64);
-    uint32_t taken = 0;
-    for (int k = 0; k < a.top; ++k) {
-        uint64_t best = 0;
-        int at = 0;
+    uint64_t left[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t v = lane + 64 * i;
-            const uint64_t o = v < a.vocab && !(taken >> i & 1) ? candidate(order(x[i]), v) : 0;
-            if (o > best) {
-                best = o;
-                at = i;
-            }
-        }
+    for (int i = 0; i < N; ++i) {
+        const uint32_t v = lane + 64 * i;
+        left[i] = v < a.vocab ? candidate(order(x[i]), v) : 0;
+    }
+    for (int k = 0; k < a.top; ++k) {
+        uint64_t best = left[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) best = left[i] > best ? left[i] : best;
         const uint64_t first = wave_best(best);
-        if (best == first) {  // candidates differ, so one lane has it
-            taken |= 1u << at;
-            write_top(a, row, k, first, t, log_sum);
-        }
+        if (lane == 0) write_top(a, row, k, first, t, log_sum);
+#pragma unroll
+        for (int i = 0; i < N; ++i) left[i] = left[i] == first ? 0 : left[i];
     }
 }
 
@@ -229,7 +244,8 @@ __global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
 
     __shared__ float joined[kBlock / 64][3];
     __shared__ uint32_t tops[kBlock];
-    __shared__ uint32_t bound, found, over;
+    __shared__ uint32_t bound, found, over, picked;
+    __shared__ uint8_t picks[kBlock];
     __shared__ uint64_t list[kList];
     const bool any = uint32_t(tid) < body - lo || uint32_t(tid) < hi - tail || uint32_t(tid) < groups;
     const uint32_t mine = any ? order(t.m) : 0;
@@ -240,7 +256,7 @@ __global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
         joined[wave][1] = t.s;
         joined[wave][2] = t.a;
     }
-    if (tid == 0) found = over = 0;
+    if (tid == 0) found = over = picked = 0;
     __syncthreads();
     t.m = joined[0][0];
     t.s = joined[0][1];
@@ -282,42 +298,50 @@ __global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
 #pragma unroll
             for (int w = 0; w < kBlock / 64; ++w) n += __popcll(__ballot(k[w] >= (at | bit)));
             if (n >= have) at |= bit;
+            if (n == have) break;  // it parts them as well as the have-th does
         }
         if (lane == 0) bound = at;
     }
     __syncthreads();
     const uint32_t least = bound;
-    auto offer = [&](float x, uint32_t v, bool equal_too) {
+    auto offer = [&](float x, uint32_t v, uint32_t from) {
         const uint32_t k = order(x);
-        if (k < least || (k == least && !equal_too)) return;
+        if (k < from) return;
         const uint32_t at = atomicAdd(&found, 1u);
         if (at < uint32_t(kList))
             list[at] = candidate(k, v);
         else
             over = 1;
     };
-    auto share = [&](bool equal_too) {
-        if (uint32_t(tid) < body - lo) offer(T::to_float(z[lo + tid]), lo + tid, equal_too);
-        if (uint32_t(tid) < hi - tail) offer(T::to_float(z[tail + tid]), tail + tid, equal_too);
-        for (uint32_t j = tid; j < groups; j += kBlock) {
-            float x[G];
-            T::unpack(zg[j], x);
+    // The shares of the threads that hold any, spread over all threads.
+    const uint32_t steps = (groups + kBlock - 1) / kBlock + 1;
+    auto look = [&](uint32_t from) {
+        if (any && mine >= from) picks[atomicAdd(&picked, 1u)] = uint8_t(tid);
+        __syncthreads();
+        for (uint32_t i = tid; i < picked * steps; i += kBlock) {
+            const uint32_t who = picks[i / steps], step = i % steps, j = who + step * kBlock;
+            if (step + 1 == steps) {  // what lies outside the groups
+                if (who < body - lo) offer(T::to_float(z[lo + who]), lo + who, from);
+                if (who < hi - tail) offer(T::to_float(z[tail + who]), tail + who, from);
+            } else if (j < groups) {
+                float x[G];
+                T::unpack(zg[j], x);
 #pragma unroll
-            for (int e = 0; e < G; ++e) offer(x[e], body + j * G + e, equal_too);
+                for (int e = 0; e < G; ++e) offer(x[e], body + j * G + e, from);
+            }
         }
+        __syncthreads();
     };
-    if (mine >= least && any) share(true);
-    __syncthreads();
+    look(least);
     if (over) {
         // Many logits equal the bound (most of a masked row, say): the ones
         // over it, which fit, then equal ones in the order of their tokens
         // until there are enough.
         __syncthreads();
-        if (tid == 0) found = 0;
+        if (tid == 0) found = picked = 0;
         __syncthreads();
-        if (mine > least && any) share(false);
+        look(least + 1);
         for (uint32_t from = lo; from < hi; from += kBlock) {
-            __syncthreads();
             if (found >= uint32_t(have)) break;
             __syncthreads();
             const uint32_t v = from + tid;
@@ -325,8 +349,8 @@ __global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
                 const uint32_t at = atomicAdd(&found, 1u);
                 list[min(at, uint32_t(kList - 1))] = candidate(least, v);
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
     // A candidate's place is the number of those before it.
     const int n = min(int(found), kList);
@@ -361,10 +385,25 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LogprobArgs a) {
     if (lane == 0) write_row<T>(a, row, t, log_sum);
     if (!a.top) return;
     log_sum = t.s == 0.0f ? -INFINITY : logf(t.s);
+    const uint64_t *const lists = a.part_top + row * a.chunks * a.top;
+    const int n = a.chunks * a.top;
+    if (a.chunks <= 64 && n <= kStaged) {  // a chunk a lane, the lists in LDS
+        __shared__ uint64_t all[kStaged];
+        for (int i = lane; i < n; i += 64) all[i] = lists[i];
+        __syncthreads();
+        int at = lane * a.top;
+        const int end = lane < a.chunks ? at + a.top : at;
+        uint64_t head = at < end ? all[at] : 0;
+        for (int k = 0; k < a.top; ++k) {
+            const uint64_t first = wave_best(head);
+            if (lane == 0) write_top(a, row, k, first, t, log_sum);
+            if (head == first) head = ++at < end ? all[at] : 0;
+        }
+        return;
+    }
     constexpr int HELD = ((1 << 24) / kChunkMost + 64) / 64;  // chunks of a lane at most
     uint64_t head[HELD];
     uint32_t taken[HELD];
-    const uint64_t *const lists = a.part_top + row * a.chunks * a.top;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
         const int k = lane + 64 * i;
@@ -499,10 +538,10 @@ void logprob_chunks(size_t rows, size_t vocab, int &chunks, int &chunk) {
     chunks = 1;
     chunk = int(vocab);
     if (vocab <= size_t(kSmall)) return;
-    // About 1024 workgroups, each of 2048 logits or more.
-    const size_t want = std::min<size_t>((1024 + rows - 1) / std::max<size_t>(rows, 1), (vocab + 2047) / 2048);
-    size_t size = (vocab + want - 1) / want;
-    size = std::min<size_t>((size + 63) / 64 * 64, size_t(kChunkMost));
+    // About 1024 workgroups, each of 2048 logits or more, and even.
+    size_t want = std::min<size_t>((1024 + rows - 1) / std::max<size_t>(rows, 1), (vocab + 2047) / 2048);
+    want = std::max<size_t>(want, (vocab + kChunkMost - 1) / kChunkMost);
+    const size_t size = std::min<size_t>(((vocab + want - 1) / want + 63) / 64 * 64, size_t(kChunkMost));
     chunk = int(size);
     chunks = int((vocab + size - 1) / size);
 }
