@@ -11,10 +11,10 @@
 // round again only where they become subnormal.
 //
 // Both directions move bytes: one wave takes 16 tokens of a head, of its keys
-// or of its values.  Keys are stored as they come; a lane takes 16 channels of
-// a token.  Values are stored transposed, 64 tokens of a channel in a row, the
-// order in which the attention's matrix product reads them; a lane takes a
-// channel of the 16 tokens.
+// or of its values.  Keys are stored as they come; a lane takes 16 bytes of a
+// token's inputs.  Values are stored transposed, 64 tokens of a channel in a row, the
+// order in which the attention's matrix product reads them; a lane takes two
+// channels of the 16 tokens.
 #include <hip/hip_runtime.h>
 
 #include <cfloat>
@@ -71,16 +71,22 @@ __device__ __forceinline__ float wave_largest(float v) {
     return v;
 }
 
-// N consecutive elements from p, those at or past `have` as 0.
+// N consecutive elements from p (N of 16 bytes, or two), those at or past `have`
+// as 0.  Aligned: whole groups are aligned to their size.
 template <class T, int N>
 __device__ __forceinline__ void load_run(const typename T::Raw *p, int have, bool aligned, float (&x)[N]) {
     if (aligned && have >= N) {
-#pragma unroll
-        for (int i = 0; i < N / T::kGroup; ++i) {
-            float g[T::kGroup];
-            T::unpack(reinterpret_cast<const uint4 *>(p)[i], g);
-#pragma unroll
-            for (int j = 0; j < T::kGroup; ++j) x[i * T::kGroup + j] = g[j];
+        if constexpr (N == T::kGroup) {
+            T::unpack(*reinterpret_cast<const uint4 *>(p), x);
+        } else if constexpr (sizeof(*p) == 4) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(p);
+            x[0] = __builtin_bit_cast(float, w.x);
+            x[1] = __builtin_bit_cast(float, w.y);
+        } else {
+            float y[8];
+            T::unpack(uint4{*reinterpret_cast<const uint32_t *>(p), 0, 0, 0}, y);
+            x[0] = y[0];
+            x[1] = y[1];
         }
         return;
     }
@@ -91,12 +97,13 @@ __device__ __forceinline__ void load_run(const typename T::Raw *p, int have, boo
 template <class T, int N>
 __device__ __forceinline__ void store_run(typename T::Raw *p, int have, bool aligned, const float (&x)[N]) {
     if (aligned && have >= N) {
-#pragma unroll
-        for (int i = 0; i < N / T::kGroup; ++i) {
-            float g[T::kGroup];
-#pragma unroll
-            for (int j = 0; j < T::kGroup; ++j) g[j] = x[i * T::kGroup + j];
-            reinterpret_cast<uint4 *>(p)[i] = T::pack(g);
+        if constexpr (N == T::kGroup) {
+            *reinterpret_cast<uint4 *>(p) = T::pack(x);
+        } else if constexpr (sizeof(*p) == 4) {
+            *reinterpret_cast<uint2 *>(p) = uint2{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1])};
+        } else {
+            const float y[8] = {x[0], x[1], 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            *reinterpret_cast<uint32_t *>(p) = T::pack(y).x;
         }
         return;
     }
@@ -105,20 +112,19 @@ __device__ __forceinline__ void store_run(typename T::Raw *p, int have, bool ali
         if (i < have) p[i] = T::from_float(x[i]);
 }
 
-template <int N>
-__device__ __forceinline__ float finite_largest(const float (&x)[N], float top) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]) <= FLT_MAX ? fabsf(x[i]) : 0.0f);
-    return top;
-}
+__device__ __forceinline__ float finite_size(float x) { return fabsf(x) <= FLT_MAX ? fabsf(x) : 0.0f; }
 
-// How a lane takes part: keys, `kRun` channels of one token, `kPasses` times 64
-// channels on; values, `kSlots` tokens of one channel.
+// How a lane takes part in keys: kRun channels (16 bytes of the inputs) of tokens
+// kRows apart, so that a wave's loads and stores are whole rows.
+template <class T, int PAD>
+struct KeyShare {
+    static constexpr int kRun = T::kGroup, kLanes = PAD / kRun, kRows = 64 / kLanes, kPasses = 16 / kRows;
+};
+// In values: two channels of kSlots tokens, kPasses times 128 channels on.
 template <int PAD>
-struct Share {
-    static constexpr int kPasses = PAD >= 64 ? PAD / 64 : 1;
-    static constexpr int kRun = PAD >= 64 ? 16 : PAD / 4;
-    static constexpr int kSlots = PAD >= 64 ? 16 : 8;
+struct ValueShare {
+    static constexpr int kPasses = PAD >= 128 ? PAD / 128 : 1;
+    static constexpr int kLanes = PAD >= 128 ? 64 : PAD / 2, kSlots = 16 * kLanes / 64;
 };
 
 // Positions [lo, hi) of the block's 16 are new; with lo past the block's first,
@@ -126,215 +132,251 @@ struct Share {
 template <class T, int PAD>
 __device__ __forceinline__ void append_keys(const Kv8AppendArgs &a, int seq, int head, size_t pair, int block, int lo,
                                             int hi, int first) {
-    using S = Share<PAD>;
-    const int lane = threadIdx.x & 63, place = 16 * block + (lane >> 2);
-    const bool fresh = place >= lo && place < hi, begun = lo > 16 * block;
-    const auto *row = static_cast<const typename T::Raw *>(a.k) + seq * a.ks.s[0] + int64_t(place - first) * a.ks.s[1] +
-                      head * a.ks.s[2];
+    using S = KeyShare<T, PAD>;
+    const int lane = threadIdx.x & 63, d = S::kRun * (lane % S::kLanes), place0 = 16 * block + lane / S::kLanes;
+    const bool begun = lo > 16 * block;
+    const auto *base = static_cast<const typename T::Raw *>(a.k) + seq * a.ks.s[0] + head * a.ks.s[2] + d;
     uint8_t *const scale = a.cache.ks + pair * (a.cache.capacity / 16) + block;
     const int was = begun ? *scale : 0;
     float x[S::kPasses][S::kRun], top = 0.0f;
 #pragma unroll
     for (int p = 0; p < S::kPasses; ++p) {
-        const int d = S::kRun * (lane & 3) + 64 * p;
-        load_run<T>(row + d, fresh ? a.cache.width - d : 0, a.aligned, x[p]);
-        top = finite_largest(x[p], top);
+        const int place = place0 + p * S::kRows;
+        const bool fresh = place >= lo && place < hi;
+        load_run<T>(base + int64_t(place - first) * a.ks.s[1], fresh ? a.cache.width - d : 0, a.aligned, x[p]);
     }
+#pragma unroll
+    for (int p = 0; p < S::kPasses; ++p)
+#pragma unroll
+        for (int i = 0; i < S::kRun; ++i) top = fmaxf(top, finite_size(x[p][i]));
     const int byte = min(max(scale_byte(wave_largest(top)), was), kHighScale);
     const float inverse = power(254 - byte), limit = byte == kHighScale ? 240.0f : 448.0f;
-    const bool lower = begun && byte > was && place < lo;
     if (lane == 0) *scale = uint8_t(byte);
-    if (!fresh && !lower) return;
-    uint8_t *const out = a.cache.k + (pair * a.cache.capacity + place) * PAD;
 #pragma unroll
     for (int p = 0; p < S::kPasses; ++p) {
-        uint32_t *const w = reinterpret_cast<uint32_t *>(out + S::kRun * (lane & 3) + 64 * p);
+        const int place = place0 + p * S::kRows;
+        const bool fresh = place >= lo && place < hi;
+        if (!fresh && !(begun && byte > was && place < lo)) continue;
+        uint32_t *const w = reinterpret_cast<uint32_t *>(a.cache.k + (pair * a.cache.capacity + place) * PAD + d);
         uint32_t c[S::kRun / 4];
-        if (fresh) {
 #pragma unroll
-            for (int i = 0; i < S::kRun / 4; ++i) {
+        for (int i = 0; i < S::kRun / 4; ++i) {
+            if (fresh) {
                 float y[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) y[j] = in_range(x[p][4 * i + j], inverse, limit);
                 c[i] = encode4(y[0], y[1], y[2], y[3]);
+            } else {
+                c[i] = lowered4(w[i], byte - was);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::kRun / 4; ++i) c[i] = lowered4(w[i], byte - was);
         }
-        if constexpr (S::kRun == 16)
-            *reinterpret_cast<uint4 *>(w) = uint4{c[0], c[1], c[2], c[3]};
-        else
+        if constexpr (S::kRun == 8)
             *reinterpret_cast<uint2 *>(w) = uint2{c[0], c[1]};
+        else
+            *w = c[0];
     }
 }
 
 template <class T, int PAD>
 __device__ __forceinline__ void append_values(const Kv8AppendArgs &a, int seq, int head, size_t pair, int block, int lo,
                                               int hi, int first) {
-    using S = Share<PAD>;
-    const int lane = threadIdx.x & 63, slot0 = PAD >= 64 ? 0 : 8 * (lane >> 5), place0 = 16 * block + slot0;
+    using S = ValueShare<PAD>;
+    const int lane = threadIdx.x & 63, slot0 = S::kSlots * (lane / S::kLanes), place0 = 16 * block + slot0;
     const bool begun = lo > 16 * block;
     const auto *base = static_cast<const typename T::Raw *>(a.v) + seq * a.vs.s[0] + head * a.vs.s[2];
     uint8_t *const scale = a.cache.vs + pair * (a.cache.capacity / 16) + block;
     const int was = begun ? *scale : 0;
-    float x[S::kPasses][S::kSlots], top = 0.0f;
+    float x[S::kPasses][2][S::kSlots], top = 0.0f;
 #pragma unroll
     for (int p = 0; p < S::kPasses; ++p) {
-        const int d = PAD >= 64 ? lane + 64 * p : lane & 31;
+        const int d = 2 * (lane % S::kLanes) + 128 * p;
 #pragma unroll
         for (int i = 0; i < S::kSlots; ++i) {
             const int place = place0 + i;
-            x[p][i] = place >= lo && place < hi && d < a.cache.width
-                          ? T::to_float(base[int64_t(place - first) * a.vs.s[1] + d])
-                          : 0.0f;
+            const bool fresh = place >= lo && place < hi;
+            float two[2];
+            load_run<T>(base + int64_t(place - first) * a.vs.s[1] + d, fresh ? a.cache.width - d : 0, a.aligned, two);
+            x[p][0][i] = two[0];
+            x[p][1][i] = two[1];
         }
-        top = finite_largest(x[p], top);
     }
+#pragma unroll
+    for (int p = 0; p < S::kPasses; ++p)
+#pragma unroll
+        for (int i = 0; i < S::kSlots; ++i)
+            top = fmaxf(top, fmaxf(finite_size(x[p][0][i]), finite_size(x[p][1][i])));
     const int byte = min(max(scale_byte(wave_largest(top)), was), kHighScale);
     const float inverse = power(254 - byte), limit = byte == kHighScale ? 240.0f : 448.0f;
     if (lane == 0) *scale = uint8_t(byte);
-    const bool whole = lo == 16 * block && hi == 16 * block + 16;
+    const bool whole = lo == 16 * block && hi == 16 * block + 16, lower = begun && byte > was;
 #pragma unroll
-    for (int p = 0; p < S::kPasses; ++p) {
-        const int d = PAD >= 64 ? lane + 64 * p : lane & 31;
-        uint8_t *const out = a.cache.v + ((pair * (a.cache.capacity / 64) + block / 4) * PAD + d) * 64 +
-                             16 * (block % 4) + slot0;
-        uint32_t c[S::kSlots / 4];
+    for (int p = 0; p < S::kPasses; ++p)
 #pragma unroll
-        for (int i = 0; i < S::kSlots / 4; ++i) {
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = in_range(x[p][4 * i + j], inverse, limit);
-            c[i] = encode4(y[0], y[1], y[2], y[3]);
-        }
-        if (!whole) {  // the bytes around the new ones: lowered where older, left where behind
-            uint32_t *const w = reinterpret_cast<uint32_t *>(out);
-            const bool lower = begun && byte > was;
+        for (int q = 0; q < 2; ++q) {
+            const int d = 2 * (lane % S::kLanes) + 128 * p + q;
+            uint32_t *const w = reinterpret_cast<uint32_t *>(
+                a.cache.v + ((pair * (a.cache.capacity / 64) + block / 4) * PAD + d) * 64 + 16 * (block % 4) + slot0);
+            uint32_t c[S::kSlots / 4];
 #pragma unroll
             for (int i = 0; i < S::kSlots / 4; ++i) {
-                const int at = place0 + 4 * i;
-                if (at + 4 <= lo ? !lower : at >= hi) continue;  // nothing of these four changes
-                const uint32_t old = w[i], low = lower ? lowered4(old, byte - was) : old;
-                uint32_t now = 0;
+                float y[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t m = 0xffu << (8 * j);
-                    now |= m & (at + j < lo ? low : at + j < hi ? c[i] : old);
-                }
-                w[i] = now;
+                for (int j = 0; j < 4; ++j) y[j] = in_range(x[p][q][4 * i + j], inverse, limit);
+                c[i] = encode4(y[0], y[1], y[2], y[3]);
             }
-            continue;
+            if (!whole) {  // the bytes around the new ones: lowered where older, left where behind
+#pragma unroll
+                for (int i = 0; i < S::kSlots / 4; ++i) {
+                    const int at = place0 + 4 * i;
+                    if (at + 4 <= lo ? !lower : at >= hi) continue;  // nothing of these four changes
+                    const uint32_t old = w[i], low = lower ? lowered4(old, byte - was) : old;
+                    uint32_t now = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t m = 0xffu << (8 * j);
+                        now |= m & (at + j < lo ? low : at + j < hi ? c[i] : old);
+                    }
+                    w[i] = now;
+                }
+                continue;
+            }
+            if constexpr (S::kSlots == 16)
+                *reinterpret_cast<uint4 *>(w) = uint4{c[0], c[1], c[2], c[3]};
+            else if constexpr (S::kSlots == 8)
+                *reinterpret_cast<uint2 *>(w) = uint2{c[0], c[1]};
+            else
+                *w = c[0];
         }
-        if constexpr (S::kSlots == 16)
-            *reinterpret_cast<uint4 *>(out) = uint4{c[0], c[1], c[2], c[3]};
-        else
-            *reinterpret_cast<uint2 *>(out) = uint2{c[0], c[1]};
-    }
 }
 
-// One wave for the keys or the values of 16 tokens of a head; waves of the
-// touched blocks of every (sequence, head).
+// A wave's part of a launch: the keys or the values of one of the blocks of 16
+// tokens from `first` on.  Four waves of a workgroup take four blocks of a tile,
+// whose lines of 64 values they fill together.
+struct Unit {
+    bool values;
+    uint32_t pair;
+    int block;
+    __device__ __forceinline__ explicit Unit(int tiles) {
+        const uint32_t wave = threadIdx.x >> 6, u = blockIdx.x >> 1;
+        values = blockIdx.x & 1;
+        pair = u / uint32_t(tiles);
+        block = 4 * int(u - pair * uint32_t(tiles)) + int(wave);
+    }
+};
+
+// Of every (sequence, head), the tiles that a run of new tokens touches at most.
 template <class T, int PAD>
-__global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a, int blocks, uint32_t units) {
-    const uint32_t u = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= units) return;
-    const uint32_t rest = u >> 1, pair = rest / uint32_t(blocks);
-    const int seq = int(pair) / a.cache.heads, head = int(pair) - seq * a.cache.heads;
+__global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a, int tiles) {
+    const Unit u(tiles);
+    const int seq = int(u.pair) / a.cache.heads, head = int(u.pair) - seq * a.cache.heads;
     const int length = a.lengths[seq], count = a.counts ? a.counts[seq] : a.count;
     if (length < 0 || length > a.cache.capacity || count < 0 || count > a.count || count > length) return;
-    const int start = length - count, block = start / 16 + int(rest - pair * uint32_t(blocks));
+    const int start = length - count, block = start / 64 * 4 + u.block;
     const int lo = max(start, 16 * block), hi = min(length, 16 * block + 16);
     if (lo >= hi) return;
     const int first = a.absolute ? 0 : start;
-    if (u & 1)
-        append_values<T, PAD>(a, seq, head, pair, block, lo, hi, first);
+    if (u.values)
+        append_values<T, PAD>(a, seq, head, u.pair, block, lo, hi, first);
     else
-        append_keys<T, PAD>(a, seq, head, pair, block, lo, hi, first);
+        append_keys<T, PAD>(a, seq, head, u.pair, block, lo, hi, first);
 }
 
 template <class T, int PAD>
 __device__ __forceinline__ void read_keys(const Kv8ReadArgs &a, int seq, int head, size_t pair, int block, int lo,
                                           int hi) {
-    using S = Share<PAD>;
-    const int lane = threadIdx.x & 63, place = 16 * block + (lane >> 2);
-    if (place < lo || place >= hi) return;
+    using S = KeyShare<T, PAD>;
+    const int lane = threadIdx.x & 63, d = S::kRun * (lane % S::kLanes), place0 = 16 * block + lane / S::kLanes;
     const float scale = power(a.cache.ks[pair * (a.cache.capacity / 16) + block]);
-    const uint8_t *const in = a.cache.k + (pair * a.cache.capacity + place) * PAD;
-    auto *row = static_cast<typename T::Raw *>(a.k) + seq * a.ks.s[0] + int64_t(place - a.first) * a.ks.s[1] +
-                head * a.ks.s[2];
+    auto *base = static_cast<typename T::Raw *>(a.k) + seq * a.ks.s[0] + head * a.ks.s[2] + d;
+    const uint8_t *const in = a.cache.k + pair * a.cache.capacity * PAD + d;
+    uint32_t w[S::kPasses][S::kRun / 4];
 #pragma unroll
     for (int p = 0; p < S::kPasses; ++p) {
-        const int d = S::kRun * (lane & 3) + 64 * p;
-        const uint32_t *const w = reinterpret_cast<const uint32_t *>(in + d);
+        const uint8_t *const row = in + size_t(place0 + p * S::kRows) * PAD;
+        if constexpr (S::kRun == 8) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(row);
+            w[p][0] = v.x;
+            w[p][1] = v.y;
+        } else {
+            w[p][0] = *reinterpret_cast<const uint32_t *>(row);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < S::kPasses; ++p) {
+        const int place = place0 + p * S::kRows;
+        if (place < lo || place >= hi) continue;
         float x[S::kRun];
 #pragma unroll
         for (int i = 0; i < S::kRun / 4; ++i) {
             float y[4];
-            decode4(w[i], y);
+            decode4(w[p][i], y);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[4 * i + j] = y[j] * scale;
         }
-        store_run<T>(row + d, a.cache.width - d, a.aligned, x);
+        store_run<T>(base + int64_t(place - a.first) * a.ks.s[1], a.cache.width - d, a.aligned, x);
     }
 }
 
 template <class T, int PAD>
 __device__ __forceinline__ void read_values(const Kv8ReadArgs &a, int seq, int head, size_t pair, int block, int lo,
                                             int hi) {
-    using S = Share<PAD>;
-    const int lane = threadIdx.x & 63, slot0 = PAD >= 64 ? 0 : 8 * (lane >> 5), place0 = 16 * block + slot0;
+    using S = ValueShare<PAD>;
+    const int lane = threadIdx.x & 63, slot0 = S::kSlots * (lane / S::kLanes), place0 = 16 * block + slot0;
     const float scale = power(a.cache.vs[pair * (a.cache.capacity / 16) + block]);
     auto *base = static_cast<typename T::Raw *>(a.v) + seq * a.vs.s[0] + head * a.vs.s[2];
 #pragma unroll
     for (int p = 0; p < S::kPasses; ++p) {
-        const int d = PAD >= 64 ? lane + 64 * p : lane & 31;
-        if (d >= a.cache.width) continue;
-        const uint32_t *const w = reinterpret_cast<const uint32_t *>(
-            a.cache.v + ((pair * (a.cache.capacity / 64) + block / 4) * PAD + d) * 64 + 16 * (block % 4) + slot0);
+        const int d = 2 * (lane % S::kLanes) + 128 * p;
+        float x[2][S::kSlots];
 #pragma unroll
-        for (int i = 0; i < S::kSlots / 4; ++i) {
-            float y[4];
-            decode4(w[i], y);
+        for (int q = 0; q < 2; ++q) {
+            const uint32_t *const w = reinterpret_cast<const uint32_t *>(
+                a.cache.v + ((pair * (a.cache.capacity / 64) + block / 4) * PAD + d + q) * 64 + 16 * (block % 4) + slot0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int place = place0 + 4 * i + j;
-                if (place >= lo && place < hi)
-                    base[int64_t(place - a.first) * a.vs.s[1] + d] = T::from_float(y[j] * scale);
+            for (int i = 0; i < S::kSlots / 4; ++i) {
+                float y[4];
+                decode4(w[i], y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[q][4 * i + j] = y[j] * scale;
             }
+        }
+#pragma unroll
+        for (int i = 0; i < S::kSlots; ++i) {
+            const int place = place0 + i;
+            const float two[2] = {x[0][i], x[1][i]};
+            if (place >= lo && place < hi)
+                store_run<T>(base + int64_t(place - a.first) * a.vs.s[1] + d, a.cache.width - d, a.aligned, two);
         }
     }
 }
 
 template <class T, int PAD>
-__global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a, int blocks, uint32_t units) {
-    const uint32_t u = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= units) return;
-    const uint32_t rest = u >> 1, pair = rest / uint32_t(blocks);
-    const int seq = int(pair) / a.cache.heads, head = int(pair) - seq * a.cache.heads;
+__global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a, int tiles) {
+    const Unit u(tiles);
+    const int seq = int(u.pair) / a.cache.heads, head = int(u.pair) - seq * a.cache.heads;
     int last = a.first + a.count;
     if (a.lengths) last = min(last, a.lengths[seq]);
-    const int block = a.first / 16 + int(rest - pair * uint32_t(blocks));
+    const int block = a.first / 64 * 4 + u.block;
     const int lo = max(a.first, 16 * block), hi = min(last, 16 * block + 16);
     if (lo >= hi) return;
-    if (u & 1)
-        read_values<T, PAD>(a, seq, head, pair, block, lo, hi);
+    if (u.values)
+        read_values<T, PAD>(a, seq, head, u.pair, block, lo, hi);
     else
-        read_keys<T, PAD>(a, seq, head, pair, block, lo, hi);
+        read_keys<T, PAD>(a, seq, head, u.pair, block, lo, hi);
 }
 
 template <class T, int PAD>
 void launch_append(const Kv8AppendArgs &a, hipStream_t stream) {
-    const int blocks = (a.count + 30) / 16;  // a run of n tokens touches at most so many
-    const uint32_t units = 2u * uint32_t(a.cache.batch) * uint32_t(a.cache.heads) * uint32_t(blocks);
-    hipLaunchKernelGGL((kv8_append_kernel<T, PAD>), dim3((units + 3) / 4), dim3(256), 0, stream, a, blocks, units);
+    const int tiles = (a.count + 126) / 64;  // a run of n tokens touches at most so many
+    hipLaunchKernelGGL((kv8_append_kernel<T, PAD>), dim3(2u * uint32_t(a.cache.batch * a.cache.heads) * uint32_t(tiles)),
+                       dim3(256), 0, stream, a, tiles);
 }
 
 template <class T, int PAD>
 void launch_read(const Kv8ReadArgs &a, hipStream_t stream) {
-    const int blocks = (a.first + a.count + 15) / 16 - a.first / 16;
-    const uint32_t units = 2u * uint32_t(a.cache.batch) * uint32_t(a.cache.heads) * uint32_t(blocks);
-    hipLaunchKernelGGL((kv8_read_kernel<T, PAD>), dim3((units + 3) / 4), dim3(256), 0, stream, a, blocks, units);
+    const int tiles = (a.first + a.count + 63) / 64 - a.first / 64;
+    hipLaunchKernelGGL((kv8_read_kernel<T, PAD>), dim3(2u * uint32_t(a.cache.batch * a.cache.heads) * uint32_t(tiles)),
+                       dim3(256), 0, stream, a, tiles);
 }
 
 template <class T>

@@ -115,7 +115,7 @@ void kv8_append(int device, const Kv8 &cache, Type type, size_t count, const voi
     require(k && v && lengths, "keys, values and lengths must not be null");
     check_aligned(k, type, "keys must be aligned to their type");
     check_aligned(v, type, "values must be aligned to their type");
-    check_grid(double(cache.batch) * cache.heads * (double(count) + 30) / 16);
+    check_grid(2.0 * cache.batch * cache.heads * ((double(count) + 126) / 64));
     const OnDevice on(device);
     kern::Kv8AppendArgs a{};
     a.cache = cache;
@@ -126,7 +126,7 @@ void kv8_append(int device, const Kv8 &cache, Type type, size_t count, const voi
     a.lengths = lengths;
     a.counts = counts;
     a.count = int(count);
-    a.aligned = aligned16(k, ks, type);
+    a.aligned = aligned16(k, ks, type) && aligned16(v, vs, type);
     kern::kv8_append(a, type, stream);
     check(hipGetLastError(), "append launch");
 }
@@ -141,7 +141,7 @@ void kv8_read(int device, const Kv8 &cache, Type type, size_t first, size_t coun
     require(k && v, "keys and values must not be null");
     check_aligned(k, type, "keys must be aligned to their type");
     check_aligned(v, type, "values must be aligned to their type");
-    check_grid(double(cache.batch) * cache.heads * (double(count) + 30) / 16);
+    check_grid(2.0 * cache.batch * cache.heads * ((double(count) + 126) / 64));
     const OnDevice on(device);
     kern::Kv8ReadArgs a{};
     a.cache = cache;
@@ -152,7 +152,7 @@ void kv8_read(int device, const Kv8 &cache, Type type, size_t first, size_t coun
     a.lengths = lengths;
     a.first = int(first);
     a.count = int(count);
-    a.aligned = aligned16(k, ks, type);
+    a.aligned = aligned16(k, ks, type) && aligned16(v, vs, type);
     kern::kv8_read(a, type, stream);
     check(hipGetLastError(), "read launch");
 }

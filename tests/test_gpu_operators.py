@@ -80,6 +80,37 @@ def test_append_writes_the_nearest_codes_and_nothing_else(kind, width, heads, co
     check_append(cache, cache.arrays(), after, L.values(k, kind), L.values(v, kind), lengths, new)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_keys_and_values_have_their_own_strides(kind):
+    """Values one element off their alignment, rows of an odd length, keys in
+    another order and with one head's rows for both (stride 0)."""
+    rng = np.random.default_rng(21)
+    cache = L.Cache(2, 2, 64, 128, rng)
+    lengths, count = np.array([37, 30], np.int32), 30
+    shape = (2, count, 2, 64)
+    k = np.broadcast_to(L.stored(rng.normal(size=(2, count, 1, 64)), kind), shape)
+    v = L.stored(rng.normal(size=shape), kind)
+    odd = np.zeros((2, count, 2, 67), v.dtype)
+    odd[..., 1:65] = v
+    cache.ks[:], cache.vs[:] = 120, 121
+    size = odd.dtype.itemsize
+    with L.Device() as dev:
+        handle = cache.on(dev)
+        kp, vp = dev.put(np.ascontiguousarray(k[:, :, 0])), dev.put(odd)
+        at = dev.put(lengths)
+        G.kv8_append(handle, L.CODES[kind], count, kp, (count * 64, 64, 0), vp + size, (count * 134, 134, 67), at)
+        after = cache.fetch(dev)
+        check_append(cache, cache.arrays(), after, L.values(k, kind), L.values(v, kind), lengths, [count] * 2)
+        outs = [dev.put(L.stored(np.full((2, 20, 2, 67), -77.0), kind)) for _ in range(2)]
+        G.kv8_read(handle, L.CODES[kind], 9, 20, outs[0], (20 * 134, 134, 67), outs[1] + size, (20 * 134, 134, 67))
+        back = [L.values(dev.get(p, (2, 20, 2, 67), L.STORED[kind]), kind) for p in outs]
+    for got, want, off in zip(back, cache.decoded(after), (0, 1)):
+        want = L.values(L.stored(want[:, :, 9:29].transpose(0, 2, 1, 3), kind), kind)
+        assert np.array_equal(got[..., off:off + 64], want, equal_nan=True)
+        rest = np.delete(got, np.s_[off:off + 64], axis=3)
+        assert (rest == -77.0).all()
+
+
 @pytest.mark.parametrize("width", [32, 64])
 def test_append_keeps_every_magnitude(width):
     """Zeros, subnormals, the largest values, infinities and NaN."""
@@ -283,6 +314,27 @@ def test_attention_of_impossible_sequences_is_nan():
         with L.Device() as dev:
             got = attend(dev, cache.on(dev), q, "f32", lengths, counts, 0.125)
         assert np.isnan(got[:3]).all() and np.isfinite(got[3]).all(), count
+
+
+@pytest.mark.parametrize("kind,count", [("f32", 1), ("bf16", 40), ("f16", 40)])
+def test_attention_rows_off_their_alignment(kind, count):
+    rng = np.random.default_rng(31)
+    lengths, width = [70, 128], 64
+    cache = L.Cache(2, 1, width, 128, rng)
+    filled(cache, lengths, rng)
+    q = L.stored(rng.normal(size=(2, count, 2, width)), kind)
+    wide = np.zeros((2, count, 2, 67), q.dtype)
+    wide[..., 1:65] = q
+    size, strides = q.dtype.itemsize, (count * 134, 134, 67)
+    with L.Device() as dev:
+        handle = cache.on(dev)
+        p = dev.put(wide)
+        room = G.kv8_attention_workspace(handle, 2, count)
+        G.kv8_attention(handle, L.CODES[kind], 2, count, p + size, strides, p + size, strides,  # in place
+                        dev.put(np.array(lengths, np.int32)), None, 0.125, dev.alloc(room) if room else None, room)
+        got = L.values(dev.get(p, wide.shape, wide.dtype), kind)
+    assert (got[..., 0] == 0).all() and (got[..., 65:] == 0).all()
+    check_attention(got[..., 1:65], q, kind, cache, lengths, [count] * 2, 0.125)
 
 
 def test_values_of_very_different_scales():
