@@ -31,11 +31,12 @@ EXPORTS = (
     "mg_equation_split", "mg_equation_batch", "mg_text_batch",
     "mg_kv8_sizes", "mg_kv8_append", "mg_kv8_read", "mg_kv8_attention_workspace", "mg_kv8_attention",
     "mg_token_logprobs_workspace", "mg_token_logprobs_noalloc", "mg_token_logprobs_backward_noalloc",
-    "mg_token_logprobs",
+    "mg_token_logprobs", "mg_set_cache",
 )
 
 MG_F32, MG_F16, MG_BF16 = range(3)  # element types of the device operators
 TOP_MAX = 32  # MG_TOP_MAX
+MG_CACHE_F32, MG_CACHE_E4M3 = range(2)  # what a model's KV cache holds
 
 IGNORE_TARGET = 0xFFFFFFFF  # MG_IGNORE_TARGET (src/gpt/mod.rs:26)
 
@@ -164,6 +165,7 @@ def lib():
         "mg_equation_batch": (i, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_double, u64, i, _szp, sz, _u32p,
                                   _u32p]),
         "mg_text_batch": (i, [_u32p, sz, _cfgp, i, sz, sz, u64, _u32p, _u32p]),
+        "mg_set_cache": (i, [vp, i]),
         "mg_kv8_sizes": (i, [_kv8p, _szp, _szp]),
         "mg_kv8_append": (i, [i, _kv8p, i, sz, vp, _strides, vp, _strides, vp, vp, vp]),
         "mg_kv8_read": (i, [i, _kv8p, i, sz, sz, vp, _strides, vp, _strides, vp, vp]),
@@ -408,6 +410,11 @@ class MeshGpt:
     def set_parameters(self, values):
         values = _f32(values)
         _check(lib().mg_set_parameters(self._h, _p(values, _f32p), values.size))
+
+    def set_cache(self, type):
+        """mg_set_cache: MG_CACHE_F32 or MG_CACHE_E4M3; drops the current batch."""
+        _check(lib().mg_set_cache(self._h, type))
+        self._batch = 0
 
     def logits(self, tokens, sequence, last_only=False):
         tokens = _u32(tokens).reshape(-1)

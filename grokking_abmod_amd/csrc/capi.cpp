@@ -202,6 +202,10 @@ int mg_set_parameters(mg_model *model, const float *values, size_t n) {
     });
 }
 
+int mg_set_cache(mg_model *model, int type) {
+    return guarded([&] { model_of(model).set_cache(CacheType(type)); });
+}
+
 int mg_logits(mg_model *model, const uint32_t *tokens, size_t n, size_t sequence, int last_only, float *out,
               size_t out_len) {
     return guarded([&] {

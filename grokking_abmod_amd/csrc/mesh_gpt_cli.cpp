@@ -41,6 +41,7 @@ struct Options {
     float temperature = 0.7f;
     std::string synthetic;
     size_t random_prompt = 0;
+    bool cache8 = false;  // --cache e4m3
     std::string prompt_file;
     std::string init = "reference";
     float init_sigma = 0.5f;
@@ -218,6 +219,11 @@ Options parse(int argc, char **argv) {
         else if (flag == "--temperature") o.temperature = value<float>(it, end, flag);
         else if (flag == "--config") o.synthetic = value<std::string>(it, end, flag);
         else if (flag == "--random-prompt") o.random_prompt = value<size_t>(it, end, flag);
+        else if (flag == "--cache") {
+            const std::string type = value<std::string>(it, end, flag);
+            if (type != "f32" && type != "e4m3") throw Error("unknown cache: " + type + "; use f32 or e4m3");
+            o.cache8 = type == "e4m3";
+        }
         else if (flag == "--prompt-file") o.prompt_file = value<std::string>(it, end, flag);
         else if (flag == "--init") o.init = value<std::string>(it, end, flag);
         else if (flag == "--init-sigma") o.init_sigma = value<float>(it, end, flag);
@@ -270,6 +276,7 @@ const char *kHelp =
     "--seed N              Initialization/data/sampling seed (default: 7)\n"
     "--device N            HIP device ordinal (default: 0)\n"
     "--config NAME         generate: synthetic seeded model: tiny, symbolic, mid, long or high\n"
+    "--cache NAME          generate: the KV cache, f32 or e4m3 (default: f32)\n"
     "--random-prompt LEN   With --config: LEN seeded uniform token ids as the prompt\n"
     "--prompt-file PATH    generate: read the prefix from PATH; with --batch N, N lines of\n"
     "                      equal token length, one prompt per sequence\n"
@@ -910,6 +917,7 @@ int run(int argc, char **argv) {
         }
         MeshGpt model(int(o.device), config, o.seed, o.batch);
         model.set_parameters(parameters.data(), parameters.size());
+        if (o.cache8) model.set_cache(CacheType::E4M3);
         std::vector<std::string> texts;
         if (!o.prompt_file.empty() && prompt.empty()) texts = prompt_lines(o);
         if (prompt.empty() && !o.batch_set) {

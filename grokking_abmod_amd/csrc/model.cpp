@@ -2,6 +2,7 @@
 // decode sequences of kernel launches, and the HIP graph that replays one
 // decode step.
 #include "model.hpp"
+#include "operators.hpp"
 #include "train.hpp"
 
 #include <algorithm>
@@ -150,6 +151,10 @@ struct MeshGpt::Impl {
     // tokens [batch_cap][tcap], lengths, SplitMix64 states and logits.
     size_t batch_cap = 0, tcap = 0;
     DevBuf kc, vc, dx, dx2, dxn, dq, part, dtokens, dlen, drng, dlogits, dflags;
+    // With the cache in 8 bits (set_cache): every layer's codes, and kc and vc
+    // hold two layers, taken in turn, whose rows are on their way to it.
+    bool cache8 = false;
+    DevBuf k8, v8, ks8, vs8;
     // Sampler states and length right after the last prefill (rewind()).
     DevBuf drng_start;
     // Sampler states a persistent decode launch writes (swapped with drng when
@@ -273,6 +278,63 @@ struct MeshGpt::Impl {
 
     size_t layer_cache_elems() const {
         return batch_cap * size_t(shape.H) * cfg.context * size_t(shape.hdp);
+    }
+
+    // Layer l of the 8-bit cache for the sequences from b0 on.
+    size_t capacity8() const { return (cfg.context + kKv8Tile - 1) / kKv8Tile * kKv8Tile; }
+    Kv8 cache8_layer(size_t l, size_t b0, size_t nb) const {
+        Kv8 c{int(nb), shape.H, shape.hd, kv8_pad(shape.hd), int(capacity8()), nullptr, nullptr, nullptr, nullptr};
+        const size_t rows = (l * batch_cap + b0) * size_t(shape.H) * capacity8();
+        c.k = k8.as<uint8_t>() + rows * c.pad;
+        c.v = v8.as<uint8_t>() + rows * c.pad;
+        c.ks = ks8.as<uint8_t>() + rows / kKv8Block;
+        c.vs = vs8.as<uint8_t>() + rows / kKv8Block;
+        return c;
+    }
+    // The rows that a block wrote to `kv` at the last `count` positions of the
+    // sequences go to its layer of the 8-bit cache.
+    void keep8(size_t l, size_t b0, size_t nb, const kern::KvView &kv, const int *len, size_t count) {
+        kern::Kv8AppendArgs a{};
+        a.cache = cache8_layer(l, b0, nb);
+        a.k = kv.k;
+        a.v = kv.v;
+        a.ks = a.vs = Strides{{int64_t(shape.H) * kv.cap * shape.hdp, shape.hdp, int64_t(kv.cap) * shape.hdp}};
+        a.lengths = len;
+        a.count = int(count);
+        a.absolute = 1;
+        a.aligned = shape.hdp % 4 == 0;
+        kern::kv8_append(a, Type::F32, stream);
+    }
+    // attn_decode over the 8-bit cache.
+    void attend8(size_t l, size_t b0, size_t nb, const float *q, const int *len, int nsplit, float *partial) {
+        kern::Kv8AttnArgs a{};
+        a.cache = cache8_layer(l, b0, nb);
+        a.q = q;
+        a.qs = Strides{{shape.W, shape.W, shape.hd}};
+        a.lengths = len;
+        a.count = a.group = a.rows = 1;
+        a.scale_log2 = float(1.4426950408889634 / std::sqrt(double(shape.hd)));
+        a.splits = nsplit;
+        a.part = partial;
+        a.stride = shape.hdp + 2;
+        a.q_aligned = shape.hd % 4 == 0;
+        kern::Kv8Plan plan{};
+        plan.row_tiles = 1;
+        kern::kv8_attention(a, Type::F32, plan, stream);
+    }
+
+    void set_cache(bool eight_bits) {
+        if (eight_bits == cache8) return;
+        if (eight_bits && shape.hd > 256) throw Error("an 8-bit cache needs head widths of at most 256", kUnsupported);
+        activate();
+        sync();
+        drop_graph();
+        for (DevBuf *b : {&kc, &vc, &k8, &v8, &ks8, &vs8}) b->release();
+        const size_t sequences = batch_cap;
+        cache8 = eight_bits;
+        batch_cap = tcap = batch = length = start_length = 0;
+        cached = kNoCache;
+        ensure_decode(std::max<size_t>(sequences, 1), 1);
     }
 
     // Splits per (sequence, head) of decode attention: about 512 workgroups
@@ -631,7 +693,14 @@ struct MeshGpt::Impl {
     void grow_decode(size_t b, size_t t, bool grow_b) {
         if (grow_b) {
             batch_cap = std::max(b, batch_cap);
-            const size_t cache = size_t(cfg.layers) * layer_cache_elems() * 4;
+            const size_t cache = (cache8 ? std::min<size_t>(cfg.layers, 2) : size_t(cfg.layers)) * layer_cache_elems() * 4;
+            if (cache8) {
+                const Kv8 one = cache8_layer(0, 0, batch_cap);
+                k8.ensure(cfg.layers * kv8_code_bytes(one));
+                v8.ensure(cfg.layers * kv8_code_bytes(one));
+                ks8.ensure(cfg.layers * kv8_scale_bytes(one));
+                vs8.ensure(cfg.layers * kv8_scale_bytes(one));
+            }
             kc.ensure(cache);
             vc.ensure(cache);
             // Padding lanes (hd < hdp) are read by vector loads and must stay zero.
@@ -701,7 +770,7 @@ struct MeshGpt::Impl {
     template <class KvOf>
     bool run_blocks(const kern::Rows &rows, int nseq, KvOf kv_of, float *x, float *x2, float *q, float *y,
                     float *xn, bool decode, hipEvent_t *events = nullptr, float *part_base = nullptr,
-                    bool last = false) {
+                    bool last = false, const int *len8 = nullptr, size_t first8 = 0) {
         if (!part_base) part_base = part.as<float>();
         const int nsplit = decode ? splits_for(size_t(rows.rows)) : 0;
         // Prefill attention on the matrix cores (XSA in its epilogue) where the
@@ -795,7 +864,12 @@ struct MeshGpt::Impl {
             else
                 kern::block(a, staged(t, a.wproj != nullptr, a.wq != nullptr), stream);
             if (l == L) break;
-            if (decode) {
+            if (len8) keep8(l, first8, size_t(nseq), kv_of(l), len8, size_t(n));
+            if (decode && len8) {
+                if (events) check(hipEventRecord(events[2 * l], stream), "hipEventRecord");
+                attend8(l, first8, size_t(nseq), q, len8, nsplit, part_base);
+                if (events) check(hipEventRecord(events[2 * l + 1], stream), "hipEventRecord");
+            } else if (decode) {
                 kern::attn_decode(shape, q, kv_of(l), rows.len, rows.rows, nsplit, part_base, stream,
                                   events ? events[2 * l] : nullptr, events ? events[2 * l + 1] : nullptr);
             } else if (compact && l + 1 == L) {
@@ -829,7 +903,7 @@ struct MeshGpt::Impl {
     }
 
     kern::KvView cache_layer(size_t l) const {
-        const size_t off = l * layer_cache_elems();
+        const size_t off = (cache8 ? l % 2 : l) * layer_cache_elems();
         return kern::KvView{kc.as<float>() + off, vc.as<float>() + off, int(cfg.context), keep_rows()};
     }
 
@@ -1306,7 +1380,7 @@ struct MeshGpt::Impl {
     // gpu.rs:2296-2313: the per-row f32 losses summed in f64 on the host.
     size_t allocated_device_bytes() const {
         size_t total = 0;
-        for (const DevBuf *b : {&params, &codes, &E, &Et, &rope, &wdec, &Edec, &q0, &kc, &vc, &dx, &dx2, &dxn, &dq,
+        for (const DevBuf *b : {&params, &codes, &E, &Et, &rope, &wdec, &Edec, &q0, &kc, &vc, &k8, &v8, &ks8, &vs8, &dx, &dx2, &dxn, &dq,
                                 &part, &dtokens, &dlen, &drng, &dlogits, &dflags, &drng_start, &drng_next, &dstage, &pxch, &pabort, &wx,
                                 &wxn, &wq, &wy, &wtok, &wlogits, &wk, &wv, &wsplit, &wlast, &tact, &tgrad, &tm, &tv, &tpart, &tin})
             total += b->bytes;
@@ -1453,7 +1527,7 @@ struct MeshGpt::Impl {
                    },
                    dx.as<float>() + b0 * W, dx2.as<float>() + b0 * W, dq.as<float>() + b0 * W, nullptr,
                    dxn.as<float>() + b0 * W, true, nullptr,
-                   part.as<float>() + slot0 * size_t(shape.H) * (shape.hdp + 2));
+                   part.as<float>() + slot0 * size_t(shape.H) * (shape.hdp + 2), false, cache8 ? rows.len : nullptr, b0);
         kern::head_sample(shape, dxn.as<float>() + b0 * W, int(nb), Et.as<float>(), vpad,
                           dlogits.as<float>() + b0 * shape.V, temperature, drng.as<uint64_t>() + b0,
                           dtokens.as<uint32_t>() + b0 * tcap, int(tcap), dlen.as<int>() + b0, dflags.as<int>(),
@@ -1494,7 +1568,7 @@ struct MeshGpt::Impl {
         known_flags = -1;
         const kern::Rows rows{int(batch), 1, dlen.as<int>(), dtokens.as<uint32_t>(), int(tcap), 0};
         run_blocks(rows, int(batch), [&](size_t l) { return cache_layer(l); }, dx.as<float>(), dx2.as<float>(),
-                   dq.as<float>(), nullptr, dxn.as<float>(), true, events);
+                   dq.as<float>(), nullptr, dxn.as<float>(), true, events, nullptr, false, cache8 ? rows.len : nullptr);
         head_and_sample(dxn.as<float>(), 1, 0);
     }
 
@@ -1534,9 +1608,11 @@ struct MeshGpt::Impl {
     void prefill_step(size_t start, size_t n) {
         ensure_workspace(batch * n, 1, false);
         const kern::Rows rows{int(batch * n), int(n), nullptr, dtokens.as<uint32_t>(), int(tcap), int(start)};
+        // Rows of a window past the context are not cached.
+        const int *len8 = cache8 && start == 0 && n == length ? dlen.as<int>() : nullptr;
         const bool compact = run_blocks(rows, int(batch), [&](size_t l) { return cache_layer(l); }, wx.as<float>(),
                                         nullptr, wq.as<float>(), wy.as<float>(), wxn.as<float>(), false, nullptr,
-                                        nullptr, true);
+                                        nullptr, true, len8);
         head_and_sample(wxn.as<float>(), compact ? 1 : int(n), compact ? 0 : int(n) - 1);
     }
 
@@ -1560,7 +1636,7 @@ struct MeshGpt::Impl {
     }
 
     // Whether tokens can be generated from whole windows in one launch.
-    bool window_usable() const { return use_window && kern::window_supported(shape, cfg.context); }
+    bool window_usable() const { return use_window && !cache8 && kern::window_supported(shape, cfg.context); }
 
     // Whether they are, against the cached decode inside the context and a
     // prefill a token past it.  What the three take is estimated (us a token):
@@ -1669,7 +1745,7 @@ struct MeshGpt::Impl {
     }
 
     bool persistent_usable() const {
-        return persistent_ok && row_decode && kern::persistent_fits(shape, int(batch), device);
+        return persistent_ok && row_decode && !cache8 && kern::persistent_fits(shape, int(batch), device);
     }
 
     // Whether `steps` decode steps should run in the persistent kernel (the
@@ -1790,6 +1866,11 @@ void MeshGpt::parameters(float *out, size_t capacity) const {
 
 void MeshGpt::set_parameters(const float *values, size_t n) { impl_->set_parameters(values, n); }
 
+void MeshGpt::set_cache(CacheType type) {
+    if (type != CacheType::F32 && type != CacheType::E4M3) throw Error("unknown cache type code");
+    impl_->set_cache(type == CacheType::E4M3);
+}
+
 std::vector<float> MeshGpt::logits(const uint32_t *tokens, size_t n, size_t sequence, bool last_only) {
     impl_->cfg.validate_tokens(tokens, n, sequence);
     std::vector<float> out((last_only ? n / sequence : n) * impl_->cfg.vocab_size);
@@ -1907,6 +1988,7 @@ void MeshGpt::prefill(const uint32_t *prompts, size_t batch, size_t prompt_len, 
 
 void MeshGpt::rewind() {
     Impl &m = *impl_;
+    if (m.cache8) throw Error("rewind needs an FP32 cache: later tokens may have rescaled an 8-bit one", kUnsupported);
     if (m.start_length == 0 || m.length < m.start_length || m.start_length > m.cfg.context)
         throw Error("rewind needs a prefilled batch");
     m.activate();

@@ -14,6 +14,10 @@
 
 namespace meshgpt {
 
+// What a model's KV cache holds: FP32, or E4M3 codes with a scale for 16 tokens
+// of a head (operators.hpp).
+enum class CacheType : int { F32 = 0, E4M3 = 1 };
+
 class MeshGpt {
   public:
     // gpu.rs:1718-1771: validates the config, seeds the weights with `seed` and
@@ -26,6 +30,10 @@ class MeshGpt {
     const GptConfig &config() const;
     std::vector<float> parameters() const;                  // gpu.rs:1846-1853
     void set_parameters(const float *values, size_t n);     // gpu.rs:1856-1872
+    // No counterpart in the reference.  Drops the current batch; an 8-bit cache
+    // decodes from quantised keys and values on the per-phase kernels, prompts
+    // attend in FP32.
+    void set_cache(CacheType type);
     // gpu.rs:1875-1887: logits of every row (or only each sequence's last row)
     std::vector<float> logits(const uint32_t *tokens, size_t n, size_t sequence, bool last_only = false);
     // The results of the calls of the same names, written to out, which holds

@@ -712,14 +712,63 @@ int og_token_embeddings(const og_config *c, const float *params, double *out) {
     return 0;
 }
 
+/* A cache rounded to 8 bits (no reference counterpart): exponents of each layer, head and 16
+ * positions for keys and values, and how near any rounding came to a tie (in steps, 0 to 0.5). */
+typedef struct {
+    int *exponent[2];
+    double margin;
+} rounding;
+
+static double e4m3(double x, double *margin) {
+    double size = fabs(x), step = ldexp(1.0, (size < ldexp(1.0, -6) ? -6 : ilogb(size)) - 3);
+    double low = floor(size / step), part = size / step - low;
+    if (fabs(part - 0.5) < *margin) *margin = fabs(part - 0.5);
+    if (part > 0.5 || (part == 0.5 && fmod(low, 2.0) == 1.0)) low += 1.0;
+    return copysign(low * step, x);
+}
+
+/* Rows [lo, hi) of one head's channels (`rows` is W apart) as an 8-bit cache holds them: the
+ * smallest power of two with 448 times which no value of 16 positions is larger; a block begun
+ * before keeps its own or takes a larger one, and its older values round again. */
+static void round_rows(double *rows, size_t W, size_t hd, size_t lo, size_t hi, int *exponent, double *margin) {
+    for (size_t block = lo / 16; block * 16 < hi; ++block) {
+        size_t from = block * 16 > lo ? block * 16 : lo, to = block * 16 + 16 < hi ? block * 16 + 16 : hi;
+        double top = 0.0, exact = 1.0;
+        for (size_t r = from; r < to; ++r)
+            for (size_t i = 0; i < hd; ++i)
+                if (fabs(rows[r * W + i]) > top) top = fabs(rows[r * W + i]);
+        int e = -117;
+        while (e < 120 && top > ldexp(448.0, e)) ++e;
+        double near = fmin(fabs(top / ldexp(448.0, e) - 1.0), fabs(top / ldexp(448.0, e - 1) - 1.0)) * 16.0;
+        if (top > 0.0 && near < *margin) *margin = near;
+        if (from > block * 16) {
+            if (exponent[block] > e) e = exponent[block];
+            for (size_t r = block * 16; r < from; ++r)
+                for (size_t i = 0; i < hd; ++i) rows[r * W + i] = ldexp(e4m3(ldexp(rows[r * W + i], -e), &exact), e);
+        }
+        exponent[block] = e;
+        for (size_t r = from; r < to; ++r)
+            for (size_t i = 0; i < hd; ++i) rows[r * W + i] = ldexp(e4m3(ldexp(rows[r * W + i], -e), margin), e);
+    }
+}
+
+static void round_cache(const og_config *c, rounding *q, size_t layer, double *ck, double *cv, size_t lo, size_t hi) {
+    size_t hd = c->width / c->heads, blocks = (c->context + 15) / 16;
+    double *rows[2] = {ck, cv};
+    for (size_t h = 0; h < c->heads; ++h)
+        for (int m = 0; m < 2; ++m)
+            round_rows(rows[m] + h * hd, c->width, hd, lo, hi, q->exponent[m] + (layer * c->heads + h) * blocks, &q->margin);
+}
+
 /* One pass of reference.rs:154-228 over n rows.  With cache_k/cache_v set, the
  * rows are positions [first_position, first_position+n) of one sequence whose
  * earlier keys/values are already cached (layer-major, context x W each); the
  * result is identical to recomputing the whole prefix because every row's
- * arithmetic depends only on its own inputs and the cached rows. */
+ * arithmetic depends only on its own inputs and the cached rows.  With `round` the cache is
+ * rounded to 8 bits: after a prompt's attention, before a single token's. */
 static void forward(const og_config *c, const float *params, const double *E, const uint32_t *tokens,
                     size_t n, size_t sequence, double *logits, double *hidden, double *cache_k,
-                    double *cache_v, size_t first_position, size_t logit_rows_from) {
+                    double *cache_v, size_t first_position, size_t logit_rows_from, rounding *round) {
     size_t W = c->width, H = c->heads, V = c->vocab_size, L = c->layers;
     size_t A = c->attention_mesh_depth, F = c->ffn_mesh_depth;
     size_t *offsets = (size_t *)malloc(sizeof(size_t) * (1 + 5 * L));
@@ -764,8 +813,10 @@ static void forward(const og_config *c, const float *params, const double *E, co
             double *ck = cache_k + b * c->context * W, *cv = cache_v + b * c->context * W;
             memcpy(ck + first_position * W, k, sizeof(double) * rw);
             memcpy(cv + first_position * W, v, sizeof(double) * rw);
+            if (round && n == 1) round_cache(c, round, b, ck, cv, first_position, first_position + n);
             for (size_t r = 0; r < n; ++r)
                 attention_row(q + r * W, ck, cv, first_position + r, W, H, scores, t1 + r * W);
+            if (round && n > 1) round_cache(c, round, b, ck, cv, first_position, first_position + n);
         } else {
             og_attention(q, k, v, n, W, H, sequence, t1);
         }
@@ -806,7 +857,7 @@ int og_logits(const og_config *c, const float *params, const uint32_t *tokens, s
     if (check_tokens(c, tokens, n, sequence)) return -1;
     double *E = (double *)malloc(sizeof(double) * c->vocab_size * c->width);
     og_token_embeddings(c, params, E);
-    forward(c, params, E, tokens, n, sequence, out, NULL, NULL, NULL, 0, 0);
+    forward(c, params, E, tokens, n, sequence, out, NULL, NULL, NULL, 0, 0, NULL);
     free(E);
     return 0;
 }
@@ -816,7 +867,7 @@ int og_hidden_states(const og_config *c, const float *params, const uint32_t *to
     if (check_tokens(c, tokens, n, sequence)) return -1;
     double *E = (double *)malloc(sizeof(double) * c->vocab_size * c->width);
     og_token_embeddings(c, params, E);
-    forward(c, params, E, tokens, n, sequence, NULL, out, NULL, NULL, 0, 0);
+    forward(c, params, E, tokens, n, sequence, NULL, out, NULL, NULL, 0, 0, NULL);
     free(E);
     return 0;
 }
@@ -907,7 +958,7 @@ int og_generate(const og_config *c, const float *params, const uint32_t *prompt,
     for (size_t step = 0; step < count; ++step) {
         size_t start = len > c->context ? len - c->context : 0;
         size_t window = len - start;
-        forward(c, params, E, out + start, window, window, logits, NULL, NULL, NULL, 0, window - 1);
+        forward(c, params, E, out + start, window, window, logits, NULL, NULL, NULL, 0, window - 1, NULL);
         for (size_t t = 0; t < V; ++t) last[t] = (float)logits[t];
         out[len++] = og_sample(last, V, temperature, &rng);
     }
@@ -917,9 +968,9 @@ int og_generate(const og_config *c, const float *params, const uint32_t *prompt,
     return 0;
 }
 
-int og_generate_cached(const og_config *c, const float *params, const uint32_t *prompt, size_t P,
-                       size_t count, float temperature, uint64_t seed, uint32_t *out,
-                       float *last_logits) {
+static int generate_cached(const og_config *c, const float *params, const uint32_t *prompt, size_t P,
+                           size_t count, float temperature, uint64_t seed, uint32_t *out,
+                           float *last_logits, rounding *round) {
     if (check_generate(c, P, temperature)) return -1;
     if (P + count > c->context) return -1;
     for (size_t i = 0; i < P; ++i)
@@ -938,7 +989,7 @@ int og_generate_cached(const og_config *c, const float *params, const uint32_t *
     for (size_t step = 0; step < count; ++step) {
         /* feed every token not yet cached (the whole prompt on the first step) */
         forward(c, params, E, out + done, len - done, c->context, logits, NULL, ck, cv, done,
-                len - done - 1);
+                len - done - 1, round);
         done = len;
         for (size_t t = 0; t < V; ++t) last[t] = (float)logits[t];
         out[len++] = og_sample(last, V, temperature, &rng);
@@ -950,6 +1001,27 @@ int og_generate_cached(const og_config *c, const float *params, const uint32_t *
     free(logits);
     free(last);
     return 0;
+}
+
+int og_generate_cached(const og_config *c, const float *params, const uint32_t *prompt, size_t P,
+                       size_t count, float temperature, uint64_t seed, uint32_t *out,
+                       float *last_logits) {
+    return generate_cached(c, params, prompt, P, count, temperature, seed, out, last_logits, NULL);
+}
+
+int og_generate_kv8(const og_config *c, const float *params, const uint32_t *prompt, size_t P,
+                    size_t count, float temperature, uint64_t seed, uint32_t *out,
+                    float *last_logits, double *margin) {
+    size_t blocks = (c->context + 15) / 16, n = (size_t)c->layers * c->heads * blocks;
+    rounding round;
+    round.exponent[0] = (int *)calloc(n, sizeof(int));
+    round.exponent[1] = (int *)calloc(n, sizeof(int));
+    round.margin = 0.5;
+    int rc = generate_cached(c, params, prompt, P, count, temperature, seed, out, last_logits, &round);
+    *margin = round.margin;
+    free(round.exponent[0]);
+    free(round.exponent[1]);
+    return rc;
 }
 
 /* ------------------------------------------------------------- datasets */

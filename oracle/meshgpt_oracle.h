@@ -125,6 +125,12 @@ int og_generate_cached(const og_config *c, const float *params, const uint32_t *
                        size_t count, float temperature, uint64_t seed, uint32_t *out,
                        float *last_logits /* V, may be NULL */);
 
+/* The same with the cache rounded to 8 bits (E4M3, a power-of-two scale for 16 positions and a
+ * head); *margin receives how near any rounding came to a tie, in steps (0 to 0.5). */
+int og_generate_kv8(const og_config *c, const float *params, const uint32_t *prompt, size_t P,
+                    size_t count, float temperature, uint64_t seed, uint32_t *out,
+                    float *last_logits /* V, may be NULL */, double *margin);
+
 /* ---- datasets used by the published-number pins ---- */
 /* TextDataset::batch (src/gpt/text.rs:63-108) over an already tokenised corpus */
 int og_text_batch(const uint32_t *tokens, size_t len, int validation, size_t sequence,

@@ -85,6 +85,9 @@ def lib():
             "og_generate_cached": (ctypes.c_int, [cp, _f32p, _u32p, ctypes.c_size_t,
                                                   ctypes.c_size_t, ctypes.c_float, ctypes.c_uint64,
                                                   _u32p, _f32p]),
+            "og_generate_kv8": (ctypes.c_int, [cp, _f32p, _u32p, ctypes.c_size_t,
+                                               ctypes.c_size_t, ctypes.c_float, ctypes.c_uint64,
+                                               _u32p, _f32p, _f64p]),
             "og_sample": (ctypes.c_uint32, [_f32p, ctypes.c_size_t, ctypes.c_float, _u64p]),
             "og_text_batch": (ctypes.c_int, [_u32p, ctypes.c_size_t, ctypes.c_int, ctypes.c_size_t,
                                              ctypes.c_size_t, ctypes.c_uint64, _u32p, _u32p]),
@@ -291,6 +294,18 @@ def generate(c, params, prompt, count, temperature, seed, cached=False):
     if rc:
         raise ValueError("oracle rejected the generation request")
     return out
+
+
+def generate_kv8(c, params, prompt, count, temperature, seed):
+    """generate(cached=True) with the cache rounded to 8 bits: (tokens, the last
+    step's logits, how near any rounding came to a tie in steps)."""
+    params, prompt = f32(params), u32(prompt)
+    out = np.zeros(prompt.size + count, dtype=np.uint32)
+    logits, margin = np.zeros(c.vocab_size, dtype=np.float32), np.zeros(1)
+    if lib().og_generate_kv8(ctypes.byref(c), ptr(params, _f32p), ptr(prompt, _u32p), prompt.size, count, temperature,
+                             seed, ptr(out, _u32p), ptr(logits, _f32p), ptr(margin, _f64p)):
+        raise ValueError("oracle rejected the generation request")
+    return out, logits, float(margin[0])
 
 
 def cpu_generate_f32(c, params, prompts, steps, temperature, seed, threads):

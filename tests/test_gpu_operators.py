@@ -388,12 +388,12 @@ def check_scores(z64, tokens, temperature, top, lp, h, ids, best):
                           (h, want[1], of_sum * (1 + 2 * log_s) + 8 * step * (1 + log_s))):
         same = np.isfinite(w)
         assert np.array_equal(got[~same], w[~same].astype(np.float32), equal_nan=True)
-        assert (np.abs(got - w)[same] <= limit[same]).all(), np.max((np.abs(got - w) / limit)[same])
+        assert (np.abs(got[same] - w[same]) <= limit[same]).all(), np.max(np.abs(got[same] - w[same]) / limit[same])
     if top:
         same = np.isfinite(want[3])
         assert np.array_equal(best[~same], want[3][~same].astype(np.float32), equal_nan=True)
         limit = of_sum[:, None] + 4 * step * np.abs(np.where(same, want[3], 0))
-        assert (np.abs(best - want[3])[same] <= limit[same]).all()
+        assert (np.abs(best[same] - want[3][same]) <= limit[same]).all()
 
 
 SCORES = [

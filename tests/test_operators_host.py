@@ -157,3 +157,11 @@ def test_the_plain_forms():
     assert np.array_equal(np.abs(L.e4m3(x) - x), near)
     for top, e in ((448.0, 0), (449.0, 1), (224.0, -1), (0.0, -117), (1e-45, -117), (3.4e38, 120)):
         assert L.scale_exponent(np.array([top, 0.0, np.nan, np.inf])) == e
+
+
+def test_the_command_line_checks_the_cache():
+    import subprocess
+    r = subprocess.run([G.CLI_PATH, "generate", "--config", "tiny", "--cache", "int4"], capture_output=True, text=True)
+    assert r.returncode != 0 and "unknown cache: int4; use f32 or e4m3" in r.stdout + r.stderr
+    r = subprocess.run([G.CLI_PATH, "--help"], capture_output=True, text=True)
+    assert "--cache NAME" in r.stdout + r.stderr
