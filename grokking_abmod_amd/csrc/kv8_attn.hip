@@ -817,11 +817,16 @@ void attn_of(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) {
 
 }  // namespace
 
-Kv8Plan kv8_plan(const Kv8 &cache, int group, int count) {
+Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count) {
     Kv8Plan p{};
     const int64_t rows = int64_t(count) * group;
     const int pairs = std::max(1, cache.batch * cache.heads);
-    p.wide = rows > 16;
+    // Up to some rows the waves of a workgroup do better to split the keys of 16,
+    // for all that several such workgroups read the same keys (us, split; not): 128 x
+    // 8000 keys of 128, 20 rows BF16 89; 68, F32 90; 109, 64 rows BF16 157; 85, F32
+    // 159; 151; 32 x 4000 keys of 64, 40 rows BF16 17.3; 20.4, F32 20.5; 27.5; 8 x 16000,
+    // 64 rows BF16 19.3; 24.1.
+    p.wide = rows > (cache.pad <= 64 ? 64 : type == Type::F32 ? 32 : 16);
     const int each = p.wide ? 32 * kWaves : 16;
     p.row_tiles = int((rows + each - 1) / each);
     // Shares of the keys, for enough workgroups (two or more a CU are resident)

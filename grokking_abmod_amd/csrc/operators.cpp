@@ -170,7 +170,10 @@ size_t kv8_attention_workspace(const Kv8 &cache, size_t heads, size_t count) {
     const int group = group_of(cache, heads);
     require(double(count) * group < double(1u << 31), "the call is too large for one launch");
     if (cache.batch == 0 || count == 0) return 0;
-    return kern::kv8_plan(cache, group, int(count)).part_floats * 4;
+    size_t floats = 0;
+    for (Type t : {Type::F32, Type::F16, Type::BF16})
+        floats = std::max(floats, kern::kv8_plan(cache, t, group, int(count)).part_floats);
+    return floats * 4;
 }
 
 void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t count, const void *q, Strides qs,
@@ -186,7 +189,7 @@ void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t
     require(q && out && lengths, "queries, output and lengths must not be null");
     check_aligned(q, type, "queries must be aligned to their type");
     check_aligned(out, type, "output must be aligned to its type");
-    const kern::Kv8Plan plan = kern::kv8_plan(cache, group, int(count));
+    const kern::Kv8Plan plan = kern::kv8_plan(cache, type, group, int(count));
     require(plan.part_floats == 0 || (workspace && workspace_bytes >= plan.part_floats * 4),
             "the workspace is too small: mg_kv8_attention_workspace gives its size");
     require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");

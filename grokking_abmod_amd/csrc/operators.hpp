@@ -84,7 +84,7 @@ struct Kv8Plan {
     int row_tiles, splits, chunk;
     size_t part_floats;
 };
-Kv8Plan kv8_plan(const Kv8 &cache, int group, int count);
+Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count);
 void kv8_attention(const Kv8AttnArgs &a, Type type, const Kv8Plan &plan, hipStream_t stream);
 
 struct LogprobArgs {

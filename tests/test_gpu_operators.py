@@ -260,6 +260,9 @@ ATTENTIONS = [
     ("bf16", 32, 2, 2, 640, 300, [300, 640], None, "sthd"),
     ("f16", 31, 1, 1, 64, 20, [20, 64, 50], [20, 19, 1], "sthd"),
     ("bf16", 64, 1, 1, 2048, 1, [2048], None, "sthd"),  # one pair, keys in shares
+    ("f32", 64, 4, 1, 2048, 30, [2048, 70], None, "sthd"),  # several tiles of 16 rows, keys in shares
+    ("bf16", 128, 4, 1, 1088, 30, [1088, 300], [30, 11], "sthd"),
+    ("f16", 32, 1, 1, 1024, 64, [1024, 64], [64, 63], "sthd"),
     ("f32", 64, 1, 1, 1024, 30, [1024, 33], [30, 30], "sthd"),
 ]
 
