@@ -168,7 +168,7 @@ int group_of(const Kv8 &cache, size_t heads) {
 size_t kv8_attention_workspace(const Kv8 &cache, size_t heads, size_t count) {
     check_count(cache, count);
     const int group = group_of(cache, heads);
-    require(double(count) * group < double(1u << 31), "the call is too large for one launch");
+    require(double(count) * group < double(1u << 30), "the call is too large for one launch");
     if (cache.batch == 0 || count == 0) return 0;
     size_t floats = 0;
     for (Type t : {Type::F32, Type::F16, Type::BF16})
@@ -183,8 +183,8 @@ void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t
     check_type(type);
     check_count(cache, count);
     const int group = group_of(cache, heads);
-    require(std::isfinite(scale) && scale > 0.0f, "scale must be finite and positive");
-    require(double(count) * group < double(1u << 31), "the call is too large for one launch");
+    require(std::isfinite(2.0f * scale) && scale > 0.0f, "scale must be finite and positive");
+    require(double(count) * group < double(1u << 30), "the call is too large for one launch");
     if (cache.batch == 0 || count == 0) return;
     require(q && out && lengths, "queries, output and lengths must not be null");
     check_aligned(q, type, "queries must be aligned to their type");
@@ -227,7 +227,8 @@ void check_rows(size_t rows, size_t vocab, size_t top) {
     require(rows < size_t(1) << 31, "rows must stay below 2^31");
 }
 void check_temperature(float temperature) {
-    require(std::isfinite(temperature) && temperature > 0.0f && std::isfinite(1.0f / temperature),
+    // Its inverse is taken in log2 units too.
+    require(std::isfinite(temperature) && temperature > 0.0f && std::isfinite(2.0f / temperature),
             "temperature must be finite and positive");
 }
 size_t stats_bytes(size_t rows, size_t chunks) { return (rows * chunks * 3 * 4 + 15) / 16 * 16; }

@@ -284,8 +284,10 @@ int mg_kv8_sizes(const mg_kv8 *cache, size_t *codes, size_t *scales);
  * ties to even (with 2^120, to at most 240).  A 16-token block that was begun by
  * an earlier call keeps its scale or, where the new tokens need it, takes a
  * larger one: then its older codes are rounded once more.  NaN and infinities
- * become NaN.  A sequence whose length is negative or over the capacity, or
- * whose count is negative or over its length or over `count`, is left as it is. */
+ * become NaN.  The positions before the new tokens have to have been written (a
+ * sequence begins at position 0).  A sequence whose length is negative or over the
+ * capacity, or whose count is negative or over its length or over `count`, is left
+ * as it is. */
 int mg_kv8_append(int device, const mg_kv8 *cache, int type, size_t count, const void *k, const int64_t k_strides[3],
                   const void *v, const int64_t v_strides[3], const int32_t *lengths, const int32_t *counts,
                   void *stream);
@@ -298,7 +300,7 @@ int mg_kv8_read(int device, const mg_kv8 *cache, int type, size_t first, size_t 
  * counts[s] (or `count`) last tokens sees the keys up to its own position, with
  * weights softmax(scale q.k).  `heads` is a multiple of kv_heads; query head h
  * reads cached head h / (heads / kv_heads).  q and out are laid out as the inputs
- * of mg_kv8_append, with `heads` heads; out may be q.  Rows behind a sequence's
+ * of mg_kv8_append, with `heads` heads; out may be q, with its strides.  Rows behind a sequence's
  * count stay as they are.  A NaN or infinity that a row sees makes what depends
  * on it NaN; what it does not see has no effect.  The rows of a sequence whose
  * length or count is impossible (as above) are filled with NaN, all `count` of

@@ -309,10 +309,11 @@ def test_what_a_row_does_not_see_has_no_effect(kind, count):
 
 def test_attention_of_impossible_sequences_is_nan():
     rng = np.random.default_rng(2)
-    for count in (1, 3, 40):
-        lengths, counts = [-1, 129, count - 1, 60], [1, 1, count, count]
-        cache = L.Cache(4, 1, 64, 128, rng)
-        filled(cache, [0, 0, 0, 60], rng)
+    for count, capacity in ((1, 128), (3, 128), (40, 128), (100, 128), (1, 2048), (3, 2048), (200, 1024)):
+        lengths, counts = [-1, capacity + 1, count - 1, count + 60], [1, 1, count, count]
+        cache = L.Cache(4, 1, 64, capacity, rng)
+        lengths[3] = min(lengths[3], capacity)
+        filled(cache, [0, 0, 0, lengths[3]], rng)
         q = rng.normal(size=(4, count, 2, 64)).astype(np.float32)
         with L.Device() as dev:
             got = attend(dev, cache.on(dev), q, "f32", lengths, counts, 0.125)
@@ -419,6 +420,18 @@ def test_log_probabilities_match_64_bits(kind, rows, vocab, stride, temperature,
     z64 = L.values(z, kind)
     check_scores(z64, tokens, temperature, top, lp, h, ids, best)
     assert np.array_equal(stats[:, 0], z64.max(1).astype(np.float32))
+
+
+def test_temperatures_from_the_smallest_to_the_largest():
+    rng = np.random.default_rng(12)
+    z = rng.normal(size=(6, 1500)).astype(np.float32)
+    tokens = z.argmax(1).astype(np.uint32)
+    for temperature in (1e-38, 1e-3, 1e3, 1e38):
+        t = float(np.float32(temperature))
+        with L.Device() as dev:
+            lp, h, _, ids, best, *_ = score(dev, z, "f32", tokens, t, 3)
+        with np.errstate(over="ignore"):
+            check_scores(z.astype(np.float64), tokens, 1 / float(np.float32(1) / np.float32(t)), 3, lp, h, ids, best)
 
 
 @pytest.mark.parametrize("vocab", [70, 1000, 6000, 40000])

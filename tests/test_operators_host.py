@@ -73,7 +73,7 @@ def test_attention_refusals():
     refused("null", call, q=None)
     refused("null", call, out=None)
     refused("null", call, lengths=None)
-    for scale in (0.0, -1.0, math.inf, math.nan):
+    for scale in (0.0, -1.0, math.inf, math.nan, 3e38):
         refused("scale must be finite and positive", call, scale=scale)
     refused("aligned to their type", call, q=257)
     refused("aligned to its type", call, out=258)
@@ -83,6 +83,7 @@ def test_attention_refusals():
     refused("workspace is too small", call, cache=long)
     refused("workspace is too small", call, cache=long, workspace=256, workspace_bytes=15)
     refused("aligned to 16", call, cache=long, workspace=264, workspace_bytes=room)
+    refused("too large", call, cache=cache(kv_heads=1, capacity=1 << 20), heads=65536, count=1 << 20)
     refused("capacity", G.kv8_attention_workspace, c, 4, 129)
     refused("multiple of the cache's heads", G.kv8_attention_workspace, c, 3, 1)
 
@@ -94,7 +95,7 @@ def test_log_probability_refusals():
     refused("1..2\\^24", call, vocab=0)
     refused("1..2\\^24", call, vocab=(1 << 24) + 1, stride=1 << 25)
     refused("stride must be at least", call, stride=99)
-    for temperature in (0.0, -1.0, math.nan, math.inf, 1e-45):
+    for temperature in (0.0, -1.0, math.nan, math.inf, 1e-45, 4e-39):
         refused("temperature must be finite and positive", call, temperature=temperature)
     refused("at most 32", call, top=33, top_tokens=256)
     refused("more alternatives than tokens", call, vocab=5, top=6, top_tokens=256)
