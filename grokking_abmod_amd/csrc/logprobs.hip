@@ -12,7 +12,7 @@
 // maximum reaches it hold any of the best k; those look at their logits again
 // (from the cache) and a few more than k of them are sorted by counting.
 // Reading the logits is what bounds it.  Rows are cut into chunks of at most
-// 128 logits a thread, so that the logits over the bound always fit the list,
+// 64 logits a thread, so that the logits over the bound always fit the list,
 // and shorter ones where there are few rows; a wave then joins a row's chunks.
 // Rows of up to 1024 logits stay in a wave's registers.
 #include <hip/hip_runtime.h>
@@ -28,7 +28,7 @@ namespace meshgpt::kern {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kSmall = 1024;           // logits of a row that one wave holds
+constexpr int kSmall = kSmallVocab;    // logits of a row that one wave holds
 constexpr int kThreadMost = 64;        // logits of a thread's share of a chunk, at most
 constexpr int kList = 2048;            // candidates of a chunk: kTopMax threads' shares
 constexpr int kStaged = 2048;          // candidates that a join holds in LDS
@@ -425,8 +425,8 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LogprobArgs a) {
     }
 }
 
-// Groups of logits a thread takes at a time, and of a row's share a workgroup.
 constexpr int kGradChunk = 16;  // 16-byte groups of a thread
+static_assert(kBlock * kGradChunk * 4 == kGradRun, "a workgroup's logits, in F32");
 
 template <class T>
 __device__ __forceinline__ float grad_of(float x, uint32_t v, const LogprobBackwardArgs &a, uint32_t token, float m,

@@ -76,9 +76,9 @@ void check_aligned(const void *p, Type type, const char *message) {
     require(reinterpret_cast<uintptr_t>(p) % type_size(type) == 0, message);
 }
 
-// Workgroups of a launch.
+// A launch counts its threads, 256 a workgroup, in 32 bits.
 void check_grid(double workgroups) {
-    require(workgroups < double(1u << 31), "the call is too large for one launch");
+    require(workgroups < double(1u << 24), "the call is too large for one launch");
 }
 
 void check_count(const Kv8 &cache, size_t count) {
@@ -195,7 +195,7 @@ void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t
     require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
     const double pairs = double(cache.batch) * cache.heads;
     check_grid((pairs + 7) * plan.splits * plan.row_tiles);
-    check_grid(pairs * double(count) * group + 1);
+    if (plan.splits > 1) check_grid(pairs * double(count) * group * cache.pad / 1024 + 1);
     const OnDevice on(device);
     kern::Kv8AttnArgs a{};
     a.cache = cache;
@@ -225,6 +225,10 @@ void check_rows(size_t rows, size_t vocab, size_t top) {
     require(top <= size_t(kern::kTopMax), "at most 32 alternatives can be asked for");
     require(top <= vocab, "there are more alternatives than tokens");
     require(rows < size_t(1) << 31, "rows must stay below 2^31");
+}
+// Rows of few logits are four to a workgroup.
+double workgroups(size_t rows, size_t vocab, double chunks) {
+    return vocab <= kern::kSmallVocab ? double(rows) / 4 + 1 : double(rows) * chunks;
 }
 void check_temperature(float temperature) {
     // Its inverse is taken in log2 units too.
@@ -260,7 +264,7 @@ void token_logprobs_noalloc(int device, Type type, const void *logits, size_t ro
     require(reinterpret_cast<uintptr_t>(workspace) % 8 == 0, "the workspace must be aligned to 8 bytes");
     kern::LogprobArgs a{};
     kern::logprob_chunks(rows, vocab, a.chunks, a.chunk);
-    check_grid(double(rows) * a.chunks);
+    check_grid(workgroups(rows, vocab, a.chunks));
     const OnDevice on(device);
     a.logits = logits;
     a.rows = rows;
@@ -296,7 +300,7 @@ void token_logprobs_backward_noalloc(int device, Type type, const void *logits, 
     require(!d_entropy || entropy, "the gradient of the entropy needs the entropy");
     check_aligned(logits, type, "logits must be aligned to their type");
     check_aligned(d_logits, type, "the gradient must be aligned to its type");
-    check_grid(double(rows) * (double(vocab) / 4096 + 1));
+    check_grid(workgroups(rows, vocab, std::ceil(double(vocab) / kern::kGradRun)));
     const OnDevice on(device);
     kern::LogprobBackwardArgs a{};
     a.logits = logits;

@@ -117,6 +117,8 @@ struct LogprobBackwardArgs {
 void token_logprobs_backward(const LogprobBackwardArgs &a, Type type, hipStream_t stream);
 
 constexpr int kTopMax = 32;
+constexpr int kSmallVocab = 1024;  // rows of so many logits take a wave, longer ones workgroups
+constexpr int kGradRun = 16384;    // F32 logits of a gradient's workgroup (twice as many in 16 bits)
 
 }  // namespace kern
 

@@ -300,13 +300,15 @@ int mg_kv8_read(int device, const mg_kv8 *cache, int type, size_t first, size_t 
  * counts[s] (or `count`) last tokens sees the keys up to its own position, with
  * weights softmax(scale q.k).  `heads` is a multiple of kv_heads; query head h
  * reads cached head h / (heads / kv_heads).  q and out are laid out as the inputs
- * of mg_kv8_append, with `heads` heads; out may be q, with its strides.  Rows behind a sequence's
- * count stay as they are.  A NaN or infinity that a row sees makes what depends
- * on it NaN; what it does not see has no effect.  The rows of a sequence whose
- * length or count is impossible (as above) are filled with NaN, all `count` of
- * them.  F32 calls keep 24 bits of the queries and probabilities, F16 and BF16
- * calls 16 and 8 of the probabilities; sums are FP32.  The workspace holds
- * mg_kv8_attention_workspace bytes, aligned to 16 (NULL where that is 0). */
+ * of mg_kv8_append, with `heads` heads; out may be q, with its strides.
+ * Rows behind a sequence's count stay as they are.  A NaN or infinity that a row
+ * sees makes what depends on it NaN; what it does not see has no effect.  The rows
+ * of a sequence whose length or count is impossible (as above) are filled with
+ * NaN, all `count` of them.  F32 calls keep 24 bits of the queries and
+ * probabilities, F16 and BF16 calls 16 and 8 of the probabilities; scores, and the
+ * sums of probabilities and of values before they are divided, are FP32 and have
+ * to stay in its range.  The workspace holds mg_kv8_attention_workspace bytes,
+ * aligned to 16 (NULL where that is 0). */
 int mg_kv8_attention_workspace(const mg_kv8 *cache, size_t heads, size_t count, size_t *bytes);
 int mg_kv8_attention(int device, const mg_kv8 *cache, int type, size_t heads, size_t count, const void *q,
                      const int64_t q_strides[3], void *out, const int64_t out_strides[3], const int32_t *lengths,
@@ -322,7 +324,9 @@ int mg_kv8_attention(int device, const mg_kv8 *cache, int type, size_t heads, si
  * top_logprobs may be NULL.  A token of MG_IGNORE_TARGET has log probability 0,
  * one outside the vocabulary NaN.  Logits of -inf are tokens that are not
  * allowed; a row without any other has log probabilities of -inf and entropy 0.
- * A NaN or +inf makes its row NaN, and its alternatives the tokens 0..top-1. */
+ * A NaN or +inf makes its row NaN, and its alternatives the tokens 0..top-1.
+ * The workspace holds mg_token_logprobs_workspace bytes, aligned to 8 (NULL where
+ * that is 0). */
 #define MG_TOP_MAX 32
 int mg_token_logprobs_workspace(size_t rows, size_t vocab, size_t top, size_t *bytes);
 int mg_token_logprobs_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab, size_t stride,

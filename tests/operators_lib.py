@@ -16,7 +16,7 @@ class Device:
     def __init__(self):
         vp, sz, i = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
         self.hip = hip = ctypes.CDLL("libamdhip64.so")
-        for name, args in dict(hipMalloc=[ctypes.POINTER(vp), sz], hipFree=[vp], hipMemcpy=[vp, vp, sz, i],
+        for name, args in dict(hipMalloc=[ctypes.POINTER(vp), sz], hipFree=[vp], hipMemcpy=[vp, vp, sz, i], hipMemset=[vp, i, sz],
                                hipDeviceSynchronize=[], hipGetDevice=[ctypes.POINTER(i)],
                                hipStreamCreate=[ctypes.POINTER(vp)], hipStreamDestroy=[vp], hipStreamSynchronize=[vp],
                                hipStreamBeginCapture=[vp, i], hipStreamEndCapture=[vp, ctypes.POINTER(vp)],
@@ -45,6 +45,11 @@ class Device:
         assert self.hip.hipMalloc(ctypes.byref(p), max(int(nbytes), 16)) == 0
         self.blocks.append(p.value)
         return p.value
+
+    def filled(self, nbytes, byte):
+        p = self.alloc(nbytes)
+        assert self.hip.hipMemset(p, byte, nbytes) == 0
+        return p
 
     def put(self, array, p=None):
         array = np.ascontiguousarray(array)

@@ -357,6 +357,87 @@ def test_values_of_very_different_scales():
 
 # ---- log probabilities ---------------------------------------------------------------
 
+@pytest.mark.parametrize("kind,count", [("f32", 1), ("bf16", 40)])
+def test_a_cache_of_more_than_4_gib(kind, count):
+    """Two sequences of 2^24 tokens of width 256, all of them zeros but the last."""
+    capacity, width = 1 << 24, 256
+    rng = np.random.default_rng(21)
+    new = [L.stored(rng.normal(size=(2, count, 1, width)), kind) for _ in range(2)]
+    q = L.stored(rng.normal(size=(2, count, 1, width)) * 6, kind)
+    at = [capacity, capacity - 70]
+    with L.Device() as dev:
+        codes, scales = 2 * capacity * width, 2 * capacity // 16
+        handle = G.Kv8(2, 1, width, capacity, dev.filled(codes, 0), dev.filled(codes, 0), dev.filled(scales, 60),
+                       dev.filled(scales, 60))
+        st = strides_of(new[0].shape)
+        G.kv8_append(handle, L.CODES[kind], count, dev.put(new[0]), st, dev.put(new[1]), st,
+                     dev.put(np.array(at, np.int32)), None, None)
+        tail = [dev.put(np.full((2, 128, 1, width), 9, np.float32)) for _ in range(2)]
+        st = strides_of((2, 128, 1, width))
+        G.kv8_read(handle, G.MG_F32, capacity - 128, 128, tail[0], st, tail[1], st, None, None)
+        k, v = (dev.get(p, (2, 128, width), np.float32).astype(np.float64) for p in tail)
+        got = attend(dev, handle, q, kind, at, None, 1 / 16)
+    qd = L.values(q, kind)[:, :, 0]
+    for s in range(2):
+        end = at[s] - (capacity - 128)
+        assert not k[s, :end - count].any() and not v[s, :end - count].any() and not v[s, end:].any()
+        for i in range(2):
+            want = L.values(new[i], kind)[s, :, 0]
+            # A block's scale is at most 2^-8 of its largest magnitude, rounded up
+            # to a power of two; a code is off by 2^-4 of it or 2^-10 scales.
+            assert (np.abs((k, v)[i][s, end - count:end] - want) <= np.abs(want) / 16 + np.abs(want).max() * 2.0**-17).all()
+        for i in range(count):
+            last = end - count + i + 1
+            x = k[s, :last] @ qd[s, i] / 16
+            e = np.exp(x)
+            total = at[s] - count + i + 1 - last + e.sum()
+            want, size = e @ v[s, :last] / total, e @ np.abs(v[s, :last]) / total
+            # 256 shares of up to 256 tiles a wave, a rounding of the sums in each,
+            # three in a share's joining: 1024 half steps and some.  A score has 256
+            # terms, and its error counts in the numerator and in the sum.  BF16
+            # calls round each probability by 2^-9 and the output by 2^-8.
+            score = (np.abs(k[s, :last]) @ np.abs(qd[s, i])).max() / 16
+            limit = size * (1200 + 600 * score) * 2.0**-24 + (0 if kind == "f32" else (size + np.abs(want)) / 256)
+            assert (np.abs(got[s, i, 0] - want) <= limit + 2.0**-126).all()
+
+
+def test_calls_on_two_streams_at_once():
+    """Each with a workspace of its own gives what it gives alone."""
+    rng = np.random.default_rng(22)
+    cases = []
+    with L.Device() as dev:
+        for i, (batch, count, rows) in enumerate(((2, 1, 3), (1, 70, 5))):
+            cache = L.Cache(batch, 2, 64, 4096, rng)
+            lengths = [4096 - 100 * s - i for s in range(batch)]
+            filled(cache, lengths, rng)
+            q = L.stored(rng.normal(size=(batch, count, 4, 64)), "bf16")
+            z = rng.normal(size=(rows, 40000)).astype(np.float32)
+            handle, stream, st = cache.on(dev), dev.stream(), strides_of(q.shape)
+            room, more = G.kv8_attention_workspace(handle, 4, count), G.token_logprobs_workspace(rows, 40000, 5)
+            assert room and more
+            p = dict(q=dev.put(q), n=dev.put(np.array(lengths, np.int32)), out=dev.alloc(q.nbytes), space=dev.alloc(room),
+                     z=dev.put(z), t=dev.put(np.arange(rows, dtype=np.uint32)), lp=dev.alloc(4 * rows),
+                     h=dev.alloc(4 * rows), ids=dev.alloc(20 * rows), best=dev.alloc(20 * rows), more=dev.alloc(more))
+
+            def run(p=p, handle=handle, stream=stream, st=st, count=count, rows=rows, room=room, more=more):
+                G.kv8_attention(handle, G.MG_BF16, 4, count, p["q"], st, p["out"], st, p["n"], None, 0.125, p["space"],
+                                room, stream)
+                G.token_logprobs_noalloc(G.MG_F32, p["z"], rows, 40000, 40000, p["t"], 1.0, p["lp"], p["h"], None, 5,
+                                         p["ids"], p["best"], p["more"], more, stream)
+
+            def results(p=p, q=q, rows=rows):
+                return [dev.get(p["out"], q.shape, np.uint16)] + [dev.get(p[n], w * rows, np.uint32)
+                                                                 for n, w in (("lp", 1), ("h", 1), ("ids", 5), ("best", 5))]
+            run()
+            cases.append((run, results, results()))
+        for _ in range(20):
+            for run, _, _ in cases:
+                run()
+        for _, results, alone in cases:
+            for a, b in zip(results(), alone):
+                assert np.array_equal(a, b)
+
+
 def score(dev, z, kind, tokens, temperature, top, stride=None, stream=None):
     rows, vocab = z.shape
     stride = vocab if stride is None else stride
@@ -405,6 +486,7 @@ SCORES = [
     ("f32", 5, 1, 1, 1.0, 1), ("f32", 3, 2, 3, 0.5, 2), ("f32", 70, 256, 256, 0.8, 5), ("bf16", 9, 99, 101, 1.0, 32),
     ("f16", 4, 1000, 1000, 1.5, 20), ("f32", 4, 1025, 1025, 1.0, 32), ("bf16", 3, 5003, 5003, 1.0, 20),
     ("f16", 2, 50257, 50264, 0.7, 5), ("f32", 1, 131072, 131072, 1.0, 32), ("bf16", 3, 131071, 131073, 2.0, 1),
+    ("f32", 2, 1000003, 1000003, 1.0, 32), ("bf16", 1, 1 << 24, 1 << 24, 1.0, 32), ("f16", 12, 200000, 200000, 1.0, 20),
     ("f32", 600, 4099, 4099, 1.0, 3), ("bf16", 1030, 2051, 2051, 1.0, 0), ("f32", 2, 64, 64, 1.0, 0)]
 
 

@@ -98,6 +98,8 @@ def test_log_probability_refusals():
     for temperature in (0.0, -1.0, math.nan, math.inf, 1e-45, 4e-39):
         refused("temperature must be finite and positive", call, temperature=temperature)
     refused("at most 32", call, top=33, top_tokens=256)
+    refused("too large", call, rows=1 << 24, vocab=2000, stride=2000, workspace=256, workspace_bytes=1 << 60)
+    refused("too large", call, rows=(1 << 26) + 4)
     refused("more alternatives than tokens", call, vocab=5, top=6, top_tokens=256)
     refused("null", call, logits=None)
     refused("null", call, tokens=None)
