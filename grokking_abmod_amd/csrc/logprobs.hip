@@ -13,7 +13,7 @@
 // (from the cache) and a few more than k of them are sorted by counting.
 // Reading the logits is what bounds it.  Rows are cut into chunks of at most
 // 64 logits a thread, so that the logits over the bound always fit the list,
-// and shorter ones where there are few rows; a wave then joins a row's chunks.
+// and shorter ones where there are few rows; a second launch joins a row's chunks.
 // Rows of up to 1024 logits stay in a wave's registers.
 #include <hip/hip_runtime.h>
 
@@ -31,7 +31,6 @@ constexpr int kBlock = 256;
 constexpr int kSmall = kSmallVocab;    // logits of a row that one wave holds
 constexpr int kThreadMost = 64;        // logits of a thread's share of a chunk, at most
 constexpr int kList = 2048;            // candidates of a chunk: kTopMax threads' shares
-constexpr int kStaged = 2048;          // candidates that a join holds in LDS
 constexpr uint32_t kIgnore = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -39,6 +38,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // behind them.
 constexpr int kChunkMost = kBlock * (kThreadMost - 16);
 static_assert(kTopMax * kThreadMost <= kList, "the logits over the bound fit the list");
+constexpr int kChunksMost = (1 << 24) / kChunkMost + 1;
 
 // Orders as the floats do, -0 with 0; NaN is not asked for.
 __device__ __forceinline__ uint32_t order(float x) {
@@ -232,15 +232,15 @@ __global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
     };
     if (uint32_t(tid) < body - lo) one(T::to_float(z[lo + tid]));
     if (uint32_t(tid) < hi - tail) one(T::to_float(z[tail + tid]));
-    uint32_t i = tid;
-    for (; i + 3 * kBlock < groups; i += 4 * kBlock) {
-        uint4 w[4];
+    // All groups of a 16-bit chunk are under way at once, half of an F32 one's.
+    for (uint32_t i = tid; i < groups; i += 6 * kBlock) {
+        uint4 w[6];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) w[u] = zg[i + u * kBlock];
+        for (int u = 0; u < 6; ++u) w[u] = zg[min(i + u * kBlock, groups - 1)];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) group(w[u]);
+        for (int u = 0; u < 6; ++u)
+            if (i + u * kBlock < groups) group(w[u]);
     }
-    for (; i < groups; i += kBlock) group(zg[i]);
 
     __shared__ float joined[kBlock / 64][3];
     __shared__ uint32_t tops[kBlock];
@@ -368,60 +368,56 @@ __global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
     if (a.chunks > 1 && tid >= have && tid < top) part[tid] = 0;
 }
 
-// Joins a row's chunks: one wave.  Lane c holds chunks c, c + 64, ... by the
-// first of their candidates that is not taken.
+// Joins a row's chunks: a workgroup, whose waves each have all the sums.  Of the
+// chunks' n-th best candidates, with n * chunks >= top, the (top / n)-th largest
+// bounds the top-th best of the row from below; the few candidates that reach it
+// take their places by counting.
 template <class T>
-__global__ void __launch_bounds__(64) logprob_join_kernel(LogprobArgs a) {
+__global__ void __launch_bounds__(kBlock) logprob_join_kernel(LogprobArgs a) {
     const size_t row = blockIdx.x;
-    const int lane = threadIdx.x;
+    const int tid = threadIdx.x, threads = blockDim.x, n = a.chunks * a.top;
     const float c = a.inv_temperature * kLog2e;
+    const uint64_t *const lists = a.part_top + row * a.chunks * a.top;
+    uint64_t next = tid < n ? lists[tid] : 0;
     Sums t;
-    for (int k = lane; k < a.chunks; k += 64) {
+    for (int k = tid & 63; k < a.chunks; k += 64) {
         const float *p = a.part_stats + (row * a.chunks + k) * 3;
         t.join(p[0], p[1], p[2], c);
     }
     wave_join(t, c);
     float log_sum = 0.0f;
-    if (lane == 0) write_row<T>(a, row, t, log_sum);
+    if (tid == 0) write_row<T>(a, row, t, log_sum);
     if (!a.top) return;
     log_sum = t.s == 0.0f ? -INFINITY : logf(t.s);
-    const uint64_t *const lists = a.part_top + row * a.chunks * a.top;
-    const int n = a.chunks * a.top;
-    if (a.chunks <= 64 && n <= kStaged) {  // a chunk a lane, the lists in LDS
-        __shared__ uint64_t all[kStaged];
-        for (int i = lane; i < n; i += 64) all[i] = lists[i];
-        __syncthreads();
-        int at = lane * a.top;
-        const int end = lane < a.chunks ? at + a.top : at;
-        uint64_t head = at < end ? all[at] : 0;
-        for (int k = 0; k < a.top; ++k) {
-            const uint64_t first = wave_best(head);
-            if (lane == 0) write_top(a, row, k, first, t, log_sum);
-            if (head == first) head = ++at < end ? all[at] : 0;
-        }
+    if (!(t.s == t.s)) {  // a NaN
+        if (tid < a.top) write_top(a, row, tid, 0, t, log_sum);
         return;
     }
-    constexpr int HELD = ((1 << 24) / kChunkMost + 64) / 64;  // chunks of a lane at most
-    uint64_t head[HELD];
-    uint32_t taken[HELD];
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const int k = lane + 64 * i;
-        taken[i] = 0;
-        head[i] = k < a.chunks ? lists[size_t(k) * a.top] : 0;
+    __shared__ uint64_t nth[kChunksMost], list[kTopMax * kTopMax], bound;
+    __shared__ uint32_t found;
+    const int each = (a.top + a.chunks - 1) / a.chunks, most = (a.top + each - 1) / each;
+    for (int k = tid; k < a.chunks; k += threads) nth[k] = lists[size_t(k) * a.top + each - 1];
+    if (tid == 0) bound = found = 0;
+    __syncthreads();
+    for (int k = tid; k < a.chunks; k += threads) {
+        const uint64_t v = nth[k];
+        int before = 0;
+        for (int o = 0; o < a.chunks; ++o) before += nth[o] > v;
+        if (v && before == most - 1) bound = v;  // 0: fewer chunks have as many
     }
-    for (int k = 0; k < a.top; ++k) {
-        uint64_t best = head[0];
-#pragma unroll
-        for (int i = 1; i < HELD; ++i) best = head[i] > best ? head[i] : best;
-        const uint64_t first = wave_best(best);
-        if (lane == 0) write_top(a, row, k, first, t, log_sum);
-#pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (head[i] == first && first) {
-                const int chunk = lane + 64 * i;
-                head[i] = int(++taken[i]) < a.top ? lists[size_t(chunk) * a.top + taken[i]] : 0;
-            }
+    __syncthreads();
+    // At most `most` chunks have more than each - 1 candidates from the bound on.
+    const uint64_t least = bound;
+    for (int i = tid; i < n; i += threads) {
+        if (i != tid) next = lists[i];
+        if (next && next >= least) list[atomicAdd(&found, 1u)] = next;
+    }
+    __syncthreads();
+    for (int j = tid; j < int(found); j += threads) {
+        const uint64_t v = list[j];
+        int before = 0;
+        for (int o = 0; o < int(found); ++o) before += list[o] > v;
+        if (before < a.top) write_top(a, row, before, v, t, log_sum);
     }
 }
 
@@ -517,7 +513,7 @@ void forward_of(const LogprobArgs &a, hipStream_t stream) {
     }
     hipLaunchKernelGGL((logprob_kernel<T>), dim3(uint32_t(a.rows * size_t(a.chunks))), dim3(kBlock), 0, stream, a);
     if (a.chunks > 1)
-        hipLaunchKernelGGL((logprob_join_kernel<T>), dim3(uint32_t(a.rows)), dim3(64), 0, stream, a);
+        hipLaunchKernelGGL((logprob_join_kernel<T>), dim3(uint32_t(a.rows)), dim3(a.top ? kBlock : 64), 0, stream, a);
 }
 
 template <class T>
