@@ -263,12 +263,13 @@ __device__ __forceinline__ void query8(const Kv8AttnArgs &a, const typename T::R
     pieces8<kPieces<T>>(x, piece);
 }
 
-// The key tiles of a share for rows that see `keys` keys.
+// The key tiles of a share for rows that see `keys` keys: equal shares, of a.least
+// tiles or more.
 struct Tiles {
-    int first, last;
+    int first, last, each;
     __device__ __forceinline__ Tiles(const Kv8AttnArgs &a, int split, int keys) {
         const int tiles = (keys + 63) / 64;
-        const int each = a.chunk ? a.chunk / 64 : (tiles + a.splits - 1) / a.splits;
+        each = max(a.least, (tiles + a.splits - 1) / a.splits);
         first = split * each;
         last = min(tiles, first + each);
     }
@@ -753,7 +754,7 @@ kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
 
 // Joins the shares of a row: a lane takes four of its channels.
 template <class T, int PAD>
-__global__ void __launch_bounds__(256) kv8_join_kernel(Kv8AttnArgs a, int64_t total) {
+__global__ void __launch_bounds__(256) kv8_join_kernel(Kv8AttnArgs a, int64_t total, int row_step) {
     constexpr int LANES = PAD / 4;
     const int64_t u = int64_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     const int d = 4 * (threadIdx.x % LANES);
@@ -766,7 +767,9 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8AttnArgs a, int64_t to
     if (s.valid) {
         // The shares of this row's tile of rows reach to the tile's last row;
         // those past this row's own keys hold nothing of it.
-        const int keys = s.length - s.count + r / a.group + 1, used = (keys + a.chunk - 1) / a.chunk;
+        const int begin = s.length - s.count, end = min((r / row_step + 1) * row_step, s.count * a.group);
+        const int each = Tiles(a, 0, begin + (end - 1) / a.group + 1).each;
+        const int used = ((begin + r / a.group + 64) / 64 + each - 1) / each;
         const float *p = a.part + size_t(u) * a.splits * a.stride;
         float m = -INFINITY, l = 0.0f;
         f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
@@ -802,7 +805,7 @@ void launch_attn(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) 
     }
     if (a.out && a.splits > 1)
         hipLaunchKernelGGL((kv8_join_kernel<T, PAD>), dim3(uint32_t((int64_t(pairs) * a.rows * (PAD / 4) + 255) / 256)),
-                           dim3(256), 0, stream, a, int64_t(pairs) * a.rows);
+                           dim3(256), 0, stream, a, int64_t(pairs) * a.rows, plan.wide ? 32 * kWaves : 16);
 }
 
 template <class T>
@@ -829,16 +832,30 @@ Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count) {
     p.wide = rows > (cache.pad <= 64 ? 64 : type == Type::F32 ? 32 : 16);
     const int each = p.wide ? 32 * kWaves : 16;
     p.row_tiles = int((rows + each - 1) / each);
-    // Shares of the keys, for enough workgroups (two or more a CU are resident)
-    // of like length.  Their join is a launch of its own, some 6 us with what it
-    // waits for, so single tokens take 1024 keys or more a share (32 x 8 heads, up
-    // to 576 keys: 10.7 us in one share, 18.8 in shares of 256), prompts, which
-    // work longer on a key, 512 (3 x 8 heads, 1001 rows, up to 1501 keys: 49.6 us in
-    // four shares, 56.3 in three, 66.0 in two).
-    const int64_t groups = int64_t(pairs) * p.row_tiles, least = p.wide ? 512 : 1024, aim = p.wide ? 1024 : 2048;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>({cache.capacity / least, 256, (aim + groups - 1) / groups}));
-    p.chunk = int((cache.capacity + want - 1) / want + 63) / 64 * 64;
-    p.splits = (cache.capacity + p.chunk - 1) / p.chunk;
+    const int64_t groups = int64_t(pairs) * p.row_tiles, tiles = cache.capacity / 64;
+    if (p.wide) {
+        // As many shares as the resident workgroups hold, two a CU, but one of width
+        // 256 and three in F32 of width 64: fewer leave CUs without work, more go
+        // over their rows' states again (us with 2; 3; 4; 5; 6 shares: 128 groups of
+        // BF16 rows of 64, 4000 keys, 46.0; 43.4; 40.8; 41.4; 40.2, of F32 rows
+        // 70.8; 68.9; 61.3; 64.3; 59.5; 152 of F16 rows of 128, 4000 keys, 109; 86;
+        // 102; 90; 93; 64 of BF16 rows of 256, 1500 keys, 54.0; 46.9; 42.9; 54.6; 55.0).
+        // The join is a launch of its own, some 6 us with what it waits for, so a
+        // share is 4 tiles or more, and shares spare 10 or more (32 groups of
+        // BF16 rows of 64, 1024 keys: 22.5 us in one, 19.4 in four; 256 of up to 1000:
+        // 23.3 in one, 28.9 in two).
+        const int64_t resident = 256 * (cache.pad == 256 ? 1 : cache.pad == 64 && type == Type::F32 ? 3 : 2);
+        p.least = 4;
+        p.splits = int(std::max<int64_t>(1, std::min(tiles / p.least, resident / groups)));
+        if (tiles - tiles / p.splits < 10) p.splits = 1;
+    } else {
+        // Single tokens wait for memory, so they take up to 2048 workgroups; but a
+        // share of 1024 keys or more (32 x 8 heads, up to 576 keys: 10.6 us in one
+        // share, 16.6 in shares of 256), of width 256 of 512 (32 pairs of 4000 keys,
+        // F16: 26.3 us, 29.4 in shares of 1024).
+        p.least = cache.pad == 256 ? 8 : 16;
+        p.splits = int(std::max<int64_t>(1, std::min<int64_t>({tiles / p.least, 256, (2048 + groups - 1) / groups})));
+    }
     p.part_floats = p.splits > 1 ? size_t(pairs) * size_t(rows) * size_t(p.splits) * size_t(kv8_part_stride(cache.pad)) : 0;
     return p;
 }

@@ -315,6 +315,7 @@ struct MeshGpt::Impl {
         a.count = a.group = a.rows = 1;
         a.scale_log2 = float(1.4426950408889634 / std::sqrt(double(shape.hd)));
         a.splits = nsplit;
+        a.least = 1;
         a.part = partial;
         a.stride = shape.hdp + 2;
         a.q_aligned = shape.hd % 4 == 0;

@@ -210,7 +210,7 @@ void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t
     a.rows = int(count) * group;
     a.scale_log2 = float(double(scale) * 1.4426950408889634);
     a.splits = plan.splits;
-    a.chunk = plan.chunk;
+    a.least = plan.least;
     a.part = static_cast<float *>(workspace);
     a.stride = kern::kv8_part_stride(cache.pad);
     a.q_aligned = aligned16(q, qs, type);

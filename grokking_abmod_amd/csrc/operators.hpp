@@ -67,7 +67,7 @@ struct Kv8AttnArgs {
     int rows;          // count * group
     float scale_log2;  // of the scores, times log2(e)
     int splits;        // shares of the keys
-    int chunk;         // keys of a share, a multiple of 64 (0: equal shares of each sequence's keys)
+    int least;         // tiles of 64 keys of a share, at least
     // With out null or splits > 1: share s of row r of (sequence, head) p leaves
     // its unnormalised output, maximum (log2 units) and sum at
     // part[((p * rows + r) * splits + s) * stride + {d, stride - 2, stride - 1}].
@@ -81,7 +81,7 @@ inline int kv8_part_stride(int pad) { return pad + 4; }
 // How a call is cut: the rows of a workgroup and the shares of the keys.
 struct Kv8Plan {
     bool wide;  // a wave has rows of its own; else the waves share a workgroup's rows and split its keys
-    int row_tiles, splits, chunk;
+    int row_tiles, splits, least;
     size_t part_floats;
 };
 Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count);

@@ -264,6 +264,9 @@ ATTENTIONS = [
     ("bf16", 128, 4, 1, 1088, 30, [1088, 300], [30, 11], "sthd"),
     ("f16", 32, 1, 1, 1024, 64, [1024, 64], [64, 63], "sthd"),
     ("f32", 64, 1, 1, 1024, 30, [1024, 33], [30, 30], "sthd"),
+    ("bf16", 64, 4, 1, 2048, 200, [2048, 300, 200], [200, 150, 200], "sthd"),  # tiles of 128 rows, keys in shares
+    ("f32", 256, 1, 1, 1024, 140, [1024, 200, 0], [140, 129, 0], "sthd"),
+    ("f16", 128, 1, 1, 1024, 400, [1000, 500], None, "shtd"),
 ]
 
 
