@@ -97,6 +97,8 @@ void kv8_check(const Kv8 &cache) {
     require(cache.batch == 0 || (cache.k && cache.v && cache.ks && cache.vs), "cache buffers must not be null");
     require((reinterpret_cast<uintptr_t>(cache.k) | reinterpret_cast<uintptr_t>(cache.v)) % 16 == 0,
             "cache keys and values must be aligned to 16 bytes");
+    require((reinterpret_cast<uintptr_t>(cache.ks) | reinterpret_cast<uintptr_t>(cache.vs)) % 4 == 0,
+            "cache scales must be aligned to 4 bytes");
 }
 
 size_t kv8_code_bytes(const Kv8 &cache) {

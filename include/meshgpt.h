@@ -265,8 +265,8 @@ enum { MG_F32 = 0, MG_F16 = 1, MG_BF16 = 2 };
  *   v_scale  the same                                  of a head: scale 2^(b - 127)
  * P is the head width (1..256) padded to 32, 64, 128 or 256; padded channels of
  * written tokens hold 0.  capacity is a multiple of 64; k and v are aligned to
- * 16 bytes.  The buffers need no clearing: positions behind a sequence's length
- * are never used, whatever they hold. */
+ * 16 bytes, k_scale and v_scale to 4.  The buffers need no clearing: positions
+ * behind a sequence's length are never used, whatever they hold. */
 typedef struct {
     uint32_t batch, kv_heads, head_width, capacity;
     uint8_t *k, *v, *k_scale, *v_scale;

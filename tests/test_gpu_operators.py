@@ -344,6 +344,38 @@ def test_attention_rows_off_their_alignment(kind, count):
     check_attention(got[..., 1:65], q, kind, cache, lengths, [count] * 2, 0.125)
 
 
+@pytest.mark.parametrize("kind,count,capacity", [("f32", 1, 128), ("bf16", 1, 2048), ("f16", 70, 128), ("f32", 140, 2048)])
+def test_attention_over_its_queries(kind, count, capacity):
+    """The output in the queries' place is that of one beside them."""
+    rng = np.random.default_rng(23)
+    lengths = [capacity, max(count, capacity - 77)]
+    cache = L.Cache(2, 2, 64, capacity, rng)
+    filled(cache, lengths, rng)
+    q = L.stored(rng.normal(size=(2, count, 4, 64)), kind)
+    with L.Device() as dev:
+        handle, st = cache.on(dev), strides_of(q.shape)
+        beside = attend(dev, handle, q, kind, lengths, None, 0.125)
+        room, at = G.kv8_attention_workspace(handle, 4, count), dev.put(q)
+        G.kv8_attention(handle, L.CODES[kind], 4, count, at, st, at, st, dev.put(np.array(lengths, np.int32)), None, 0.125,
+                        dev.alloc(room) if room else None, room)
+        assert np.array_equal(L.values(dev.get(at, q.shape, L.STORED[kind]), kind), beside)
+
+
+def test_queries_that_heads_and_tokens_share():
+    """Strides of 0 for heads and tokens: one query a sequence."""
+    rng = np.random.default_rng(24)
+    cache = L.Cache(2, 2, 64, 192, rng)
+    filled(cache, [192, 100], rng)
+    q = rng.normal(size=(2, 1, 1, 64)).astype(np.float32)
+    with L.Device() as dev:
+        handle, n = cache.on(dev), dev.put(np.array([192, 100], np.int32))
+        whole = np.ascontiguousarray(np.broadcast_to(q, (2, 20, 4, 64)))
+        want = attend(dev, handle, whole, "f32", [192, 100], None, 0.125)
+        out = dev.alloc(whole.nbytes)
+        G.kv8_attention(handle, G.MG_F32, 4, 20, dev.put(q), (64, 0, 0), out, strides_of(whole.shape), n, None, 0.125)
+        assert np.array_equal(dev.get(out, whole.shape, np.float32), want)
+
+
 def test_values_of_very_different_scales():
     """Blocks 2^200 apart: a block's scale meets its own probabilities."""
     rng = np.random.default_rng(4)
@@ -613,6 +645,40 @@ def test_the_gradient_is_that_of_the_forward_pass():
             # size 4 off by 40 roundings over 2 step.
             limit = 4 * step**2 / 6 + 2 * 4 * 40 * 2.0**-24 / (2 * step)
             assert np.abs(got - slope).max() <= limit
+
+
+def test_a_scored_step_and_its_gradient_as_a_graph():
+    """Rows in several chunks, replayed with new logits in the same buffers, with
+    eager calls of other data between the replays."""
+    rng = np.random.default_rng(25)
+    rows, vocab = 6, 30000
+    t = rng.integers(0, vocab, rows).astype(np.uint32)
+    g, gh = (rng.normal(size=rows).astype(np.float32) for _ in range(2))
+    with L.Device() as dev:
+        stream = dev.stream()
+        room = G.token_logprobs_workspace(rows, vocab, 4)
+        assert room
+        zp, dz, tp, gp, ghp = dev.alloc(4 * rows * vocab), dev.alloc(4 * rows * vocab), dev.put(t), dev.put(g), dev.put(gh)
+        lp, h, st, ids, best, space = (dev.alloc(n) for n in (4 * rows, 4 * rows, 8 * rows, 16 * rows, 16 * rows, room))
+
+        def enqueue(on=stream, z=zp, more=space):
+            G.token_logprobs_noalloc(G.MG_F32, z, rows, vocab, vocab, tp, 0.9, lp, h, st, 4, ids, best, more, room, on)
+            G.token_logprobs_backward_noalloc(G.MG_F32, z, rows, vocab, vocab, tp, 0.9, st, h, gp, ghp, dz, vocab, on)
+
+        def results():
+            return [dev.get(p, n, np.uint32) for p, n in ((lp, rows), (h, rows), (st, 2 * rows), (ids, 4 * rows),
+                                                         (best, 4 * rows), (dz, rows * vocab))]
+        step = dev.graph(stream, enqueue)
+        other, spare = dev.put(rng.normal(size=(rows, vocab)).astype(np.float32)), dev.alloc(room)
+        for i in range(4):
+            z = (rng.normal(size=(rows, vocab)) * (1 + i)).astype(np.float32)
+            dev.put(z, zp)
+            dev.replay(step, stream)
+            replayed = results()
+            enqueue(None, other, spare)
+            enqueue(None)
+            for a, b in zip(replayed, results()):
+                assert np.array_equal(a, b), i
 
 
 def test_host_arrays_give_the_same():

@@ -12,7 +12,7 @@ import operators_lib as L
 S = (64, 64, 64)
 
 
-def cache(batch=2, kv_heads=2, head_width=64, capacity=128, k=256, v=256, ks=1, vs=1):
+def cache(batch=2, kv_heads=2, head_width=64, capacity=128, k=256, v=256, ks=256, vs=256):
     return G.Kv8(batch, kv_heads, head_width, capacity, k, v, ks, vs)
 
 
@@ -28,13 +28,13 @@ def refused(match, f, *args, **kw):
     (dict(kv_heads=0), "heads must be in 1..4096"), (dict(kv_heads=5000), "heads must be in 1..4096"),
     (dict(batch=(1 << 24) + 1), "out of range"), (dict(batch=1 << 24, kv_heads=4096), "below 2\\^31"),
     (dict(k=0), "must not be null"), (dict(vs=0), "must not be null"), (dict(k=264), "aligned to 16"),
-    (dict(v=257), "aligned to 16")])
+    (dict(v=257), "aligned to 16"), (dict(ks=257), "aligned to 4"), (dict(vs=258), "aligned to 4")])
 def test_caches_that_cannot_be(kw, match):
     c = cache(**kw)
     refused(match, G.kv8_append, c, G.MG_F32, 1, 256, S, 256, S, 256)
     refused(match, G.kv8_read, c, G.MG_F32, 0, 1, 256, S, 256, S)
     refused(match, G.kv8_attention, c, G.MG_F32, 5000 if "kv_heads" in kw else 2, 1, 256, S, 256, S, 256, None, 1.0)
-    if not {"k", "v", "vs"} & set(kw):
+    if not {"k", "v", "ks", "vs"} & set(kw):
         refused(match, G.kv8_sizes, c)
 
 
