@@ -18,8 +18,7 @@
 // 128001 logits with 20 alternatives take 65 us (3.9 TB/s) and 5.3 us for the join,
 // 32 F32 rows of 256 with 5 take 5 us.
 //
-// The gradient reads and writes each logit once: 4096 BF16 rows of 50257 logits
-// take 169 to 191 us (4.3 to 4.9 TB/s).
+// The gradient reads and writes each logit once, which bounds it.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -426,8 +425,13 @@ __global__ void __launch_bounds__(kBlock) logprob_join_kernel(LogprobArgs a) {
     }
 }
 
-constexpr int kGradChunk = 16;  // 16-byte groups of a thread
-static_assert(kBlock * kGradChunk * 4 == kGradRun, "a workgroup's logits, in F32");
+constexpr int kGradGroups = 3;  // 16-byte groups of a lane
+template <class T>
+constexpr size_t kLine = 128 / sizeof(typename T::Raw);
+// Logits of a share at most, beside what moves a row's shares to whole lines.
+template <class T>
+constexpr size_t kGradMost = 64 * kGradGroups * T::kGroup - kLine<T>;
+static_assert(kGradMost<F32> == kGradRun && kGradMost<BF16> >= kGradRun, "as the launch's size is checked");
 
 template <class T>
 __device__ __forceinline__ float grad_of(float x, uint32_t v, const LogprobBackwardArgs &a, uint32_t token, float m,
@@ -440,13 +444,19 @@ __device__ __forceinline__ float grad_of(float x, uint32_t v, const LogprobBackw
     return d * a.inv_temperature;
 }
 
+// A wave's share of a row: `size` logits, all under way at once.  Shares end at
+// 128-byte lines.  Short shares keep what is read and written at a time close
+// together in memory: 4096 BF16 rows of 50257 take 192 us with 32768 logits a
+// workgroup, 146 with 2048 a wave, 140 with 1536 (5.9 TB/s), 147 with 1024.
 template <class T>
-__global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwardArgs a, uint32_t chunks) {
+__global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwardArgs a, uint32_t shares, uint32_t size) {
     using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
-    const int tid = threadIdx.x;
-    const size_t row = blockIdx.x / chunks;
-    const uint32_t chunk = blockIdx.x - uint32_t(row) * chunks;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t unit = blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const size_t row = unit / shares;
+    if (row >= a.rows) return;
+    const uint32_t share = unit - uint32_t(row) * shares;
     const auto *z = static_cast<const Raw *>(a.logits) + row * a.stride;
     auto *out = static_cast<Raw *>(a.d_logits) + row * a.d_stride;
     const uint32_t token = a.tokens ? a.tokens[row] : kIgnore;
@@ -458,52 +468,34 @@ __global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwar
     auto grad = [&](float x, uint32_t v) {
         return none ? 0.0f : grad_of<T>(x, v, a, token, m, log_sum, g, h, entropy);
     };
-    const uint32_t size = kBlock * kGradChunk * G, lo = chunk * size;
-    const uint32_t hi = uint32_t(min(size_t(lo) + size, a.vocab));
-    const uint32_t in_off = uint32_t(reinterpret_cast<uintptr_t>(z + lo) % 16);
-    if (in_off != uint32_t(reinterpret_cast<uintptr_t>(out + lo) % 16)) {  // no common 16-byte groups
-        for (uint32_t v = lo + tid; v < hi; v += kBlock) out[v] = T::from_float(grad(T::to_float(z[v]), v));
+    const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(z) % 128 / sizeof(Raw));
+    const uint32_t lo = share ? share * size - shift : 0;
+    const uint32_t hi = share + 1 == shares ? uint32_t(a.vocab) : (share + 1) * size - shift;
+    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(z + lo) % 16);
+    if (off != uint32_t(reinterpret_cast<uintptr_t>(out + lo) % 16)) {  // no common 16-byte groups
+        for (uint32_t v = lo + lane; v < hi; v += 64) out[v] = T::from_float(grad(T::to_float(z[v]), v));
         return;
     }
-    const uint32_t body = min(hi, lo + (G - in_off / uint32_t(sizeof(Raw))) % G), groups = (hi - body) / G,
+    const uint32_t body = min(hi, lo + (G - off / uint32_t(sizeof(Raw))) % G), groups = (hi - body) / G,
                    tail = body + groups * G;
-    if (uint32_t(tid) < body - lo) out[lo + tid] = T::from_float(grad(T::to_float(z[lo + tid]), lo + tid));
-    if (uint32_t(tid) < hi - tail) out[tail + tid] = T::from_float(grad(T::to_float(z[tail + tid]), tail + tid));
+    if (lane < body - lo) out[lo + lane] = T::from_float(grad(T::to_float(z[lo + lane]), lo + lane));
+    if (lane < hi - tail) out[tail + lane] = T::from_float(grad(T::to_float(z[tail + lane]), tail + lane));
+    if (groups == 0) return;
     const uint4 *const zg = reinterpret_cast<const uint4 *>(z + body);
     uint4 *const og = reinterpret_cast<uint4 *>(out + body);
-    auto one = [&](uint4 w, uint32_t i) {
+    uint4 w[kGradGroups];
+#pragma unroll
+    for (int u = 0; u < kGradGroups; ++u) w[u] = zg[min(lane + 64 * u, groups - 1)];
+#pragma unroll
+    for (int u = 0; u < kGradGroups; ++u) {
+        const uint32_t i = lane + 64 * u;
+        if (i >= groups) continue;
         float x[G];
-        T::unpack(w, x);
+        T::unpack(w[u], x);
 #pragma unroll
         for (int j = 0; j < G; ++j) x[j] = grad(x[j], body + i * G + j);
         og[i] = T::pack(x);
-    };
-    uint32_t i = tid;
-    for (; i + 3 * kBlock < groups; i += 4 * kBlock) {
-        uint4 w[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) w[u] = zg[i + u * kBlock];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) one(w[u], i + u * kBlock);
     }
-    for (; i < groups; i += kBlock) one(zg[i], i);
-}
-
-// Short rows: a wave a row.
-template <class T>
-__global__ void __launch_bounds__(kBlock) logprob_backward_small_kernel(LogprobBackwardArgs a) {
-    const size_t row = size_t(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
-    if (row >= a.rows) return;
-    const auto *z = static_cast<const typename T::Raw *>(a.logits) + row * a.stride;
-    auto *out = static_cast<typename T::Raw *>(a.d_logits) + row * a.d_stride;
-    const uint32_t token = a.tokens ? a.tokens[row] : kIgnore;
-    const float m = a.stats[2 * row], log_sum = a.stats[2 * row + 1];
-    float g = a.d_logprob && token != kIgnore ? a.d_logprob[row] : 0.0f;
-    if (token != kIgnore && token >= a.vocab) g = __builtin_nanf("");
-    const float h = a.d_entropy ? a.d_entropy[row] : 0.0f, entropy = a.d_entropy ? a.entropy[row] : 0.0f;
-    for (uint32_t v = threadIdx.x & 63; v < a.vocab; v += 64)
-        out[v] = T::from_float(m == -INFINITY ? 0.0f
-                                              : grad_of<T>(T::to_float(z[v]), v, a, token, m, log_sum, g, h, entropy));
 }
 
 template <class T>
@@ -523,14 +515,13 @@ void forward_of(const LogprobArgs &a, hipStream_t stream) {
 
 template <class T>
 void backward_of(const LogprobBackwardArgs &a, hipStream_t stream) {
-    if (a.vocab <= size_t(kSmall)) {
-        hipLaunchKernelGGL((logprob_backward_small_kernel<T>), dim3(uint32_t((a.rows + kBlock / 64 - 1) / (kBlock / 64))),
-                           dim3(kBlock), 0, stream, a);
-        return;
-    }
-    const size_t size = size_t(kBlock) * kGradChunk * T::kGroup, chunks = (a.vocab + size - 1) / size;
-    hipLaunchKernelGGL((logprob_backward_kernel<T>), dim3(uint32_t(a.rows * chunks)), dim3(kBlock), 0, stream, a,
-                       uint32_t(chunks));
+    // Equal shares, of whole lines; the first is shorter by what its row lies off a
+    // line, the last may be longer by as much.
+    const size_t parts = (a.vocab + kGradMost<T> - 1) / kGradMost<T>, even = (a.vocab + parts - 1) / parts;
+    const size_t size = (even + kLine<T> - 1) / kLine<T> * kLine<T>, shares = (a.vocab + size - 1) / size;
+    const size_t units = a.rows * shares;
+    hipLaunchKernelGGL((logprob_backward_kernel<T>), dim3(uint32_t((units + kBlock / 64 - 1) / (kBlock / 64))), dim3(kBlock),
+                       0, stream, a, uint32_t(shares), uint32_t(size));
 }
 
 }  // namespace

@@ -228,10 +228,6 @@ void check_rows(size_t rows, size_t vocab, size_t top) {
     require(top <= vocab, "there are more alternatives than tokens");
     require(rows < size_t(1) << 31, "rows must stay below 2^31");
 }
-// Rows of few logits are four to a workgroup.
-double workgroups(size_t rows, size_t vocab, double chunks) {
-    return vocab <= kern::kSmallVocab ? double(rows) / 4 + 1 : double(rows) * chunks;
-}
 void check_temperature(float temperature) {
     // Its inverse is taken in log2 units too.
     require(std::isfinite(temperature) && temperature > 0.0f && std::isfinite(2.0f / temperature),
@@ -266,7 +262,7 @@ void token_logprobs_noalloc(int device, Type type, const void *logits, size_t ro
     require(reinterpret_cast<uintptr_t>(workspace) % 8 == 0, "the workspace must be aligned to 8 bytes");
     kern::LogprobArgs a{};
     kern::logprob_chunks(rows, vocab, a.chunks, a.chunk);
-    check_grid(workgroups(rows, vocab, a.chunks));
+    check_grid(vocab <= kern::kSmallVocab ? double(rows) / 4 + 1 : double(rows) * a.chunks);  // small: a wave a row
     const OnDevice on(device);
     a.logits = logits;
     a.rows = rows;
@@ -302,7 +298,7 @@ void token_logprobs_backward_noalloc(int device, Type type, const void *logits, 
     require(!d_entropy || entropy, "the gradient of the entropy needs the entropy");
     check_aligned(logits, type, "logits must be aligned to their type");
     check_aligned(d_logits, type, "the gradient must be aligned to its type");
-    check_grid(workgroups(rows, vocab, std::ceil(double(vocab) / kern::kGradRun)));
+    check_grid(double(rows) * std::ceil(double(vocab) / kern::kGradRun) / 4 + 1);
     const OnDevice on(device);
     kern::LogprobBackwardArgs a{};
     a.logits = logits;

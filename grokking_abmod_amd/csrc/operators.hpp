@@ -118,7 +118,7 @@ void token_logprobs_backward(const LogprobBackwardArgs &a, Type type, hipStream_
 
 constexpr int kTopMax = 32;
 constexpr int kSmallVocab = 1024;  // rows of so many logits take a wave, longer ones workgroups
-constexpr int kGradRun = 16384;    // F32 logits of a gradient's workgroup (twice as many in 16 bits)
+constexpr int kGradRun = 736;      // F32 logits of a gradient's wave (twice as many in 16 bits)
 
 }  // namespace kern
 

@@ -580,11 +580,14 @@ def test_log_probabilities_of_masked_and_odd_rows(vocab):
 
 
 GRADIENTS = [("f32", 5, 1, 1, 1.0), ("f32", 70, 99, 99, 0.8), ("bf16", 9, 1001, 1003, 1.0), ("f16", 4, 1024, 1024, 1.5),
-             ("f32", 3, 1025, 1027, 1.0), ("bf16", 3, 40001, 40001, 1.0), ("f16", 2, 33000, 33008, 0.7)]
+             ("f32", 3, 1025, 1027, 1.0), ("bf16", 3, 40001, 40001, 1.0), ("f16", 2, 33000, 33008, 0.7),
+             # about the ends of a wave's share, rows off their lines by any amount
+             ("f32", 40, 736, 737, 1.0), ("f32", 40, 737, 737, 1.0), ("f32", 40, 1473, 1475, 1.0),
+             ("bf16", 70, 1472, 1473, 1.0), ("bf16", 70, 1473, 1473, 1.0), ("f16", 70, 2945, 2951, 1.0)]
 
 
 @pytest.mark.parametrize("kind,rows,vocab,stride,temperature", GRADIENTS)
-@pytest.mark.parametrize("which", ["both", "logprob", "entropy", "in place"])
+@pytest.mark.parametrize("which", ["both", "logprob", "entropy", "in place", "apart"])
 def test_the_gradient_matches_64_bits(kind, rows, vocab, stride, temperature, which):
     rng = np.random.default_rng(vocab + rows)
     z = rng.normal(size=(rows, vocab)) * 3
@@ -598,11 +601,15 @@ def test_the_gradient_matches_64_bits(kind, rows, vocab, stride, temperature, wh
     z64 = L.values(z, kind)
     with L.Device() as dev:
         lp, h, stats, _, _, zp, (_, hp, sp) = score(dev, z, kind, tokens, temperature, 0, stride)
-        out = zp if which == "in place" else dev.put(L.stored(np.full((rows, stride), -77.0), kind))
+        # Apart: the gradient has a stride and an alignment of its own.
+        wide, off = (stride + 3, 1) if which == "apart" else (stride, 0)
+        out = zp if which == "in place" else dev.put(L.stored(np.full(rows * wide + off, -77.0), kind))
         G.token_logprobs_backward_noalloc(L.CODES[kind], zp, rows, vocab, stride, dev.put(tokens), temperature, sp,
                                           hp if which != "logprob" else None, dev.put(g) if which != "entropy" else None,
-                                          dev.put(e) if which != "logprob" else None, out, stride)
-        got = L.values(dev.get(out, (rows, stride), L.STORED[kind]), kind)
+                                          dev.put(e) if which != "logprob" else None, out + off * z.itemsize, wide)
+        got = L.values(dev.get(out, rows * wide + off, L.STORED[kind]), kind)
+    assert which == "in place" or (got[:off] == -77.0).all()
+    got = got[off:].reshape(rows, wide)
     if which != "in place":
         assert (got[:, vocab:] == -77.0).all()
     gg, ee = g * (which != "entropy"), e * (which != "logprob")
