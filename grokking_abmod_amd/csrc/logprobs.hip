@@ -220,30 +220,36 @@ __global__ void __launch_bounds__(kBlock) logprob_kernel(LogprobArgs a) {
         if (x > t.m) t.raise(x, c);
         add(x, fmaxf(t.m, -FLT_MAX), c, t.s, t.a);
     };
-    auto group = [&](uint4 w) {
-        float x[G];
-        T::unpack(w, x);
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < G; ++j) top = fmaxf(top, x[j]);
-        if (top > t.m) t.raise(top, c);
-        const float base = fmaxf(t.m, -FLT_MAX);
-        float s = 0.0f, q = 0.0f;
-#pragma unroll
-        for (int j = 0; j < G; ++j) add(x[j], base, c, s, q);
-        t.s += s;
-        t.a += q;
-    };
     if (uint32_t(tid) < body - lo) one(T::to_float(z[lo + tid]));
     if (uint32_t(tid) < hi - tail) one(T::to_float(z[tail + tid]));
-    // All groups of a 16-bit chunk are under way at once, half of an F32 one's.
+    // All groups of a 16-bit chunk are under way at once, half of an F32 one's, and
+    // their maximum comes first, so that sums are raised once.
     for (uint32_t i = tid; i < groups; i += 6 * kBlock) {
         uint4 w[6];
 #pragma unroll
         for (int u = 0; u < 6; ++u) w[u] = zg[min(i + u * kBlock, groups - 1)];
+        float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 6; ++u)
-            if (i + u * kBlock < groups) group(w[u]);
+        for (int u = 0; u < 6; ++u) {
+            float x[G];
+            T::unpack(w[u], x);
+            if (i + u * kBlock >= groups) continue;
+#pragma unroll
+            for (int j = 0; j < G; ++j) top = fmaxf(top, x[j]);
+        }
+        if (top > t.m) t.raise(top, c);
+        const float base = fmaxf(t.m, -FLT_MAX);
+#pragma unroll
+        for (int u = 0; u < 6; ++u) {
+            if (i + u * kBlock >= groups) continue;
+            float x[G];
+            T::unpack(w[u], x);
+            float s = 0.0f, q = 0.0f;
+#pragma unroll
+            for (int j = 0; j < G; ++j) add(x[j], base, c, s, q);
+            t.s += s;
+            t.a += q;
+        }
     }
 
     __shared__ float joined[kBlock / 64][3];
