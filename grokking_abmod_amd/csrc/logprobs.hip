@@ -16,7 +16,7 @@
 // and shorter ones where there are few rows; a second launch joins a row's chunks.
 // Rows of up to 1024 logits stay in a wave's registers.  1000 BF16 rows of
 // 128001 logits with 20 alternatives take 61 us (4.2 TB/s) and 5.4 us for the join,
-// 32 F32 rows of 256 with 5 take 5 us.
+// 20000 of 1000 with 32 take 33 us, and 22 with none.
 //
 // The gradient reads and writes each logit once, which bounds it.
 #include <hip/hip_runtime.h>
@@ -35,6 +35,7 @@ constexpr int kBlock = 256;
 constexpr int kSmall = kSmallVocab;    // logits of a row that one wave holds
 constexpr int kThreadMost = 64;        // logits of a thread's share of a chunk, at most
 constexpr int kList = 2048;            // candidates of a chunk: kTopMax threads' shares
+constexpr int kHeld = 128;             // candidates of such a row
 constexpr uint32_t kIgnore = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -102,24 +103,6 @@ __device__ __forceinline__ void wave_join(Sums &t, float c) {
     t.a = wave_sum(t.a);
 }
 
-template <int CTRL, int ROW_MASK = 0xf>
-__device__ __forceinline__ uint32_t largest_of(uint32_t v) {
-    return max(v, uint32_t(__builtin_amdgcn_update_dpp(int(v), int(v), CTRL, ROW_MASK, 0xf, false)));
-}
-__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
-    v = largest_of<0xB1>(v);
-    v = largest_of<0x4E>(v);
-    v = largest_of<0x141>(v);
-    v = largest_of<0x140>(v);
-    v = largest_of<0x142, 0xa>(v);
-    v = largest_of<0x143, 0xc>(v);
-    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
-}
-__device__ __forceinline__ uint64_t wave_best(uint64_t v) {
-    const uint32_t high = wave_largest(uint32_t(v >> 32));
-    return (uint64_t(high) << 32) | wave_largest(uint32_t(v >> 32) == high ? uint32_t(v) : 0);
-}
-
 // A row's results from its sums (a in log2 units); one thread.
 template <class T>
 __device__ __forceinline__ void write_row(const LogprobArgs &a, size_t row, const Sums &t, float &log_sum) {
@@ -181,20 +164,63 @@ __global__ void __launch_bounds__(kBlock) logprob_small_kernel(LogprobArgs a) {
     if (lane == 0) write_row<T>(a, row, t, log_sum);
     if (!a.top) return;
     log_sum = __shfl(log_sum, 0, 64);
-    uint64_t left[N];
+    if (!(t.s == t.s)) {  // a NaN
+        if (lane < a.top) write_top(a, row, lane, 0, t, log_sum);
+        return;
+    }
+    uint32_t k[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) k[i] = lane + 64 * i < int(a.vocab) ? order(x[i]) : 0;
+    // As in a chunk, the top-th largest of the lanes' maxima bounds the top-th
+    // largest logit; where too many reach it (equal ones), that one itself.
+    uint32_t best = k[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) best = max(best, k[i]);
+    uint32_t least = 0;
+    for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+        const int n = __popcll(__ballot(best >= (least | bit)));
+        if (n >= a.top) least |= bit;
+        if (n == a.top) break;  // it parts them as well as the top-th does
+    }
+    __shared__ uint64_t list[kBlock / 64][kHeld];
+    uint64_t *const mine = list[threadIdx.x >> 6];
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    int n = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const uint32_t v = lane + 64 * i;
-        left[i] = v < a.vocab ? candidate(order(x[i]), v) : 0;
+        const uint64_t all = __ballot(k[i] >= least);
+        const int at = n + __popcll(all & below);
+        if (k[i] >= least && at < kHeld) mine[at] = candidate(k[i], lane + 64 * i);
+        n += __popcll(all);
     }
-    for (int k = 0; k < a.top; ++k) {
-        uint64_t best = left[0];
+    if (n > kHeld) {
+        least = 0;
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+            n = 0;
 #pragma unroll
-        for (int i = 1; i < N; ++i) best = left[i] > best ? left[i] : best;
-        const uint64_t first = wave_best(best);
-        if (lane == 0) write_top(a, row, k, first, t, log_sum);
+            for (int i = 0; i < N; ++i) n += __popcll(__ballot(k[i] >= (least | bit)));
+            if (n >= a.top) least |= bit;
+        }
+        // The larger ones, and of equal ones the first.
+        int larger = 0, equal = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) left[i] = left[i] == first ? 0 : left[i];
+        for (int i = 0; i < N; ++i) equal += __popcll(__ballot(k[i] > least));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint64_t above = __ballot(k[i] > least), same = __ballot(k[i] == least);
+            const int at = k[i] > least ? larger + __popcll(above & below) : equal + __popcll(same & below);
+            if (k[i] >= least && at < a.top) mine[at] = candidate(k[i], lane + 64 * i);
+            larger += __popcll(above);
+            equal += __popcll(same);
+        }
+        n = a.top;
+    }
+    __builtin_amdgcn_wave_barrier();
+    for (int j = lane; j < n; j += 64) {
+        const uint64_t v = mine[j];
+        int before = 0;
+        for (int o = 0; o < n; ++o) before += mine[o] > v;
+        if (before < a.top) write_top(a, row, before, v, t, log_sum);
     }
 }
 
