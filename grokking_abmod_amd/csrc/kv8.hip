@@ -80,10 +80,11 @@ __device__ __forceinline__ float wave_largest(float v) {
 }
 
 // N consecutive elements from p (N of 16 bytes, or two), those at or past `have`
-// as 0.  Aligned: whole groups are aligned to their size.
+// as 0.  Aligned: to 16 bytes, so that whole groups are aligned to their size, to
+// 4, or (0) to the element.
 template <class T, int N>
-__device__ __forceinline__ void load_run(const typename T::Raw *p, int have, bool aligned, float (&x)[N]) {
-    if (aligned && have >= N) {
+__device__ __forceinline__ void load_run(const typename T::Raw *p, int have, int aligned, float (&x)[N]) {
+    if (aligned == 16 && have >= N) {
         if constexpr (N == T::kGroup) {
             T::unpack(*reinterpret_cast<const uint4 *>(p), x);
         } else if constexpr (sizeof(*p) == 4) {
@@ -98,13 +99,30 @@ __device__ __forceinline__ void load_run(const typename T::Raw *p, int have, boo
         }
         return;
     }
+    if constexpr (sizeof(*p) == 2) {
+        if (aligned) {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                uint32_t w = 0;
+                if (i + 1 < have)
+                    w = *reinterpret_cast<const uint32_t *>(p + i);
+                else if (i < have)
+                    w = __builtin_bit_cast(uint16_t, p[i]);
+                float y[8];
+                T::unpack(uint4{w, 0, 0, 0}, y);
+                x[i] = y[0];
+                x[i + 1] = y[1];
+            }
+            return;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = i < have ? T::to_float(p[i]) : 0.0f;
 }
 
 template <class T, int N>
-__device__ __forceinline__ void store_run(typename T::Raw *p, int have, bool aligned, const float (&x)[N]) {
-    if (aligned && have >= N) {
+__device__ __forceinline__ void store_run(typename T::Raw *p, int have, int aligned, const float (&x)[N]) {
+    if (aligned == 16 && have >= N) {
         if constexpr (N == T::kGroup) {
             *reinterpret_cast<uint4 *>(p) = T::pack(x);
         } else if constexpr (sizeof(*p) == 4) {
@@ -114,6 +132,19 @@ __device__ __forceinline__ void store_run(typename T::Raw *p, int have, bool ali
             *reinterpret_cast<uint32_t *>(p) = T::pack(y).x;
         }
         return;
+    }
+    if constexpr (sizeof(*p) == 2) {
+        if (aligned) {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const float y[8] = {x[i], x[i + 1], 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                if (i + 1 < have)
+                    *reinterpret_cast<uint32_t *>(p + i) = T::pack(y).x;
+                else if (i < have)
+                    p[i] = T::from_float(x[i]);
+            }
+            return;
+        }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)

@@ -302,7 +302,7 @@ struct MeshGpt::Impl {
         a.lengths = len;
         a.count = int(count);
         a.absolute = 1;
-        a.aligned = shape.hdp % 4 == 0;
+        a.aligned = shape.hdp % 4 == 0 ? 16 : 0;
         kern::kv8_append(a, Type::F32, stream);
     }
     // attn_decode over the 8-bit cache.

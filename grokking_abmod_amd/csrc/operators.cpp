@@ -65,11 +65,17 @@ void check_type(Type type) {
     require(type == Type::F32 || type == Type::F16 || type == Type::BF16, "unknown element type code");
 }
 
-bool aligned16(const void *p, const Strides &s, Type type) {
+bool aligned_to(int bytes, const void *p, const Strides &s, Type type) {
     const int64_t size = int64_t(type_size(type));
-    bool ok = reinterpret_cast<uintptr_t>(p) % 16 == 0;
-    for (int64_t v : s.s) ok = ok && v * size % 16 == 0;
+    bool ok = reinterpret_cast<uintptr_t>(p) % size_t(bytes) == 0;
+    for (int64_t v : s.s) ok = ok && v % bytes * size % bytes == 0;
     return ok;
+}
+// 16, 4, or 0 for less.
+int alignment(const void *k, const Strides &ks, const void *v, const Strides &vs, Type type) {
+    for (int bytes : {16, 4})
+        if (aligned_to(bytes, k, ks, type) && aligned_to(bytes, v, vs, type)) return bytes;
+    return 0;
 }
 
 void check_aligned(const void *p, Type type, const char *message) {
@@ -128,7 +134,7 @@ void kv8_append(int device, const Kv8 &cache, Type type, size_t count, const voi
     a.lengths = lengths;
     a.counts = counts;
     a.count = int(count);
-    a.aligned = aligned16(k, ks, type) && aligned16(v, vs, type);
+    a.aligned = alignment(k, ks, v, vs, type);
     kern::kv8_append(a, type, stream);
     check(hipGetLastError(), "append launch");
 }
@@ -154,7 +160,7 @@ void kv8_read(int device, const Kv8 &cache, Type type, size_t first, size_t coun
     a.lengths = lengths;
     a.first = int(first);
     a.count = int(count);
-    a.aligned = aligned16(k, ks, type) && aligned16(v, vs, type);
+    a.aligned = alignment(k, ks, v, vs, type);
     kern::kv8_read(a, type, stream);
     check(hipGetLastError(), "read launch");
 }
@@ -215,8 +221,8 @@ void kv8_attention(int device, const Kv8 &cache, Type type, size_t heads, size_t
     a.least = plan.least;
     a.part = static_cast<float *>(workspace);
     a.stride = kern::kv8_part_stride(cache.pad);
-    a.q_aligned = aligned16(q, qs, type);
-    a.o_aligned = aligned16(out, os, type);
+    a.q_aligned = aligned_to(16, q, qs, type);
+    a.o_aligned = aligned_to(16, out, os, type);
     kern::kv8_attention(a, type, plan, stream);
     check(hipGetLastError(), "attention launch");
 }

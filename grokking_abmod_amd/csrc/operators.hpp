@@ -43,7 +43,7 @@ struct Kv8AppendArgs {
     const int *counts;   // new tokens of each sequence (null: count)
     int count;
     int absolute;  // 1: token i of the inputs is position i of the sequence, 0: the first new token is token 0
-    int aligned;   // 16-byte loads of whole 16-byte groups are possible
+    int aligned;   // of inputs and strides: 16 bytes, 4, or 0 for less
 };
 void kv8_append(const Kv8AppendArgs &a, Type type, hipStream_t stream);
 
@@ -53,7 +53,7 @@ struct Kv8ReadArgs {
     Strides ks, vs;
     const int *lengths;  // positions behind a sequence's own are not written (null: all are)
     int first, count;
-    int aligned;
+    int aligned;   // as above, of the outputs
 };
 void kv8_read(const Kv8ReadArgs &a, Type type, hipStream_t stream);
 

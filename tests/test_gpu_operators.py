@@ -111,6 +111,34 @@ def test_keys_and_values_have_their_own_strides(kind):
         assert (rest == -77.0).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("width,pitch,off", [(50, 54, 2), (51, 54, 2), (51, 64, 0), (33, 48, 8), (1, 2, 0), (130, 135, 1)])
+def test_rows_of_16_bits_at_every_alignment(kind, width, pitch, off):
+    """Rows on 16 bytes, on 4 and on 2, of even and odd lengths."""
+    rng = np.random.default_rng(26)
+    cache = L.Cache(2, 2, width, 128, rng)
+    lengths, count = np.array([37, 30], np.int32), 30
+    x = [L.stored(rng.normal(size=(2, count, 2, width)), kind) for _ in range(2)]
+    wide = [np.zeros((2, count, 2, pitch), x[0].dtype) for _ in range(2)]
+    cache.ks[:], cache.vs[:] = 120, 121
+    where, st = np.s_[..., off:off + width], (count * 2 * pitch, 2 * pitch, pitch)
+    with L.Device() as dev:
+        handle = cache.on(dev)
+        for w, y in zip(wide, x):
+            w[where] = y
+        kp, vp = (dev.put(np.append(w, np.zeros(off, w.dtype))) + 2 * off for w in wide)
+        G.kv8_append(handle, L.CODES[kind], count, kp, st, vp, st, dev.put(lengths))
+        after = cache.fetch(dev)
+        check_append(cache, cache.arrays(), after, *(L.values(y, kind) for y in x), lengths, [count] * 2)
+        outs = [dev.put(L.stored(np.full((2, count, 2, pitch), -77.0), kind)) for _ in range(2)]
+        G.kv8_read(handle, L.CODES[kind], 0, count, outs[0] + 2 * off, st, outs[1] + 2 * off, st)
+        back = [L.values(dev.get(p, (2, count, 2, pitch), L.STORED[kind]), kind) for p in outs]
+    for got, want in zip(back, cache.decoded(after)):
+        want = L.values(L.stored(want[:, :, :count].transpose(0, 2, 1, 3), kind), kind)
+        assert np.array_equal(got[where], want, equal_nan=True)
+        assert (np.delete(got, np.s_[off:off + width], axis=3) == -77.0).all()
+
+
 @pytest.mark.parametrize("width", [32, 64])
 def test_append_keeps_every_magnitude(width):
     """Zeros, subnormals, the largest values, infinities and NaN."""
