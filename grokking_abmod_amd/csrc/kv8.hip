@@ -16,7 +16,7 @@
 // order in which the attention's matrix product reads them; a lane takes two
 // channels of the 16 tokens.  Memory bounds both where there is enough of it: 8
 // prompts of up to 4000 tokens, 8 heads of 128, BF16, are written in 32 us (3.8
-// TB/s read and written), 16 caches of 8000 tokens read back as F16 in 142 us (5.5
+// TB/s read and written), 16 caches of 8000 tokens read back as F16 in 135 us (5.8
 // TB/s); a step of 32 sequences takes 4.6 us.
 #include <hip/hip_runtime.h>
 
@@ -28,6 +28,8 @@
 
 namespace meshgpt::kern {
 namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Scales from 2^-117 (a code is at least 2^-9, so every value is a normal f32)
 // to 2^120, where codes end at 240: 256 * 2^120 is no f32.
@@ -120,16 +122,24 @@ __device__ __forceinline__ void load_run(const typename T::Raw *p, int have, int
     for (int i = 0; i < N; ++i) x[i] = i < have ? T::to_float(p[i]) : 0.0f;
 }
 
-template <class T, int N>
+template <bool STREAM, class W>
+__device__ __forceinline__ void put(void *p, W w) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(w, static_cast<W *>(p));
+    else
+        *static_cast<W *>(p) = w;
+}
+
+template <class T, bool STREAM, int N>
 __device__ __forceinline__ void store_run(typename T::Raw *p, int have, int aligned, const float (&x)[N]) {
     if (aligned == 16 && have >= N) {
         if constexpr (N == T::kGroup) {
-            *reinterpret_cast<uint4 *>(p) = T::pack(x);
+            put<STREAM>(p, __builtin_bit_cast(u32x4, T::pack(x)));
         } else if constexpr (sizeof(*p) == 4) {
-            *reinterpret_cast<uint2 *>(p) = uint2{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1])};
+            put<STREAM>(p, f32x2{x[0], x[1]});
         } else {
             const float y[8] = {x[0], x[1], 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            *reinterpret_cast<uint32_t *>(p) = T::pack(y).x;
+            put<STREAM>(p, T::pack(y).x);
         }
         return;
     }
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a, int ti
         append_keys<T, PAD>(a, seq, head, pair, block, lo, hi, first);
 }
 
-template <class T, int PAD>
+template <class T, int PAD, bool STREAM>
 __device__ __forceinline__ void read_keys(const Kv8ReadArgs &a, int seq, int head, size_t pair, int block, int lo,
                                           int hi) {
     using S = KeyShare<T, PAD>;
@@ -357,11 +367,11 @@ __device__ __forceinline__ void read_keys(const Kv8ReadArgs &a, int seq, int hea
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[4 * i + j] = y[j] * scale;
         }
-        store_run<T>(base + int64_t(place - a.first) * a.ks.s[1], a.cache.width - d, a.aligned, x);
+        store_run<T, STREAM>(base + int64_t(place - a.first) * a.ks.s[1], a.cache.width - d, a.aligned, x);
     }
 }
 
-template <class T, int PAD>
+template <class T, int PAD, bool STREAM>
 __device__ __forceinline__ void read_values(const Kv8ReadArgs &a, int seq, int head, size_t pair, int block, int lo,
                                             int hi) {
     using S = ValueShare<PAD>;
@@ -389,12 +399,12 @@ __device__ __forceinline__ void read_values(const Kv8ReadArgs &a, int seq, int h
             const int place = place0 + i;
             const float two[2] = {x[0][i], x[1][i]};
             if (place >= lo && place < hi)
-                store_run<T>(base + int64_t(place - a.first) * a.vs.s[1] + d, a.cache.width - d, a.aligned, two);
+                store_run<T, STREAM>(base + int64_t(place - a.first) * a.vs.s[1] + d, a.cache.width - d, a.aligned, two);
         }
     }
 }
 
-template <class T, int PAD>
+template <class T, int PAD, bool STREAM>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a, int tiles) {
     const Unit u(a.cache.heads, tiles);
     const int seq = u.seq, head = u.head;
@@ -405,9 +415,9 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a, int tiles)
     const int lo = max(a.first, 16 * block), hi = min(last, 16 * block + 16);
     if (lo >= hi) return;
     if (u.values)
-        read_values<T, PAD>(a, seq, head, pair, block, lo, hi);
+        read_values<T, PAD, STREAM>(a, seq, head, pair, block, lo, hi);
     else
-        read_keys<T, PAD>(a, seq, head, pair, block, lo, hi);
+        read_keys<T, PAD, STREAM>(a, seq, head, pair, block, lo, hi);
 }
 
 template <class T, int PAD>
@@ -420,8 +430,13 @@ void launch_append(const Kv8AppendArgs &a, hipStream_t stream) {
 template <class T, int PAD>
 void launch_read(const Kv8ReadArgs &a, hipStream_t stream) {
     const int tiles = (a.first + a.count + 63) / 64 - a.first / 64;
-    hipLaunchKernelGGL((kv8_read_kernel<T, PAD>), dim3(2u * uint32_t(a.cache.batch * a.cache.heads) * uint32_t(tiles)),
-                       dim3(256), 0, stream, a, tiles);
+    const dim3 grid(2u * uint32_t(a.cache.batch * a.cache.heads) * uint32_t(tiles));
+    // Outputs of more than the Infinity Cache's 256 MB are not found there by their
+    // reader, and are stored past the caches (524 MB, F16: 135 us, 142 otherwise).
+    if (2.0 * a.cache.batch * a.cache.heads * a.cache.width * double(a.count) * sizeof(typename T::Raw) > double(256u << 20))
+        hipLaunchKernelGGL((kv8_read_kernel<T, PAD, true>), grid, dim3(256), 0, stream, a, tiles);
+    else
+        hipLaunchKernelGGL((kv8_read_kernel<T, PAD, false>), grid, dim3(256), 0, stream, a, tiles);
 }
 
 template <class T>

@@ -226,6 +226,27 @@ def test_read_gives_the_values_of_the_codes(kind, width, first, count, lengths, 
         assert np.array_equal(L.values(got, kind), want, equal_nan=True)
 
 
+@pytest.mark.parametrize("kind,batch,width,count", [("f32", 4, 100, 11000), ("f16", 8, 128, 9000)])
+def test_read_of_more_than_the_caches_hold(kind, batch, width, count):
+    rng = np.random.default_rng(27)
+    heads, capacity, first = 8, (count + 127) // 64 * 64, 37
+    cache = L.Cache(batch, heads, width, capacity, rng)
+    cache.ks[:], cache.vs[:] = (rng.integers(120, 128, cache.ks.shape, dtype=np.uint8) for _ in range(2))
+    shape = (batch, count, heads, width)
+    size = int(np.prod(shape)) * np.dtype(L.STORED[kind]).itemsize
+    assert 2 * size > 256 << 20
+    with L.Device() as dev:
+        handle, outs, st = cache.on(dev), [dev.alloc(size) for _ in range(2)], strides_of(shape)
+        G.kv8_read(handle, L.CODES[kind], first, count, outs[0], st, outs[1], st)
+        table = L.E4M3.astype(np.float32)
+        for which, codes in enumerate((cache.k, cache.v.transpose(0, 1, 2, 4, 3).reshape(cache.k.shape))):
+            got = dev.get(outs[which], shape, L.STORED[kind])
+            scale = np.ldexp(np.float32(1), np.repeat((cache.ks, cache.vs)[which], 16, 2).astype(np.int32) - 127)
+            for s in range(batch):  # exact: 4 bits times a power of two
+                want = table[codes[s, :, first:first + count, :width]] * scale[s, :, first:first + count, None]
+                assert np.array_equal(got[s], want.transpose(1, 0, 2).astype(got.dtype), equal_nan=True)
+
+
 def filled(cache, lengths, rng, spread=4):
     """Codes and scales of ordinary tokens inside the sequences; behind them stays
     whatever was there, NaN codes and scales of every kind among it."""
