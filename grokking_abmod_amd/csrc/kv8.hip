@@ -29,8 +29,6 @@
 namespace meshgpt::kern {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 // Scales from 2^-117 (a code is at least 2^-9, so every value is a normal f32)
 // to 2^120, where codes end at 240: 256 * 2^120 is no f32.
 constexpr int kLowScale = 10, kHighScale = 247;
@@ -120,14 +118,6 @@ __device__ __forceinline__ void load_run(const typename T::Raw *p, int have, int
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = i < have ? T::to_float(p[i]) : 0.0f;
-}
-
-template <bool STREAM, class W>
-__device__ __forceinline__ void put(void *p, W w) {
-    if constexpr (STREAM)
-        __builtin_nontemporal_store(w, static_cast<W *>(p));
-    else
-        *static_cast<W *>(p) = w;
 }
 
 template <class T, bool STREAM, int N>
@@ -431,9 +421,8 @@ template <class T, int PAD>
 void launch_read(const Kv8ReadArgs &a, hipStream_t stream) {
     const int tiles = (a.first + a.count + 63) / 64 - a.first / 64;
     const dim3 grid(2u * uint32_t(a.cache.batch * a.cache.heads) * uint32_t(tiles));
-    // Outputs of more than the Infinity Cache's 256 MB are not found there by their
-    // reader, and are stored past the caches (524 MB, F16: 135 us, 142 otherwise).
-    if (2.0 * a.cache.batch * a.cache.heads * a.cache.width * double(a.count) * sizeof(typename T::Raw) > double(256u << 20))
+    // 524 MB of F16 take 135 us past the caches, 142 otherwise.
+    if (2.0 * a.cache.batch * a.cache.heads * a.cache.width * double(a.count) * sizeof(typename T::Raw) > kCached)
         hipLaunchKernelGGL((kv8_read_kernel<T, PAD, true>), grid, dim3(256), 0, stream, a, tiles);
     else
         hipLaunchKernelGGL((kv8_read_kernel<T, PAD, false>), grid, dim3(256), 0, stream, a, tiles);

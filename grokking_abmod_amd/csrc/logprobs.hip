@@ -479,8 +479,9 @@ __device__ __forceinline__ float grad_of(float x, uint32_t v, const LogprobBackw
 // A wave's share of a row: `size` logits, all under way at once.  Shares end at
 // 128-byte lines.  Short shares keep what is read and written at a time close
 // together in memory: 4096 BF16 rows of 50257 take 192 us with 32768 logits a
-// workgroup, 146 with 2048 a wave, 140 with 1536 (5.9 TB/s), 147 with 1024.
-template <class T>
+// workgroup, 146 with 2048 a wave, 140 with 1536, 147 with 1024; past the caches
+// 133 (6.2 TB/s).
+template <class T, bool STREAM>
 __global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwardArgs a, uint32_t shares, uint32_t size) {
     using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwar
     uint4 *const og = reinterpret_cast<uint4 *>(out + body);
     uint4 w[kGradGroups];
 #pragma unroll
-    for (int u = 0; u < kGradGroups; ++u) w[u] = zg[min(lane + 64 * u, groups - 1)];
+    for (int u = 0; u < kGradGroups; ++u) w[u] = get<STREAM>(zg + min(lane + 64 * u, groups - 1));
 #pragma unroll
     for (int u = 0; u < kGradGroups; ++u) {
         const uint32_t i = lane + 64 * u;
@@ -526,7 +527,7 @@ __global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwar
         T::unpack(w[u], x);
 #pragma unroll
         for (int j = 0; j < G; ++j) x[j] = grad(x[j], body + i * G + j);
-        og[i] = T::pack(x);
+        put<STREAM>(og + i, __builtin_bit_cast(u32x4, T::pack(x)));
     }
 }
 
@@ -552,8 +553,13 @@ void backward_of(const LogprobBackwardArgs &a, hipStream_t stream) {
     const size_t parts = (a.vocab + kGradMost<T> - 1) / kGradMost<T>, even = (a.vocab + parts - 1) / parts;
     const size_t size = (even + kLine<T> - 1) / kLine<T> * kLine<T>, shares = (a.vocab + size - 1) / size;
     const size_t units = a.rows * shares;
-    hipLaunchKernelGGL((logprob_backward_kernel<T>), dim3(uint32_t((units + kBlock / 64 - 1) / (kBlock / 64))), dim3(kBlock),
-                       0, stream, a, uint32_t(shares), uint32_t(size));
+    const dim3 grid(uint32_t((units + kBlock / 64 - 1) / (kBlock / 64)));
+    if (double(a.rows) * double(a.vocab) * sizeof(typename T::Raw) > kCached)
+        hipLaunchKernelGGL((logprob_backward_kernel<T, true>), grid, dim3(kBlock), 0, stream, a, uint32_t(shares),
+                           uint32_t(size));
+    else
+        hipLaunchKernelGGL((logprob_backward_kernel<T, false>), grid, dim3(kBlock), 0, stream, a, uint32_t(shares),
+                           uint32_t(size));
 }
 
 }  // namespace

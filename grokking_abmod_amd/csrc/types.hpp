@@ -8,6 +8,7 @@ namespace meshgpt::kern {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct F32 {
     using Raw = float;
@@ -69,5 +70,23 @@ struct BF16 {
         return {w[0], w[1], w[2], w[3]};
     }
 };
+
+// Inputs and outputs of more than the Infinity Cache's 256 MB: whoever comes next
+// does not find them there, so they are moved past the caches (STREAM).
+constexpr double kCached = double(256u << 20);
+template <bool STREAM, class W>
+__device__ __forceinline__ void put(void *p, W w) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(w, static_cast<W *>(p));
+    else
+        *static_cast<W *>(p) = w;
+}
+template <bool STREAM>
+__device__ __forceinline__ uint4 get(const uint4 *p) {
+    if constexpr (STREAM)
+        return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p)));
+    else
+        return *p;
+}
 
 }  // namespace meshgpt::kern

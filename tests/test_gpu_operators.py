@@ -675,6 +675,28 @@ def test_the_gradient_matches_64_bits(kind, rows, vocab, stride, temperature, wh
     assert (np.abs(got[:, :vocab] - want) <= limit).all(), np.max(np.abs(got[:, :vocab] - want) / limit)
 
 
+def test_the_gradient_of_more_than_the_caches_hold():
+    """The same rows again and again, beside those of a small call."""
+    rng = np.random.default_rng(28)
+    rows, vocab, times = 8, 50257, 340
+    assert rows * times * vocab * 2 > 256 << 20
+    z = L.stored(rng.normal(size=(rows, vocab)) * 3, "bf16")
+    t = rng.integers(0, vocab, rows).astype(np.uint32)
+    g, e = (rng.normal(size=rows).astype(np.float32) for _ in range(2))
+    with L.Device() as dev:
+        *_, zp, (_, hp, sp) = score(dev, z, "bf16", t, 1.0, 0)
+        out = dev.alloc(z.nbytes)
+        G.token_logprobs_backward_noalloc(G.MG_BF16, zp, rows, vocab, vocab, dev.put(t), 1.0, sp, hp, dev.put(g), dev.put(e),
+                                          out, vocab)
+        want, h, stats = dev.get(out, z.shape, np.uint16), dev.get(hp, rows, np.float32), dev.get(sp, (rows, 2), np.float32)
+        many = dev.put(np.tile(z, (times, 1)))
+        G.token_logprobs_backward_noalloc(G.MG_BF16, many, rows * times, vocab, vocab, dev.put(np.tile(t, times)), 1.0,
+                                          dev.put(np.tile(stats, (times, 1))), dev.put(np.tile(h, times)),
+                                          dev.put(np.tile(g, times)), dev.put(np.tile(e, times)), many, vocab)
+        got = dev.get(many, (times, rows, vocab), np.uint16)
+    assert (got == want).all()
+
+
 def test_the_gradient_is_that_of_the_forward_pass():
     """Differences of the forward kernel's own log probability and entropy."""
     rng = np.random.default_rng(1)
