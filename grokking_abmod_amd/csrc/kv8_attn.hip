@@ -3,12 +3,16 @@
 //
 // Every product runs on the BF16 matrix cores.  An E4M3 code is exact in BF16,
 // so keys and values go there as codes, two an instruction, and their scales
-// meet the scores and the probabilities in FP32.  Queries and probabilities go
-// there as one BF16 (BF16 calls: half a step, 2^-9, of each probability, of
-// random sign and of the size of the result's own rounding), as two (F16 calls:
-// 16 bits of the probabilities, queries exact) or as three (F32 calls: 24 bits,
-// exact), each piece a product of its own.  Scores, maxima, sums and outputs are
-// FP32.
+// meet the scores in FP32 and the values, exactly, in their conversion.  Queries
+// go there exactly: as one BF16 (BF16 calls), two (F16) or three (F32).
+// Probabilities go there as two in 16-bit calls, which leaves 2^-15 of each, or as
+// three in F32 calls, which leaves nothing.  Each piece is a product of its own.
+// One BF16 would leave 2^-8 of each probability, as much as the output's own
+// rounding: the error against 64 bits was then 1.35 times that of the output's
+// rounding alone.  The second piece takes nothing where memory bounds (64 sequences of
+// 2000 to 16000 tokens, 32 heads over 8 of 128: 231 us with one, 232 with two) and up
+// to a quarter more where products do (4 prompts of 4096: 586 us, 753).  Scores, maxima,
+// sums and outputs are FP32.
 //
 // A wave takes tiles of 64 keys for 16 query rows at a time; query heads that
 // share a cached head are rows of the same tile.  The scores are computed
@@ -36,11 +40,13 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 4;
 
-// Pieces of a query or probability in BF16.
+// Pieces of a query and of a probability in BF16.
 template <class T>
-constexpr int kPieces = sizeof(typename T::Raw) == 4 ? 3 : 1;
+constexpr int kQueryPieces = sizeof(typename T::Raw) == 4 ? 3 : 1;
 template <>
-constexpr int kPieces<F16> = 2;
+constexpr int kQueryPieces<F16> = 2;
+template <class T>
+constexpr int kProbPieces = sizeof(typename T::Raw) == 4 ? 3 : 2;
 
 __device__ __forceinline__ float bits(uint32_t u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ uint32_t bits(float f) { return __builtin_bit_cast(uint32_t, f); }
@@ -245,7 +251,7 @@ __device__ __forceinline__ void store4(const Kv8AttnArgs &a, typename T::Raw *o,
 // Eight elements of a query from d as pieces, zeros where there are none.
 template <class T>
 __device__ __forceinline__ void query8(const Kv8AttnArgs &a, const typename T::Raw *q, bool real, int d,
-                                       bf16x8 (&piece)[kPieces<T>]) {
+                                       bf16x8 (&piece)[kQueryPieces<T>]) {
     float x[8];
     if (a.q_aligned && real && d + 8 <= a.cache.width) {
 #pragma unroll
@@ -259,7 +265,7 @@ __device__ __forceinline__ void query8(const Kv8AttnArgs &a, const typename T::R
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = real && d + j < a.cache.width ? T::to_float(q[d + j]) : 0.0f;
     }
-    pieces8<kPieces<T>>(x, piece);
+    pieces8<kQueryPieces<T>>(x, piece);
 }
 
 // The key tiles of a share for rows that see `keys` keys: equal shares, of a.least
@@ -287,7 +293,7 @@ __device__ __forceinline__ void fill_nan(const Kv8AttnArgs &a, const Sequence &s
 // 32 heads over 8 of 128, BF16, take 233 us (5.0 TB/s).
 template <class T, int PAD>
 __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, int pairs, int row_tiles) {
-    constexpr int NP = kPieces<T>, STEPS = PAD / 32, DT = PAD / 16;
+    constexpr int NQ = kQueryPieces<T>, NP = kProbPieces<T>, STEPS = PAD / 32, DT = PAD / 16;
     constexpr int WORDS = PAD >= 64 ? PAD / 16 : 2;  // 4-byte words of a key that a lane holds
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int id = int(blockIdx.x), pair = id % pairs, split = id / pairs % a.splits;
@@ -304,7 +310,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
     const Tiles tiles(a, split, begin + (row_end - 1) / a.group + 1);
     if (tiles.first >= tiles.last && a.out) return;  // the join does not read it
 
-    bf16x8 qf[NP][STEPS];
+    bf16x8 qf[NQ][STEPS];
     const int row = row0 + n, place = row < rows ? begin + row / a.group : -1;
     {
         const int i = row / a.group;
@@ -312,10 +318,10 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
                         (s.head * a.group + row - i * a.group) * a.qs.s[2];
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
-            bf16x8 piece[NP];
+            bf16x8 piece[NQ];
             query8<T>(a, q, row < rows, PAD >= 64 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 8 * g, piece);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) qf[p][k] = piece[p];
+            for (int p = 0; p < NQ; ++p) qf[p][k] = piece[p];
         }
     }
 
@@ -378,7 +384,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, in
             for (int k = 0; k < STEPS; ++k) {
                 const bf16x8 kf = codes8(kw[t][2 * k], kw[t][2 * k + 1]);
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
+                for (int p = NQ - 1; p >= 0; --p)
                     st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[p][k], st[t], 0, 0, 0);
             }
         }
@@ -576,7 +582,7 @@ __device__ __forceinline__ void mark_nan32(const uint8_t *vpair, int from, int t
 template <class T, int PAD, int SUB>
 __global__ void __launch_bounds__(64 * kWaves, PAD == 256 ? 1 : 2)
 kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
-    constexpr int NP = kPieces<T>, DT = PAD / 32, ROWS = 32 * kWaves;
+    constexpr int NQ = kQueryPieces<T>, NP = kProbPieces<T>, DT = PAD / 32, ROWS = 32 * kWaves;
     // A tile's groups: 64 lanes' 16 codes of the keys (32 u + ..., 32 c + ...), then
     // of the values; in LDS two operands of 8 elements for each lane.
     static_assert(kWaves == 4, "two waves take the keys, two the values");
@@ -637,7 +643,7 @@ kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
     };
     load_tile(tiles.first);
 
-    bf16x8 qf[NP][DT][2];
+    bf16x8 qf[NQ][DT][2];
     const int r = row0 + n, place = r < rows ? begin + r / a.group : -1;
     {
         const int i = r / a.group;
@@ -647,10 +653,10 @@ kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
         for (int c = 0; c < DT; ++c)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                bf16x8 piece[NP];
+                bf16x8 piece[NQ];
                 query8<T>(a, q, r < rows, 32 * c + 16 * g + 8 * k, piece);
 #pragma unroll
-                for (int p = 0; p < NP; ++p) qf[p][c][k] = piece[p];
+                for (int p = 0; p < NQ; ++p) qf[p][c][k] = piece[p];
             }
     }
     float m = -INFINITY, l = 0.0f;
@@ -694,10 +700,10 @@ kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
                     for (int u = 0; u < SUB; ++u) {
                         const bf16x8 kf = now[(step + u) * DT + c][k][lane];
 #pragma unroll
-                        for (int p = NP - 1; p >= 0; --p)
+                        for (int p = NQ - 1; p >= 0; --p)
                             st[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[p][c][k], st[u], 0, 0, 0);
                     }
-            paced<2 * DT * SUB, NP>();
+            paced<2 * DT * SUB, NQ>();
             int key0[SUB];  // of the lane's 16 keys
             float kscale[SUB], slack = kSlack;
 #pragma unroll
@@ -798,7 +804,7 @@ template <class T, int PAD>
 void launch_attn(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) {
     const int pairs = a.cache.batch * a.cache.heads;
     if (plan.wide) {
-        constexpr int SUB = PAD <= 64 || (PAD == 128 && kPieces<T> == 1) ? 2 : 1;
+        constexpr int SUB = PAD <= 64 || (PAD == 128 && kQueryPieces<T> == 1) ? 2 : 1;
         const int pairs8 = (pairs + 7) / 8 * 8;
         hipLaunchKernelGGL((kv8_tiles_kernel<T, PAD, SUB>),
                            dim3(uint32_t(pairs8) * uint32_t(a.splits) * uint32_t(plan.row_tiles)), dim3(64 * kWaves), 0,

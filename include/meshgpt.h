@@ -305,7 +305,7 @@ int mg_kv8_read(int device, const mg_kv8 *cache, int type, size_t first, size_t 
  * sees makes what depends on it NaN; what it does not see has no effect.  The rows
  * of a sequence whose length or count is impossible (as above) are filled with
  * NaN, all `count` of them.  F32 calls keep 24 bits of the queries and
- * probabilities, F16 and BF16 calls 16 and 8 of the probabilities; scores, and the
+ * probabilities, F16 and BF16 calls 15 bits of the probabilities; scores, and the
  * sums of probabilities and of values before they are divided, are FP32 and have
  * to stay in its range.  The workspace holds mg_kv8_attention_workspace bytes,
  * aligned to 16 (NULL where that is 0). */

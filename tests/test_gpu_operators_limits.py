@@ -1,0 +1,41 @@
+"""GPU: the device operators (mg_kv8_attention) where their
+precision or their inputs are at an end, against the plain 64-bit forms."""
+import math
+
+import numpy as np
+import pytest
+
+import operators_lib as L
+from test_gpu_operators import attend, filled
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("width,heads,kv_heads,capacity,count,lengths", [
+    (128, 8, 2, 128, 1, [1, 7, 20, 33]), (64, 2, 2, 2048, 1, [40, 1500, 3]), (256, 2, 1, 64, 3, [33, 5]),
+    (32, 8, 1, 64, 2, [30, 21]), (50, 4, 4, 64, 1, [11, 29]),  # single tokens, a few
+    (32, 2, 1, 256, 200, [200, 204]), (64, 2, 2, 128, 100, [100, 103]), (64, 1, 1, 1024, 200, [1024, 230]),
+    (128, 2, 1, 128, 70, [70, 80]), (256, 1, 1, 192, 140, [140, 150]), (80, 1, 1, 128, 100, [100, 101])])  # prompts
+def test_probabilities_of_16_bit_calls_keep_15_bits(kind, width, heads, kv_heads, capacity, count, lengths):
+    """Beside the output's own rounding, a half step of the type, a call in 16 bits
+    is off by no more than two BF16 pieces of each probability leave: the first one
+    cut after 8 bits, the rest, under 2^-7 of it, rounded by 2^-8 of itself; once in
+    the sum over the values, once in that of the probabilities.  Flat weights over
+    few keys, so that little else adds to it."""
+    rng = np.random.default_rng(width + count)
+    cache = L.Cache(len(lengths), kv_heads, width, capacity, rng)
+    filled(cache, lengths, rng)
+    q = L.stored(rng.normal(size=(len(lengths), count, heads, width)), kind)
+    scale = 0.2 / math.sqrt(width)
+    with L.Device() as dev:
+        got = attend(dev, cache.on(dev), q, kind, lengths, None, scale)
+    k, v = cache.decoded()
+    want, size, mass, far = L.attention(L.values(q, kind), k, v, lengths, [count] * len(lengths), scale)
+    # As attention_tolerance, whose terms for scores, sums and the output stand.
+    step = 2.0**-24
+    exponent = 2 * (width + 2) * step * mass + 6 * step * (1.5 * far + 1)
+    sums = (max(lengths) / 8 + 64) * step
+    least = {"f16": 2.0**-25, "bf16": 2.0**-133}[kind]
+    limit = (2 * exponent + 2 * sums + 2 * 2.0**-15) * size * 1.01 + L.HALF_STEP[kind] * np.abs(want) * 1.01 + least
+    assert (np.abs(got - want) <= limit).all(), np.max(np.abs(got - want) / limit)
