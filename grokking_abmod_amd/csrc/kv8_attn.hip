@@ -112,9 +112,9 @@ __device__ __forceinline__ float soften(f32x4 (&st)[4], bool masked, float kscal
     if (masked) {
         __builtin_amdgcn_sched_barrier(0);  // a branch: few tiles are masked
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (key0 + j > place) st[j / 4][j % 4] = -INFINITY;
-        if (key0 > place) kscale = 1.0f;  // the scale may be anything too
+        for (int j = 0; j < 16; ++j)  // scaled first: the scale may be 0, or anything where no key counts
+            st[j / 4][j % 4] = key0 + j > place ? -INFINITY : st[j / 4][j % 4] * kscale;
+        kscale = 1.0f;
     }
     float top = st[0][0];
 #pragma unroll
@@ -496,9 +496,8 @@ __device__ __forceinline__ float soften32(f32x16 (&st)[SUB], bool masked, float 
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (key0[u] + j > place) st[u][j] = -INFINITY;
-            if (key0[u] > place) kscale[u] = 1.0f;  // the scale may be anything too
+            for (int j = 0; j < 16; ++j) st[u][j] = key0[u] + j > place ? -INFINITY : st[u][j] * kscale[u];
+            kscale[u] = 1.0f;
         }
     }
     float top = -INFINITY;

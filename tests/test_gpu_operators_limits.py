@@ -1,5 +1,5 @@
-"""GPU: the device operators (mg_kv8_attention) where their
-precision or their inputs are at an end, against the plain 64-bit forms."""
+"""GPU: mg_kv8_attention where its precision or its inputs are at an end, against
+the plain 64-bit form."""
 import math
 
 import numpy as np
@@ -39,3 +39,28 @@ def test_probabilities_of_16_bit_calls_keep_15_bits(kind, width, heads, kv_heads
     least = {"f16": 2.0**-25, "bf16": 2.0**-133}[kind]
     limit = (2 * exponent + 2 * sums + 2 * 2.0**-15) * size * 1.01 + L.HALF_STEP[kind] * np.abs(want) * 1.01 + least
     assert (np.abs(got - want) <= limit).all(), np.max(np.abs(got - want) / limit)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("count,lengths", [(1, [5, 16, 70, 128]), (40, [40, 41, 90, 128]), (130, [130, 131, 300, 320])])
+@pytest.mark.parametrize("scale", [1e-11, 1e-30, 1e-42])
+def test_scales_that_leave_the_scores_nothing(kind, count, lengths, scale):
+    """Zero keys, whose blocks have the smallest scale, under a scale with which
+    their product is no f32 any more: every key that a row sees weighs the same."""
+    rng = np.random.default_rng(count)
+    width, capacity = 64, 320
+    cache = L.Cache(len(lengths), 1, width, capacity, rng)
+    filled(cache, lengths, rng, spread=1)
+    for s, n in enumerate(lengths):
+        cache.k[s, :, :n] = 0
+        cache.ks[s, :, :(n + 15) // 16] = 10
+    q = L.stored(rng.normal(size=(len(lengths), count, 1, width)), kind)
+    with L.Device() as dev:
+        got = attend(dev, cache.on(dev), q, kind, lengths, None, scale)
+    _, v = cache.decoded()
+    for s, n in enumerate(lengths):
+        for i in range(count):
+            seen = v[s, 0, :n - count + i + 1]
+            want, size = seen.mean(0), np.abs(seen).mean(0)
+            limit = 2 * (max(lengths) / 8 + 64) * 2.0**-24 * size + L.HALF_STEP[kind] * np.abs(want) * 1.01
+            assert (np.abs(got[s, i, 0] - want) <= limit + 2.0**-25).all(), (s, i)
