@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwar
     const uint32_t token = a.tokens ? a.tokens[row] : kIgnore;
     const float m = a.stats[2 * row], log_sum = a.stats[2 * row + 1];
     float g = a.d_logprob && token != kIgnore ? a.d_logprob[row] : 0.0f;
-    if (token != kIgnore && token >= a.vocab) g = __builtin_nanf("");
+    if (a.d_logprob && token != kIgnore && token >= a.vocab) g = __builtin_nanf("");
     const float h = a.d_entropy ? a.d_entropy[row] : 0.0f, entropy = a.d_entropy ? a.entropy[row] : 0.0f;
     const bool none = m == -INFINITY;  // no token is allowed: nothing depends on the logits
     auto grad = [&](float x, uint32_t v) {

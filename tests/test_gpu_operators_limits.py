@@ -1,12 +1,13 @@
-"""GPU: mg_kv8_attention where its precision or its inputs are at an end, against
-the plain 64-bit form."""
+"""GPU: the device operators (mg_kv8_attention, mg_token_logprobs*) where their
+precision or their inputs are at an end, against the plain 64-bit forms."""
 import math
 
 import numpy as np
 import pytest
 
+import grokking_abmod_amd as G
 import operators_lib as L
-from test_gpu_operators import attend, filled
+from test_gpu_operators import attend, filled, score
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,29 @@ def test_scales_that_leave_the_scores_nothing(kind, count, lengths, scale):
             want, size = seen.mean(0), np.abs(seen).mean(0)
             limit = 2 * (max(lengths) / 8 + 64) * 2.0**-24 * size + L.HALF_STEP[kind] * np.abs(want) * 1.01
             assert (np.abs(got[s, i, 0] - want) <= limit + 2.0**-25).all(), (s, i)
+
+
+def gradient(dev, z, kind, tokens, stats, entropy, d_logprob, d_entropy, temperature=1.0):
+    rows, vocab = z.shape
+    out = dev.alloc(z.nbytes)
+    G.token_logprobs_backward_noalloc(L.CODES[kind], dev.put(z), rows, vocab, vocab,
+                                      None if tokens is None else dev.put(np.asarray(tokens, np.uint32)), temperature, stats,
+                                      entropy, None if d_logprob is None else dev.put(d_logprob),
+                                      None if d_entropy is None else dev.put(d_entropy), out, vocab)
+    return L.values(dev.get(out, z.shape, L.STORED[kind]), kind)
+
+
+def test_tokens_do_not_matter_to_the_entropys_gradient():
+    """Without a gradient of the log probabilities, a token outside the vocabulary
+    is like any other."""
+    rng = np.random.default_rng(1)
+    z, e = (rng.normal(size=s).astype(np.float32) for s in ((4, 300), 4))
+    with L.Device() as dev:
+        *_, (_, h, st) = score(dev, z, "f32", [1, 2, 3, 4], 1.0, 0)
+        plain = gradient(dev, z, "f32", [1, 2, 3, 4], st, h, None, e)
+        assert np.isfinite(plain).all() and np.abs(plain).max() > 0
+        for tokens in ([300, 1 << 31, G.IGNORE_TARGET - 1, 7], None):
+            assert np.array_equal(gradient(dev, z, "f32", tokens, st, h, None, e), plain)
+        # With one, its row alone is NaN.
+        got = gradient(dev, z, "f32", [300, 2, 3, 4], st, h, e, None)
+        assert np.isnan(got[0]).all() and np.isfinite(got[1:]).all()
