@@ -494,10 +494,13 @@ __global__ void __launch_bounds__(kBlock) logprob_backward_kernel(LogprobBackwar
     auto *out = static_cast<Raw *>(a.d_logits) + row * a.d_stride;
     const uint32_t token = a.tokens ? a.tokens[row] : kIgnore;
     const float m = a.stats[2 * row], log_sum = a.stats[2 * row + 1];
-    float g = a.d_logprob && token != kIgnore ? a.d_logprob[row] : 0.0f;
-    if (a.d_logprob && token != kIgnore && token >= a.vocab) g = __builtin_nanf("");
+    const bool scored = a.d_logprob && token != kIgnore;
+    float g = scored ? a.d_logprob[row] : 0.0f;
+    if (scored && token >= a.vocab) g = __builtin_nanf("");
     const float h = a.d_entropy ? a.d_entropy[row] : 0.0f, entropy = a.d_entropy ? a.entropy[row] : 0.0f;
-    const bool none = m == -INFINITY;  // no token is allowed: nothing depends on the logits
+    // No token is allowed, so that nothing depends on the logits, or nothing is asked
+    // of the row, whose logits may then be anything (0 times its NaN would be NaN).
+    const bool none = m == -INFINITY || (!scored && h == 0.0f);
     auto grad = [&](float x, uint32_t v) {
         return none ? 0.0f : grad_of<T>(x, v, a, token, m, log_sum, g, h, entropy);
     };

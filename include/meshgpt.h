@@ -337,7 +337,8 @@ int mg_token_logprobs_noalloc(int device, int type, const void *logits, size_t r
  * log probabilities and of the entropies (rows floats each; either may be NULL)
  * and the forward call's stats and entropies.  Rows of MG_IGNORE_TARGET take
  * nothing from d_logprob, rows of a token outside the vocabulary NaN; a row without
- * an allowed token has gradient 0.
+ * an allowed token has gradient 0, and so has one that takes nothing from d_logprob
+ * and whose d_entropy is 0 or not given, whatever its logits are.
  * d_logits may be the logits, with the same stride. */
 int mg_token_logprobs_backward_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab,
                                        size_t stride, const uint32_t *tokens, float temperature, const float *stats,

@@ -91,3 +91,29 @@ def test_tokens_do_not_matter_to_the_entropys_gradient():
         # With one, its row alone is NaN.
         got = gradient(dev, z, "f32", [300, 2, 3, 4], st, h, e, None)
         assert np.isnan(got[0]).all() and np.isfinite(got[1:]).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [40, 5000])
+def test_ignored_rows_take_no_gradient_whatever_they_hold(kind, vocab):
+    """Rows behind a sequence, as a padded batch has them: their logits may be
+    anything, NaN and infinities among it, and so may their d_logprob."""
+    rng = np.random.default_rng(vocab)
+    z = (rng.normal(size=(6, vocab)) * 3).astype(np.float32)
+    z[1] = np.nan
+    z[2, 3] = np.inf
+    z[3, 4], z[3, 5] = -np.inf, np.nan
+    z[4] = -np.inf
+    z = L.stored(z, kind)
+    tokens = np.full(6, G.IGNORE_TARGET, np.uint32)
+    tokens[5] = 7
+    g = np.array([1, 2, np.nan, np.inf, 3, 1], np.float32)
+    e = np.array([0, 0, -0.0, 0, 0, 0.5], np.float32)
+    with L.Device() as dev:
+        lp, h, *_, (_, hp, st) = score(dev, z, kind, tokens, 1.0, 0)
+        assert (lp[:5] == 0).all() and np.isnan(h[1:4]).all()
+        for d_entropy in (None, e):
+            got = gradient(dev, z, kind, tokens, st, hp, g, d_entropy)
+            assert (got[:5] == 0).all() and np.isfinite(got[5]).all() and np.abs(got[5]).max() > 0
+        # The entropy of such a row is NaN, and asked for, its gradient is.
+        assert np.isnan(gradient(dev, z, kind, tokens, st, hp, None, np.ones(6, np.float32))[1:4]).all()
