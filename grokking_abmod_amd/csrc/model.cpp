@@ -1621,7 +1621,9 @@ struct MeshGpt::Impl {
     void step() {
         if (length + 1 > tcap) throw Error("generation exceeds the reserved token capacity");
         known_flags = -1;
-        if (length <= cfg.context && cached == length - 1) {
+        // A prompt of one token is a decode step from an empty cache, but not with 8
+        // bits, where prompts attend before they are quantised.
+        if (length <= cfg.context && cached == length - 1 && !(cache8 && cached == 0)) {
             decode_step();
             cached = length;
         } else if (length <= cfg.context) {

@@ -765,7 +765,8 @@ static void round_cache(const og_config *c, rounding *q, size_t layer, double *c
  * earlier keys/values are already cached (layer-major, context x W each); the
  * result is identical to recomputing the whole prefix because every row's
  * arithmetic depends only on its own inputs and the cached rows.  With `round` the cache is
- * rounded to 8 bits: after a prompt's attention, before a single token's. */
+ * rounded to 8 bits: after the attention of a prompt, of one token too, and before that of a
+ * token that follows cached ones. */
 static void forward(const og_config *c, const float *params, const double *E, const uint32_t *tokens,
                     size_t n, size_t sequence, double *logits, double *hidden, double *cache_k,
                     double *cache_v, size_t first_position, size_t logit_rows_from, rounding *round) {
@@ -813,10 +814,10 @@ static void forward(const og_config *c, const float *params, const double *E, co
             double *ck = cache_k + b * c->context * W, *cv = cache_v + b * c->context * W;
             memcpy(ck + first_position * W, k, sizeof(double) * rw);
             memcpy(cv + first_position * W, v, sizeof(double) * rw);
-            if (round && n == 1) round_cache(c, round, b, ck, cv, first_position, first_position + n);
+            if (round && first_position > 0) round_cache(c, round, b, ck, cv, first_position, first_position + n);
             for (size_t r = 0; r < n; ++r)
                 attention_row(q + r * W, ck, cv, first_position + r, W, H, scores, t1 + r * W);
-            if (round && n > 1) round_cache(c, round, b, ck, cv, first_position, first_position + n);
+            if (round && first_position == 0) round_cache(c, round, b, ck, cv, first_position, first_position + n);
         } else {
             og_attention(q, k, v, n, W, H, sequence, t1);
         }
