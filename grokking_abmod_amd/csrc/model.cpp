@@ -330,12 +330,21 @@ struct MeshGpt::Impl {
         activate();
         sync();
         drop_graph();
-        for (DevBuf *b : {&kc, &vc, &k8, &v8, &ks8, &vs8}) b->release();
+        auto release = [&] {
+            for (DevBuf *b : {&kc, &vc, &k8, &v8, &ks8, &vs8}) b->release();
+        };
+        release();
         const size_t sequences = batch_cap;
         cache8 = eight_bits;
         batch_cap = tcap = batch = length = start_length = 0;
         cached = kNoCache;
-        ensure_decode(std::max<size_t>(sequences, 1), 1);
+        try {
+            ensure_decode(std::max<size_t>(sequences, 1), 1);
+        } catch (...) {
+            release();
+            cache8 = !eight_bits;  // the next batch allocates what there was
+            throw;
+        }
     }
 
     // Splits per (sequence, head) of decode attention: about 512 workgroups

@@ -184,10 +184,36 @@ void scores_without_memory() {
     fake::memory = size_t(1) << 33;
 }
 
+// A cache of another type that finds no memory leaves the model with the type that
+// it had and no batch.
+void cache_without_memory() {
+    for (CacheType type : {CacheType::E4M3, CacheType::F32}) {
+        const CacheType other = type == CacheType::E4M3 ? CacheType::F32 : CacheType::E4M3;
+        MeshGpt m(0, shape(128, 4, 256, type == CacheType::E4M3 ? 2 : 8), 7, 64);
+        m.set_cache(other);
+        generate(m, 64, 16, 4);
+        // Two layers in 8 bits take more than in FP32, eight layers less.
+        fake::memory = fake::used;
+        expect(status_of([&] { m.set_cache(type); }) == kOutOfMemory, "no memory for the other cache");
+        bool rounded = false;
+        fake::on_launch = [&](const fake::Launch &l) { rounded |= l.kernel.find("kv8_append_kernel") != std::string::npos; };
+        expect(status_of([&] { m.decode(1); }) != 0, "the batch is gone");
+        expect(status_of([&] { generate(m, 64, 16, 4); }) == 0, "the model generates in the memory that it had");
+        expect(rounded == (other == CacheType::E4M3), "from the cache that it had");
+        fake::memory = size_t(1) << 33;
+        rounded = false;
+        expect(status_of([&] { m.set_cache(type); }) == 0, "the type changes where there is memory");
+        generate(m, 64, 16, 4);
+        expect(rounded == (type == CacheType::E4M3), "and the model generates from it");
+        fake::on_launch = nullptr;
+    }
+}
+
 const std::map<std::string, void (*)()> kChecks = {
     {"refused_launches", refused_launches},
     {"foreign_errors", foreign_errors},
     {"scores_without_memory", scores_without_memory},
+    {"cache_without_memory", cache_without_memory},
 };
 
 }  // namespace
