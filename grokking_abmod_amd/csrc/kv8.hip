@@ -412,9 +412,9 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a, int tiles)
 
 template <class T, int PAD>
 void launch_append(const Kv8AppendArgs &a, hipStream_t stream) {
-    const int tiles = (a.count + 126) / 64;  // a run of n tokens touches at most so many
-    hipLaunchKernelGGL((kv8_append_kernel<T, PAD>), dim3(2u * uint32_t(a.cache.batch * a.cache.heads) * uint32_t(tiles)),
-                       dim3(256), 0, stream, a, tiles);
+    const size_t groups = kv8_append_workgroups(size_t(a.cache.batch) * size_t(a.cache.heads), size_t(a.count));
+    const int tiles = int(groups / (2 * size_t(a.cache.batch) * size_t(a.cache.heads)));
+    hipLaunchKernelGGL((kv8_append_kernel<T, PAD>), dim3(uint32_t(groups)), dim3(256), 0, stream, a, tiles);
 }
 
 template <class T, int PAD>

@@ -295,15 +295,19 @@ struct MeshGpt::Impl {
     // sequences go to its layer of the 8-bit cache.
     void keep8(size_t l, size_t b0, size_t nb, const kern::KvView &kv, const int *len, size_t count) {
         kern::Kv8AppendArgs a{};
-        a.cache = cache8_layer(l, b0, nb);
-        a.k = kv.k;
-        a.v = kv.v;
         a.ks = a.vs = Strides{{int64_t(shape.H) * kv.cap * shape.hdp, shape.hdp, int64_t(kv.cap) * shape.hdp}};
-        a.lengths = len;
         a.count = int(count);
         a.absolute = 1;
         a.aligned = shape.hdp % 4 == 0 ? 16 : 0;
-        kern::kv8_append(a, Type::F32, stream);
+        // A launch counts its threads in 32 bits: as many sequences as that allows.
+        const size_t most = std::max<size_t>(1, kern::kLaunchMost / kern::kv8_append_workgroups(size_t(shape.H), count));
+        for (size_t b = 0; b < nb; b += most) {
+            a.cache = cache8_layer(l, b0 + b, std::min(most, nb - b));
+            a.k = kv.k + int64_t(b) * a.ks.s[0];
+            a.v = kv.v + int64_t(b) * a.vs.s[0];
+            a.lengths = len + b;
+            kern::kv8_append(a, Type::F32, stream);
+        }
     }
     // attn_decode over the 8-bit cache.
     void attend8(size_t l, size_t b0, size_t nb, const float *q, const int *len, int nsplit, float *partial) {

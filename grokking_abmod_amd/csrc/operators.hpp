@@ -46,6 +46,10 @@ struct Kv8AppendArgs {
     int aligned;   // of inputs and strides: 16 bytes, 4, or 0 for less
 };
 void kv8_append(const Kv8AppendArgs &a, Type type, hipStream_t stream);
+// Workgroups of an append: a run of n tokens touches at most (n + 126) / 64 tiles.
+inline size_t kv8_append_workgroups(size_t pairs, size_t count) { return 2 * pairs * ((count + 126) / kKv8Tile); }
+// Workgroups of a launch at most: it counts its threads, 256 each, in 32 bits.
+constexpr size_t kLaunchMost = (size_t(1) << 24) - 1;
 
 struct Kv8ReadArgs {
     Kv8 cache;

@@ -209,11 +209,40 @@ void cache_without_memory() {
     }
 }
 
+// A launch counts its threads in 32 bits: where a batch has more rows to quantise,
+// they take several, which between them have every sequence once.
+void many_sequences() {
+    const size_t batch = (1 << 20) + 3;
+    fake::memory = size_t(1) << 40;
+    MeshGpt m(0, shape(32, 8, 2, 1), 7, 1);
+    m.set_cache(CacheType::E4M3);
+    size_t appended = 0, attended = 0;
+    const uint8_t *keys = nullptr;
+    fake::on_launch = [&](const fake::Launch &l) {
+        expect(size_t(l.grid.x) * l.block.x < size_t(1) << 32, "a launch's threads are counted in 32 bits: " + l.kernel);
+        if (l.kernel.find("kv8_append_kernel") != std::string::npos) {
+            const auto *a = static_cast<const kern::Kv8AppendArgs *>(l.args[0]);
+            const int tiles = *static_cast<const int *>(l.args[1]);
+            expect(l.grid.x == 2u * unsigned(a->cache.batch * a->cache.heads * tiles), "a workgroup for each tile");
+            expect(appended % batch == 0 || a->cache.k == keys, "the sequences follow one another");
+            appended += size_t(a->cache.batch);
+            keys = a->cache.k + kv8_code_bytes(a->cache);
+        }
+        if (l.kernel.find("kv8_rows_kernel") != std::string::npos)
+            attended += size_t(static_cast<const kern::Kv8AttnArgs *>(l.args[0])->cache.batch);
+    };
+    generate(m, batch, 1, 2);
+    fake::on_launch = nullptr;
+    expect(appended == 2 * batch && attended == batch, "every sequence once a token");
+    fake::memory = size_t(1) << 33;
+}
+
 const std::map<std::string, void (*)()> kChecks = {
     {"refused_launches", refused_launches},
     {"foreign_errors", foreign_errors},
     {"scores_without_memory", scores_without_memory},
     {"cache_without_memory", cache_without_memory},
+    {"many_sequences", many_sequences},
 };
 
 }  // namespace

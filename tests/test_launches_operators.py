@@ -28,7 +28,8 @@ def checks(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("name", ["refused_launches", "foreign_errors", "scores_without_memory", "cache_without_memory"])
+@pytest.mark.parametrize("name", ["refused_launches", "foreign_errors", "scores_without_memory", "cache_without_memory",
+                                  "many_sequences"])
 def test_launches(checks, name):
     run = subprocess.run([checks, name], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout == "ok\n", run.stdout + run.stderr
