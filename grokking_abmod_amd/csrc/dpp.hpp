@@ -27,6 +27,17 @@ __device__ __forceinline__ float wave_sum(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+// The largest value of the wave, in every lane, by the same moves.
+__device__ __forceinline__ float wave_largest(float v) {
+    v = fmaxf(v, dpp_move<0xB1>(v, v));
+    v = fmaxf(v, dpp_move<0x4E>(v, v));
+    v = fmaxf(v, dpp_move<0x141>(v, v));
+    v = fmaxf(v, dpp_move<0x140>(v, v));
+    v = fmaxf(v, dpp_move<0x142, 0xa>(v, v));
+    v = fmaxf(v, dpp_move<0x143, 0xc>(v, v));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 // wave_sum of eight values at once: lane l returns the sum over the wave of
 // v[l & 7].  The lanes add the same pairs level by level as wave_sum does
 // (lane bits 0, 1, 2, 3, 4, 5), and f32 addition is commutative, so every

@@ -69,16 +69,6 @@ __device__ __forceinline__ uint32_t lowered4(uint32_t w, int drop) {
     return encode4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
 }
 
-__device__ __forceinline__ float wave_largest(float v) {
-    v = fmaxf(v, dpp_move<0xB1>(v, v));
-    v = fmaxf(v, dpp_move<0x4E>(v, v));
-    v = fmaxf(v, dpp_move<0x141>(v, v));
-    v = fmaxf(v, dpp_move<0x140>(v, v));
-    v = fmaxf(v, dpp_move<0x142, 0xa>(v, v));
-    v = fmaxf(v, dpp_move<0x143, 0xc>(v, v));
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
-
 // N consecutive elements from p (N of 16 bytes, or two), those at or past `have`
 // as 0.  Aligned: to 16 bytes, so that whole groups are aligned to their size, to
 // 4, or (0) to the element.

@@ -14,15 +14,18 @@
 // to a quarter more where products do (4 prompts of 4096: 586 us, 753).  Scores, maxima,
 // sums and outputs are FP32.
 //
-// A wave takes tiles of 64 keys for 16 query rows at a time; query heads that
-// share a cached head are rows of the same tile.  The scores are computed
-// transposed, S^T = K Q^T: a lane then holds 16 keys of one row, all of them in
-// one block of 16 tokens when the rows of K are taken in the order
-// 16 (m / 4) + 4 t + m % 4 for matrix row m of product t.  So one scale of the
-// keys and one of the values serve a lane, the maximum and the sum need two lane
-// exchanges, and the probabilities are where the second product, O^T = V^T P^T,
-// takes them: nothing moves between lanes.  Its values come in 16-byte loads
-// because the cache holds them transposed.
+// A wave takes tiles of 64 keys for 16 query rows at a time (few rows,
+// kv8_rows_kernel) or 32 (prompts, kv8_tiles_kernel); query heads that share a
+// cached head are rows of the same tile.  The scores are computed transposed,
+// S^T = K Q^T: a lane then holds 16 keys of one row, all of them in one block of 16
+// tokens, when the rows of K are taken in the right order: of 16 rows 16 (m / 4) +
+// 4 t + m % 4 for matrix row m of product t, of 32 rows 16 (m / 4 % 2) + 4 (m / 8) +
+// m % 4 for row m.  So one scale of the keys and one of the values serve a lane, the
+// maximum needs two lane exchanges (one), and the probabilities are where the second
+// product, O^T = V^T P^T, takes them: nothing moves between lanes.  Its values come
+// in 16-byte loads because the cache holds them transposed.  The sums of 16 rows are
+// a product with ones, those of 32 are added in each lane and exchanged once at the
+// end.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -292,7 +295,7 @@ __device__ __forceinline__ void fill_nan(const Kv8AttnArgs &a, const Sequence &s
 // the end.  The bytes of the cache bound it: 64 sequences of 2000 to 16000 tokens,
 // 32 heads over 8 of 128, BF16, take 233 us (5.0 TB/s).
 template <class T, int PAD>
-__global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, int pairs, int row_tiles) {
+__global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, int pairs) {
     constexpr int NQ = kQueryPieces<T>, NP = kProbPieces<T>, STEPS = PAD / 32, DT = PAD / 16;
     constexpr int WORDS = PAD >= 64 ? PAD / 16 : 2;  // 4-byte words of a key that a lane holds
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
@@ -486,8 +489,8 @@ __device__ __forceinline__ void paced() {
     }
 }
 
-// As soften(), mark_nan() and load_queries() for the products of 32 x 32: a lane
-// holds 16 keys of a row in each 32, one block of 16 tokens, and a row is two lanes.
+// As soften() and mark_nan() for the products of 32 x 32: a lane holds 16 keys of a
+// row in each 32, one block of 16 tokens, and a row is two lanes.
 template <int NP, int SUB>
 __device__ __forceinline__ float soften32(f32x16 (&st)[SUB], bool masked, float (&kscale)[SUB], float slack,
                                           const int (&key0)[SUB], int place, float &m, float &l, bf16x8 (&pf)[SUB][NP][2]) {
@@ -810,7 +813,7 @@ void launch_attn(const Kv8AttnArgs &a, const Kv8Plan &plan, hipStream_t stream) 
                            stream, a, pairs, pairs8, plan.row_tiles);
     } else {
         hipLaunchKernelGGL((kv8_rows_kernel<T, PAD>), dim3(uint32_t(pairs) * uint32_t(a.splits) * uint32_t(plan.row_tiles)),
-                           dim3(64 * kWaves), 0, stream, a, pairs, plan.row_tiles);
+                           dim3(64 * kWaves), 0, stream, a, pairs);
     }
     if (a.out && a.splits > 1)
         hipLaunchKernelGGL((kv8_join_kernel<T, PAD>), dim3(uint32_t((int64_t(pairs) * a.rows * (PAD / 4) + 255) / 256)),

@@ -87,18 +87,8 @@ __device__ __forceinline__ void add(float x, float base, float c, float &s, floa
     a = fmaf(e, d, a);
 }
 
-__device__ __forceinline__ float wave_top(float v) {
-    v = fmaxf(v, dpp_move<0xB1>(v, v));
-    v = fmaxf(v, dpp_move<0x4E>(v, v));
-    v = fmaxf(v, dpp_move<0x141>(v, v));
-    v = fmaxf(v, dpp_move<0x140>(v, v));
-    v = fmaxf(v, dpp_move<0x142, 0xa>(v, v));
-    v = fmaxf(v, dpp_move<0x143, 0xc>(v, v));
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
-
 __device__ __forceinline__ void wave_join(Sums &t, float c) {
-    t.raise(wave_top(t.m), c);
+    t.raise(wave_largest(t.m), c);
     t.s = wave_sum(t.s);
     t.a = wave_sum(t.a);
 }

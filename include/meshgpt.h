@@ -207,7 +207,8 @@ int mg_last_call_ms(mg_model *model, float *ms);
  * type stays what it was.  With 8 bits prompts attend in FP32 and are then
  * quantised, and decode steps attend over the quantised keys and values (the
  * exclusive projection keeps a token's own value in FP32), on the per-phase
- * kernels: mg_decode_traced and mg_decode_rewind return MG_UNSUPPORTED.  Head widths up to 256.  No reference counterpart. */
+ * kernels: mg_decode_traced and mg_decode_rewind return MG_UNSUPPORTED.  Head
+ * widths up to 256.  No reference counterpart. */
 enum { MG_CACHE_F32 = 0, MG_CACHE_E4M3 = 1 };
 int mg_set_cache(mg_model *model, int type);
 /* Current tokens per sequence (prompt + generated). */
