@@ -15,9 +15,10 @@
 // token's inputs.  Values are stored transposed, 64 tokens of a channel in a row, the
 // order in which the attention's matrix product reads them; a lane takes two
 // channels of the 16 tokens.  Memory bounds both where there is enough of it: 8
-// prompts of up to 4000 tokens, 8 heads of 128, BF16, are written in 32 us (3.8
-// TB/s read and written), 16 caches of 8000 tokens read back as F16 in 135 us (5.8
-// TB/s); a step of 32 sequences takes 4.6 us.
+// prompts of up to 4000 tokens, 8 heads of 128, BF16, are written in 37 us (3.3 TB/s
+// read and written), or in 32 where the inputs lie in the Infinity Cache; 16 caches
+// of 8000 tokens are read back as F16 in 135 us (5.8 TB/s); a step of 32 sequences
+// takes 4.6 us.
 #include <hip/hip_runtime.h>
 
 #include <cfloat>

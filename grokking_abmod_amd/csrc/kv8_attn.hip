@@ -5,14 +5,14 @@
 // so keys and values go there as codes, two an instruction, and their scales
 // meet the scores in FP32 and the values, exactly, in their conversion.  Queries
 // go there exactly: as one BF16 (BF16 calls), two (F16) or three (F32).
-// Probabilities go there as two in 16-bit calls, which leaves 2^-15 of each, or as
+// Probabilities go there as two in 16-bit calls, which leaves 2^-16 of each, or as
 // three in F32 calls, which leaves nothing.  Each piece is a product of its own.
 // One BF16 would leave 2^-8 of each probability, as much as the output's own
-// rounding: the error against 64 bits was then 1.35 times that of the output's
-// rounding alone.  The second piece takes nothing where memory bounds (64 sequences of
-// 2000 to 16000 tokens, 32 heads over 8 of 128: 231 us with one, 232 with two) and up
-// to a quarter more where products do (4 prompts of 4096: 586 us, 753).  Scores, maxima,
-// sums and outputs are FP32.
+// rounding: BF16 calls were then off by 0.0023 against 64 bits (root mean square),
+// by 0.0017 with two, which is the output's rounding.  The second piece takes nothing
+// where memory bounds (64 sequences of 2000 to 16000 tokens, 32 heads over 8 of 128:
+// 229 us either way) and a third more where products do (4 prompts of 4096: 575 us
+// with one, 758 with two).  Scores, maxima, sums and outputs are FP32.
 //
 // A wave takes tiles of 64 keys for 16 query rows at a time (few rows,
 // kv8_rows_kernel) or 32 (prompts, kv8_tiles_kernel); query heads that share a
@@ -293,7 +293,8 @@ __device__ __forceinline__ void fill_nan(const Kv8AttnArgs &a, const Sequence &s
 // Up to 16 rows of a pair a workgroup, as in single tokens: its waves take the
 // key tiles in turn, straight from memory into operands, and join their states at
 // the end.  The bytes of the cache bound it: 64 sequences of 2000 to 16000 tokens,
-// 32 heads over 8 of 128, BF16, take 233 us (5.0 TB/s).
+// 32 heads over 8 of 128, BF16, take 224 to 231 us (5.1 to 5.3 TB/s; each byte is
+// fetched once, and the matrix units are busy for a ninth of the time).
 template <class T, int PAD>
 __global__ void __launch_bounds__(64 * kWaves) kv8_rows_kernel(Kv8AttnArgs a, int pairs) {
     constexpr int NQ = kQueryPieces<T>, NP = kProbPieces<T>, STEPS = PAD / 32, DT = PAD / 16;
@@ -577,10 +578,12 @@ __device__ __forceinline__ void mark_nan32(const uint8_t *vpair, int from, int t
 // bytes a lane.  The products are of 32 x 32: the vector unit waits less for them
 // than for 16 x 16 (beside as many exponentials a product of the same size took 12.9
 // cycles against 22).  SUB times 32 keys are softened together, as the registers
-// allow.  The matrix unit and the exponentials bound it, which two waves a SIMD
-// hardly overlap: 4 prompts of 4096, 32 heads over 8 of 128, BF16, take 580 us, 0.95
-// PFLOP/s; 3 ragged ones of up to 1001 behind up to 500, 8 heads of 64, F32 with
-// three products each, 31 us.
+// allow.  The matrix unit and the vector unit bound it, which two waves a SIMD hardly
+// overlap: 4 prompts of 4096, 32 heads over 8 of 128, BF16, take 755 us, 1.09 PFLOP/s of
+// the three products, with the matrix units busy for 52 % of the cycles and the
+// vector units for about as many; 3 ragged ones of up to 1001 behind up to 500, 8
+// heads of 64, F32 with three products each, 31 us.  Width 256 leaves one wave a SIMD
+// and in F32 not registers enough even so: 48 of them are spilled (196 bytes a lane).
 template <class T, int PAD, int SUB>
 __global__ void __launch_bounds__(64 * kWaves, PAD == 256 ? 1 : 2)
 kv8_tiles_kernel(Kv8AttnArgs a, int pairs, int pairs8, int row_tiles) {
@@ -838,9 +841,9 @@ Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count) {
     const int pairs = std::max(1, cache.batch * cache.heads);
     // Up to some rows the waves of a workgroup do better to split the keys of 16,
     // for all that several such workgroups read the same keys (us, split; not): 128 x
-    // 8000 keys of 128, 20 rows BF16 89; 68, F32 90; 109, 64 rows BF16 157; 85, F32
-    // 159; 151; 32 x 4000 keys of 64, 40 rows BF16 17.3; 20.4, F32 20.5; 27.5; 8 x 16000,
-    // 64 rows BF16 19.3; 24.1.
+    // 8000 keys of 128, 20 rows BF16 90; 67, F16 89; 79, F32 91; 104, 64 rows BF16 163;
+    // 96, F32 161; 153; 32 x 4000 keys of 64, 40 rows BF16 18.1; 22.7, F32 19.1; 25.9; 8 x
+    // 16000, 64 rows BF16 20.3; 32.7.
     p.wide = rows > (cache.pad <= 64 ? 64 : type == Type::F32 ? 32 : 16);
     const int each = p.wide ? 32 * kWaves : 16;
     p.row_tiles = int((rows + each - 1) / each);
@@ -849,13 +852,13 @@ Kv8Plan kv8_plan(const Kv8 &cache, Type type, int group, int count) {
         // As many shares as the resident workgroups hold, two a CU, but one of width
         // 256 and three in F32 of width 64: fewer leave CUs without work, more go
         // over their rows' states again (us with 2; 3; 4; 5; 6 shares: 128 groups of
-        // BF16 rows of 64, 4000 keys, 46.0; 43.4; 40.8; 41.4; 40.2, of F32 rows
-        // 70.8; 68.9; 61.3; 64.3; 59.5; 152 of F16 rows of 128, 4000 keys, 109; 86;
-        // 102; 90; 93; 64 of BF16 rows of 256, 1500 keys, 54.0; 46.9; 42.9; 54.6; 55.0).
+        // BF16 rows of 64, 4000 keys, 58.5; 54.3; 48.8; 50.6; 46.8, of F32 rows
+        // 74.5; 72.5; 62.4; 63.4; 59.3; 152 of F16 rows of 128, 4000 keys, 102; 110;
+        // 98; 99; 108; 64 of BF16 rows of 256, 1500 keys, 64.7; 53.4; 47.1; 61.0; 61.1).
         // The join is a launch of its own, some 6 us with what it waits for, so a
         // share is 4 tiles or more, and shares spare 10 or more (32 groups of
-        // BF16 rows of 64, 1024 keys: 22.5 us in one, 19.4 in four; 256 of up to 1000:
-        // 23.3 in one, 28.9 in two).
+        // BF16 rows of 64, 1024 keys: 26.8 us in one, 18.9 in four; 256 of up to 1000:
+        // 30.3 in one, 34.8 in two).
         const int64_t resident = 256 * (cache.pad == 256 ? 1 : cache.pad == 64 && type == Type::F32 ? 3 : 2);
         p.least = 4;
         p.splits = int(std::max<int64_t>(1, std::min(tiles / p.least, resident / groups)));

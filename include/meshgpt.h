@@ -202,8 +202,10 @@ int mg_decode_rewind(mg_model *model);
  * a decode launch without the host's synchronisation. */
 int mg_last_call_ms(mg_model *model, float *ms);
 /* What the model's KV cache holds: MG_CACHE_F32 (the default), or MG_CACHE_E4M3,
- * an 8-bit cache as of mg_kv8_append, a quarter of the bytes that a decode step
- * reads.  A change drops the current batch; where there is no memory for it, the
+ * an 8-bit cache as of mg_kv8_append: from head widths of 17 on a quarter of the
+ * bytes that a decode step reads (rows are padded to 32 bytes at least, so width 16
+ * reads half, width 8 as much).  Beside it stay two layers in FP32, from which rows
+ * are quantised: models of up to two layers hold more than before.  A change drops the current batch; where there is no memory for it, the
  * type stays what it was.  With 8 bits prompts attend in FP32 and are then
  * quantised, and decode steps attend over the quantised keys and values (the
  * exclusive projection keeps a token's own value in FP32), on the per-phase
@@ -306,7 +308,7 @@ int mg_kv8_read(int device, const mg_kv8 *cache, int type, size_t first, size_t 
  * sees makes what depends on it NaN; what it does not see has no effect.  The rows
  * of a sequence whose length or count is impossible (as above) are filled with
  * NaN, all `count` of them.  F32 calls keep 24 bits of the queries and
- * probabilities, F16 and BF16 calls 15 bits of the probabilities; scores, and the
+ * probabilities, F16 and BF16 calls 16 bits of the probabilities; scores, and the
  * sums of probabilities and of values before they are divided, are FP32 and have
  * to stay in its range.  The workspace holds mg_kv8_attention_workspace bytes,
  * aligned to 16 (NULL where that is 0). */
