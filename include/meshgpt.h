@@ -205,12 +205,12 @@ int mg_last_call_ms(mg_model *model, float *ms);
  * an 8-bit cache as of mg_kv8_append: from head widths of 17 on a quarter of the
  * bytes that a decode step reads (rows are padded to 32 bytes at least, so width 16
  * reads half, width 8 as much).  Beside it stay two layers in FP32, from which rows
- * are quantised: models of up to two layers hold more than before.  A change drops the current batch; where there is no memory for it, the
- * type stays what it was.  With 8 bits prompts attend in FP32 and are then
- * quantised, and decode steps attend over the quantised keys and values (the
- * exclusive projection keeps a token's own value in FP32), on the per-phase
- * kernels: mg_decode_traced and mg_decode_rewind return MG_UNSUPPORTED.  Head
- * widths up to 256.  No reference counterpart. */
+ * are quantised: models of up to two layers hold more than before.  A change drops
+ * the current batch; where there is no memory for it, the type stays what it was.
+ * With 8 bits prompts attend in FP32 and are then quantised, and decode steps attend
+ * over the quantised keys and values (the exclusive projection keeps a token's own
+ * value in FP32), on the per-phase kernels: mg_decode_traced and mg_decode_rewind
+ * return MG_UNSUPPORTED.  Head widths up to 256.  No reference counterpart. */
 enum { MG_CACHE_F32 = 0, MG_CACHE_E4M3 = 1 };
 int mg_set_cache(mg_model *model, int type);
 /* Current tokens per sequence (prompt + generated). */
