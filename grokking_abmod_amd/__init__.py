@@ -32,11 +32,15 @@ EXPORTS = (
     "mg_kv8_sizes", "mg_kv8_append", "mg_kv8_read", "mg_kv8_attention_workspace", "mg_kv8_attention",
     "mg_token_logprobs_workspace", "mg_token_logprobs_noalloc", "mg_token_logprobs_backward_noalloc",
     "mg_token_logprobs", "mg_set_cache",
+    "mg_sample_filtered_noalloc", "mg_rope_frequencies", "mg_rope_apply", "mg_rope_backward",
+    "mg_rms_norm", "mg_rms_norm_e4m3", "mg_rms_norm_backward_workspace", "mg_rms_norm_backward",
 )
 
 MG_F32, MG_F16, MG_BF16 = range(3)  # element types of the device operators
 TOP_MAX = 32  # MG_TOP_MAX
 MG_CACHE_F32, MG_CACHE_E4M3 = range(2)  # what a model's KV cache holds
+MG_ROPE_HALF, MG_ROPE_INTERLEAVED = range(2)  # which channels are a pair
+MG_ROPE_UNSCALED, MG_ROPE_LINEAR, MG_ROPE_BASE, MG_ROPE_BANDS = range(4)  # frequencies for longer contexts
 
 IGNORE_TARGET = 0xFFFFFFFF  # MG_IGNORE_TARGET (src/gpt/mod.rs:26)
 
@@ -90,6 +94,13 @@ class Kv8(ctypes.Structure):
         (name, ctypes.c_void_p) for name in ("k", "v", "k_scale", "v_scale")]
 
 
+class Rope(ctypes.Structure):
+    """mg_rope: how heads turn; `frequencies` is a device pointer (an int)."""
+
+    _fields_ = [(name, ctypes.c_uint32) for name in ("head_width", "rotary", "layout")] + [
+        ("magnitude", ctypes.c_float), ("frequencies", ctypes.c_void_p)]
+
+
 class MeshGptError(RuntimeError):
     def __init__(self, status, message):
         super().__init__(message)
@@ -102,7 +113,9 @@ _f32p = ctypes.POINTER(ctypes.c_float)
 _szp = ctypes.POINTER(ctypes.c_size_t)
 _cfgp = ctypes.POINTER(GptConfig)
 _kv8p = ctypes.POINTER(Kv8)
+_ropep = ctypes.POINTER(Rope)
 _strides = ctypes.c_int64 * 3
+_stridesp = ctypes.POINTER(ctypes.c_int64)  # or None
 _lib = None
 
 
@@ -116,6 +129,7 @@ def lib():
                           "(or make -C grokking_abmod_amd/csrc)")
     L = ctypes.CDLL(LIB_PATH)
     vp, sz, i, u64, f = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint64, ctypes.c_float
+    d = ctypes.c_double
     sigs = {
         "mg_last_error": (ctypes.c_char_p, []),
         "mg_config_default": (None, [_cfgp]),
@@ -174,6 +188,16 @@ def lib():
         "mg_token_logprobs_workspace": (i, [sz, sz, sz, _szp]),
         "mg_token_logprobs_noalloc": (i, [i, i, vp, sz, sz, sz, vp, f, vp, vp, vp, sz, vp, vp, vp, sz, vp]),
         "mg_token_logprobs_backward_noalloc": (i, [i, i, vp, sz, sz, sz, vp, f, vp, vp, vp, vp, vp, sz, vp]),
+        "mg_sample_filtered_noalloc": (i, [i, i, vp, sz, sz, sz, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "mg_rope_frequencies": (i, [sz, d, i, d, d, d, d, ctypes.POINTER(d)]),
+        "mg_rope_apply": (i, [i, _ropep, i, sz, sz, sz, vp, _stridesp, vp, _stridesp, sz, vp, _stridesp, vp, _stridesp, vp,
+                              vp, vp, vp]),
+        "mg_rope_backward": (i, [i, _ropep, i, sz, sz, sz, vp, _stridesp, vp, _stridesp, sz, vp, _stridesp, vp, _stridesp,
+                                 vp, vp, vp, vp]),
+        "mg_rms_norm": (i, [i, i, sz, sz, vp, sz, vp, sz, vp, sz, vp, f, vp, sz, vp, vp]),
+        "mg_rms_norm_e4m3": (i, [i, i, sz, sz, vp, sz, vp, sz, vp, sz, vp, f, vp, sz, vp, sz, vp, vp]),
+        "mg_rms_norm_backward_workspace": (i, [sz, sz, _szp]),
+        "mg_rms_norm_backward": (i, [i, i, sz, sz, vp, sz, vp, vp, vp, sz, vp, sz, vp, sz, vp, vp, sz, vp]),
         "mg_token_logprobs": (i, [i, _f32p, sz, sz, _u32p, f, _f32p, _f32p, sz, _u32p, _f32p]),
     }
     for name, (res, args) in sigs.items():
@@ -326,6 +350,71 @@ def token_logprobs(logits, tokens, temperature=1.0, top=0, device=0):
     _check(lib().mg_token_logprobs(device, _p(logits, _f32p), rows, vocab, _p(tokens, _u32p), temperature,
                                    _p(logprob, _f32p), _p(entropy, _f32p), top, _p(ids, _u32p), _p(best, _f32p)))
     return logprob, entropy, ids, best
+
+
+def sample_filtered_noalloc(type, logits, rows, vocab, stride, temperatures, top_k, top_p, min_p, uniforms, tokens,
+                            logprob=None, stream=None, device=0):
+    """mg_sample_filtered_noalloc on device pointers (ints), None for what is not
+    wanted; enqueued on `stream`."""
+    _check(lib().mg_sample_filtered_noalloc(device, type, logits, rows, vocab, stride, temperatures, top_k, top_p, min_p,
+                                            uniforms, tokens, logprob, stream))
+
+
+def rope_frequencies(rotary, base=10000.0, scaling=MG_ROPE_UNSCALED, factor=1.0, context=0.0, low=1.0, high=32.0):
+    """mg_rope_frequencies: radians a position of each pair, for a device array of doubles."""
+    out = np.empty(rotary // 2, dtype=np.float64)
+    _check(lib().mg_rope_frequencies(rotary, base, scaling, factor, context, low, high,
+                                     _p(out, ctypes.POINTER(ctypes.c_double))))
+    return out
+
+
+def rope(rope, type, batch, count, heads, q, q_strides, q_out, q_out_strides, kv_heads, k, k_strides, k_out, k_out_strides,
+         lengths=None, counts=None, positions=None, stream=None, device=0):
+    """mg_rope_apply on device pointers (ints); strides are (sequence, token, head)
+    in elements, of what has 0 heads None; enqueued on `stream`."""
+    _check(lib().mg_rope_apply(device, rope, type, batch, count, heads, q, _three(q_strides), q_out, _three(q_out_strides),
+                               kv_heads, k, _three(k_strides), k_out, _three(k_out_strides), lengths, counts, positions,
+                               stream))
+
+
+def rope_backward(rope, type, batch, count, heads, d_q_out, d_q_out_strides, d_q, d_q_strides, kv_heads, d_k_out,
+                  d_k_out_strides, d_k, d_k_strides, lengths=None, counts=None, positions=None, stream=None, device=0):
+    """mg_rope_backward on device pointers (ints); enqueued on `stream`."""
+    _check(lib().mg_rope_backward(device, rope, type, batch, count, heads, d_q_out, _three(d_q_out_strides), d_q,
+                                  _three(d_q_strides), kv_heads, d_k_out, _three(d_k_out_strides), d_k,
+                                  _three(d_k_strides), lengths, counts, positions, stream))
+
+
+def _three(strides):
+    return None if strides is None else _strides(*strides)
+
+
+def rms_norm(type, rows, width, x, x_stride, residual, residual_stride, sum, sum_stride, weight, epsilon, out, out_stride,
+             rstd=None, stream=None, device=0):
+    """mg_rms_norm on device pointers (ints), None for what there is not; enqueued on `stream`."""
+    _check(lib().mg_rms_norm(device, type, rows, width, x, x_stride, residual, residual_stride, sum, sum_stride, weight,
+                             epsilon, out, out_stride, rstd, stream))
+
+
+def rms_norm_e4m3(type, rows, width, x, x_stride, residual, residual_stride, sum, sum_stride, weight, epsilon, codes,
+                  codes_stride, scales, scales_stride, rstd=None, stream=None, device=0):
+    """mg_rms_norm_e4m3 on device pointers (ints), None for what there is not; enqueued on `stream`."""
+    _check(lib().mg_rms_norm_e4m3(device, type, rows, width, x, x_stride, residual, residual_stride, sum, sum_stride,
+                                  weight, epsilon, codes, codes_stride, scales, scales_stride, rstd, stream))
+
+
+def rms_norm_backward_workspace(rows, width):
+    """mg_rms_norm_backward_workspace: bytes of scratch that a call with d_weight needs."""
+    n = ctypes.c_size_t()
+    _check(lib().mg_rms_norm_backward_workspace(rows, width, ctypes.byref(n)))
+    return n.value
+
+
+def rms_norm_backward(type, rows, width, sum, sum_stride, weight, rstd, d_out, d_out_stride, d_sum, d_sum_stride, d_x,
+                      d_x_stride, d_weight=None, workspace=None, workspace_bytes=0, stream=None, device=0):
+    """mg_rms_norm_backward on device pointers (ints), None for what there is not; enqueued on `stream`."""
+    _check(lib().mg_rms_norm_backward(device, type, rows, width, sum, sum_stride, weight, rstd, d_out, d_out_stride, d_sum,
+                                      d_sum_stride, d_x, d_x_stride, d_weight, workspace, workspace_bytes, stream))
 
 
 def device_expf(x, device=0):

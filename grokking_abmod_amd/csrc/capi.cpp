@@ -133,6 +133,15 @@ Strides to_strides(const int64_t *s) {
     return Strides{{s[0], s[1], s[2]}};
 }
 
+Rope to_rope(const mg_rope *r) {
+    require(r != nullptr, "rope must not be null");
+    require(r->layout <= 1, "unknown rotary layout code");
+    return Rope{r->head_width, r->rotary, r->layout == MG_ROPE_INTERLEAVED, r->magnitude, r->frequencies};
+}
+
+// Of queries or keys that a call may go without.
+Strides side_strides(size_t heads, const int64_t *s) { return heads ? to_strides(s) : Strides{{0, 0, 0}}; }
+
 }  // namespace
 
 extern "C" {
@@ -477,6 +486,80 @@ int mg_token_logprobs(int device, const float *logits, size_t rows, size_t vocab
     return guarded([&] {
         token_logprobs(device, logits, rows, vocab, tokens, temperature, logprob, entropy, top, top_tokens,
                        top_logprobs);
+    });
+}
+
+int mg_sample_filtered_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab, size_t stride,
+                               const float *temperatures, const int32_t *top_k, const float *top_p, const float *min_p,
+                               const float *uniforms, uint32_t *tokens, float *logprob, void *stream) {
+    return guarded([&] {
+        sample_filtered_noalloc(device, Type(type), logits, rows, vocab, stride, temperatures, top_k, top_p, min_p,
+                                uniforms, tokens, logprob, static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_rope_frequencies(size_t rotary, double base, int scaling, double factor, double context, double low, double high,
+                        double *out) {
+    return guarded([&] { rope_frequencies(rotary, base, RopeScaling(scaling), factor, context, low, high, out); });
+}
+
+int mg_rope_apply(int device, const mg_rope *r, int type, size_t batch, size_t count, size_t heads, const void *q,
+                  const int64_t q_strides[3], void *q_out, const int64_t q_out_strides[3], size_t kv_heads, const void *k,
+                  const int64_t k_strides[3], void *k_out, const int64_t k_out_strides[3], const int32_t *lengths,
+                  const int32_t *counts, const int32_t *positions, void *stream) {
+    return guarded([&] {
+        rope(device, to_rope(r), Type(type), batch, count, heads, q, side_strides(heads, q_strides), q_out,
+             side_strides(heads, q_out_strides), kv_heads, k, side_strides(kv_heads, k_strides), k_out,
+             side_strides(kv_heads, k_out_strides), lengths, counts, positions, false, static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_rope_backward(int device, const mg_rope *r, int type, size_t batch, size_t count, size_t heads,
+                     const void *d_q_out, const int64_t d_q_out_strides[3], void *d_q, const int64_t d_q_strides[3],
+                     size_t kv_heads, const void *d_k_out, const int64_t d_k_out_strides[3], void *d_k,
+                     const int64_t d_k_strides[3], const int32_t *lengths, const int32_t *counts,
+                     const int32_t *positions, void *stream) {
+    return guarded([&] {
+        rope(device, to_rope(r), Type(type), batch, count, heads, d_q_out, side_strides(heads, d_q_out_strides), d_q,
+             side_strides(heads, d_q_strides), kv_heads, d_k_out, side_strides(kv_heads, d_k_out_strides), d_k,
+             side_strides(kv_heads, d_k_strides), lengths, counts, positions, true, static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_rms_norm(int device, int type, size_t rows, size_t width, const void *x, size_t x_stride, const void *residual,
+                size_t residual_stride, void *sum, size_t sum_stride, const void *weight, float epsilon, void *out,
+                size_t out_stride, float *rstd, void *stream) {
+    return guarded([&] {
+        rms_norm(device, Type(type), rows, width, x, x_stride, residual, residual_stride, sum, sum_stride, weight,
+                 epsilon, out, out_stride, rstd, static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_rms_norm_e4m3(int device, int type, size_t rows, size_t width, const void *x, size_t x_stride,
+                     const void *residual, size_t residual_stride, void *sum, size_t sum_stride, const void *weight,
+                     float epsilon, uint8_t *codes, size_t codes_stride, uint8_t *scales, size_t scales_stride,
+                     float *rstd, void *stream) {
+    return guarded([&] {
+        rms_norm_e4m3(device, Type(type), rows, width, x, x_stride, residual, residual_stride, sum, sum_stride, weight,
+                      epsilon, codes, codes_stride, scales, scales_stride, rstd, static_cast<hipStream_t>(stream));
+    });
+}
+
+int mg_rms_norm_backward_workspace(size_t rows, size_t width, size_t *bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "output must not be null");
+        *bytes = rms_norm_backward_workspace(rows, width);
+    });
+}
+
+int mg_rms_norm_backward(int device, int type, size_t rows, size_t width, const void *sum, size_t sum_stride,
+                         const void *weight, const float *rstd, const void *d_out, size_t d_out_stride,
+                         const void *d_sum, size_t d_sum_stride, void *d_x, size_t d_x_stride, float *d_weight,
+                         void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        rms_norm_backward(device, Type(type), rows, width, sum, sum_stride, weight, rstd, d_out, d_out_stride, d_sum,
+                          d_sum_stride, d_x, d_x_stride, d_weight, workspace, workspace_bytes,
+                          static_cast<hipStream_t>(stream));
     });
 }
 

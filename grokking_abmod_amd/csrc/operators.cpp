@@ -1,50 +1,13 @@
 // The checked entry points of the operators on device buffers: arguments are
 // looked at, the work is enqueued on the caller's stream, and the caller's
 // current device is what it was.
-#include "operators.hpp"
+#include "operators_host.hpp"
 
 #include <algorithm>
 #include <cmath>
-#include <string>
-
-#include "meshgpt_types.hpp"
 
 namespace meshgpt {
 namespace {
-
-void check(hipError_t e, const char *what) {
-    if (e == hipSuccess) return;
-    (void)hipGetLastError();  // reported here
-    throw Error(std::string(what) + ": " + hipGetErrorString(e), e == hipErrorOutOfMemory ? kOutOfMemory : kDeviceError);
-}
-
-void require(bool ok, const char *message) {
-    if (!ok) throw Error(message);
-}
-
-// `device` is the current device while this lives.  What earlier calls left as
-// the thread's last error is not this call's.
-class OnDevice {
-  public:
-    explicit OnDevice(int device) {
-        int count = 0;
-        check(hipGetDeviceCount(&count), "hipGetDeviceCount");
-        if (device < 0 || device >= count) throw Error("invalid device ordinal", kDeviceError);
-        check(hipGetDevice(&caller_), "hipGetDevice");
-        switched_ = caller_ != device;
-        if (switched_) check(hipSetDevice(device), "hipSetDevice");
-        (void)hipGetLastError();
-    }
-    ~OnDevice() {
-        if (switched_) (void)hipSetDevice(caller_);
-    }
-    OnDevice(const OnDevice &) = delete;
-    OnDevice &operator=(const OnDevice &) = delete;
-
-  private:
-    int caller_ = 0;
-    bool switched_ = false;
-};
 
 class Buffer {
   public:
@@ -60,32 +23,6 @@ class Buffer {
   private:
     void *p_ = nullptr;
 };
-
-void check_type(Type type) {
-    require(type == Type::F32 || type == Type::F16 || type == Type::BF16, "unknown element type code");
-}
-
-bool aligned_to(int bytes, const void *p, const Strides &s, Type type) {
-    const int64_t size = int64_t(type_size(type));
-    bool ok = reinterpret_cast<uintptr_t>(p) % size_t(bytes) == 0;
-    for (int64_t v : s.s) ok = ok && v % bytes * size % bytes == 0;
-    return ok;
-}
-// 16, 4, or 0 for less.
-int alignment(const void *k, const Strides &ks, const void *v, const Strides &vs, Type type) {
-    for (int bytes : {16, 4})
-        if (aligned_to(bytes, k, ks, type) && aligned_to(bytes, v, vs, type)) return bytes;
-    return 0;
-}
-
-void check_aligned(const void *p, Type type, const char *message) {
-    require(reinterpret_cast<uintptr_t>(p) % type_size(type) == 0, message);
-}
-
-// A launch counts its threads, 256 a workgroup, in 32 bits.
-void check_grid(double workgroups) {
-    require(workgroups < double(1u << 24), "the call is too large for one launch");
-}
 
 void check_count(const Kv8 &cache, size_t count) {
     require(count <= size_t(cache.capacity), "count must not exceed the cache's capacity");

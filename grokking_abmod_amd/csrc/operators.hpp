@@ -1,7 +1,8 @@
 // Operators on device buffers that the caller owns: the 8-bit KV cache with
-// its attention (kv8.hip, kv8_attn.hip) and the log probabilities of tokens
-// with their gradient (logprobs.hip).  Host code (operators.cpp, model.cpp)
-// calls only these.
+// its attention (kv8.hip, kv8_attn.hip), the log probabilities of tokens with
+// their gradient (logprobs.hip), sampling with filters (sample.hip), rotary
+// positions (rope.hip) and the root-mean-square norm (norm.hip).  Host code
+// (operators.cpp, step_operators.cpp, model.cpp) calls only these.
 #pragma once
 
 #include <hip/hip_runtime_api.h>
@@ -120,6 +121,61 @@ struct LogprobBackwardArgs {
 };
 void token_logprobs_backward(const LogprobBackwardArgs &a, Type type, hipStream_t stream);
 
+struct SampleArgs {
+    const void *logits;
+    size_t rows, vocab, stride;
+    // One a row; null: temperature 1, no filter.
+    const float *temperatures;
+    const int *top_k;
+    const float *top_p, *min_p;
+    const float *uniforms;
+    uint32_t *tokens;
+    float *logprob;  // null: not wanted
+};
+void sample_filtered(const SampleArgs &a, Type type, hipStream_t stream);
+
+struct RopeSide {  // queries or keys
+    const void *x;
+    void *out;
+    Strides xs, os;
+    int heads;
+};
+struct RopeArgs {
+    RopeSide side[2];
+    const double *frequencies;  // radians a position, of each pair
+    float magnitude;
+    const int *lengths, *counts, *positions;  // null: none, `count` each, by the lengths
+    int batch, count, width, rotary;
+    bool interleaved, backward;
+};
+void rope(const RopeArgs &a, Type type, hipStream_t stream);
+
+struct NormArgs {
+    const void *x, *residual;  // residual null: none
+    void *sum;                 // null: not kept
+    const void *weight;        // null: 1
+    void *out;                 // null: codes are wanted
+    uint8_t *codes, *scales;
+    float *rstd;  // null: not wanted
+    size_t rows, xs, rs, ss, os, scs;
+    int width;
+    float epsilon;
+};
+void rms_norm(const NormArgs &a, Type type, hipStream_t stream);
+
+struct NormBackwardArgs {
+    const void *x, *weight, *d_out, *d_sum;  // weight and d_sum may be null
+    const float *rstd;
+    void *d_x;
+    float *d_weight, *part;  // null: not wanted; parts x width
+    size_t rows, xs, dos, dss, dxs;
+    int width;
+};
+// Partial sums of the weight's gradient that a call makes.
+size_t norm_parts(size_t rows, size_t width);
+void rms_norm_backward(const NormBackwardArgs &a, Type type, hipStream_t stream);
+constexpr size_t kNormWidth = 32768;  // at most
+
 constexpr int kTopMax = 32;
 constexpr int kSmallVocab = 1024;  // rows of so many logits take a wave, longer ones workgroups
 constexpr int kGradRun = 736;      // F32 logits of a gradient's wave (twice as many in 16 bits)
@@ -153,5 +209,37 @@ void token_logprobs_backward_noalloc(int device, Type type, const void *logits, 
 void token_logprobs(int device, const float *logits, size_t rows, size_t vocab, const uint32_t *tokens,
                     float temperature, float *logprob, float *entropy, size_t top, uint32_t *top_tokens,
                     float *top_logprobs);
+
+// step_operators.cpp
+void sample_filtered_noalloc(int device, Type type, const void *logits, size_t rows, size_t vocab, size_t stride,
+                             const float *temperatures, const int *top_k, const float *top_p, const float *min_p,
+                             const float *uniforms, uint32_t *tokens, float *logprob, hipStream_t stream);
+
+struct Rope {
+    size_t width, rotary;
+    bool interleaved;
+    float magnitude;
+    const double *frequencies;
+};
+enum class RopeScaling : int { None = 0, Linear = 1, Base = 2, Bands = 3 };
+void rope_frequencies(size_t rotary, double base, RopeScaling scaling, double factor, double context, double low,
+                      double high, double *out);
+void rope(int device, const Rope &r, Type type, size_t batch, size_t count, size_t heads, const void *q, Strides qs,
+          void *q_out, Strides qos, size_t kv_heads, const void *k, Strides ks, void *k_out, Strides kos,
+          const int *lengths, const int *counts, const int *positions, bool backward, hipStream_t stream);
+
+// out, or codes and scales.
+void rms_norm(int device, Type type, size_t rows, size_t width, const void *x, size_t x_stride, const void *residual,
+              size_t residual_stride, void *sum, size_t sum_stride, const void *weight, float epsilon, void *out,
+              size_t out_stride, float *rstd, hipStream_t stream);
+void rms_norm_e4m3(int device, Type type, size_t rows, size_t width, const void *x, size_t x_stride,
+                   const void *residual, size_t residual_stride, void *sum, size_t sum_stride, const void *weight,
+                   float epsilon, uint8_t *codes, size_t codes_stride, uint8_t *scales, size_t scales_stride,
+                   float *rstd, hipStream_t stream);
+size_t rms_norm_backward_workspace(size_t rows, size_t width);
+void rms_norm_backward(int device, Type type, size_t rows, size_t width, const void *sum, size_t sum_stride,
+                       const void *weight, const float *rstd, const void *d_out, size_t d_out_stride, const void *d_sum,
+                       size_t d_sum_stride, void *d_x, size_t d_x_stride, float *d_weight, void *workspace,
+                       size_t workspace_bytes, hipStream_t stream);
 
 }  // namespace meshgpt

@@ -71,6 +71,15 @@ struct BF16 {
     }
 };
 
+// 16 bytes at any element: the compiler's loads and stores for this target allow it.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ uint4 get_any(const void *p) {
+    return __builtin_bit_cast(uint4, u32x4(*static_cast<const u32x4_any *>(p)));
+}
+__device__ __forceinline__ void put_any(void *p, uint4 w) {
+    *static_cast<u32x4_any *>(p) = __builtin_bit_cast(u32x4, w);
+}
+
 // Inputs and outputs of more than the Infinity Cache's 256 MB: whoever comes next
 // does not find them there, so they are moved past the caches (STREAM).
 constexpr double kCached = double(256u << 20);

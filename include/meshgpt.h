@@ -353,6 +353,100 @@ int mg_token_logprobs(int device, const float *logits, size_t rows, size_t vocab
                       float temperature, float *logprob, float *entropy, size_t top, uint32_t *top_tokens,
                       float *top_logprobs);
 
+/* Draws a token from each row of `vocab` logits (rows `stride` elements of `type`
+ * apart).  Tokens are ranked by their logits, the largest first, of equal ones the
+ * lowest first; a token's weight is exp((logit - largest) / temperature).  Of the
+ * ranking are left, one after the other: the first top_k tokens; the shortest run
+ * from the first whose weights reach top_p of theirs; the tokens whose weight is at
+ * least min_p.  The token drawn is the first in rank at which the sum of what is
+ * left exceeds uniforms[r] times the whole, and logprob[r] the log of its share.
+ * temperatures, top_k, top_p and min_p have a value for each row; NULL is 1 and no
+ * filter.  Temperature 0 takes the first of the largest logits (logprob 0, filters
+ * and random number not looked at).  A top_k of 0 or less, or of `vocab` or more, a
+ * top_p of 1 or more and a min_p of 0 or less filter nothing; the first token is
+ * always left.  A row gets the token 0xFFFFFFFF and a logprob of NaN where its
+ * logits hold a NaN or +inf or are all -inf, its temperature is negative, NaN or
+ * infinite, top_p or min_p is NaN, or its random number is not in [0, 1).  Sums are
+ * exact to about 2^-34 of a weight and the same in every call; tokens of less than
+ * e^-31.9 of the largest weight are not drawn.  logprob may be NULL.  Fewer than 2^22
+ * rows, up to 2^24 tokens; no workspace. */
+int mg_sample_filtered_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab, size_t stride,
+                               const float *temperatures, const int32_t *top_k, const float *top_p, const float *min_p,
+                               const float *uniforms, uint32_t *tokens, float *logprob, void *stream);
+
+/* Rotary positions: `rotary` channels (even) of each head of `head_width` (up to
+ * 1024) turn in pairs, channels i and i + rotary / 2 (MG_ROPE_HALF) or 2 i and
+ * 2 i + 1 (MG_ROPE_INTERLEAVED), by position times frequencies[i] radians, and are
+ * multiplied by `magnitude`; the channels behind stay as they are.  frequencies holds
+ * rotary / 2 doubles on the device, because an angle at a far position needs them. */
+enum { MG_ROPE_HALF = 0, MG_ROPE_INTERLEAVED = 1 };
+typedef struct {
+    uint32_t head_width, rotary, layout;
+    float magnitude;
+    const double *frequencies;
+} mg_rope;
+/* Frequencies base^(-2 i / rotary) into the host array out (rotary / 2 doubles), or
+ * scaled for contexts `factor` times as long: MG_ROPE_LINEAR divides them by factor;
+ * MG_ROPE_BASE multiplies the base by factor^(rotary / (rotary - 2)), which divides
+ * the last by factor and leaves the first; MG_ROPE_BANDS divides those that turn
+ * less than `low` times over the original `context`, leaves those that turn more than
+ * `high` times, and mixes in proportion to the turns between.  What a scaling does
+ * not use is not looked at. */
+enum { MG_ROPE_UNSCALED = 0, MG_ROPE_LINEAR = 1, MG_ROPE_BASE = 2, MG_ROPE_BANDS = 3 };
+int mg_rope_frequencies(size_t rotary, double base, int scaling, double factor, double context, double low, double high,
+                        double *out);
+/* Turns the queries (`heads` heads) and keys (`kv_heads`) of `count` tokens of each
+ * sequence, laid out as the inputs of mg_kv8_append, into q_out and k_out; either
+ * may have 0 heads and is then not looked at.  Outputs may be the inputs, with the same
+ * strides; else they must not overlap them.  Token i of sequence s has position
+ * positions[s * count + i]; without positions (NULL), those of mg_kv8_append: lengths[s]
+ * tokens with the new ones, counts[s] of them new; lengths NULL: i; counts NULL:
+ * `count` each.  Rows behind a sequence's count stay as they are, and so do all rows of
+ * a sequence whose count is negative or over `count`, or whose length is under its
+ * count. */
+int mg_rope_apply(int device, const mg_rope *r, int type, size_t batch, size_t count, size_t heads, const void *q,
+                  const int64_t q_strides[3], void *q_out, const int64_t q_out_strides[3], size_t kv_heads, const void *k,
+                  const int64_t k_strides[3], void *k_out, const int64_t k_out_strides[3], const int32_t *lengths,
+                  const int32_t *counts, const int32_t *positions, void *stream);
+/* The gradients of the inputs from those of the outputs: turned back, and multiplied
+ * by the magnitude.  Everything else is as above. */
+int mg_rope_backward(int device, const mg_rope *r, int type, size_t batch, size_t count, size_t heads,
+                     const void *d_q_out, const int64_t d_q_out_strides[3], void *d_q, const int64_t d_q_strides[3],
+                     size_t kv_heads, const void *d_k_out, const int64_t d_k_out_strides[3], void *d_k,
+                     const int64_t d_k_strides[3], const int32_t *lengths, const int32_t *counts,
+                     const int32_t *positions, void *stream);
+
+/* The root-mean-square norm of rows of `width` (1..32768; fewer than 2^22 rows,
+ * strides in elements): h = x + residual (NULL: x), rounded to `type` and written to
+ * sum (NULL: not); rstd = 1 / sqrt(mean(h^2) + epsilon); out = h * rstd * weight (of
+ * `type`; NULL: 1).  sum and out may be x or the residual, with their strides, but not
+ * each other.  rstd (rows floats, or NULL) is what the gradient needs.  A row's sum of
+ * squares is FP64: no finite value overflows it.  A NaN makes its row NaN; an infinity
+ * is NaN in its place and makes the others 0. */
+int mg_rms_norm(int device, int type, size_t rows, size_t width, const void *x, size_t x_stride, const void *residual,
+                size_t residual_stride, void *sum, size_t sum_stride, const void *weight, float epsilon, void *out,
+                size_t out_stride, float *rstd, void *stream);
+/* The same with outputs in 8 bits: E4M3 codes (rows codes_stride bytes apart), and
+ * for each 32 channels of a row, the last ones fewer, a byte b (rows scales_stride
+ * apart): scale 2^(b - 127), the smallest power of two from 2^-117 to 2^120 with which
+ * the largest magnitude of the 32 is at most 448.  Codes are the nearest, ties to even;
+ * NaN, infinities and what the largest scale cannot hold become NaN. */
+int mg_rms_norm_e4m3(int device, int type, size_t rows, size_t width, const void *x, size_t x_stride,
+                     const void *residual, size_t residual_stride, void *sum, size_t sum_stride, const void *weight,
+                     float epsilon, uint8_t *codes, size_t codes_stride, uint8_t *scales, size_t scales_stride,
+                     float *rstd, void *stream);
+/* The gradients of mg_rms_norm from that of its output and (d_sum, or NULL) of the
+ * kept sum, which what follows may have used too: d_x, which is the residual's as
+ * well, and d_weight (`width` floats, or NULL: not wanted).  sum is what the forward
+ * call normalised: its kept sum, or x where there was no residual.  d_x may be sum,
+ * d_out or d_sum, with its stride.  d_weight is added up in one order, and needs the
+ * workspace of mg_rms_norm_backward_workspace bytes, aligned to 4 (else NULL, 0). */
+int mg_rms_norm_backward_workspace(size_t rows, size_t width, size_t *bytes);
+int mg_rms_norm_backward(int device, int type, size_t rows, size_t width, const void *sum, size_t sum_stride,
+                         const void *weight, const float *rstd, const void *d_out, size_t d_out_stride,
+                         const void *d_sum, size_t d_sum_stride, void *d_x, size_t d_x_stride, float *d_weight,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
 /* out[i] = the f32 exp the sampler of mg_generate uses (the reference's
  * f32::exp, i.e. the C library's expf), evaluated on `device`.  No separate
  * reference call: it lets tests compare the device exp with the host's. */
