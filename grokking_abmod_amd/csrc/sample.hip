@@ -6,19 +6,14 @@
 // top_p of theirs; of these the ones with w >= min_p; and u picks the first
 // token in rank at which the sum of what is left exceeds u times the whole.
 // Everything is a prefix of the ranking, so no row is sorted: a border is found
-// by the weights of bins, and inside one bin by sorting that bin.
-//
-// A row has a workgroup.  Where the candidates are few (top_k bounds them by
-// the k-th largest of the threads' maxima, min_p by itself), they are gathered
-// and sorted.  Else the row goes into kBins bins of (max z - z) / T, 64 for each
-// power of e, and the bins that hold a border or the drawn token are gathered.
-// A bin with too many tokens is divided by the bits of its logits until it has
-// few enough or all are equal.
+// by the weights of bins, and inside one bin by ranking that bin.
 //
 // Sums decide which of many close borders is met: at 100000 equally likely
-// tokens one is 1e-5 of the whole.  So weights are summed in 64 bits: a bin's as
-// a count and a fixed-point sum of 1 - w / (w at its begin), in one LDS word, exact
-// to 2^-34 of a weight and the same in any order; gathered ones in FP64.
+// tokens one is 1e-5 of the whole.  So weights are summed in 64 bits, in an
+// order that is the same in every call.
+//
+// A row has a workgroup.  Up to kShort logits, every token counts those before it;
+// else they go into bins of (max z - z) / T (sample_bins_kernel).
 #include <cfloat>
 
 #include "dpp.hpp"
@@ -28,10 +23,9 @@
 namespace meshgpt::kern {
 namespace {
 
-constexpr int kBins = 2048;
-constexpr double kPerUnit = 64.0;  // bins of a factor e
-constexpr int kMost = 2048;        // tokens that are sorted at a time, in long rows
-constexpr int kShort = 1024;       // rows of so many logits are sorted whole
+constexpr int kShort = 256;
+constexpr int kPerUnit = 64;       // bins of a factor e
+constexpr double kReach = 31.9;    // powers of e that are looked at: 2041.6 bins
 constexpr uint32_t kNoToken = 0xffffffffu;
 
 // Logits as integers in the same order; -0 is 0.
@@ -42,39 +36,94 @@ __device__ __forceinline__ uint32_t order(float x) {
 __device__ __forceinline__ float unordered(uint32_t k) {
     return __builtin_bit_cast(float, k ^ (uint32_t(int32_t(~k) >> 31) | 0x80000000u));
 }
-// Ranked by the logit, then the lowest token.
-__device__ __forceinline__ uint64_t candidate(float x, uint32_t token) {
-    return uint64_t(order(x)) << 32 | uint32_t(~token);
+
+// A value that all lanes have, in scalar registers.
+__device__ __forceinline__ double uniform(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(b)), hi = __builtin_amdgcn_readfirstlane(uint32_t(b >> 32));
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
 }
 
-// f(logit, token) for every logit of a row, 16 bytes a load, four loads under way.
+// f(logit) for every logit of a row, 16 bytes a load, four loads under way.
 template <class T, int THREADS, class F>
 __device__ __forceinline__ void each(const typename T::Raw *z, uint32_t vocab, F &&f) {
     constexpr int G = T::kGroup, U = 4;
     const uint32_t groups = vocab / G;
-    uint32_t j = threadIdx.x;
-    for (; j + (U - 1) * THREADS < groups; j += U * THREADS) {
+    for (uint32_t j = threadIdx.x; j < groups; j += U * THREADS) {
         uint4 w[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) w[u] = get_any(z + size_t(j + u * THREADS) * G);
+        for (int u = 0; u < U; ++u)  // behind the end: its first group again
+            w[u] = get_any(z + size_t(j + u * THREADS < groups ? j + u * THREADS : j) * G);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float x[G];
             T::unpack(w[u], x);
 #pragma unroll
-            for (int e = 0; e < G; ++e) f(x[e], (j + u * THREADS) * G + e);
+            for (int e = 0; e < G; ++e) f(x[e]);
         }
     }
-    for (; j < groups; j += THREADS) {
-        float x[G];
-        T::unpack(get_any(z + size_t(j) * G), x);
-#pragma unroll
-        for (int e = 0; e < G; ++e) f(x[e], j * G + e);
-    }
     const uint32_t last = groups * G + threadIdx.x;
-    if (last < vocab) f(T::to_float(z[last]), last);
+    if (last < vocab) f(T::to_float(z[last]));
 }
 
+// The same for what takes long with each logit: the next group is under way meanwhile.
+template <class T, int THREADS, class F>
+__device__ __forceinline__ void each_slowly(const typename T::Raw *z, uint32_t vocab, F &&f) {
+    constexpr int G = T::kGroup;
+    const uint32_t groups = vocab / G;
+    uint32_t j = threadIdx.x;
+    uint4 now{}, next{};
+    if (j < groups) now = get_any(z + size_t(j) * G);
+    if (j + THREADS < groups) next = get_any(z + size_t(j + THREADS) * G);
+#pragma unroll 1
+    for (; j < groups; j += THREADS) {
+        uint4 later{};
+        if (j + 2 * THREADS < groups) later = get_any(z + size_t(j + 2 * THREADS) * G);
+        float x[G];
+        T::unpack(now, x);
+#pragma unroll
+        for (int e = 0; e < G; ++e) f(x[e]);
+        now = next;
+        next = later;
+    }
+    const uint32_t last = groups * G + threadIdx.x;
+    if (last < vocab) f(T::to_float(z[last]));
+}
+
+// f(logit, token) for the few logits of a row from lo to hi.
+template <class T, int THREADS, class F>
+__device__ __forceinline__ void each_in(const typename T::Raw *z, uint32_t vocab, float lo, float hi, F &&f) {
+    constexpr int G = T::kGroup, U = 4;
+    const uint32_t groups = vocab / G;
+#pragma unroll 1
+    for (uint32_t j = threadIdx.x; j < groups; j += U * THREADS) {
+        uint4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = get_any(z + size_t(min(j + u * THREADS, groups - 1)) * G);
+        uint32_t those = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x[G];
+            T::unpack(w[u], x);
+            uint32_t here = 0;
+#pragma unroll
+            for (int e = 0; e < G; ++e) here |= uint32_t(x[e] >= lo && x[e] <= hi) << e;
+            if (j + u * THREADS < groups) those |= here << (u * G);
+        }
+        while (those) {
+            const uint32_t b = __builtin_ctz(those), token = (j + b / G * THREADS) * G + b % G;
+            those &= those - 1;
+            f(T::to_float(z[token]), token);
+        }
+    }
+    const uint32_t last = groups * G + threadIdx.x;
+    if (last < vocab) {
+        const float x = T::to_float(z[last]);
+        if (x >= lo && x <= hi) f(x, last);
+    }
+}
+
+// Running sums over a wave's lanes.
 template <class V>
 __device__ __forceinline__ V wave_scan(V v, int lane) {
 #pragma unroll
@@ -84,120 +133,301 @@ __device__ __forceinline__ V wave_scan(V v, int lane) {
     }
     return v;
 }
+template <class V>
+__device__ __forceinline__ V wave_total(V v) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+// The sum of the values of the threads before, and of all of them.
+template <int THREADS, class V>
+__device__ __forceinline__ V block_scan(V v, V *room, V &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const V in = wave_scan(v, lane);
+    __syncthreads();
+    if (lane == 63) room[wave] = in;
+    __syncthreads();
+    V base = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        const V o = room[w];
+        if (w < wave) base += o;
+        sum += o;
+    }
+    total = sum;
+    return base + in - v;
+}
+template <int THREADS, class V>
+__device__ __forceinline__ V block_total(V v, V *room) {
+    v = wave_total(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
+    __syncthreads();
+    V sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) sum += room[w];
+    return sum;
+}
 
 struct Settings {
     double temperature, top_p, min_p, uniform;
     uint32_t top_k;  // 0: all
-    bool with_p, with_min;
+    bool with_p, with_min, greedy, valid;
+};
+__device__ __forceinline__ Settings settings_of(const SampleArgs &a, size_t row) {
+    Settings s;
+    s.temperature = uniform(a.temperatures ? double(a.temperatures[row]) : 1.0);
+    s.top_p = uniform(a.top_p ? double(a.top_p[row]) : 1.0);
+    s.min_p = uniform(fmin(a.min_p ? double(a.min_p[row]) : 0.0, 1.0));  // the largest is always left
+    s.uniform = uniform(double(a.uniforms[row]));
+    const int k = a.top_k ? a.top_k[row] : 0;
+    s.top_k = k > 0 && size_t(k) < a.vocab ? uint32_t(k) : 0;
+    s.with_p = s.top_p < 1.0;
+    s.with_min = s.min_p > 0.0;
+    s.greedy = s.temperature == 0.0;
+    s.valid = s.temperature >= 0.0 && s.temperature <= double(FLT_MAX) && s.top_p == s.top_p && !(a.min_p && a.min_p[row] != a.min_p[row]) &&
+              (s.greedy || (s.uniform >= 0.0 && s.uniform < 1.0));
+    return s;
+}
+
+__device__ __forceinline__ void write(const SampleArgs &a, size_t row, uint32_t token, float logprob) {
+    a.tokens[row] = token;
+    if (a.logprob) a.logprob[row] = logprob;
+}
+
+// How many of n equal weights w reach t, at least 1, and which of them the first to exceed it is.
+__device__ __forceinline__ uint32_t equal_reach(double t, double w, uint32_t n) {
+    const double steps = t / w;
+    return steps >= double(n) ? n : steps > 1.0 ? uint32_t(ceil(steps)) : 1;
+}
+__device__ __forceinline__ uint32_t equal_draw(double t, double w, uint32_t n) {
+    const double steps = t / w;
+    return steps >= double(n - 1) ? n - 1 : steps > 0.0 ? uint32_t(steps) : 0;
+}
+
+// ---- short rows -------------------------------------------------------------------
+
+// A thread has a token and counts those before it, four to an LDS read; then it
+// has a place in the ranking, with the running sum of the weights up to there.
+template <class T>
+__global__ void __launch_bounds__(kShort) sample_short_kernel(SampleArgs a) {
+    using Raw = typename T::Raw;
+    constexpr int WAVES = kShort / 64;
+    __shared__ uint4 keys[kShort / 4];
+    __shared__ double weights[kShort], sums[kShort], room_d[WAVES];
+    __shared__ uint32_t tokens[kShort], room_u[WAVES], bads[WAVES];
+    __shared__ float tops[WAVES];
+    const size_t row = blockIdx.x;
+    const uint32_t tid = threadIdx.x, vocab = uint32_t(a.vocab), wave = tid / 64, lane = tid % 64;
+    const Settings set = settings_of(a, row);
+    const float x = tid < vocab ? T::to_float(static_cast<const Raw *>(a.logits)[row * a.stride + tid]) : -INFINITY;
+    const uint32_t key = order(x);
+    reinterpret_cast<uint32_t *>(keys)[tid] = key;
+    const float wave_top = wave_largest(x);
+    const bool wave_bad = __ballot(!(x < INFINITY)) != 0;
+    if (lane == 0) {
+        tops[wave] = wave_top;
+        bads[wave] = wave_bad;
+    }
+    weights[tid] = 0.0;
+    __syncthreads();
+    float top = -INFINITY;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        top = fmaxf(top, tops[w]);
+        bad |= bads[w];
+    }
+    if (bad || top == -INFINITY || !set.valid) {
+        if (tid == 0) write(a, row, kNoToken, NAN);
+        return;
+    }
+    // Of equal keys those of lower tokens are before: all in the waves before, the lanes before in this one.
+    uint32_t before = 0;
+    const uint32_t mine = __builtin_amdgcn_readfirstlane(wave * 16), end = (vocab + 3) / 4;
+    for (uint32_t j = 0; j < min(mine, end); ++j) {
+        const uint4 k = keys[j];
+        before += (k.x >= key) + (k.y >= key) + (k.z >= key) + (k.w >= key);
+    }
+    for (uint32_t j = mine + 16; j < end; ++j) {
+        const uint4 k = keys[j];
+        before += (k.x > key) + (k.y > key) + (k.z > key) + (k.w > key);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) {
+        const uint4 k = keys[mine + j];
+        before += (k.x > key || (k.x == key && 4 * j < lane)) + (k.y > key || (k.y == key && 4 * j + 1 < lane)) +
+                  (k.z > key || (k.z == key && 4 * j + 2 < lane)) + (k.w > key || (k.w == key && 4 * j + 3 < lane));
+    }
+    if (set.greedy) {
+        if (before == 0) write(a, row, tid, 0.0f);
+        return;
+    }
+    const double weight = exp((double(x) - double(top)) / set.temperature);
+    if (tid < vocab) {
+        weights[before] = weight;
+        tokens[before] = tid;
+    }
+    __syncthreads();
+    // From here on a thread has a place in the ranking.
+    const double w = weights[tid];
+    double whole;
+    const double sum = block_scan<kShort>(w, room_d, whole) + w;
+    sums[tid] = sum;
+    __syncthreads();
+    const auto count = [&](bool is) {
+        const uint32_t c = uint32_t(__popcll(__ballot(is)));
+        if (lane == 0) room_u[wave] = c;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) all += room_u[v];
+        __syncthreads();
+        return all;
+    };
+    uint32_t left = count(w > 0.0);
+    if (set.top_k) left = min(left, set.top_k);
+    if (set.with_p) {
+        const double t = set.top_p * sums[left - 1];
+        left = min(left, count(tid < left && sum < t) + 1);
+    }
+    if (set.with_min) left = max(1u, count(tid < left && w >= set.min_p));
+    whole = sums[left - 1];
+    const uint32_t at = min(left - 1, count(tid < left && sum <= set.uniform * whole));
+    if (tid == at) write(a, row, tokens[tid], float(log(w / whole)));
+}
+
+// ---- weights by bins of 1/64 of a power of e -------------------------------------------
+
+struct Powers {
+    double wholes[32], parts[kPerUnit];  // e^-i, e^(-i / 64)
 };
 
-// Where a prefix of the ranking ends: inside a bin, after `in` of its tokens,
-// with the sum of all weights up to there.
-struct Border {
-    int bin;
-    uint32_t in;
-    double weight;
+struct Weights {
+    const Powers &powers;  // in LDS
+    double top, scale;     // the largest logit, bins of a unit of a logit
+
+    // Makes the powers; a barrier has to follow.
+    static __device__ __forceinline__ void prepare(Powers &p) {
+        if (threadIdx.x < 32) p.wholes[threadIdx.x] = exp(-double(threadIdx.x));
+        if (threadIdx.x < kPerUnit) p.parts[threadIdx.x] = exp(-double(threadIdx.x) / kPerUnit);
+    }
+    // Bins from the largest logit.
+    __device__ __forceinline__ double place(float x) const { return (top - double(x)) * scale; }
+    // The weight where a bin begins.
+    __device__ __forceinline__ double begin_of(int bin) const { return powers.wholes[bin / kPerUnit] * powers.parts[bin % kPerUnit]; }
+    // e^(-r / 64) - 1 for r from 0 to 1: the sixth term of the series is under 2^-45.  r = 0 is
+    // exact, and with it the sum of weights that equal the largest.
+    static __device__ __forceinline__ double rest(double r) {
+        return r * fma(r, fma(r, fma(r, fma(r, -0x1p-30 / 120, 0x1p-24 / 24), -0x1p-18 / 6), 0x1p-12 / 2), -0x1p-6);
+    }
+    __device__ __forceinline__ double of(float x) const {
+        const double y = place(x), at = floor(y);
+        if (!(y < kReach * kPerUnit)) return 0.0;
+        const double begin = begin_of(int(at));
+        return fma(begin, rest(y - at), begin);
+    }
 };
 
-enum class Ask { Count, Reach, Draw };
+// ---- the general way -----------------------------------------------------------------
 
-template <class T, int THREADS, int MOST, bool LONG>
-struct Row {
-    using Element = T;
-    static constexpr int kThreads = THREADS, kWaves = THREADS / 64, kMostRanked = MOST;
+// The row's largest logit; then either few candidates (top_k bounds them by the
+// k-th largest of the threads' maxima, min_p by itself), which are gathered and
+// ranked, or bins of (max z - z) / T, 64 for each power of e.  A bin keeps its
+// tokens' count and the fixed-point sum of w / (w where it begins) - 1 in one LDS
+// word, exact to 2^-34 of a weight and the same in any order.  Where a border falls
+// into a bin, its tokens are gathered and ranked; if they are more than MOST, the
+// bin is divided by the bits of their logits until they are few enough or equal.
+enum Ask { kCount, kReachP, kLeast, kDraw, kAsks };
+
+template <class T, int THREADS, int BINS, int MOST>
+struct Bins {
+    static constexpr int kEach = BINS / THREADS;
+    static_assert(BINS == 32 * kPerUnit && BINS > kReach * kPerUnit && BINS % THREADS == 0 && MOST % THREADS == 0, "every place has a bin");
+    static constexpr int kCounted = THREADS / 4;  // up to so many are ranked by counting
+
+    struct Bin {
+        int at;
+        uint32_t taken, count;  // tokens before it and in it
+        double base, weight;    // weights before it and in it
+    };
     struct Shared {
-        uint64_t list[MOST];
-        union {
-            double sums[MOST];  // running sums of the sorted list
-            uint64_t bins[LONG ? kBins : 1];
-            uint32_t counts[LONG ? kBins : 1];
-        };
-        double before[LONG ? kBins + 1 : 1];    // weights of the bins before each
-        uint32_t tokens[LONG ? kBins + 1 : 1];  // and their tokens
-        double wave_d[kWaves + 1];
-        uint32_t wave_u[kWaves + 1];
-        float wave_f[kWaves];
-        uint32_t n, lo, hi, found;
-        double weight;
+        uint64_t bins[BINS], fine[THREADS], list[MOST];
+        double sums[MOST];
+        double before[THREADS];   // weights before a thread's bins
+        uint32_t taken[THREADS];  // and tokens
+        double room_d[THREADS / 64], base;
+        Bin found_by[THREADS / 64];
+        uint32_t room_u[THREADS / 64], n, lo, hi, found;
+        float room_f[THREADS / 64];
+        Powers powers;
     };
 
     const typename T::Raw *z;
     uint32_t vocab;
     Shared &s;
-    int tid, lane, wave;
+    int tid;
     float top;
-    double inv, scale;  // 1 / T, bins of a unit of a logit
+    double scale, until_min;  // bins of a unit of a logit, and to min_p
     int dev_bits, shift;
 
-    __device__ Row(const typename T::Raw *z_, uint32_t vocab_, Shared &s_) : z(z_), vocab(vocab_), s(s_) {
-        tid = threadIdx.x;
-        lane = tid & 63;
-        wave = tid >> 6;
+    __device__ __forceinline__ Bins(const typename T::Raw *z_, uint32_t vocab_, Shared &s_)
+        : z(z_), vocab(vocab_), s(s_), tid(threadIdx.x) {}
+
+    __device__ __forceinline__ Weights weights() const { return {s.powers, double(top), scale}; }
+    __device__ __forceinline__ double place(float x) const { return weights().place(x); }
+    __device__ __forceinline__ double weight_of(float x) const { return weights().of(x); }
+    __device__ __forceinline__ double begin_of(int bin) const { return weights().begin_of(bin); }
+    // A logit at or below every logit with place < `until`, and one at or above those with place >= `from`.
+    __device__ __forceinline__ float least(double until) const {
+        const double down = until / scale, x = double(top) - down - (fabs(double(top)) + down) * 0x1p-20;
+        return x > -double(FLT_MAX) ? float(x) : -FLT_MAX;
+    }
+    __device__ __forceinline__ float most(double from) const {
+        const double down = from / scale, x = double(top) - down + (fabs(double(top)) + down) * 0x1p-20;
+        return x < double(FLT_MAX) ? float(x) : FLT_MAX;
     }
 
-    __device__ double weight_of(float x) const { return exp((double(x) - double(top)) * inv); }
-    // Bins from the largest logit.
-    __device__ double place(float x) const { return (double(top) - double(x)) * scale; }
-
-    // The sum over the workgroup of each thread's value, and (scan) of the threads before.
-    template <class V>
-    __device__ V block_scan(V v, V *room, V &total) {
-        const V in = wave_scan(v, lane);
-        if (lane == 63) room[wave] = in;
-        __syncthreads();
-        V base = 0, sum = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const V o = room[w];
-            if (w < wave) base += o;
-            sum += o;
-        }
-        total = sum;
-        __syncthreads();
-        return base + in - v;
-    }
-    __device__ uint32_t block_count(uint32_t v) {
-        uint32_t total;
-        block_scan<uint32_t>(v, s.wave_u, total);
-        return total;
+    __device__ __forceinline__ void append(float x, uint32_t token) {
+        const uint32_t at = atomicAdd(&s.n, 1u);
+        if (at < uint32_t(MOST)) s.list[at] = uint64_t(order(x)) << 32 | uint32_t(~token);
     }
 
-    // Appends what `in` takes; more than MOST are only counted.
-    template <class In>
-    __device__ uint32_t gather(In &&in) {
-        if (tid == 0) s.n = 0;
-        __syncthreads();
-        each<T, THREADS>(z, vocab, [&](float x, uint32_t token) {
-            if (in(x)) {
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < uint32_t(MOST)) s.list[at] = candidate(x, token);
+    // Ranks the first n of the list and makes their running sums.
+    __device__ __forceinline__ void rank(uint32_t n) {
+        if (n <= uint32_t(kCounted)) {  // four threads a token count those before it
+            const uint32_t i = tid / 4;
+            const uint64_t v = i < n ? s.list[i] : 0;
+            uint32_t before = 0;
+            if (i < n) {
+#pragma unroll 4
+                for (uint32_t j = tid % 4; j < n; j += 4) before += s.list[j] > v;
             }
-        });
-        __syncthreads();
-        const uint32_t n = s.n;
-        __syncthreads();
-        return n;
-    }
-
-    // Sorts the first n of the list, the first in rank first, and makes their running sums.
-    __device__ void rank(uint32_t n) {
-        uint32_t size = 2;
-        while (size < n) size *= 2;
-        for (uint32_t i = n + tid; i < size; i += THREADS) s.list[i] = 0;
-        __syncthreads();
-        for (uint32_t k = 2; k <= size; k *= 2)
-            for (uint32_t j = k / 2; j > 0; j /= 2) {
-                for (uint32_t i = tid; i < size / 2; i += THREADS) {
-                    const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
-                    const uint64_t x = s.list[a], y = s.list[b];
-                    if ((x < y) == ((a & k) == 0)) {
-                        s.list[a] = y;
-                        s.list[b] = x;
+            before += __shfl_xor(before, 1, 64);
+            before += __shfl_xor(before, 2, 64);
+            __syncthreads();
+            if (i < n && tid % 4 == 0) s.list[before] = v;
+            __syncthreads();
+        } else {
+            uint32_t size = 2 * kCounted;
+            while (size < n) size *= 2;
+            for (uint32_t i = n + tid; i < size; i += THREADS) s.list[i] = 0;
+            __syncthreads();
+            for (uint32_t k = 2; k <= size; k *= 2)
+                for (uint32_t j = k / 2; j > 0; j /= 2) {
+                    for (uint32_t i = tid; i < size / 2; i += THREADS) {
+                        const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
+                        const uint64_t x = s.list[a], y = s.list[b];
+                        if ((x < y) == ((a & k) == 0)) {
+                            s.list[a] = y;
+                            s.list[b] = x;
+                        }
                     }
+                    __syncthreads();
                 }
-                __syncthreads();
-            }
-        constexpr int E = (MOST + THREADS - 1) / THREADS;
+        }
+        constexpr int E = MOST / THREADS;
         double w[E], sum = 0.0, total;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -205,7 +435,7 @@ struct Row {
             w[e] = i < n ? weight_of(unordered(uint32_t(s.list[i] >> 32))) : 0.0;
             sum += w[e];
         }
-        double run = block_scan<double>(sum, s.wave_d, total);
+        double run = block_scan<THREADS>(sum, s.room_d, total);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const uint32_t i = tid * E + e;
@@ -216,469 +446,387 @@ struct Row {
     }
 
     // How many of the n ranked ones' running sums lie under t, or (up) do not exceed it.
-    __device__ uint32_t below(uint32_t n, double t, bool up) {
+    __device__ __forceinline__ uint32_t below(uint32_t n, double t, bool up) {
         uint32_t c = 0;
         for (uint32_t i = tid; i < n; i += THREADS) c += up ? s.sums[i] <= t : s.sums[i] < t;
-        return block_count(c);
+        return block_total<THREADS>(c, s.room_u);
     }
 
-    // Bins of the row, or (within) the keys lo..hi of bin `of`, 2^step keys each.
-    __device__ void fill_bins(bool within, int of, uint32_t lo, uint32_t hi, int step) {
-        for (int i = tid; i < kBins; i += THREADS) s.bins[i] = 0;
+    __device__ __forceinline__ void finish(const SampleArgs &a, size_t row, uint64_t v, double whole) {
+        if (tid == 0) write(a, row, ~uint32_t(v), float(log(weight_of(unordered(uint32_t(v >> 32))) / whole)));
+    }
+
+    // Draws from the n candidates of the list.
+    __device__ __forceinline__ void draw_few(const SampleArgs &a, size_t row, const Settings &set, uint32_t n) {
+        rank(n);
+        if (set.top_k) n = min(n, set.top_k);
+        if (set.with_p) n = min(n, below(n, set.top_p * s.sums[n - 1], false) + 1);
+        if (set.with_min) {
+            uint32_t c = 0;
+            for (uint32_t i = tid; i < n; i += THREADS)
+                c += weight_of(unordered(uint32_t(s.list[i] >> 32))) >= set.min_p;
+            n = max(1u, block_total<THREADS>(c, s.room_u));
+        }
+        const double whole = s.sums[n - 1];
+        finish(a, row, s.list[min(below(n, set.uniform * whole, true), n - 1)], whole);
+    }
+
+    // The bin of the k-th largest of the threads' maxima bounds the k-th largest logit
+    // from below; what lies past the last bin cannot be drawn.
+    __device__ __forceinline__ int bound_bin(float mine, uint32_t k) {
+        uint32_t *const counts = reinterpret_cast<uint32_t *>(s.bins);
+        for (int i = tid; i < BINS; i += THREADS) counts[i] = 0;
+        if (tid == 0) s.found = BINS - 1;
         __syncthreads();
-        // e^-r - 1 for r from 0 to 1/64, in units of 2^-dev_bits: the sixth term is under 2^-45.
-        // (r = 0, and so the sum of weights that equal the largest, is exact.)
-        const double unit = double(uint64_t(1) << dev_bits), c1 = -unit * 0x1p-6, c2 = unit * (0x1p-12 / 2),
-                     c3 = -unit * (0x1p-18 / 6), c4 = unit * (0x1p-24 / 24), c5 = -unit * (0x1p-30 / 120);
-        const uint64_t one = uint64_t(1) << shift;
-        each<T, THREADS>(z, vocab, [&](float x, uint32_t) {
-            const double y = place(x);
-            int bin;
-            double r;
-            if (within) {
-                const uint32_t k = order(x);
-                if (k < lo || k > hi) return;
-                bin = int((hi - k) >> step);
-                r = y - double(of);
-            } else {
-                if (!(y < double(kBins - 1))) return;
-                const double at = floor(y);
-                bin = int(at);
-                r = y - at;
-            }
-            const double d = r * fma(r, fma(r, fma(r, fma(r, c5, c4), c3), c2), c1);
-            atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[bin]),
-                      static_cast<unsigned long long>(one + uint64_t(int64_t(int32_t(rint(d))))));
+        const double y = place(mine);
+        if (y < double(kReach * kPerUnit)) atomicAdd(&counts[int(y)], 1u);
+        __syncthreads();
+        uint32_t c[kEach], sum = 0, total;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum += c[e] = counts[tid * kEach + e];
+        uint32_t before = block_scan<THREADS>(sum, s.room_u, total);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (before < k && before + c[e] >= k) s.found = uint32_t(tid * kEach + e);
+            before += c[e];
+        }
+        __syncthreads();
+        return int(s.found);
+    }
+
+    // 1 for a token, and w / (w where the bin begins) - 1, r bins from there: the series of
+    // Weights::rest in units of 2^-dev_bits, rounded by the addition of 1.5 * 2^52.
+    __device__ __forceinline__ uint64_t term(double r) const {
+        const auto units = [&](double v) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, v) + (uint64_t(dev_bits) << 52)); };
+        const double d = fma(r, fma(r, fma(r, fma(r, units(-0x1p-30 / 120), units(0x1p-24 / 24)), units(-0x1p-18 / 6)),
+                                    units(0x1p-12 / 2)),
+                             units(-0x1p-6));
+        const double rounded = fma(r, d, 0x1.8p52);
+        return __builtin_bit_cast(uint64_t, rounded) + ((uint64_t(1) << shift) - __builtin_bit_cast(uint64_t, 0x1.8p52));
+    }
+    __device__ __forceinline__ void split(uint64_t h, double begin, uint32_t &tokens, double &weight) const {
+        const int64_t dev = int64_t(h << (64 - shift)) >> (64 - shift);
+        tokens = uint32_t((h - uint64_t(dev)) >> shift);
+        weight = begin * fma(double(dev), __builtin_bit_cast(double, uint64_t(1023 - dev_bits) << 52), double(tokens));
+    }
+    __device__ __forceinline__ void fill(uint32_t &all_c, double &all_w) {
+        // A bin's sum of `vocab` terms under 0.0156 stays in its field.
+        shift = 63 - (32 - __clz(int(vocab)));
+        dev_bits = min(36, 2 * shift - 58);
+        for (int i = tid; i < BINS; i += THREADS) s.bins[i] = 0;
+        __syncthreads();
+        const float from = least(kReach * kPerUnit);
+        each_slowly<T, THREADS>(z, vocab, [&](float x) {
+            if (x < from) return;
+            const double y = place(x), at = floor(y);
+            if (y < kReach * kPerUnit)
+                atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(at)]),
+                          static_cast<unsigned long long>(term(y - at)));
         });
         __syncthreads();
-    }
-
-    static constexpr int kEach = (kBins + THREADS - 1) / THREADS;  // bins of a thread
-
-    // A thread's bins with the weights and tokens before them; `of` as above, or -1.
-    struct Mine {
-        double weight[kEach], before, total;
-        uint32_t tokens[kEach], taken, all;
-    };
-    __device__ Mine scan_bins(int of) {
-        Mine m;
         double w = 0.0;
         uint32_t c = 0;
-        const double unit = 1.0 / double(uint64_t(1) << dev_bits);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int b = tid * kEach + e;
-            const uint64_t h = s.bins[b];
-            const int64_t dev = int64_t(h << (64 - shift)) >> (64 - shift);
-            m.tokens[e] = uint32_t((h - uint64_t(dev)) >> shift);
-            m.weight[e] = exp(-double(of < 0 ? b : of) / kPerUnit) * (double(m.tokens[e]) + double(dev) * unit);
-            w += m.weight[e];
-            c += m.tokens[e];
+            uint32_t tokens;
+            double weight;
+            split(s.bins[tid * kEach + e], begin_of(tid * kEach + e), tokens, weight);
+            w += weight;
+            c += tokens;
         }
-        m.before = block_scan<double>(w, s.wave_d, m.total);
-        m.taken = block_scan<uint32_t>(c, s.wave_u, m.all);
-        return m;
-    }
-    __device__ void keep_bins() {
-        Mine m = scan_bins(-1);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            s.before[tid * kEach + e] = m.before;
-            s.tokens[tid * kEach + e] = m.taken;
-            m.before += m.weight[e];
-            m.taken += m.tokens[e];
-        }
-        if (tid == 0) {
-            s.before[kBins] = m.total;
-            s.tokens[kBins] = m.all;
-        }
+        s.before[tid] = block_scan<THREADS>(w, s.room_d, all_w);
+        s.taken[tid] = block_scan<THREADS>(c, s.room_u, all_c);
         __syncthreads();
     }
-    // The first bin that `is` takes, kBins where there is none.
+
+    // The first bin that `is` takes; there has to be one.
     template <class Is>
-    __device__ int first_bin(Is &&is) {
-        if (tid == 0) s.found = kBins;
-        __syncthreads();
-        for (int b = tid; b < kBins; b += THREADS)
-            if (is(b)) {
-                atomicMin(&s.found, uint32_t(b));
-                break;
+    __device__ __forceinline__ Bin find(Is &&is) {
+        Bin b{tid * kEach, s.taken[tid], 0, s.before[tid], 0.0};
+        bool mine = false;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (!mine) {
+                split(s.bins[b.at], begin_of(b.at), b.count, b.weight);
+                mine = is(b);
             }
+            if (!mine) b = {b.at + 1, b.taken + b.count, 0, b.base + b.weight, 0.0};
+        }
+        const uint64_t those = __ballot(mine);
+        if (those == 0) {
+            if (tid % 64 == 0) s.found_by[tid / 64].at = BINS;
+        } else if (int(tid % 64) == __builtin_ctzll(those)) {
+            s.found_by[tid / 64] = b;
+        }
         __syncthreads();
-        const int b = int(s.found);
+        int w = 0;
+        while (w + 1 < THREADS / 64 && s.found_by[w].at == BINS) ++w;
+        b = s.found_by[w];
+        b.base = uniform(b.base);
+        b.weight = uniform(b.weight);
         __syncthreads();
         return b;
     }
 
-    // The n-th token, from 0, whose logit is that of key k.
-    __device__ uint32_t nth_of(uint32_t k, uint32_t n) {
-        const uint32_t share = (vocab + THREADS - 1) / THREADS * 64, from = min(vocab, wave * share),
+    // The n-th token, from 0, whose logit has key k.
+    __device__ __forceinline__ uint32_t nth_of(uint32_t k, uint32_t n) {
+        const int lane = tid & 63;
+        const uint32_t share = (vocab + THREADS - 1) / THREADS * 64, from = min(vocab, (tid >> 6) * share),
                        to = min(vocab, from + share);
-        uint32_t c = 0;
+        uint32_t c = 0, total;
         for (uint32_t i = from + lane; i < to; i += 64) c += order(T::to_float(z[i])) == k;
-        uint32_t total, before = block_scan<uint32_t>(c, s.wave_u, total);
-        const uint32_t first = __shfl(before, 0, 64);
-        uint32_t here = __shfl(before + c, 63, 64) - first;
-        if (n >= first && n < first + here) {  // this wave has it
+        const uint32_t before = block_scan<THREADS>(c, s.room_u, total);
+        const uint32_t first = __shfl(before, 0, 64), here = __shfl(before + c, 63, 64) - first;
+        if (n >= first && n - first < here) {  // this wave has it
             uint32_t left = n - first;
             for (uint32_t i = from; i < to; i += 64) {
                 const bool is = i + lane < to && order(T::to_float(z[i + lane])) == k;
                 const uint64_t mask = __ballot(is);
-                const uint32_t c64 = uint32_t(__popcll(mask));
-                if (left < c64) {
+                const uint32_t step = uint32_t(__popcll(mask));
+                if (left < step) {
                     if (is && uint32_t(__popcll(mask & ((uint64_t(1) << lane) - 1))) == left) s.found = i + lane;
                     break;
                 }
-                left -= c64;
+                left -= step;
             }
         }
         __syncthreads();
-        const uint32_t token = s.found;
-        __syncthreads();
-        return token;
+        return s.found;
     }
 
-    struct Answer {
-        uint32_t in;    // tokens of the bin up to the border
-        double weight;  // of all up to there (Draw: of the token)
-        uint32_t token;
-    };
-    // In n ranked tokens, after `taken` of the bin and weights of `base`.
-    __device__ Answer answer(uint32_t n, Ask ask, double t, uint32_t q, double base, uint32_t taken) {
-        if (ask == Ask::Draw) {
-            const uint32_t at = min(below(n, t - base, true), min(n, q - taken) - 1);
-            const uint64_t v = s.list[at];
-            return {0, weight_of(unordered(uint32_t(v >> 32))), ~uint32_t(v)};
-        }
-        const uint32_t c = ask == Ask::Count ? min(n, q - taken) : min(n, below(n, t - base, false) + 1);
-        return {taken + c, base + s.sums[c - 1], 0};
-    }
-
-    // Inside a bin that holds tokens: its first q tokens (Count); the tokens up to
-    // where the sum of all weights reaches t (Reach); the first of its first q
-    // tokens at which that sum exceeds t, or the last of them (Draw).
-    __device__ Answer resolve(int bin, Ask ask, double t, uint32_t q) {
-        const double from = double(bin), until = double(bin + 1);
-        double base = s.before[bin];
-        uint32_t taken = 0;
-        const uint32_t n = gather([&](float x) {
-            const double y = place(x);
-            return y >= from && y < until;
-        });
-        if (n <= uint32_t(MOST)) {
-            rank(n);
-            return answer(n, ask, t, q, base, 0);
-        }
-        if (tid == 0) {
-            s.lo = 0xffffffffu;
-            s.hi = 0;
-        }
-        __syncthreads();
-        uint32_t lo = 0xffffffffu, hi = 0, count = n;
-        each<T, THREADS>(z, vocab, [&](float x, uint32_t) {
-            const double y = place(x);
-            if (y >= from && y < until) {
-                lo = min(lo, order(x));
-                hi = max(hi, order(x));
-            }
-        });
-        atomicMin(&s.lo, lo);
-        atomicMax(&s.hi, hi);
-        __syncthreads();
-        lo = s.lo;
-        hi = s.hi;
-        __syncthreads();
-        while (lo != hi) {
-            const int step = max(0, 32 - __clz(int(hi - lo)) - 11);  // (hi - lo) >> step < kBins
-            fill_bins(true, bin, lo, hi, step);
-            const Mine m = scan_bins(bin);
-            if (tid == 0) {
-                s.found = kBins;
-                s.n = 0;
-            }
-            __syncthreads();
-            double w = base + m.before;
-            uint32_t c = taken + m.taken;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                w += m.weight[e];
-                c += m.tokens[e];
-                if (!m.tokens[e]) continue;
-                atomicMax(&s.n, uint32_t(tid * kEach + e));
-                if (ask == Ask::Count ? c >= q : ask == Ask::Reach ? w >= t : w > t || c >= q)
-                    atomicMin(&s.found, uint32_t(tid * kEach + e));
-            }
-            __syncthreads();
-            const uint32_t sub = s.found < uint32_t(kBins) ? s.found : s.n;
-            __syncthreads();
-            w = base + m.before;
-            c = taken + m.taken;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                if (sub == uint32_t(tid * kEach + e)) {
-                    s.weight = w;
-                    s.lo = c;
-                    s.hi = m.tokens[e];
-                }
-                w += m.weight[e];
-                c += m.tokens[e];
-            }
-            __syncthreads();
-            base = s.weight;
-            taken = s.lo;
-            count = s.hi;
-            __syncthreads();
-            hi -= sub << step;
-            const uint32_t span = (uint32_t(1) << step) - 1;
-            if (hi - lo > span) lo = hi - span;
-            if (count <= uint32_t(MOST)) {
-                gather([&](float x) { return order(x) >= lo && order(x) <= hi; });
-                rank(count);
-                return answer(count, ask, t, q, base, taken);
-            }
-        }
-        // Equal logits, in the order of their tokens.
-        const double w = weight_of(unordered(lo)), steps = (t - base) / w;
-        if (ask == Ask::Draw) {
-            const uint32_t last = min(count, q - taken) - 1;
-            const uint32_t at = steps >= double(last) ? last : steps > 0.0 ? uint32_t(steps) : 0;
-            return {0, w, nth_of(lo, at)};
-        }
-        const uint32_t c = ask == Ask::Count       ? min(count, q - taken)
-                           : steps >= double(count) ? count
-                           : steps > 1.0            ? uint32_t(ceil(steps))
-                                                    : 1;
-        return {taken + c, base + double(c) * w, 0};
-    }
-};
-
-struct Drawn {
-    uint32_t token;
-    double weight, of;
-};
-
-// Draws from the n first in rank, of which the whole is `whole` to top_p, or (negative) their own.
-template <class R>
-__device__ Drawn draw_ranked(R &r, uint32_t n, const Settings &set, double whole) {
-    r.rank(n);
-    if (set.top_k) n = min(n, set.top_k);
-    if (set.with_p) n = min(n, r.below(n, set.top_p * (whole < 0.0 ? r.s.sums[n - 1] : whole), false) + 1);
-    if (set.with_min) {
-        uint32_t c = 0;
-        for (uint32_t i = r.tid; i < n; i += blockDim.x)
-            c += r.weight_of(unordered(uint32_t(r.s.list[i] >> 32))) >= set.min_p;
-        n = max(1u, r.block_count(c));
-    }
-    const double all = r.s.sums[n - 1];
-    const uint64_t v = r.s.list[min(r.below(n, set.uniform * all, true), n - 1)];
-    return {~uint32_t(v), r.weight_of(unordered(uint32_t(v >> 32))), all};
-}
-
-// The bin of the k-th largest of the threads' maxima bounds the k-th largest logit
-// from below; bins past the last with a weight hold nothing that can be drawn.
-template <class R>
-__device__ int bound_bin(R &r, float mine, uint32_t k) {
-    for (int i = r.tid; i < kBins; i += int(blockDim.x)) r.s.counts[i] = 0;
-    __syncthreads();
-    const double y = r.place(mine);
-    if (y < double(kBins - 1)) atomicAdd(&r.s.counts[int(y)], 1u);
-    __syncthreads();
-    constexpr int E = R::kEach;
-    uint32_t c[E], sum = 0, total;
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum += c[e] = r.s.counts[r.tid * E + e];
-    uint32_t before = r.template block_scan<uint32_t>(sum, r.s.wave_u, total);
-    if (r.tid == 0) r.s.found = kBins - 2;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (before < k && before + c[e] >= k) r.s.found = uint32_t(r.tid * E + e);
-        before += c[e];
-    }
-    __syncthreads();
-    const int b = int(r.s.found);
-    __syncthreads();
-    return b;
-}
-
-// A logit that is at or below every logit with place < `until`.
-template <class R>
-__device__ float least_of(const R &r, double until) {
-    const double down = until / r.scale, x = double(r.top) - down - (fabs(double(r.top)) + down) * 0x1p-20;
-    return x > -double(FLT_MAX) ? float(x) : -FLT_MAX;
-}
-
-// The whole row by its bins.
-template <class R>
-__device__ Drawn draw_long(R &r, const Settings &set) {
-    auto &s = r.s;
-    r.shift = 63 - max(1, 32 - __clz(int(r.vocab)));
-    r.dev_bits = min(36, 2 * r.shift - 58);  // a bin's sum, vocab terms under 0.0156, stays in its field
-    r.fill_bins(false, 0, 0, 0, 0);
-    r.keep_bins();
-    const auto few = [&](int b) { return s.tokens[b + 1] <= uint32_t(R::kMostRanked); };
-    const auto ranked = [&](int b, double whole) {
-        const double until = double(b + 1);
-        const uint32_t n = r.gather([&](float x) { return r.place(x) < until; });
-        return draw_ranked(r, n, set, whole);
-    };
-    Border end{kBins, 0, s.before[kBins]};
-    double whole = -1.0;
-    if (set.top_k && set.top_k < s.tokens[kBins]) {
-        const int b = r.first_bin([&](int i) { return s.tokens[i + 1] >= set.top_k; });
-        if (few(b)) return ranked(b, -1.0);
-        const auto at = r.resolve(b, Ask::Count, 0.0, set.top_k - s.tokens[b]);
-        end = {b, at.in, at.weight};
-    }
-    if (set.with_p) {
-        whole = end.weight;
-        const double t = set.top_p * whole;
-        const int b = r.first_bin([&](int i) { return s.before[i + 1] >= t; });
-        if (b < kBins && b <= end.bin) {
-            if (few(b)) return ranked(b, whole);
-            const auto at = r.resolve(b, Ask::Reach, t, 0);
-            if (b < end.bin || at.in < end.in) end = {b, at.in, at.weight};
-        }
-    }
-    if (set.with_min) {
-        const double y = -log(set.min_p) * kPerUnit;
-        const int b = y < double(kBins - 1) ? max(0, int(y)) : kBins;
-        if (b < kBins && b <= end.bin) {
-            if (few(b)) return ranked(b, whole);
-            const double from = double(b), until = double(b + 1);
-            double w = 0.0, in;
-            uint32_t c = 0;
-            each<typename R::Element, R::kThreads>(r.z, r.vocab, [&](float x, uint32_t) {
-                const double at = r.place(x);
-                if (at >= from && at < until) {
-                    const double v = r.weight_of(x);
-                    if (v >= set.min_p) {
-                        w += v;
-                        ++c;
+    // From the bins: one border after the other, then the token.
+    __device__ __forceinline__ void draw_bins(const SampleArgs &a, size_t row, const Settings &set) {
+        // What is left: the first `left` tokens, with the weight `whole`.
+        uint32_t left;
+        double whole;
+        fill(left, whole);
+        whole = uniform(whole);
+#pragma unroll 1
+        for (int ask = kCount; ask < kAsks; ++ask) {
+            // What depends on them alone is made where it is used, not kept in registers over the loop.
+            asm volatile("" : "+v"(tid), "+s"(z));
+            // The weight that is asked for, in all that is left or (kCount) its first tokens.
+            double t = 0.0;
+            if (ask == kCount) {
+                if (!set.top_k || set.top_k >= left) continue;
+                left = set.top_k;
+            } else if (ask == kReachP) {
+                if (!set.with_p) continue;
+                t = uniform(set.top_p * whole);
+            } else if (ask == kLeast) {
+                if (!set.with_min) continue;
+                // The bin of min_p, and its tokens from min_p on.
+                if (!(until_min < kReach * kPerUnit)) continue;
+                const int at = int(until_min);
+                const float from = least(double(at + 1)), to = most(double(at));
+                double w = 0.0;
+                uint32_t c = 0;
+                each_in<T, THREADS>(z, vocab, from, to, [&](float x, uint32_t) {
+                    const double o = place(x);
+                    if (o >= double(at) && o < double(at + 1)) {
+                        const double v = weight_of(x);
+                        if (v >= set.min_p) {
+                            w += v;
+                            ++c;
+                        }
                     }
+                });
+                w = block_total<THREADS>(w, s.room_d);
+                c = block_total<THREADS>(c, s.room_u);
+                const Bin b = find([&](const Bin &o) { return o.at == at; });
+                if (b.taken + c < left) {
+                    left = b.taken + c;
+                    whole = uniform(b.base + w);
                 }
+                continue;
+            } else {
+                t = uniform(set.uniform * whole);
+            }
+            const Bin b = find([&](const Bin &o) {
+                return o.count && (o.taken + o.count >= left || (ask == kReachP ? o.base + o.weight >= t
+                                                                                : ask == kDraw && o.base + o.weight > t));
             });
-            r.template block_scan<double>(w, s.wave_d, in);
-            c = r.block_count(c);
-            if (b < end.bin || c < end.in) end = {b, c, s.before[b] + in};
+            const uint32_t q = left - b.taken;  // tokens of the bin that are left, or more
+            // Inside the bin.
+            const double from = double(b.at), until = double(b.at + 1);
+            const float x_from = least(until), x_to = most(from);
+            double base = b.base;
+            uint32_t taken = 0, n = b.count;
+            uint32_t lo = 0, hi = 0;
+            bool ranked = n <= uint32_t(MOST);
+            if (ranked) {
+                if (tid == 0) s.n = 0;
+                __syncthreads();
+                each_in<T, THREADS>(z, vocab, x_from, x_to, [&](float x, uint32_t token) {
+                    const double y = place(x);
+                    if (y >= from && y < until) append(x, token);
+                });
+                __syncthreads();
+                n = min(s.n, uint32_t(MOST));
+            } else {
+                lo = 0xffffffffu;
+                each_in<T, THREADS>(z, vocab, x_from, x_to, [&](float x, uint32_t) {
+                    const double y = place(x);
+                    if (y >= from && y < until) {
+                        lo = min(lo, order(x));
+                        hi = max(hi, order(x));
+                    }
+                });
+                if (tid == 0) {
+                    s.lo = 0xffffffffu;
+                    s.hi = 0;
+                }
+                __syncthreads();
+                atomicMin(&s.lo, lo);
+                atomicMax(&s.hi, hi);
+                __syncthreads();
+                lo = s.lo;
+                hi = s.hi;
+                __syncthreads();
+            }
+            const double begin = begin_of(b.at);
+            while (!ranked && lo != hi) {
+                constexpr int kBits = 31 - __builtin_clz(THREADS);
+                const int step = max(0, 32 - __clz(int(hi - lo)) - kBits);  // (hi - lo) >> step < THREADS
+                s.fine[tid] = 0;
+                __syncthreads();
+                each_in<T, THREADS>(z, vocab, unordered(lo), unordered(hi), [&](float x, uint32_t) {
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&s.fine[(hi - order(x)) >> step]),
+                              static_cast<unsigned long long>(term(place(x) - from)));
+                });
+                if (tid == 0) {
+                    s.found = THREADS;
+                    s.n = 0;
+                }
+                __syncthreads();
+                uint32_t c, all_c;
+                double w, all_w;
+                split(s.fine[tid], begin, c, w);
+                const double before_w = base + block_scan<THREADS>(w, s.room_d, all_w);
+                const uint32_t before_c = taken + block_scan<THREADS>(c, s.room_u, all_c);
+                if (c) {
+                    atomicMax(&s.n, uint32_t(tid));
+                    if (before_c + c >= q || (ask == kReachP ? before_w + w >= t : ask == kDraw && before_w + w > t))
+                        atomicMin(&s.found, uint32_t(tid));
+                }
+                __syncthreads();
+                const uint32_t sub = s.found < uint32_t(THREADS) ? s.found : s.n;
+                __syncthreads();
+                if (sub == uint32_t(tid)) {
+                    s.base = before_w;
+                    s.lo = before_c;
+                    s.hi = c;
+                }
+                __syncthreads();
+                base = uniform(s.base);
+                taken = s.lo;
+                n = s.hi;
+                hi -= sub << step;
+                const uint32_t span = (uint32_t(1) << step) - 1;
+                if (hi - lo > span) lo = hi - span;
+                ranked = n <= uint32_t(MOST);
+                if (ranked) {
+                    if (tid == 0) s.n = 0;
+                    __syncthreads();
+                    each_in<T, THREADS>(z, vocab, unordered(lo), unordered(hi),
+                                        [&](float x, uint32_t token) { append(x, token); });
+                }
+                __syncthreads();
+            }
+            if (ranked) {
+                rank(n);
+                if (ask == kDraw) {
+                    finish(a, row, s.list[min(below(n, t - base, true), min(n, q - taken) - 1)], whole);
+                    return;
+                }
+                const uint32_t c = ask == kCount ? min(n, q - taken) : min(min(n, q - taken), below(n, t - base, false) + 1);
+                left = b.taken + taken + c;
+                whole = uniform(base + s.sums[c - 1]);
+                __syncthreads();
+            } else {  // equal logits, in the order of their tokens
+                const double w = weight_of(unordered(lo));
+                n = min(n, q - taken);
+                if (ask == kDraw) {
+                    const uint32_t token = nth_of(lo, equal_draw(t - base, w, n));
+                    if (tid == 0) write(a, row, token, float(log(w / whole)));
+                    return;
+                }
+                const uint32_t c = ask == kCount ? n : equal_reach(t - base, w, n);
+                left = b.taken + taken + c;
+                whole = uniform(base + double(c) * w);
+            }
         }
     }
-    const double t = set.uniform * end.weight;
-    int b = r.first_bin([&](int i) { return s.before[i + 1] > t && s.tokens[i + 1] > s.tokens[i]; });
-    if (b >= end.bin && (end.in == 0 || b >= kBins)) {  // rounding: the last that is left
-        if (end.bin < kBins && end.in)
-            b = end.bin;
-        else
-            b = kBins - 1 - r.first_bin([&](int i) {
-                const int j = kBins - 1 - i;
-                return j < end.bin && s.tokens[j + 1] > s.tokens[j];
-            });
-    }
-    b = min(b, end.bin);
-    const auto at = r.resolve(b, Ask::Draw, t, b == end.bin ? end.in : s.tokens[b + 1] - s.tokens[b]);
-    return {at.token, at.weight, end.weight};
-}
+};
 
-template <class T, int THREADS, int MOST, bool LONG>
-__global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
-    using R = Row<T, THREADS, MOST, LONG>;
-    __shared__ typename R::Shared shared;
+template <class T, int THREADS, int BINS, int MOST>
+__global__ void __launch_bounds__(THREADS) sample_bins_kernel(SampleArgs a) {
+    using B = Bins<T, THREADS, BINS, MOST>;
+    __shared__ typename B::Shared s;
     const size_t row = blockIdx.x;
-    R r(static_cast<const typename T::Raw *>(a.logits) + row * a.stride, uint32_t(a.vocab), shared);
-    Settings set;
-    set.temperature = a.temperatures ? double(a.temperatures[row]) : 1.0;
-    set.top_p = a.top_p ? double(a.top_p[row]) : 1.0;
-    set.min_p = a.min_p ? double(a.min_p[row]) : 0.0;
-    set.uniform = double(a.uniforms[row]);
-    const int k = a.top_k ? a.top_k[row] : 0;
-    set.top_k = k > 0 && uint32_t(k) < r.vocab ? uint32_t(k) : 0;
-    set.with_p = set.top_p < 1.0;
-    set.with_min = set.min_p > 0.0;
-    const bool greedy = set.temperature == 0.0;
-    const bool valid = set.temperature >= 0.0 && set.temperature <= double(FLT_MAX) && set.top_p == set.top_p &&
-                       set.min_p == set.min_p && (greedy || (set.uniform >= 0.0 && set.uniform < 1.0));
-    set.min_p = fmin(set.min_p, 1.0);  // the largest is always left
-
+    B b(static_cast<const typename T::Raw *>(a.logits) + row * a.stride, uint32_t(a.vocab), s);
+    const Settings set = settings_of(a, row);
+    b.until_min = uniform(set.with_min ? -log(set.min_p) * kPerUnit : 0.0);
+    Weights::prepare(s.powers);
     float mine = -INFINITY;
     bool bad = false;
-    each<T, THREADS>(r.z, r.vocab, [&](float x, uint32_t) {
+    each<T, THREADS>(b.z, b.vocab, [&](float x) {
         mine = fmaxf(mine, x);
         bad |= !(x < INFINITY);
     });
     const float wave_top = wave_largest(mine);
     const bool wave_bad = __ballot(bad) != 0;
-    if (r.lane == 0) {
-        shared.wave_f[r.wave] = wave_top;
-        shared.wave_u[r.wave] = wave_bad;
+    if (b.tid % 64 == 0) {
+        s.room_f[b.tid / 64] = wave_top;
+        s.room_u[b.tid / 64] = wave_bad;
+    }
+    if (b.tid == 0) {
+        s.n = 0;
+        s.found = kNoToken;
     }
     __syncthreads();
-    r.top = -INFINITY;
+    b.top = -INFINITY;
     uint32_t any_bad = 0;
 #pragma unroll
-    for (int w = 0; w < R::kWaves; ++w) {
-        r.top = fmaxf(r.top, shared.wave_f[w]);
-        any_bad |= shared.wave_u[w];
+    for (int w = 0; w < THREADS / 64; ++w) {
+        b.top = fmaxf(b.top, s.room_f[w]);
+        any_bad |= s.room_u[w];
     }
-    __syncthreads();
-    if (any_bad || r.top == -INFINITY || !valid) {
-        if (r.tid == 0) {
-            a.tokens[row] = kNoToken;
-            if (a.logprob) a.logprob[row] = NAN;
-        }
+    b.top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(uint32_t, b.top)));
+    if (any_bad || b.top == -INFINITY || !set.valid) {
+        if (b.tid == 0) write(a, row, kNoToken, NAN);
         return;
     }
-    if (greedy) {
-        if (r.tid == 0) shared.found = kNoToken;
+    if (set.greedy) {
+        uint32_t first = kNoToken;
+        each_in<T, THREADS>(b.z, b.vocab, b.top, b.top, [&](float, uint32_t token) { first = min(first, token); });
+        if (first != kNoToken) atomicMin(&s.found, first);
         __syncthreads();
-        uint32_t least = kNoToken;
-        each<T, THREADS>(r.z, r.vocab, [&](float x, uint32_t token) {
-            if (x == r.top) least = min(least, token);
-        });
-        if (least != kNoToken) atomicMin(&shared.found, least);
-        __syncthreads();
-        if (r.tid == 0) {
-            a.tokens[row] = shared.found;
-            if (a.logprob) a.logprob[row] = 0.0f;
-        }
+        if (b.tid == 0) write(a, row, s.found, 0.0f);
         return;
     }
-    r.inv = 1.0 / set.temperature;
-    r.scale = kPerUnit * r.inv;
-
-    float least = 0.0f;
-    bool few = true;
-    if constexpr (LONG) {
-        if (set.top_k && set.top_k <= uint32_t(THREADS / 2))
-            least = least_of(r, double(bound_bin(r, mine, set.top_k) + 1));
-        else if (set.with_min && !set.with_p)
-            least = least_of(r, -log(set.min_p) * kPerUnit);
-        else
-            few = false;
-    } else {
-        least = -FLT_MAX;
+    b.scale = uniform(kPerUnit / set.temperature);
+    const bool by_k = set.top_k && set.top_k <= uint32_t(THREADS / 2);
+    if (by_k || (set.with_min && !set.with_p)) {
+        const float from = by_k ? b.least(double(b.bound_bin(mine, set.top_k) + 1)) : b.least(b.until_min);
+        each_in<T, THREADS>(b.z, b.vocab, from, FLT_MAX, [&](float x, uint32_t token) { b.append(x, token); });
+        __syncthreads();
+        const uint32_t n = s.n;
+        if (n <= uint32_t(MOST)) return b.draw_few(a, row, set, n);
+        __syncthreads();
     }
-    Drawn d;
-    uint32_t n = 0;
-    if (few) {
-        n = r.gather([&](float x) { return x >= least; });
-        few = n <= uint32_t(MOST);
-    }
-    if constexpr (LONG)
-        d = few ? draw_ranked(r, n, set, -1.0) : draw_long(r, set);
-    else
-        d = draw_ranked(r, n, set, -1.0);
-    if (r.tid == 0) {
-        a.tokens[row] = d.token;
-        if (a.logprob) a.logprob[row] = float(log(d.weight / d.of));
-    }
+    b.draw_bins(a, row, set);
 }
 
 template <class T>
 void launch(const SampleArgs &a, hipStream_t stream) {
+    const dim3 rows(static_cast<unsigned>(a.rows));
     if (a.vocab <= size_t(kShort))
-        sample_kernel<T, 256, kShort, false><<<dim3(unsigned(a.rows)), 256, 0, stream>>>(a);
+        sample_short_kernel<T><<<rows, kShort, 0, stream>>>(a);
+    else if (a.vocab <= 8192)
+        sample_bins_kernel<T, 256, 2048, 1024><<<rows, 256, 0, stream>>>(a);
     else
-        sample_kernel<T, 1024, kMost, true><<<dim3(unsigned(a.rows)), 1024, 0, stream>>>(a);
+        sample_bins_kernel<T, 1024, 2048, 2048><<<rows, 1024, 0, stream>>>(a);
 }
 
 }  // namespace
