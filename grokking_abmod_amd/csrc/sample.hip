@@ -12,8 +12,10 @@
 // tokens one is 1e-5 of the whole.  So weights are summed in 64 bits, in an
 // order that is the same in every call.
 //
-// A row has a workgroup.  Up to kShort logits, every token counts those before it;
-// else they go into bins of (max z - z) / T (sample_bins_kernel).
+// A row has a workgroup, in one of three ways:
+//   up to kShort logits: every token counts the tokens and weights before it;
+//   16-bit logits: a count for each of their 65536 values (sample_codes_kernel);
+//   else: bins of (max z - z) / T (sample_bins_kernel).
 #include <cfloat>
 
 #include "dpp.hpp"
@@ -122,6 +124,8 @@ __device__ __forceinline__ void each_in(const typename T::Raw *z, uint32_t vocab
         if (x >= lo && x <= hi) f(x, last);
     }
 }
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // Running sums over a wave's lanes.
 template <class V>
@@ -308,10 +312,18 @@ struct Weights {
     const Powers &powers;  // in LDS
     double top, scale;     // the largest logit, bins of a unit of a logit
 
-    // Makes the powers; a barrier has to follow.
+    // Makes the powers, as products of e^(-2^b / 64) (to 6 * 2^-53); a barrier has to follow.
     static __device__ __forceinline__ void prepare(Powers &p) {
-        if (threadIdx.x < 32) p.wholes[threadIdx.x] = exp(-double(threadIdx.x));
-        if (threadIdx.x < kPerUnit) p.parts[threadIdx.x] = exp(-double(threadIdx.x) / kPerUnit);
+        const uint32_t i = threadIdx.x;
+        if (i >= 96) return;
+        const double of[11] = {0x1.f80feabfeefa5p-1, 0x1.f03f56a88b5d8p-1, 0x1.e0fabfbc702a4p-1, 0x1.c3d6a24ed8222p-1,
+                               0x1.8ebef9eac820bp-1, 0x1.368b2fc6f960ap-1, 0x1.78b56362cef38p-2, 0x1.152aaa3bf81ccp-3,
+                               0x1.2c155b8213cf4p-6, 0x1.5fc21041027adp-12, 0x1.e355bbaee85cbp-24};
+        double w = 1.0;
+#pragma unroll
+        for (int b = 0; b < 6; ++b)
+            if (i >> b & 1) w *= i < kPerUnit ? of[b] : of[min(6 + b, 10)];
+        (i < kPerUnit ? p.parts[i] : p.wholes[i - kPerUnit]) = w;
     }
     // Bins from the largest logit.
     __device__ __forceinline__ double place(float x) const { return (top - double(x)) * scale; }
@@ -329,6 +341,360 @@ struct Weights {
         return fma(begin, rest(y - at), begin);
     }
 };
+
+// ---- rows of 16 bits ------------------------------------------------------------------
+
+// Logits of 16 bits have 65536 values: one pass counts each, two to an LDS word, with
+// the row kept in registers, and all the rest follows from the counts, the weights of
+// the values and (the n-th of equal logits) a look through the registers.
+//
+// In rank order the values are q = 0..65535: the positive ones downwards, q = 0x7fff
+// minus the code, then the negative ones, q = the code.  They are summed in segments
+// of 64.  One code is counted apart, without its LDS word, which all lanes would meet
+// in: -inf, or what a sample of the row is full of (a mask's value).  No other code can
+// overflow its 16 bits unless it has more than half of the row; then it is looked for
+// and counted apart in a second pass.
+constexpr int kCodeThreads = 1024;
+constexpr int kCodeGroups = 16;  // of 8 logits a thread
+constexpr uint32_t kCodeMost = 131071;
+static_assert(kCodeMost < kCodeThreads * kCodeGroups * 8, "a row fits the registers");
+
+template <class T>
+struct Codes {
+    static constexpr int THREADS = kCodeThreads, WAVES = THREADS / 64, GROUPS = kCodeGroups;
+    static constexpr uint32_t kInf = std::is_same<T, F16>::value ? 0x7c00 : 0x7f80, kNegative = 0x8000 | kInf;
+
+    struct Part {
+        uint32_t segment, taken;
+        double base;
+    };
+    struct Shared {
+        uint32_t counts[32768 + 64];  // two codes a word; a word for each lane, of the code counted apart
+        uint32_t in_segment[THREADS];
+        double weights[THREADS];
+        Powers powers;
+        double room_d[WAVES];
+        uint32_t room_u[WAVES];
+        uint32_t matches[(GROUPS + 1) * WAVES];
+        Part parts[WAVES];
+    };
+
+    Shared &s;
+    uint32_t tid, lane, wave;
+    uint32_t hot, hot_count;  // counted apart
+    Weights weights;
+
+    static __device__ __forceinline__ uint32_t code_at(uint32_t q) { return q < 0x8000 ? 0x7fff - q : q; }
+    static __device__ __forceinline__ uint32_t segment_of(uint32_t code) { return (code < 0x8000 ? 0x7fff - code : code) / 64; }
+    static __device__ __forceinline__ float value(uint32_t code) { return T::to_float(__builtin_bit_cast(typename T::Raw, uint16_t(code))); }
+    __device__ __forceinline__ uint32_t count_of(uint32_t code) const {
+        if (code == hot) return hot_count;
+        return s.counts[code / 2] >> (code % 2 * 16) & 0xffff;
+    }
+
+    // The first segment that `is` takes ((weights, tokens) before and in it), or segment THREADS.
+    template <class Is>
+    __device__ __forceinline__ Part first(double base, uint32_t taken, Is &&is) {
+        const bool mine = is();
+        const uint64_t those = __ballot(mine);
+        if (those == 0) {
+            if (lane == 0) s.parts[wave].segment = THREADS;
+        } else if (int(lane) == __builtin_ctzll(those)) {
+            s.parts[wave] = {tid, taken, base};
+        }
+        __syncthreads();
+        int w = 0;
+        while (w + 1 < WAVES && s.parts[w].segment == uint32_t(THREADS)) ++w;
+        Part p = s.parts[w];
+        p.segment = __builtin_amdgcn_readfirstlane(p.segment);
+        p.taken = __builtin_amdgcn_readfirstlane(p.taken);
+        p.base = uniform(p.base);
+        __syncthreads();
+        return p;
+    }
+
+    // The values of a segment, one a lane, with what is before each.
+    struct Value {
+        uint32_t code, count, taken;
+        double weight, base;
+    };
+    __device__ __forceinline__ Value value_of(uint32_t segment) const {
+        Value v{};
+        v.code = code_at(segment * 64 + lane);
+        v.count = count_of(v.code);
+        if (v.code == kNegative) v.count = 0;
+        v.weight = v.count ? weights.of(value(v.code)) : 0.0;
+        if (v.weight == 0.0) v.count = 0;
+        return v;
+    }
+    __device__ __forceinline__ Value value_in(const Part &p) const {
+        Value v = value_of(p.segment);
+        const double w = double(v.count) * v.weight;
+        v.base = p.base + wave_scan(w, int(lane)) - w;
+        v.taken = p.taken + wave_scan(v.count, int(lane)) - v.count;
+        return v;
+    }
+    // Lane l's.
+    static __device__ __forceinline__ Value lane_of(Value v, int l) {
+        v.code = __builtin_amdgcn_readlane(v.code, l);
+        v.count = __builtin_amdgcn_readlane(v.count, l);
+        v.taken = __builtin_amdgcn_readlane(v.taken, l);
+        v.weight = uniform(__shfl(v.weight, l, 64));
+        v.base = uniform(__shfl(v.base, l, 64));
+        return v;
+    }
+};
+
+// One of the groups, which are in registers (a choice by masks: one by an index would put them into memory).
+__device__ __forceinline__ u32x4 group_of(const u32x4 (&w)[kCodeGroups], int at) {
+    u32x4 g = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < kCodeGroups; ++j) g |= w[j] & (at == j ? 0xffffffffu : 0u);
+    return g;
+}
+
+// The code that most of a sample of the row has, if it has a quarter of a wave's.
+template <class C>
+__device__ __forceinline__ uint32_t sampled_code(C &c, const u32x4 (&w)[kCodeGroups]) {
+    const u32x4 g = group_of(w, int(c.wave));
+    const uint32_t word = c.lane & 4 ? (c.lane & 2 ? g[3] : g[2]) : (c.lane & 2 ? g[1] : g[0]);
+    const uint32_t code = word >> (c.lane % 2 * 16) & 0xffff;
+    uint64_t rest = ~uint64_t(0);
+    uint32_t most = 15, at = 0;
+#pragma unroll 1
+    for (int i = 0; i < 4 && rest; ++i) {
+        const uint32_t one = __builtin_amdgcn_readlane(code, __builtin_ctzll(rest));
+        const uint64_t same = __ballot(code == one);
+        rest &= ~same;
+        if (uint32_t(__popcll(same)) > most) {
+            most = uint32_t(__popcll(same));
+            at = one;
+        }
+    }
+    if (c.lane == 0) c.s.room_u[c.wave] = most << 16 | at;
+    __syncthreads();
+    uint32_t best = 0;
+#pragma unroll
+    for (int v = 0; v < C::WAVES; ++v) best = max(best, c.s.room_u[v]);
+    __syncthreads();
+    return best >> 16 > 15 ? best & 0xffff : C::kNegative;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a) {
+    using C = Codes<T>;
+    using Raw = typename T::Raw;
+    __shared__ typename C::Shared s;
+    const size_t row = blockIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, vocab = uint32_t(a.vocab);
+    const Raw *const z = static_cast<const Raw *>(a.logits) + row * a.stride;
+    const uint32_t groups = vocab / 8, tail = vocab % 8;
+    u32x4 w[kCodeGroups];
+#pragma unroll
+    for (int j = 0; j < kCodeGroups; ++j) w[j] = *reinterpret_cast<const u32x4_any *>(z + size_t(min(j * C::THREADS + tid, groups - 1)) * 8);
+    const uint32_t last = tid < tail ? uint32_t(__builtin_bit_cast(uint16_t, z[groups * 8 + tid])) : 0;
+    const Settings set = settings_of(a, row);
+    Weights::prepare(s.powers);
+    C c{s, tid, lane, wave, 0, 0, {s.powers, 0.0, set.greedy ? 1.0 : uniform(kPerUnit / set.temperature)}};
+    c.hot = sampled_code(c, w);
+    uint32_t mine;  // tokens of a thread's segment, without those of -inf
+#pragma unroll 1
+    for (bool again = false;; again = true) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) reinterpret_cast<uint4 *>(s.counts)[i * C::THREADS + tid] = uint4{0, 0, 0, 0};
+        if (tid < 64) s.counts[32768 + tid] = 0;
+        __syncthreads();
+        // What is counted apart goes to the lane's own word.
+        const uint32_t own = 32768 + lane;
+        const auto count = [&](uint32_t code) {
+            const bool is = code == c.hot;
+            atomicAdd(&s.counts[is ? own : code / 2], is || !(code & 1) ? 1u : 65536u);
+        };
+#pragma unroll
+        for (int j = 0; j < kCodeGroups; ++j) {
+            if (j * C::THREADS + tid < groups) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) count(w[j][e / 2] >> (e % 2 * 16) & 0xffff);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // one group's registers at a time
+        }
+        if (tid < tail) count(last);
+        __syncthreads();
+        c.hot_count = wave_total(s.counts[32768 + lane]);
+        // A thread's segment: 32 words in a row, begun at another one in each lane.
+        const uint32_t from = tid < 512 ? 16384 - 32 * (tid + 1) : 32 * tid;
+        uint32_t n = 0;
+#pragma unroll 8
+        for (uint32_t i = 0; i < 32; ++i) n = __builtin_amdgcn_sad_u16(s.counts[from + (i + tid) % 32], 0, n);
+        const uint32_t all = block_total<C::THREADS>(n, s.room_u);
+        if (tid == C::segment_of(C::kNegative) && c.hot != C::kNegative) n -= c.count_of(C::kNegative);
+        if (tid == C::segment_of(c.hot) && c.hot != C::kNegative) n += c.hot_count;
+        mine = n;
+        if (again || all + c.hot_count == vocab) break;
+        // Some code has overflowed: it has most of the row, and each of its bits most of theirs.
+        uint32_t ones[16];
+        if (tid < 16) s.matches[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < 16; ++b) ones[b] = 0;
+#pragma unroll 1
+        for (uint32_t i = tid; i < (vocab + 63) / 64 * 64; i += C::THREADS) {
+            const uint32_t code = i < vocab ? __builtin_bit_cast(uint16_t, z[i]) : 0;
+#pragma unroll
+            for (int b = 0; b < 16; ++b) ones[b] += uint32_t(__popcll(__ballot(code >> b & 1)));
+        }
+#pragma unroll
+        for (int b = 0; b < 16; ++b)
+            if (lane == 0) atomicAdd(&s.matches[b], ones[b]);
+        __syncthreads();
+        c.hot = uint32_t(__ballot(lane < 16 && 2 * s.matches[lane % 16] > vocab));
+        __syncthreads();
+    }
+
+    // What is not a number or +inf comes first in the order, and last, with -inf.
+    const bool odd = mine && (tid <= C::segment_of(C::kInf) || tid >= C::segment_of(C::kNegative));
+    s.in_segment[tid] = mine;
+    s.weights[tid] = 0.0;
+    const typename C::Part begin = c.first(0.0, 0, [&] { return mine != 0; });
+    const bool bad = block_total<C::THREADS>(uint32_t(odd), s.room_u) != 0;
+    if (bad || begin.segment == uint32_t(C::THREADS) || !set.valid) {
+        if (tid == 0) write(a, row, kNoToken, NAN);
+        return;
+    }
+    uint32_t code = C::code_at(begin.segment * 64 + lane), at = 0;
+    code = __builtin_amdgcn_readlane(code, __builtin_ctzll(__ballot(c.count_of(code) != 0)));
+    double share = 1.0;  // of the token that is drawn
+    if (!set.greedy) {
+        c.weights.top = uniform(double(C::value(code)));
+        // The segments' weights, a wave a segment; and what is over min_p.
+        double over = 0.0;
+        uint32_t over_count = 0;
+        uint64_t full = __ballot(s.in_segment[wave + C::WAVES * lane] != 0);
+        while (full) {
+            const uint32_t segment = wave + C::WAVES * uint32_t(__builtin_ctzll(full));
+            full &= full - 1;
+            const typename C::Value v = c.value_of(segment);
+            const double sum = double(v.count) * v.weight;
+            if (set.with_min && v.weight >= set.min_p) {
+                over += sum;
+                over_count += v.count;
+            }
+            const double weight = wave_total(sum);
+            const uint32_t count = wave_total(v.count);
+            if (lane == 0) {
+                s.weights[segment] = weight;
+                s.in_segment[segment] = count;
+            }
+        }
+        __syncthreads();
+        // What is left: the first `left` tokens, with the weight `whole`.
+        const double weight = s.weights[tid];
+        const uint32_t count = s.in_segment[tid];
+        double whole;
+        uint32_t left;
+        const double base = block_scan<C::THREADS>(weight, s.room_d, whole);
+        const uint32_t taken = block_scan<C::THREADS>(count, s.room_u, left);
+        whole = uniform(whole);
+        // The value at which the tokens reach `left`, or (p) the weights t, or exceed it.
+        const auto find = [&](double t, bool p, bool over_t) {
+            const typename C::Part part = c.first(base, taken, [&] {
+                return count && (taken + count >= left || (p && base + weight >= t) || (over_t && base + weight > t));
+            });
+            const typename C::Value v = c.value_in(part);
+            const double until = v.base + double(v.count) * v.weight;
+            const uint64_t any = __ballot(v.count != 0);
+            const uint64_t those = __ballot(v.count && (v.taken + v.count >= left || (p && until >= t) || (over_t && until > t)));
+            return C::lane_of(v, those ? __builtin_ctzll(those) : 63 - __builtin_clzll(any));
+        };
+        if (set.top_k && set.top_k < left) {
+            left = set.top_k;
+            const typename C::Value v = find(0.0, false, false);
+            whole = v.base + double(left - v.taken) * v.weight;
+        }
+        if (set.with_p) {
+            const double t = set.top_p * whole;
+            const typename C::Value v = find(t, true, false);
+            const uint32_t n = equal_reach(t - v.base, v.weight, min(v.count, left - v.taken));
+            left = v.taken + n;
+            whole = v.base + double(n) * v.weight;
+        }
+        if (set.with_min) {
+            over = block_total<C::THREADS>(over, s.room_d);
+            over_count = block_total<C::THREADS>(over_count, s.room_u);
+            if (over_count < left) {
+                left = over_count;
+                whole = over;
+            }
+        }
+        const double t = set.uniform * whole;
+        const typename C::Value v = find(t, false, true);
+        at = equal_draw(t - v.base, v.weight, min(v.count, left - v.taken));
+        code = v.code;
+        share = uniform(v.weight / whole);
+    }
+
+    // The at-th token of that code, from 0; the two zeros are equal.
+    const bool zero = (code & 0x7fff) == 0;
+    if (code == 0x8000) at += c.count_of(0);
+    const uint32_t bits = zero ? 0x7fff7fffu : 0xffffffffu, wanted = (code & bits) * 0x10001u;
+    const auto matches = [&](u32x4 g) {  // of its 8 logits: those whose difference has no bit
+        uint32_t n = 8;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u16x2 d = __builtin_bit_cast(u16x2, (g[e] & bits) ^ wanted);
+            n -= __builtin_amdgcn_sad_u16(__builtin_bit_cast(uint32_t, __builtin_elementwise_min(d, u16x2{1, 1})), 0, 0);
+        }
+        return n;
+    };
+#pragma unroll
+    for (int j = 0; j <= kCodeGroups; ++j) {
+        uint32_t n;
+        if (j < kCodeGroups)
+            n = j * C::THREADS + tid < groups ? matches(w[j < kCodeGroups ? j : 0]) : 0;
+        else
+            n = tid < tail && (last & bits) == (wanted & 0xffff);
+        uint32_t all = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) all += uint32_t(__popcll(__ballot(n >> b & 1))) << b;
+        if (lane == 0) s.matches[j * C::WAVES + wave] = all;
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+    // Every wave looks for the group and the wave of the at-th, and the one that has it goes on.
+    uint32_t here = 0;
+    if (lane <= uint32_t(kCodeGroups)) {
+#pragma unroll
+        for (int v = 0; v < C::WAVES; ++v) here += s.matches[lane * C::WAVES + v];
+    }
+    uint32_t sum = wave_scan(here, int(lane));
+    const int j = __builtin_ctzll(__ballot(sum > at));  // there is one
+    uint32_t before = __builtin_amdgcn_readlane(sum - here, j);
+    here = lane < C::WAVES ? s.matches[j * C::WAVES + lane] : 0;
+    sum = before + wave_scan(here, int(lane));
+    if (uint32_t(__builtin_ctzll(__ballot(sum > at))) != wave) return;
+    before = __builtin_amdgcn_readlane(sum - here, int(wave));
+    const u32x4 g = group_of(w, j);
+    const bool in_tail = j == kCodeGroups;
+    uint32_t n;
+    if (in_tail)
+        n = tid < tail && (last & bits) == (wanted & 0xffff);
+    else
+        n = j * C::THREADS + tid < groups ? matches(g) : 0;
+    here = before + wave_scan(n, int(lane)) - n;
+    if (at < here || at >= here + n) return;
+    uint32_t token = groups * 8 + tid;
+    if (!in_tail) {
+        token = (j * C::THREADS + tid) * 8;
+        uint32_t skip = at - here;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool is = ((g[e / 2] >> (e % 2 * 16) ^ wanted) & bits & 0xffff) == 0;
+            if (is && skip == 0) token += e;
+            if (is) --skip;
+        }
+    }
+    write(a, row, token, float(log(share)));
+}
 
 // ---- the general way -----------------------------------------------------------------
 
@@ -825,8 +1191,10 @@ void launch(const SampleArgs &a, hipStream_t stream) {
         sample_short_kernel<T><<<rows, kShort, 0, stream>>>(a);
     else if (a.vocab <= 8192)
         sample_bins_kernel<T, 256, 2048, 1024><<<rows, 256, 0, stream>>>(a);
-    else
+    else if (sizeof(typename T::Raw) == 4 || a.vocab > size_t(kCodeMost))
         sample_bins_kernel<T, 1024, 2048, 2048><<<rows, 1024, 0, stream>>>(a);
+    else if constexpr (sizeof(typename T::Raw) == 2)
+        sample_codes_kernel<T><<<rows, kCodeThreads, 0, stream>>>(a);
 }
 
 }  // namespace
