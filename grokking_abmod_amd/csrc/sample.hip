@@ -127,51 +127,61 @@ __device__ __forceinline__ void each_in(const typename T::Raw *z, uint32_t vocab
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
-// Running sums over a wave's lanes.
+// v of the lane that the DPP pattern CTRL names, 0 where there is none.
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROW_MASK, 0xf, false));
+}
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ double moved(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, uint64_t(moved<CTRL, ROW_MASK>(uint32_t(b >> 32))) << 32 | moved<CTRL, ROW_MASK>(uint32_t(b)));
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, uint64_t(lane_value(uint32_t(b >> 32), lane)) << 32 | lane_value(uint32_t(b), lane));
+}
+// Running sums over the lanes of a row of 16, and over a wave's.
 template <class V>
-__device__ __forceinline__ V wave_scan(V v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const V o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
+__device__ __forceinline__ V row_scan(V v) {
+    v += moved<0x111>(v);  // row_shr:1
+    v += moved<0x112>(v);
+    v += moved<0x114>(v);
+    v += moved<0x118>(v);
+    return v;
+}
+template <class V>
+__device__ __forceinline__ V wave_scan(V v) {
+    v = row_scan(v);
+    v += moved<0x142, 0xa>(v);  // row_bcast:15
+    v += moved<0x143, 0xc>(v);  // row_bcast:31
     return v;
 }
 template <class V>
 __device__ __forceinline__ V wave_total(V v) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
-    return v;
+    return lane_value(wave_scan(v), 63);
 }
 
 // The sum of the values of the threads before, and of all of them.
 template <int THREADS, class V>
 __device__ __forceinline__ V block_scan(V v, V *room, V &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const V in = wave_scan(v, lane);
+    constexpr int WAVES = THREADS / 64;
+    static_assert(WAVES <= 16, "a row of lanes has the waves' sums");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const V in = wave_scan(v);
     __syncthreads();
     if (lane == 63) room[wave] = in;
     __syncthreads();
-    V base = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-        const V o = room[w];
-        if (w < wave) base += o;
-        sum += o;
-    }
-    total = sum;
-    return base + in - v;
+    const V own = lane < WAVES ? room[lane] : V(0), sums = row_scan(own);
+    total = lane_value(sums, WAVES - 1);
+    return lane_value(sums - own, wave) + (in - v);
 }
 template <int THREADS, class V>
 __device__ __forceinline__ V block_total(V v, V *room) {
-    v = wave_total(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
-    __syncthreads();
-    V sum = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) sum += room[w];
-    return sum;
+    V total;
+    block_scan<THREADS>(v, room, total);
+    return total;
 }
 
 struct Settings {
@@ -369,18 +379,18 @@ struct Codes {
         double base;
     };
     struct Shared {
-        uint32_t counts[32768 + 64];  // two codes a word; a word for each lane, of the code counted apart
+        uint32_t counts[32768 + 64];  // of a code and its negative; then of the code counted apart, a word a lane
         uint32_t in_segment[THREADS];
         double weights[THREADS];
         Powers powers;
         double room_d[WAVES];
         uint32_t room_u[WAVES];
-        uint32_t matches[(GROUPS + 1) * WAVES];
+        uint32_t bits[16];
         Part parts[WAVES];
     };
 
     Shared &s;
-    uint32_t tid, lane, wave;
+    uint32_t tid, lane, wave, each;
     uint32_t hot, hot_count;  // counted apart
     Weights weights;
 
@@ -389,7 +399,7 @@ struct Codes {
     static __device__ __forceinline__ float value(uint32_t code) { return T::to_float(__builtin_bit_cast(typename T::Raw, uint16_t(code))); }
     __device__ __forceinline__ uint32_t count_of(uint32_t code) const {
         if (code == hot) return hot_count;
-        return s.counts[code / 2] >> (code % 2 * 16) & 0xffff;
+        return s.counts[code & 0x7fff] >> (code / 0x8000 * 16) & 0xffff;
     }
 
     // The first segment that `is` takes ((weights, tokens) before and in it), or segment THREADS.
@@ -430,8 +440,8 @@ struct Codes {
     __device__ __forceinline__ Value value_in(const Part &p) const {
         Value v = value_of(p.segment);
         const double w = double(v.count) * v.weight;
-        v.base = p.base + wave_scan(w, int(lane)) - w;
-        v.taken = p.taken + wave_scan(v.count, int(lane)) - v.count;
+        v.base = p.base + wave_scan(w) - w;
+        v.taken = p.taken + wave_scan(v.count) - v.count;
         return v;
     }
     // Lane l's.
@@ -439,8 +449,8 @@ struct Codes {
         v.code = __builtin_amdgcn_readlane(v.code, l);
         v.count = __builtin_amdgcn_readlane(v.count, l);
         v.taken = __builtin_amdgcn_readlane(v.taken, l);
-        v.weight = uniform(__shfl(v.weight, l, 64));
-        v.base = uniform(__shfl(v.base, l, 64));
+        v.weight = lane_value(v.weight, l);
+        v.base = lane_value(v.base, l);
         return v;
     }
 };
@@ -456,7 +466,7 @@ __device__ __forceinline__ u32x4 group_of(const u32x4 (&w)[kCodeGroups], int at)
 // The code that most of a sample of the row has, if it has a quarter of a wave's.
 template <class C>
 __device__ __forceinline__ uint32_t sampled_code(C &c, const u32x4 (&w)[kCodeGroups]) {
-    const u32x4 g = group_of(w, int(c.wave));
+    const u32x4 g = group_of(w, int(c.wave % c.each));
     const uint32_t word = c.lane & 4 ? (c.lane & 2 ? g[3] : g[2]) : (c.lane & 2 ? g[1] : g[0]);
     const uint32_t code = word >> (c.lane % 2 * 16) & 0xffff;
     uint64_t rest = ~uint64_t(0);
@@ -488,14 +498,20 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
     const size_t row = blockIdx.x;
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, vocab = uint32_t(a.vocab);
     const Raw *const z = static_cast<const Raw *>(a.logits) + row * a.stride;
-    const uint32_t groups = vocab / 8, tail = vocab % 8;
+    // A wave has `each` times 64 groups in a row, and a lane every 64th of them.
+    const uint32_t groups = vocab / 8, tail = vocab % 8, each = (groups + C::THREADS - 1) / C::THREADS;
+    const auto group = [&](int g) { return (wave * each + uint32_t(g)) * 64 + lane; };
     u32x4 w[kCodeGroups];
 #pragma unroll
-    for (int j = 0; j < kCodeGroups; ++j) w[j] = *reinterpret_cast<const u32x4_any *>(z + size_t(min(j * C::THREADS + tid, groups - 1)) * 8);
+    for (int j = 0; j < kCodeGroups; ++j)
+        if (uint32_t(j) < each) {
+            w[j] = *reinterpret_cast<const u32x4_any *>(z + size_t(min(group(j), groups - 1)) * 8);
+            w[j] |= group(j) < groups ? 0 : 0x7fff7fffu;  // NaN, which no token that is drawn is
+        }
     const uint32_t last = tid < tail ? uint32_t(__builtin_bit_cast(uint16_t, z[groups * 8 + tid])) : 0;
     const Settings set = settings_of(a, row);
     Weights::prepare(s.powers);
-    C c{s, tid, lane, wave, 0, 0, {s.powers, 0.0, set.greedy ? 1.0 : uniform(kPerUnit / set.temperature)}};
+    C c{s, tid, lane, wave, each, 0, 0, {s.powers, 0.0, set.greedy ? 1.0 : uniform(kPerUnit / set.temperature)}};
     c.hot = sampled_code(c, w);
     uint32_t mine;  // tokens of a thread's segment, without those of -inf
 #pragma unroll 1
@@ -507,12 +523,12 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         // What is counted apart goes to the lane's own word.
         const uint32_t own = 32768 + lane;
         const auto count = [&](uint32_t code) {
-            const bool is = code == c.hot;
-            atomicAdd(&s.counts[is ? own : code / 2], is || !(code & 1) ? 1u : 65536u);
+            atomicAdd(&s.counts[code == c.hot ? own : code & 0x7fff], code & 0x8000 ? 65536u : 1u);
         };
 #pragma unroll
         for (int j = 0; j < kCodeGroups; ++j) {
-            if (j * C::THREADS + tid < groups) {
+            asm volatile("" : "+v"(w[j]));  // what is made of it is not kept from one pass for the other
+            if (uint32_t(j) < each && group(j) < groups) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) count(w[j][e / 2] >> (e % 2 * 16) & 0xffff);
             }
@@ -520,12 +536,12 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         }
         if (tid < tail) count(last);
         __syncthreads();
-        c.hot_count = wave_total(s.counts[32768 + lane]);
-        // A thread's segment: 32 words in a row, begun at another one in each lane.
-        const uint32_t from = tid < 512 ? 16384 - 32 * (tid + 1) : 32 * tid;
+        c.hot_count = wave_total(__builtin_amdgcn_sad_u16(s.counts[32768 + lane], 0, 0));
+        // A thread's segment: one half of 64 words in a row, begun at another one in each lane.
+        const uint32_t from = tid < 512 ? 32768 - 64 * (tid + 1) : 64 * (tid - 512), half = tid < 512 ? 0 : 16;
         uint32_t n = 0;
 #pragma unroll 8
-        for (uint32_t i = 0; i < 32; ++i) n = __builtin_amdgcn_sad_u16(s.counts[from + (i + tid) % 32], 0, n);
+        for (uint32_t i = 0; i < 64; ++i) n += s.counts[from + (i + tid) % 64] >> half & 0xffff;
         const uint32_t all = block_total<C::THREADS>(n, s.room_u);
         if (tid == C::segment_of(C::kNegative) && c.hot != C::kNegative) n -= c.count_of(C::kNegative);
         if (tid == C::segment_of(c.hot) && c.hot != C::kNegative) n += c.hot_count;
@@ -533,7 +549,7 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         if (again || all + c.hot_count == vocab) break;
         // Some code has overflowed: it has most of the row, and each of its bits most of theirs.
         uint32_t ones[16];
-        if (tid < 16) s.matches[tid] = 0;
+        if (tid < 16) s.bits[tid] = 0;
         __syncthreads();
 #pragma unroll
         for (int b = 0; b < 16; ++b) ones[b] = 0;
@@ -545,9 +561,9 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         }
 #pragma unroll
         for (int b = 0; b < 16; ++b)
-            if (lane == 0) atomicAdd(&s.matches[b], ones[b]);
+            if (lane == 0) atomicAdd(&s.bits[b], ones[b]);
         __syncthreads();
-        c.hot = uint32_t(__ballot(lane < 16 && 2 * s.matches[lane % 16] > vocab));
+        c.hot = uint32_t(__ballot(lane < 16 && 2 * s.bits[lane % 16] > vocab));
         __syncthreads();
     }
 
@@ -570,21 +586,32 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         double over = 0.0;
         uint32_t over_count = 0;
         uint64_t full = __ballot(s.in_segment[wave + C::WAVES * lane] != 0);
-        while (full) {
-            const uint32_t segment = wave + C::WAVES * uint32_t(__builtin_ctzll(full));
-            full &= full - 1;
-            const typename C::Value v = c.value_of(segment);
-            const double sum = double(v.count) * v.weight;
-            if (set.with_min && v.weight >= set.min_p) {
-                over += sum;
-                over_count += v.count;
+        while (full) {  // two at a time: each is a chain
+            uint32_t segment[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                segment[i] = full ? wave + C::WAVES * uint32_t(__builtin_ctzll(full)) : segment[0];
+                full &= full - 1;
             }
-            const double weight = wave_total(sum);
-            const uint32_t count = wave_total(v.count);
-            if (lane == 0) {
-                s.weights[segment] = weight;
-                s.in_segment[segment] = count;
+            const typename C::Value v[2] = {c.value_of(segment[0]), c.value_of(segment[1])};
+            double weight[2];
+            uint32_t count[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const double sum = double(v[i].count) * v[i].weight;
+                if (set.with_min && v[i].weight >= set.min_p && (i == 0 || segment[1] != segment[0])) {
+                    over += sum;
+                    over_count += v[i].count;
+                }
+                weight[i] = wave_total(sum);
+                count[i] = wave_total(v[i].count);
             }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (lane == 0) {
+                    s.weights[segment[i]] = weight[i];
+                    s.in_segment[segment[i]] = count[i];
+                }
         }
         __syncthreads();
         // What is left: the first `left` tokens, with the weight `whole`.
@@ -637,58 +664,59 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
     const bool zero = (code & 0x7fff) == 0;
     if (code == 0x8000) at += c.count_of(0);
     const uint32_t bits = zero ? 0x7fff7fffu : 0xffffffffu, wanted = (code & bits) * 0x10001u;
-    const auto matches = [&](u32x4 g) {  // of its 8 logits: those whose difference has no bit
-        uint32_t n = 8;
+    const auto others = [&](u32x4 g) {  // of its 8 logits, in two halves: a difference has a bit
+        u16x2 n = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const u16x2 d = __builtin_bit_cast(u16x2, (g[e] & bits) ^ wanted);
-            n -= __builtin_amdgcn_sad_u16(__builtin_bit_cast(uint32_t, __builtin_elementwise_min(d, u16x2{1, 1})), 0, 0);
-        }
+        for (int e = 0; e < 4; ++e)
+            n += __builtin_elementwise_min(__builtin_bit_cast(u16x2, (g[e] & bits) ^ wanted), u16x2{1, 1});
         return n;
     };
+    const auto matches = [&](u32x4 g) {
+        const u16x2 n = others(g);
+        return uint32_t(8 - n[0] - n[1]);
+    };
+    const auto in_group = [&](int g) { return uint32_t(g) < each ? matches(w[g]) : 0; };
+    u16x2 apart = {0, 0};
 #pragma unroll
-    for (int j = 0; j <= kCodeGroups; ++j) {
-        uint32_t n;
-        if (j < kCodeGroups)
-            n = j * C::THREADS + tid < groups ? matches(w[j < kCodeGroups ? j : 0]) : 0;
-        else
-            n = tid < tail && (last & bits) == (wanted & 0xffff);
-        uint32_t all = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) all += uint32_t(__popcll(__ballot(n >> b & 1))) << b;
-        if (lane == 0) s.matches[j * C::WAVES + wave] = all;
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int g = 0; g < kCodeGroups; ++g)
+        if (uint32_t(g) < each) apart += others(w[g]);
+    uint32_t n = 8 * each - apart[0] - apart[1];
+    // The wave that has it, or the tail behind the waves; there the group; there the lane.
+    n = wave_total(n);
+    if (lane == 0) s.room_u[wave] = n;
     __syncthreads();
-    // Every wave looks for the group and the wave of the at-th, and the one that has it goes on.
-    uint32_t here = 0;
-    if (lane <= uint32_t(kCodeGroups)) {
+    uint32_t own = lane < C::WAVES ? s.room_u[lane] : 0, sum = row_scan(own);
+    uint64_t those = __ballot(lane < C::WAVES && sum > at);
+    const bool in_tail = those == 0;
+    if ((in_tail ? 0 : uint32_t(__builtin_ctzll(those))) != wave) return;
+    uint32_t before = in_tail ? lane_value(sum, C::WAVES - 1) : lane_value(sum - own, int(wave)), skip;
+    int g = 0;
+    if (in_tail) {
+        own = tid < tail && (last & bits) == (wanted & 0xffff);
+    } else {
+        uint32_t pairs[kCodeGroups / 2];  // two groups' sums, of up to 512 each, a word
 #pragma unroll
-        for (int v = 0; v < C::WAVES; ++v) here += s.matches[lane * C::WAVES + v];
+        for (int i = 0; i < kCodeGroups / 2; ++i) pairs[i] = wave_scan(in_group(2 * i) | in_group(2 * i + 1) << 16);
+#pragma unroll
+        for (int i = 0; i < kCodeGroups; ++i) {
+            const uint32_t here = lane_value(pairs[i / 2], 63) >> (i % 2 * 16) & 0xffff;
+            if (before + here > at || g != i) continue;
+            before += here;
+            ++g;
+        }
+        own = matches(group_of(w, g));
     }
-    uint32_t sum = wave_scan(here, int(lane));
-    const int j = __builtin_ctzll(__ballot(sum > at));  // there is one
-    uint32_t before = __builtin_amdgcn_readlane(sum - here, j);
-    here = lane < C::WAVES ? s.matches[j * C::WAVES + lane] : 0;
-    sum = before + wave_scan(here, int(lane));
-    if (uint32_t(__builtin_ctzll(__ballot(sum > at))) != wave) return;
-    before = __builtin_amdgcn_readlane(sum - here, int(wave));
-    const u32x4 g = group_of(w, j);
-    const bool in_tail = j == kCodeGroups;
-    uint32_t n;
-    if (in_tail)
-        n = tid < tail && (last & bits) == (wanted & 0xffff);
-    else
-        n = j * C::THREADS + tid < groups ? matches(g) : 0;
-    here = before + wave_scan(n, int(lane)) - n;
-    if (at < here || at >= here + n) return;
+    sum = before + wave_scan(own);
+    those = __ballot(sum > at);
+    if (those == 0 || lane != uint32_t(__builtin_ctzll(those))) return;
+    skip = at - (sum - own);
     uint32_t token = groups * 8 + tid;
     if (!in_tail) {
-        token = (j * C::THREADS + tid) * 8;
-        uint32_t skip = at - here;
+        const u32x4 v = group_of(w, g);
+        token = group(g) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bool is = ((g[e / 2] >> (e % 2 * 16) ^ wanted) & bits & 0xffff) == 0;
+            const bool is = ((v[e / 2] >> (e % 2 * 16) ^ wanted) & bits & 0xffff) == 0;
             if (is && skip == 0) token += e;
             if (is) --skip;
         }
@@ -942,7 +970,7 @@ struct Bins {
         uint32_t c = 0, total;
         for (uint32_t i = from + lane; i < to; i += 64) c += order(T::to_float(z[i])) == k;
         const uint32_t before = block_scan<THREADS>(c, s.room_u, total);
-        const uint32_t first = __shfl(before, 0, 64), here = __shfl(before + c, 63, 64) - first;
+        const uint32_t first = lane_value(before, 0), here = lane_value(before + c, 63) - first;
         if (n >= first && n - first < here) {  // this wave has it
             uint32_t left = n - first;
             for (uint32_t i = from; i < to; i += 64) {
