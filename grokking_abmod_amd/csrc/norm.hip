@@ -19,27 +19,43 @@
 namespace meshgpt::kern {
 namespace {
 
-// Group g of a row, zero behind its end.
+// Group g of a row, zero behind its end.  The row's last group, where it is cut, is moved
+// element by element (in a loop: unrolled it would take the registers of all groups).
 template <class T>
 __device__ __forceinline__ uint4 load_group(const typename T::Raw *row, int g, int width) {
-    constexpr int G = T::kGroup;
+    constexpr int G = T::kGroup, SIZE = sizeof(typename T::Raw);
     const int at = g * G;
-    if (at + G <= width) return get_any(row + at);
-    float x[G];
-#pragma unroll
-    for (int e = 0; e < G; ++e) x[e] = at + e < width ? T::to_float(row[at + e]) : 0.0f;
-    return T::pack(x);
+    if (at + G <= width) return get_any(reinterpret_cast<const char *>(row) + uint32_t(g) * 16u);  // 32 bits beside the row's address
+    uint4 w{0, 0, 0, 0};
+#pragma unroll 1
+    for (int e = 0; at + e < width; ++e) {
+        uint32_t x;
+        if constexpr (SIZE == 4)
+            x = __builtin_bit_cast(uint32_t, row[at + e]);
+        else
+            x = uint32_t(__builtin_bit_cast(uint16_t, row[at + e])) << (e % 2 * 16);
+        const int word = e * SIZE / 4;
+        w.x |= word == 0 ? x : 0;
+        w.y |= word == 1 ? x : 0;
+        w.z |= word == 2 ? x : 0;
+        w.w |= word == 3 ? x : 0;
+    }
+    return w;
 }
 template <class T>
 __device__ __forceinline__ void store_group(typename T::Raw *row, int g, int width, uint4 w) {
-    constexpr int G = T::kGroup;
+    constexpr int G = T::kGroup, SIZE = sizeof(typename T::Raw);
     const int at = g * G;
-    if (at + G <= width) return put_any(row + at, w);
-    float x[G];
-    T::unpack(w, x);
-#pragma unroll
-    for (int e = 0; e < G; ++e)
-        if (at + e < width) row[at + e] = T::from_float(x[e]);
+    if (at + G <= width) return put_any(reinterpret_cast<char *>(row) + uint32_t(g) * 16u, w);
+#pragma unroll 1
+    for (int e = 0; at + e < width; ++e) {
+        const int word = e * SIZE / 4;
+        const uint32_t x = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
+        if constexpr (SIZE == 4)
+            row[at + e] = __builtin_bit_cast(float, x);
+        else
+            row[at + e] = __builtin_bit_cast(typename T::Raw, uint16_t(x >> (e % 2 * 16)));
+    }
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -48,26 +64,29 @@ __device__ __forceinline__ double wave_sum64(double v) {
     return v;
 }
 
-// The sum of a team's values, in all of its lanes.
-template <int WAVES>
-__device__ __forceinline__ double team_sum(double v, double *room) {
-    v = wave_sum64(v);
-    if constexpr (WAVES > 1) {
-        const int wave = threadIdx.x / 64;
-        __syncthreads();  // of the row before
-        if (threadIdx.x % 64 == 0) room[wave] = v;
-        __syncthreads();
-        v = 0.0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += room[w];
+// How a row is held: in a wave's registers, four rows a workgroup (BLOCK false), or in
+// those of a workgroup of whole waves.
+template <bool BLOCK>
+struct Team {
+    int lane, lanes, of;  // this thread in its team, the team's threads, the team in its workgroup
+    __device__ __forceinline__ Team()
+        : lane(BLOCK ? threadIdx.x : threadIdx.x % 64), lanes(BLOCK ? blockDim.x : 64),
+          of(BLOCK ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) {}
+    // The sum of its values, in all of its threads.
+    __device__ __forceinline__ double sum(double v, double *room) const {
+        v = wave_sum64(v);
+        if constexpr (BLOCK) {
+            __syncthreads();  // of the row before
+            if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
+            __syncthreads();
+            v = 0.0;
+            for (int w = 0; w < lanes / 64; ++w) v += room[w];
+        }
+        return v;
     }
-    return v;
-}
-
-template <int WAVES>
-constexpr int kTeams = WAVES == 1 ? 4 : 1;  // of a workgroup
-template <int WAVES>
-constexpr int kThreads = 64 * WAVES * kTeams<WAVES>;
+};
+constexpr int kTeams = 4;  // waves of a workgroup that have a row each
+constexpr int kWavesMost = 8;
 
 typedef uint32_t u32_any __attribute__((aligned(1)));
 
@@ -77,24 +96,25 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
 }
 
-template <class T, int WAVES, int GROUPS, bool CODES>
-__global__ void __launch_bounds__(kThreads<WAVES>) norm_kernel(NormArgs a) {
+template <class T, bool BLOCK, int GROUPS, bool CODES>
+__global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_kernel(NormArgs a) {
     using Raw = typename T::Raw;
-    constexpr int G = T::kGroup, LANES = 64 * WAVES;
-    __shared__ double room[WAVES];
-    const int lane = threadIdx.x % LANES, width = a.width;
-    const size_t row = size_t(blockIdx.x) * kTeams<WAVES> + threadIdx.x / LANES;
-    if (row >= a.rows) return;  // of one wave a row, or all of the workgroup
+    constexpr int G = T::kGroup;
+    __shared__ double room[kWavesMost];
+    const Team<BLOCK> team;
+    const int lane = team.lane, lanes = team.lanes, width = a.width;
+    const size_t row = BLOCK ? blockIdx.x : size_t(blockIdx.x) * kTeams + team.of;
+    if (row >= a.rows) return;  // a whole wave
     const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs;
     const Raw *const weight = static_cast<const Raw *>(a.weight);
     uint4 h[GROUPS];
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) h[i] = load_group<T>(x, lane + i * LANES, width);
+    for (int i = 0; i < GROUPS; ++i) h[i] = load_group<T>(x, lane + i * lanes, width);
     if (a.residual) {
         const Raw *const r = static_cast<const Raw *>(a.residual) + row * a.rs;
         uint4 add[GROUPS];
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) add[i] = load_group<T>(r, lane + i * LANES, width);
+        for (int i = 0; i < GROUPS; ++i) add[i] = load_group<T>(r, lane + i * lanes, width);
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             float u[G], v[G];
@@ -116,16 +136,16 @@ __global__ void __launch_bounds__(kThreads<WAVES>) norm_kernel(NormArgs a) {
     if (a.sum) {
         Raw *const s = static_cast<Raw *>(a.sum) + row * a.ss;
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) store_group<T>(s, lane + i * LANES, width, h[i]);
+        for (int i = 0; i < GROUPS; ++i) store_group<T>(s, lane + i * lanes, width, h[i]);
     }
-    const double rstd = 1.0 / sqrt(team_sum<WAVES>(square, room) / double(width) + double(a.epsilon));
+    const double rstd = 1.0 / sqrt(team.sum(square, room) / double(width) + double(a.epsilon));
     if (a.rstd && lane == 0) a.rstd[row] = float(rstd);
     if constexpr (CODES) {
         constexpr int SHARE = 32 / G;  // lanes of a scale
         uint8_t *const codes = a.codes + row * a.os, *const scales = a.scales + row * a.scs;
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            const int g = lane + i * LANES, at = g * G;
+            const int g = lane + i * lanes, at = g * G;
             float u[G], w[G];
             T::unpack(h[i], u);
             if (weight) {
@@ -168,7 +188,7 @@ __global__ void __launch_bounds__(kThreads<WAVES>) norm_kernel(NormArgs a) {
         Raw *const out = static_cast<Raw *>(a.out) + row * a.os;
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            const int g = lane + i * LANES;
+            const int g = lane + i * lanes;
             float u[G];
             T::unpack(h[i], u);
 #pragma unroll
@@ -184,168 +204,189 @@ __global__ void __launch_bounds__(kThreads<WAVES>) norm_kernel(NormArgs a) {
     }
 }
 
-template <class T, int WAVES, int GROUPS>
-__global__ void __launch_bounds__(kThreads<WAVES>) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
+// A team has every teams-th row, and its lanes the same channels of each: the sums of
+// the weight's gradient stay in registers, and so does the weight (KEEP), and the next
+// row's loads are under way while a row's mean is joined (AHEAD), where there is room.
+// 8192 x 4096 BF16 with a residual: 53 us (5 TB/s); a wave a row, without loads ahead, 114.
+template <class T, bool BLOCK, int GROUPS, bool AHEAD>
+__global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
     using Raw = typename T::Raw;
-    constexpr int G = T::kGroup, LANES = 64 * WAVES;
-    __shared__ double room[WAVES];
-    __shared__ float joined[WAVES == 1 ? LANES * GROUPS * G : 1];
-    const int lane = threadIdx.x % LANES, width = a.width;
-    const int team = threadIdx.x / LANES;
+    constexpr int G = T::kGroup;
+    constexpr bool KEEP = GROUPS * G <= 16;  // more would not fit beside the rest
+    __shared__ double room[kWavesMost];
+    __shared__ float joined[BLOCK ? 1 : 64 * GROUPS * G];
+    const Team<BLOCK> team;
+    const int lane = team.lane, lanes = team.lanes, width = a.width;
     const Raw *const weight = static_cast<const Raw *>(a.weight);
-    float dw[GROUPS][G];
-#pragma unroll
-    for (int i = 0; i < GROUPS; ++i)
-#pragma unroll
-        for (int e = 0; e < G; ++e) dw[i][e] = 0.0f;
-    for (size_t row = size_t(blockIdx.x) * kTeams<WAVES> + team; row < a.rows; row += teams) {
-        const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs, *const dy = static_cast<const Raw *>(a.d_out) + row * a.dos;
-        uint4 h[GROUPS], d[GROUPS];
+    struct Groups {
+        uint4 h[GROUPS], d[GROUPS], s[GROUPS];
+        float rstd;
+    };
+    const auto load = [&](size_t row, Groups &g) {
+        const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs, *const dy = static_cast<const Raw *>(a.d_out) + row * a.dos,
+                        *const ds = static_cast<const Raw *>(a.d_sum) + row * a.dss;
+        g.rstd = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(uint32_t, a.rstd[row])));
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            h[i] = load_group<T>(x, lane + i * LANES, width);
-            d[i] = load_group<T>(dy, lane + i * LANES, width);
+            g.h[i] = load_group<T>(x, lane + i * lanes, width);
+            g.d[i] = load_group<T>(dy, lane + i * lanes, width);
+            if (KEEP && a.d_sum) g.s[i] = load_group<T>(ds, lane + i * lanes, width);
         }
-        const float rstd = a.rstd[row];
-        const float pre = rstd < 0x1p-100f ? 0x1p-64f : 1.0f, by = rstd / pre;
+    };
+    const double share = 1.0 / double(width);
+    uint4 w[GROUPS];
+    float dw[GROUPS][G];
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+        if (KEEP && weight) w[i] = load_group<T>(weight, lane + i * lanes, width);
+#pragma unroll
+        for (int e = 0; e < G; ++e) dw[i][e] = 0.0f;
+    }
+    size_t row = BLOCK ? blockIdx.x : size_t(blockIdx.x) * kTeams + team.of;
+    Groups now, next;
+    if (row < a.rows) load(row, now);
+    for (; row < a.rows; row += teams) {
+        if (AHEAD && row + teams < a.rows) load(row + teams, next);
+        // As in the forward pass, a rstd of rows over 1e30 is moved into FP32's range.
+        const float pre = now.rstd < 0x1p-100f ? 0x1p-64f : 1.0f, by = now.rstd / pre;
         double dot = 0.0;
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            float u[G], v[G], w[G];
-            T::unpack(h[i], u);
-            T::unpack(d[i], v);
-            if (weight) T::unpack(load_group<T>(weight, lane + i * LANES, width), w);
-            float part = 0.0f;
+            float u[G], v[G], k[G], part = 0.0f;
+            T::unpack(now.h[i], u);
+            T::unpack(now.d[i], v);
+            if (weight) T::unpack(KEEP ? w[i] : load_group<T>(weight, lane + i * lanes, width), k);
 #pragma unroll
             for (int e = 0; e < G; ++e) {
                 const float hat = u[e] * pre * by;
                 dw[i][e] = fmaf(v[e], hat, dw[i][e]);
-                part = fmaf(weight ? v[e] * w[e] : v[e], hat, part);
+                part = fmaf(weight ? v[e] * k[e] : v[e], hat, part);
             }
             dot += double(part);
+            if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);
         }
-        const float mean = float(team_sum<WAVES>(dot, room) / double(width));
+        const float mean = float(team.sum(dot, room) * share);
         Raw *const dx = static_cast<Raw *>(a.d_x) + row * a.dxs;
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            const int g = lane + i * LANES;
-            float u[G], v[G], w[G];
-            T::unpack(h[i], u);
-            T::unpack(d[i], v);
-            if (weight) T::unpack(load_group<T>(weight, g, width), w);
+            float u[G], v[G], k[G];
+            T::unpack(now.h[i], u);
+            T::unpack(now.d[i], v);
+            if (weight) T::unpack(KEEP ? w[i] : load_group<T>(weight, lane + i * lanes, width), k);
 #pragma unroll
-            for (int e = 0; e < G; ++e) u[e] = rstd * fmaf(-(u[e] * pre * by), mean, weight ? v[e] * w[e] : v[e]);
+            for (int e = 0; e < G; ++e) u[e] = now.rstd * fmaf(-(u[e] * pre * by), mean, weight ? v[e] * k[e] : v[e]);
             if (a.d_sum) {
-                T::unpack(load_group<T>(static_cast<const Raw *>(a.d_sum) + row * a.dss, g, width), v);
+                T::unpack(KEEP ? now.s[i] : load_group<T>(static_cast<const Raw *>(a.d_sum) + row * a.dss, lane + i * lanes, width), v);
 #pragma unroll
                 for (int e = 0; e < G; ++e) u[e] += v[e];
             }
-            store_group<T>(dx, g, width, T::pack(u));
+            store_group<T>(dx, lane + i * lanes, width, T::pack(u));
+            if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (AHEAD)
+            now = next;
+        else if (row + teams < a.rows)
+            load(row + teams, now);
     }
     if (!a.part) return;
     float *const part = a.part + size_t(blockIdx.x) * width;
-    if constexpr (WAVES == 1) {  // the waves one after the other, in one order
-        for (int t = 0; t < kTeams<WAVES>; ++t) {
-            if (team == t) {
+    if constexpr (!BLOCK) {  // the waves one after the other, in one order
+        for (int t = 0; t < kTeams; ++t) {
+            if (team.of == t) {
 #pragma unroll
                 for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
                     for (int e = 0; e < G; ++e) {
-                        float &at = joined[(i * G + e) * LANES + lane];
+                        float &at = joined[(i * G + e) * 64 + lane];
                         if (t) dw[i][e] += at;
                         at = dw[i][e];
                     }
             }
             __syncthreads();
         }
-        if (team != kTeams<WAVES> - 1) return;
+        if (team.of != kTeams - 1) return;
     }
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
         for (int e = 0; e < G; ++e) {
-            const int at = (lane + i * LANES) * G + e;
+            const int at = (lane + i * lanes) * G + e;
             if (at < width) part[at] = dw[i][e];
         }
 }
 
-// Sums 64 channels over the parts.
-constexpr int kJoin = 1024;
-__global__ void __launch_bounds__(kJoin) norm_join_kernel(const float *part, uint32_t parts, int width, float *out) {
-    __shared__ double room[kJoin / 64][64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, at = int(blockIdx.x) * 64 + lane;
+// Sums 32 channels over the parts, 32 threads each.
+__global__ void __launch_bounds__(1024) norm_join_kernel(const float *part, uint32_t parts, int width, float *out) {
+    __shared__ double room[32][33];
+    const int channel = threadIdx.x % 32, share = threadIdx.x / 32, at = int(blockIdx.x) * 32 + channel;
     double sum = 0.0;
-    if (at < width)
-        for (uint32_t p = wave; p < parts; p += kJoin / 64) sum += double(part[size_t(p) * width + at]);
-    room[wave][lane] = sum;
+    if (at < width) {
+#pragma unroll 8
+        for (uint32_t p = share; p < parts; p += 32) sum += double(part[size_t(p) * width + at]);
+    }
+    room[share][channel] = sum;
     __syncthreads();
-    if (wave || at >= width) return;
-    for (int w = 1; w < kJoin / 64; ++w) sum += room[w][lane];
+    if (share) return;
+    if (at >= width) return;
+#pragma unroll 8
+    for (int w = 1; w < 32; ++w) sum += room[w][channel];
     out[at] = float(sum);
 }
 
-// Waves and 16-byte groups of a lane that a row takes.
+// A row's 16-byte groups a lane, and its waves (0: a wave of a workgroup of kTeams).
 struct Cut {
-    int waves, groups;
+    int groups, waves;
 };
 Cut cut_of(size_t width, int group) {
-    const size_t groups = (width + group - 1) / group;
-    for (int waves : {1, 4, 16})
-        for (int n : {1, 2, 4, 8})
-            if (groups <= size_t(64 * waves * n)) return {waves, n};
-    return {0, 0};
+    const size_t n = (width + group - 1) / group;
+    if (n <= 64) return {1, 0};
+    if (n <= 128) return {2, 0};
+    for (int groups : {2, 4})
+        if (n <= size_t(64 * kWavesMost * groups)) return {groups, int((n + 64 * groups - 1) / (64 * groups))};
+    return {8, int((n + 64 * 8 - 1) / (64 * 8))};
 }
 
-template <class T, int WAVES, int GROUPS>
-void launch_norm(const NormArgs &a, hipStream_t stream) {
-    const dim3 grid(unsigned((a.rows + kTeams<WAVES> - 1) / kTeams<WAVES>));
-    if (a.codes)
-        norm_kernel<T, WAVES, GROUPS, true><<<grid, kThreads<WAVES>, 0, stream>>>(a);
-    else
-        norm_kernel<T, WAVES, GROUPS, false><<<grid, kThreads<WAVES>, 0, stream>>>(a);
-}
-
-uint32_t parts_of(size_t rows, int waves) {
-    const size_t teams = waves == 1 ? 4 : 1;
-    return uint32_t(std::min<size_t>((rows + teams - 1) / teams, 512));
-}
-
-template <class T, int WAVES, int GROUPS>
-void launch_backward(const NormBackwardArgs &a, hipStream_t stream) {
-    const uint32_t parts = parts_of(a.rows, WAVES);
-    if (parts)
-        norm_backward_kernel<T, WAVES, GROUPS><<<dim3(parts), kThreads<WAVES>, 0, stream>>>(a, parts * kTeams<WAVES>);
-    if (a.d_weight)
-        norm_join_kernel<<<dim3(unsigned((a.width + 63) / 64)), kJoin, 0, stream>>>(a.part, parts, a.width, a.d_weight);
-}
-
-// f(WAVES, GROUPS) for a row's width.
+// f(BLOCK, GROUPS) for a row's width.
 template <class T, class F>
-void for_cut(size_t width, F &&f) {
-    const Cut c = cut_of(width, T::kGroup);
-    const auto groups = [&](auto waves) {
-        switch (c.groups) {
-            case 1: return f(waves, std::integral_constant<int, 1>());
-            case 2: return f(waves, std::integral_constant<int, 2>());
-            case 4: return f(waves, std::integral_constant<int, 4>());
-            default: return f(waves, std::integral_constant<int, 8>());
-        }
-    };
-    switch (c.waves) {
-        case 1: return groups(std::integral_constant<int, 1>());
-        case 4: return groups(std::integral_constant<int, 4>());
-        default: return groups(std::integral_constant<int, 16>());
-    }
+void for_cut(const Cut &c, F &&f) {
+    using std::integral_constant;
+    if (c.waves == 0)
+        return c.groups == 1 ? f(std::false_type(), integral_constant<int, 1>()) : f(std::false_type(), integral_constant<int, 2>());
+    if (c.groups == 2) return f(std::true_type(), integral_constant<int, 2>());
+    if (c.groups == 4) return f(std::true_type(), integral_constant<int, 4>());
+    if constexpr (T::kGroup == 4) f(std::true_type(), integral_constant<int, 8>());  // 16-bit rows end before
 }
 
 template <class T>
 void norm_of(const NormArgs &a, hipStream_t stream) {
-    for_cut<T>(size_t(a.width), [&](auto w, auto g) { launch_norm<T, w.value, g.value>(a, stream); });
+    const Cut c = cut_of(size_t(a.width), T::kGroup);
+    const int threads = c.waves ? 64 * c.waves : 64 * kTeams;
+    const dim3 grid(unsigned(c.waves ? a.rows : (a.rows + kTeams - 1) / kTeams));
+    for_cut<T>(c, [&](auto block, auto groups) {
+        if (a.codes)
+            norm_kernel<T, block.value, groups.value, true><<<grid, threads, 0, stream>>>(a);
+        else
+            norm_kernel<T, block.value, groups.value, false><<<grid, threads, 0, stream>>>(a);
+    });
 }
+
+uint32_t parts_of(size_t rows, int waves) {
+    const size_t teams = waves ? 1 : kTeams;
+    return uint32_t(std::min<size_t>((rows + teams - 1) / teams, 512));
+}
+
 template <class T>
 void backward_of(const NormBackwardArgs &a, hipStream_t stream) {
-    for_cut<T>(size_t(a.width), [&](auto w, auto g) { launch_backward<T, w.value, g.value>(a, stream); });
+    const Cut c = cut_of(size_t(a.width), T::kGroup);
+    const uint32_t parts = parts_of(a.rows, c.waves);
+    const int threads = c.waves ? 64 * c.waves : 64 * kTeams;
+    if (parts)
+        for_cut<T>(c, [&](auto block, auto groups) {
+            norm_backward_kernel<T, block.value, groups.value, (groups.value * T::kGroup <= 16)>
+                <<<dim3(parts), threads, 0, stream>>>(a, parts * (c.waves ? 1 : kTeams));
+        });
+    if (a.d_weight)
+        norm_join_kernel<<<dim3(unsigned((a.width + 31) / 32)), 1024, 0, stream>>>(a.part, parts, a.width, a.d_weight);
 }
 
 }  // namespace

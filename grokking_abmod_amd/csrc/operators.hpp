@@ -174,7 +174,7 @@ struct NormBackwardArgs {
 // Partial sums of the weight's gradient that a call makes.
 size_t norm_parts(size_t rows, size_t width);
 void rms_norm_backward(const NormBackwardArgs &a, Type type, hipStream_t stream);
-constexpr size_t kNormWidth = 32768;  // at most
+constexpr size_t kNormWidth = 16384;  // at most
 
 constexpr int kTopMax = 32;
 constexpr int kSmallVocab = 1024;  // rows of so many logits take a wave, longer ones workgroups

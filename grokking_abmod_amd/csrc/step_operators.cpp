@@ -107,7 +107,7 @@ void rope(int device, const Rope &r, Type type, size_t batch, size_t count, size
 
 namespace {
 void check_norm(size_t rows, size_t width) {
-    require(width >= 1 && width <= kern::kNormWidth, "width must be in 1..32768");
+    require(width >= 1 && width <= kern::kNormWidth, "width must be in 1..16384");
     require(rows < size_t(1) << 22, "rows must stay below 2^22");  // of up to 1024 threads each, counted in 32 bits
 }
 

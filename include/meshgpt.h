@@ -416,7 +416,7 @@ int mg_rope_backward(int device, const mg_rope *r, int type, size_t batch, size_
                      const int64_t d_k_strides[3], const int32_t *lengths, const int32_t *counts,
                      const int32_t *positions, void *stream);
 
-/* The root-mean-square norm of rows of `width` (1..32768; fewer than 2^22 rows,
+/* The root-mean-square norm of rows of `width` (1..16384; fewer than 2^22 rows,
  * strides in elements): h = x + residual (NULL: x), rounded to `type` and written to
  * sum (NULL: not); rstd = 1 / sqrt(mean(h^2) + epsilon); out = h * rstd * weight (of
  * `type`; NULL: 1).  sum and out may be x or the residual, with their strides, but not

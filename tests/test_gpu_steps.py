@@ -360,7 +360,7 @@ def norm_tolerance(y, kind):
 
 
 NORMS = [(3, 1), (5, 2), (2, 7), (4, 8), (3, 31), (9, 32), (2, 33), (5, 100), (33, 256), (32, 512), (3, 1000), (2, 2048), (3, 2049),
-         (2, 4096), (3, 4097), (1, 5120), (2, 8192), (2, 8200), (1, 16384), (2, 16385), (1, 32768), (1030, 40), (700, 3001)]
+         (2, 4096), (3, 4097), (1, 5120), (2, 8192), (2, 8200), (2, 16383), (1, 16384), (1030, 40), (700, 3001)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -391,7 +391,7 @@ def test_norms_are_those_of_the_formulas(kind, rows, width):
 @pytest.mark.parametrize("kind", KINDS)
 def test_norms_over_their_inputs(kind):
     rng = np.random.default_rng(12)
-    for rows, width in ((5, 100), (3, 5001), (2, 20000)):
+    for rows, width in ((5, 100), (3, 5001), (2, 16000)):
         x, r, w = norm_inputs(rng, rows, width, kind)
         kept, h, rstd, y = S.norm(x, r, w, 1e-6, kind)
         with L.Device() as dev:
@@ -442,7 +442,7 @@ def test_nan_and_infinities_stay_in_their_rows(codes):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("rows,width", [(3, 1), (4, 31), (5, 32), (3, 33), (2, 100), (7, 512), (2, 2049), (3, 4104), (2, 9000), (1, 17000)])
+@pytest.mark.parametrize("rows,width", [(3, 1), (4, 31), (5, 32), (3, 33), (2, 100), (7, 512), (2, 2049), (3, 4104), (2, 9000), (1, 16200)])
 def test_8_bit_norms_are_the_nearest_codes(kind, rows, width):
     rng = np.random.default_rng(rows + width)
     x, r, w = norm_inputs(rng, rows, width, kind)

@@ -113,8 +113,8 @@ def norm_call(f=G.rms_norm, **kw):
 def test_norm_refusals(f):
     call = lambda **kw: norm_call(f, **kw)  # noqa: E731
     refused("element type", call, type=3)
-    refused("width must be in 1..32768", call, width=0)
-    refused("width must be in 1..32768", call, width=32769)
+    refused("width must be in 1..16384", call, width=0)
+    refused("width must be in 1..16384", call, width=16385)
     refused("rows must stay below", call, rows=1 << 22)
     for name in ("x_stride", "residual_stride", "sum_stride"):
         refused("row strides", call, **{name: 63})
@@ -147,7 +147,7 @@ def test_norm_gradient_refusals():
     call = lambda **kw: G.rms_norm_backward(**{**base, **kw})  # noqa: E731
     refused("element type", call, type=-1)
     refused("width must be", call, width=0)
-    refused("width must be", G.rms_norm_backward_workspace, rows=1, width=32769)
+    refused("width must be", G.rms_norm_backward_workspace, rows=1, width=16385)
     refused("rows must stay below", call, rows=1 << 22)
     refused("rows must stay below", call, rows=1 << 40, d_weight=None)
     for name in ("sum_stride", "d_out_stride", "d_sum_stride", "d_x_stride"):
