@@ -19,43 +19,18 @@
 namespace meshgpt::kern {
 namespace {
 
-// Group g of a row, zero behind its end.  The row's last group, where it is cut, is moved
-// element by element (in a loop: unrolled it would take the registers of all groups).
+// Group g of a row, zero behind its end.
 template <class T>
 __device__ __forceinline__ uint4 load_group(const typename T::Raw *row, int g, int width) {
-    constexpr int G = T::kGroup, SIZE = sizeof(typename T::Raw);
-    const int at = g * G;
-    if (at + G <= width) return get_any(reinterpret_cast<const char *>(row) + uint32_t(g) * 16u);  // 32 bits beside the row's address
-    uint4 w{0, 0, 0, 0};
-#pragma unroll 1
-    for (int e = 0; at + e < width; ++e) {
-        uint32_t x;
-        if constexpr (SIZE == 4)
-            x = __builtin_bit_cast(uint32_t, row[at + e]);
-        else
-            x = uint32_t(__builtin_bit_cast(uint16_t, row[at + e])) << (e % 2 * 16);
-        const int word = e * SIZE / 4;
-        w.x |= word == 0 ? x : 0;
-        w.y |= word == 1 ? x : 0;
-        w.z |= word == 2 ? x : 0;
-        w.w |= word == 3 ? x : 0;
-    }
-    return w;
+    const int have = width - g * T::kGroup;
+    if (have >= T::kGroup) return get_any(reinterpret_cast<const char *>(row) + uint32_t(g) * 16u);  // 32 bits beside the row's address
+    return get_part<T>(row + g * T::kGroup, have);
 }
 template <class T>
 __device__ __forceinline__ void store_group(typename T::Raw *row, int g, int width, uint4 w) {
-    constexpr int G = T::kGroup, SIZE = sizeof(typename T::Raw);
-    const int at = g * G;
-    if (at + G <= width) return put_any(reinterpret_cast<char *>(row) + uint32_t(g) * 16u, w);
-#pragma unroll 1
-    for (int e = 0; at + e < width; ++e) {
-        const int word = e * SIZE / 4;
-        const uint32_t x = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
-        if constexpr (SIZE == 4)
-            row[at + e] = __builtin_bit_cast(float, x);
-        else
-            row[at + e] = __builtin_bit_cast(typename T::Raw, uint16_t(x >> (e % 2 * 16)));
-    }
+    const int have = width - g * T::kGroup;
+    if (have >= T::kGroup) return put_any(reinterpret_cast<char *>(row) + uint32_t(g) * 16u, w);
+    put_part<T>(row + g * T::kGroup, have, w);
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {

@@ -8,7 +8,10 @@
 // Angles are taken in FP64 as turns and reduced to an eighth of one, because at
 // position 10^6 an FP32 product is off by a thirtieth of a radian; sine and
 // cosine of what is left are FP32 series.  A workgroup makes them once for its
-// tokens, in LDS, and applies them to all heads, 16 bytes of each half a thread.
+// tokens, in LDS, and applies them to all heads, 16 bytes of each half a thread, with the
+// next head's loads under way.
+#include <algorithm>
+
 #include "operators.hpp"
 #include "types.hpp"
 
@@ -32,108 +35,126 @@ __device__ __forceinline__ float2 turned(double t) {
     return {q == 1 || q == 2 ? -a : a, q >= 2 ? -b : b};
 }
 
-template <class T, int N>
-__device__ __forceinline__ void load(const typename T::Raw *p, int have, float (&x)[N]) {
-    if (have >= N) return T::unpack(get_any(p), x);
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = i < have ? T::to_float(p[i]) : 0.0f;
+template <class T>
+__device__ __forceinline__ uint4 load(const typename T::Raw *p, int have) {
+    return have >= T::kGroup ? get_any(p) : get_part<T>(p, have);
 }
-template <class T, int N>
-__device__ __forceinline__ void store(typename T::Raw *p, int have, const float (&x)[N]) {
-    if (have >= N) return put_any(p, T::pack(x));
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i < have) p[i] = T::from_float(x[i]);
+template <class T, bool STREAM>
+__device__ __forceinline__ void store(typename T::Raw *p, int have, uint4 w) {
+    if (have >= T::kGroup) return put_any<STREAM>(p, w);
+    put_part<T>(p, have, w);
 }
 
-template <class T>
+// A head's work is cut into items of 16 bytes: of neighbours that are pairs, all of the
+// head; else of its first half of turning channels, with those of the second, and then of
+// what stays.
+template <class T, bool INTERLEAVED, bool STREAM>
 __global__ void __launch_bounds__(kBlock) rope_kernel(RopeArgs a, int tile, int items, int slots) {
     using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
     __shared__ float2 table[kPairs];
-    __shared__ int64_t places[kTokens];  // sequence << 32 | token, -1: not there
-    __shared__ int positions[kTokens];
+    __shared__ int tokens[kTokens];  // in its sequence, -1: not there
+    __shared__ int sequences[kTokens], positions[kTokens];
     const int tid = threadIdx.x, half = a.rotary / 2;
-    const int64_t first = int64_t(blockIdx.x) * tile, all = int64_t(a.batch) * a.count;
+    const uint32_t first = blockIdx.x * uint32_t(tile), all = uint32_t(a.batch) * uint32_t(a.count);
     if (tid < tile) {
-        const int64_t t = first + tid;
-        places[tid] = -1;
-        if (t < all) {
-            const int64_t s = t / a.count;
-            const int i = int(t - s * a.count), n = a.counts ? a.counts[s] : a.count;
-            const int length = a.lengths ? a.lengths[s] : n;
-            if (n >= 0 && n <= a.count && length >= n && i < n) {
-                places[tid] = s << 32 | i;
-                positions[tid] = a.positions ? a.positions[t] : length - n + i;
-            }
-        }
+        const uint32_t t = first + tid, s = min(t, all - 1) / uint32_t(a.count);
+        const int i = int(t - s * uint32_t(a.count)), n = a.counts ? a.counts[s] : a.count;
+        const int length = a.lengths ? a.lengths[s] : n;
+        const bool there = t < all && n >= 0 && n <= a.count && length >= n && i < n;
+        tokens[tid] = there ? i : -1;
+        sequences[tid] = int(s);
+        positions[tid] = there && a.positions ? a.positions[t] : length - n + i;
     }
     __syncthreads();
+
+    // A thread has one item of a head, in every slots-th head of the tokens.
+    const int slot = tid / items, item = tid - slot * items;
+    const int heads = a.side[0].heads + a.side[1].heads;
+    const int turning = INTERLEAVED ? items : (half + G - 1) / G;
+    const bool turns = item < turning;
+    const int at = turns ? item * G : a.rotary + (item - turning) * G;
+    const int have = (INTERLEAVED || !turns ? a.width : half) - at;
+    int t = 0, h = slot;
+    struct Place {
+        const Raw *x;
+        Raw *o;
+        int t;  // of the tile, or -1: nothing
+    };
+    const auto next = [&] {
+        Place p{nullptr, nullptr, -1};
+        for (;; h += slots) {
+            while (h >= heads) {
+                h -= heads;
+                ++t;
+            }
+            if (slot >= slots || t >= tile) return p;
+            if (tokens[t] < 0) continue;
+            const bool second = h >= a.side[0].heads;
+            const RopeSide &side = a.side[second];
+            const int64_t s = sequences[t], i = tokens[t], head = second ? h - a.side[0].heads : h;
+            p.x = static_cast<const Raw *>(side.x) + s * side.xs.s[0] + i * side.xs.s[1] + head * side.xs.s[2] + at;
+            p.o = static_cast<Raw *>(side.out) + s * side.os.s[0] + i * side.os.s[1] + head * side.os.s[2] + at;
+            p.t = t;
+            h += slots;
+            return p;
+        }
+    };
+    const auto fetch = [&](const Place &p, uint4 &x, uint4 &y) {
+        if (p.t < 0) return;
+        x = load<T>(p.x, have);
+        if (!INTERLEAVED && turns) y = load<T>(p.x + half, have);
+    };
+    Place now = next();
+    uint4 x{}, y{};
+    fetch(now, x, y);  // under way while the angles are made
     for (int i = tid; i < tile * half; i += kBlock) {
-        const int t = i / half;
-        if (places[t] < 0) continue;
-        float2 cs = turned(double(positions[t]) * (a.frequencies[i - t * half] * 0.15915494309189535));
+        const int of = i / half;
+        if (tokens[of] < 0) continue;
+        float2 cs = turned(double(positions[of]) * (a.frequencies[i - of * half] * 0.15915494309189535));
         if (a.backward) cs.y = -cs.y;
         table[i] = {cs.x * a.magnitude, cs.y * a.magnitude};
     }
     __syncthreads();
-
-    // A thread has one group of a head, in every slots-th head of the tokens.
-    const int slot = tid / items, item = tid - slot * items;
-    if (slot >= slots) return;
-    const int heads = a.side[0].heads + a.side[1].heads;
-    const int groups = a.interleaved ? (a.rotary + G - 1) / G : (half + G - 1) / G;  // that turn
-    int t = 0, h = slot;
-    for (;;) {
-        while (h >= heads) {
-            h -= heads;
-            ++t;
-        }
-        if (t >= tile) return;
-        const int64_t place = places[t];
-        if (place >= 0) {
-            const bool second = h >= a.side[0].heads;
-            const RopeSide &side = a.side[second];
-            const int64_t s = place >> 32, i = place & 0xffffffff, head = second ? h - a.side[0].heads : h;
-            const Raw *const x = static_cast<const Raw *>(side.x) + s * side.xs.s[0] + i * side.xs.s[1] + head * side.xs.s[2];
-            Raw *const o = static_cast<Raw *>(side.out) + s * side.os.s[0] + i * side.os.s[1] + head * side.os.s[2];
-            const float2 *const row = table + t * half;
-            if (item >= groups) {  // stays as it is
-                const int at = a.rotary + (item - groups) * G, have = a.width - at;
-                if (have >= G) {
-                    put_any(o + at, get_any(x + at));
-                } else {
-                    for (int e = 0; e < have; ++e) o[at + e] = x[at + e];
-                }
-            } else if (a.interleaved) {
-                const int at = item * G, have = a.rotary - at;
-                float v[G];
-                load<T>(x + at, have, v);
+    while (now.t >= 0) {
+        const Place then = next();
+        uint4 x2{}, y2{};
+        fetch(then, x2, y2);
+        const float2 *const row = table + now.t * half;
+        float p[G], q[G];
+        T::unpack(x, p);
+        if constexpr (INTERLEAVED) {
 #pragma unroll
-                for (int e = 0; e < G; e += 2) {
-                    const float2 cs = row[min(at + e, a.rotary - 2) / 2];
-                    const float p = v[e], q = v[e + 1];
-                    v[e] = p * cs.x - q * cs.y;
-                    v[e + 1] = q * cs.x + p * cs.y;
-                }
-                store<T>(o + at, have, v);
-            } else {
-                const int at = item * G, have = half - at;
-                float p[G], q[G];
-                load<T>(x + at, have, p);
-                load<T>(x + at + half, have, q);
-#pragma unroll
-                for (int e = 0; e < G; ++e) {
-                    const float2 cs = row[min(at + e, half - 1)];
-                    const float v = p[e], w = q[e];
-                    p[e] = v * cs.x - w * cs.y;
-                    q[e] = w * cs.x + v * cs.y;
-                }
-                store<T>(o + at, have, p);
-                store<T>(o + at + half, have, q);
+            for (int e = 0; e < G; e += 2) {
+                const float2 cs = row[max(0, min(at + e, a.rotary - 2)) / 2];
+                const float v = p[e], w = p[e + 1];
+                p[e] = v * cs.x - w * cs.y;
+                p[e + 1] = w * cs.x + v * cs.y;
             }
+            uint4 turned = T::pack(p);
+            if (at + G > a.rotary) {  // some channels stay: whole words, for pairs turn
+                const int words = (a.rotary - at) * int(sizeof(Raw)) / 4;
+                turned = {words > 0 ? turned.x : x.x, words > 1 ? turned.y : x.y, words > 2 ? turned.z : x.z,
+                          words > 3 ? turned.w : x.w};
+            }
+            store<T, STREAM>(now.o, have, turned);
+        } else if (turns) {
+            T::unpack(y, q);
+#pragma unroll
+            for (int e = 0; e < G; ++e) {
+                const float2 cs = row[min(at + e, half - 1)];
+                const float v = p[e], w = q[e];
+                p[e] = v * cs.x - w * cs.y;
+                q[e] = w * cs.x + v * cs.y;
+            }
+            store<T, STREAM>(now.o, have, T::pack(p));
+            store<T, STREAM>(now.o + half, have, T::pack(q));
+        } else {
+            store<T, STREAM>(now.o, have, x);
         }
-        h += slots;
+        now = then;
+        x = x2;
+        y = y2;
     }
 }
 
@@ -145,13 +166,27 @@ void launch(const RopeArgs &a, hipStream_t stream) {
     for (const RopeSide &s : a.side)
         if (s.heads)
             same = same && s.x == s.out && s.xs.s[0] == s.os.s[0] && s.xs.s[1] == s.os.s[1] && s.xs.s[2] == s.os.s[2];
-    const int turning = a.interleaved ? (a.rotary + G - 1) / G : (half + G - 1) / G;
-    const int items = turning + (same ? 0 : (a.width - a.rotary + G - 1) / G);
+    const int turning = ((a.interleaved ? a.rotary : half) + G - 1) / G;
+    const int items = same            ? turning
+                      : a.interleaved ? (a.width + G - 1) / G
+                                      : turning + (a.width - a.rotary + G - 1) / G;
     if (items == 0) return;
-    const int64_t tokens = int64_t(a.batch) * a.count;
-    const int most = half ? kPairs / half : kTokens;
-    const int tile = int(std::max<int64_t>(1, std::min<int64_t>({tokens / 2048, kTokens, most})));
-    rope_kernel<T><<<dim3(unsigned((tokens + tile - 1) / tile)), kBlock, 0, stream>>>(a, tile, items, kBlock / items);
+    // Two or three heads a thread, where there are tokens enough for that: 32768 tokens of 40
+    // heads of 128 BF16 took 128 us with 2 tokens a workgroup (2.5 heads), 142 with 1, 139
+    // with 8 and 152 with 16; past the caches 121, with loads ahead 116 (5.8 TB/s).
+    const int64_t tokens = int64_t(a.batch) * a.count, heads = a.side[0].heads + a.side[1].heads;
+    const int slots = kBlock / items, most = half ? std::min(kTokens, kPairs / half) : kTokens;
+    const int tile = int(std::max<int64_t>(1, std::min<int64_t>({tokens / 1024, 5 * slots / (2 * heads), most})));
+    const dim3 grid(unsigned((tokens + tile - 1) / tile));
+    const bool past = double(tokens) * double(heads) * a.width * sizeof(typename T::Raw) > kCached;
+    if (a.interleaved && past)
+        rope_kernel<T, true, true><<<grid, kBlock, 0, stream>>>(a, tile, items, slots);
+    else if (a.interleaved)
+        rope_kernel<T, true, false><<<grid, kBlock, 0, stream>>>(a, tile, items, slots);
+    else if (past)
+        rope_kernel<T, false, true><<<grid, kBlock, 0, stream>>>(a, tile, items, slots);
+    else
+        rope_kernel<T, false, false><<<grid, kBlock, 0, stream>>>(a, tile, items, slots);
 }
 
 }  // namespace

@@ -220,98 +220,6 @@ __device__ __forceinline__ uint32_t equal_draw(double t, double w, uint32_t n) {
     return steps >= double(n - 1) ? n - 1 : steps > 0.0 ? uint32_t(steps) : 0;
 }
 
-// ---- short rows -------------------------------------------------------------------
-
-// A thread has a token and counts those before it, four to an LDS read; then it
-// has a place in the ranking, with the running sum of the weights up to there.
-template <class T>
-__global__ void __launch_bounds__(kShort) sample_short_kernel(SampleArgs a) {
-    using Raw = typename T::Raw;
-    constexpr int WAVES = kShort / 64;
-    __shared__ uint4 keys[kShort / 4];
-    __shared__ double weights[kShort], sums[kShort], room_d[WAVES];
-    __shared__ uint32_t tokens[kShort], room_u[WAVES], bads[WAVES];
-    __shared__ float tops[WAVES];
-    const size_t row = blockIdx.x;
-    const uint32_t tid = threadIdx.x, vocab = uint32_t(a.vocab), wave = tid / 64, lane = tid % 64;
-    const Settings set = settings_of(a, row);
-    const float x = tid < vocab ? T::to_float(static_cast<const Raw *>(a.logits)[row * a.stride + tid]) : -INFINITY;
-    const uint32_t key = order(x);
-    reinterpret_cast<uint32_t *>(keys)[tid] = key;
-    const float wave_top = wave_largest(x);
-    const bool wave_bad = __ballot(!(x < INFINITY)) != 0;
-    if (lane == 0) {
-        tops[wave] = wave_top;
-        bads[wave] = wave_bad;
-    }
-    weights[tid] = 0.0;
-    __syncthreads();
-    float top = -INFINITY;
-    uint32_t bad = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        top = fmaxf(top, tops[w]);
-        bad |= bads[w];
-    }
-    if (bad || top == -INFINITY || !set.valid) {
-        if (tid == 0) write(a, row, kNoToken, NAN);
-        return;
-    }
-    // Of equal keys those of lower tokens are before: all in the waves before, the lanes before in this one.
-    uint32_t before = 0;
-    const uint32_t mine = __builtin_amdgcn_readfirstlane(wave * 16), end = (vocab + 3) / 4;
-    for (uint32_t j = 0; j < min(mine, end); ++j) {
-        const uint4 k = keys[j];
-        before += (k.x >= key) + (k.y >= key) + (k.z >= key) + (k.w >= key);
-    }
-    for (uint32_t j = mine + 16; j < end; ++j) {
-        const uint4 k = keys[j];
-        before += (k.x > key) + (k.y > key) + (k.z > key) + (k.w > key);
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < 16; ++j) {
-        const uint4 k = keys[mine + j];
-        before += (k.x > key || (k.x == key && 4 * j < lane)) + (k.y > key || (k.y == key && 4 * j + 1 < lane)) +
-                  (k.z > key || (k.z == key && 4 * j + 2 < lane)) + (k.w > key || (k.w == key && 4 * j + 3 < lane));
-    }
-    if (set.greedy) {
-        if (before == 0) write(a, row, tid, 0.0f);
-        return;
-    }
-    const double weight = exp((double(x) - double(top)) / set.temperature);
-    if (tid < vocab) {
-        weights[before] = weight;
-        tokens[before] = tid;
-    }
-    __syncthreads();
-    // From here on a thread has a place in the ranking.
-    const double w = weights[tid];
-    double whole;
-    const double sum = block_scan<kShort>(w, room_d, whole) + w;
-    sums[tid] = sum;
-    __syncthreads();
-    const auto count = [&](bool is) {
-        const uint32_t c = uint32_t(__popcll(__ballot(is)));
-        if (lane == 0) room_u[wave] = c;
-        __syncthreads();
-        uint32_t all = 0;
-#pragma unroll
-        for (int v = 0; v < WAVES; ++v) all += room_u[v];
-        __syncthreads();
-        return all;
-    };
-    uint32_t left = count(w > 0.0);
-    if (set.top_k) left = min(left, set.top_k);
-    if (set.with_p) {
-        const double t = set.top_p * sums[left - 1];
-        left = min(left, count(tid < left && sum < t) + 1);
-    }
-    if (set.with_min) left = max(1u, count(tid < left && w >= set.min_p));
-    whole = sums[left - 1];
-    const uint32_t at = min(left - 1, count(tid < left && sum <= set.uniform * whole));
-    if (tid == at) write(a, row, tokens[tid], float(log(w / whole)));
-}
-
 // ---- weights by bins of 1/64 of a power of e -------------------------------------------
 
 struct Powers {
@@ -351,6 +259,93 @@ struct Weights {
         return fma(begin, rest(y - at), begin);
     }
 };
+
+// ---- short rows -------------------------------------------------------------------
+
+// Four threads count the tokens before a token, a quarter of the row each, four to an
+// LDS read; then a thread has a place in the ranking, with the running sum of the weights
+// up to there.
+constexpr int kShortThreads = 4 * kShort;
+
+template <class T>
+__global__ void __launch_bounds__(kShortThreads) sample_short_kernel(SampleArgs a) {
+    using Raw = typename T::Raw;
+    constexpr int WAVES = kShort / 64;
+    __shared__ uint4 keys[kShort / 4];
+    __shared__ double weights[kShort], sums[kShort], room_d[kShortThreads / 64];
+    __shared__ uint32_t tokens[kShort], room_u[kShortThreads / 64], bads[WAVES];
+    __shared__ float tops[WAVES];
+    __shared__ Powers powers;
+    const size_t row = blockIdx.x;
+    const uint32_t tid = threadIdx.x, vocab = uint32_t(a.vocab);
+    const Raw *const z = static_cast<const Raw *>(a.logits) + row * a.stride;
+    const Settings set = settings_of(a, row);
+    const uint32_t token = tid / 4, quarter = tid % 4;
+    const float x = token < vocab ? T::to_float(z[token]) : -INFINITY;
+    if (tid < kShort) {
+        const float y = tid < vocab ? T::to_float(z[tid]) : -INFINITY;
+        reinterpret_cast<uint32_t *>(keys)[tid] = order(y);
+        weights[tid] = 0.0;
+        const float wave_top = wave_largest(y);
+        const bool wave_bad = __ballot(!(y < INFINITY)) != 0;
+        if (tid % 64 == 0) {
+            tops[tid / 64] = wave_top;
+            bads[tid / 64] = wave_bad;
+        }
+    }
+    Weights::prepare(powers);
+    const double scale = set.greedy ? 1.0 : uniform(kPerUnit / set.temperature);
+    __syncthreads();
+    float top = -INFINITY;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        top = fmaxf(top, tops[w]);
+        bad |= bads[w];
+    }
+    if (bad || top == -INFINITY || !set.valid) {
+        if (tid == 0) write(a, row, kNoToken, NAN);
+        return;
+    }
+    // Of equal keys those of lower tokens are before.  Each quarter begins at other banks.
+    const uint32_t key = order(x);
+    uint32_t before = 0;
+#pragma unroll 4
+    for (uint32_t j = 0; j < kShort / 16; ++j) {
+        const uint32_t at = quarter * (kShort / 16) + (j + 4 * quarter) % (kShort / 16);
+        const uint4 k = keys[at];
+        const int lower = int(token) - int(4 * at);  // so many of the four are lower tokens
+        before += (k.x > key - (lower > 0)) + (k.y > key - (lower > 1)) + (k.z > key - (lower > 2)) + (k.w > key - (lower > 3));
+    }
+    before += moved<0xB1>(before);  // quad_perm [1,0,3,2]
+    before += moved<0x4E>(before);  // quad_perm [2,3,0,1]
+    if (set.greedy) {
+        if (before == 0 && quarter == 0) write(a, row, token, 0.0f);
+        return;
+    }
+    if (quarter == 0 && token < vocab) {
+        weights[before] = Weights{powers, double(top), scale}.of(x);
+        tokens[before] = token;
+    }
+    __syncthreads();
+    // From here on a thread has a place in the ranking.
+    const double w = tid < kShort ? weights[tid] : 0.0;
+    double whole;
+    const double sum = block_scan<kShortThreads>(w, room_d, whole) + w;
+    if (tid < kShort) sums[tid] = sum;
+    __syncthreads();
+    const auto count = [&](bool is) { return block_total<kShortThreads>(uint32_t(is), room_u); };
+    uint32_t left = count(w > 0.0);
+    if (set.top_k) left = min(left, set.top_k);
+    if (set.with_p) {
+        const double t = set.top_p * sums[left - 1];
+        left = min(left, count(tid < left && sum < t) + 1);
+    }
+    if (set.with_min) left = max(1u, count(tid < left && w >= set.min_p));
+    whole = sums[left - 1];
+    const uint32_t at = min(left - 1, count(tid < left && sum <= set.uniform * whole));
+    if (tid == at) write(a, row, tokens[tid], float(log(w / whole)));
+}
 
 // ---- rows of 16 bits ------------------------------------------------------------------
 
@@ -1217,7 +1212,7 @@ template <class T>
 void launch(const SampleArgs &a, hipStream_t stream) {
     const dim3 rows(static_cast<unsigned>(a.rows));
     if (a.vocab <= size_t(kShort))
-        sample_short_kernel<T><<<rows, kShort, 0, stream>>>(a);
+        sample_short_kernel<T><<<rows, kShortThreads, 0, stream>>>(a);
     else if (a.vocab <= 8192)
         sample_bins_kernel<T, 256, 2048, 1024><<<rows, 256, 0, stream>>>(a);
     else if (sizeof(typename T::Raw) == 4 || a.vocab > size_t(kCodeMost))

@@ -80,6 +80,41 @@ __device__ __forceinline__ void put_any(void *p, uint4 w) {
     *static_cast<u32x4_any *>(p) = __builtin_bit_cast(u32x4, w);
 }
 
+// The first `have` of a group's elements, the rest zero; and back.  (Loops: unrolled, the
+// rare end of a row would take the registers of everything around it.)
+template <class T>
+__device__ __forceinline__ uint4 get_part(const typename T::Raw *p, int have) {
+    constexpr int SIZE = sizeof(typename T::Raw);
+    uint4 w{0, 0, 0, 0};
+#pragma unroll 1
+    for (int e = 0; e < have; ++e) {
+        uint32_t x;
+        if constexpr (SIZE == 4)
+            x = __builtin_bit_cast(uint32_t, p[e]);
+        else
+            x = uint32_t(__builtin_bit_cast(uint16_t, p[e])) << (e % 2 * 16);
+        const int word = e * SIZE / 4;
+        w.x |= word == 0 ? x : 0;
+        w.y |= word == 1 ? x : 0;
+        w.z |= word == 2 ? x : 0;
+        w.w |= word == 3 ? x : 0;
+    }
+    return w;
+}
+template <class T>
+__device__ __forceinline__ void put_part(typename T::Raw *p, int have, uint4 w) {
+    constexpr int SIZE = sizeof(typename T::Raw);
+#pragma unroll 1
+    for (int e = 0; e < have; ++e) {
+        const int word = e * SIZE / 4;
+        const uint32_t x = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
+        if constexpr (SIZE == 4)
+            p[e] = __builtin_bit_cast(float, x);
+        else
+            p[e] = __builtin_bit_cast(typename T::Raw, uint16_t(x >> (e % 2 * 16)));
+    }
+}
+
 // Inputs and outputs of more than the Infinity Cache's 256 MB: whoever comes next
 // does not find them there, so they are moved past the caches (STREAM).
 constexpr double kCached = double(256u << 20);
@@ -89,6 +124,13 @@ __device__ __forceinline__ void put(void *p, W w) {
         __builtin_nontemporal_store(w, static_cast<W *>(p));
     else
         *static_cast<W *>(p) = w;
+}
+template <bool STREAM>
+__device__ __forceinline__ void put_any(void *p, uint4 w) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, w), static_cast<u32x4_any *>(p));
+    else
+        put_any(p, w);
 }
 template <bool STREAM>
 __device__ __forceinline__ uint4 get(const uint4 *p) {
