@@ -26,8 +26,8 @@ namespace meshgpt::kern {
 namespace {
 
 constexpr int kShort = 256;
-constexpr int kPerUnit = 64;       // bins of a factor e
-constexpr double kReach = 31.9;    // powers of e that are looked at: 2041.6 bins
+constexpr int kPerUnit = 128;      // bins of a factor e
+constexpr double kReach = 31.9;    // powers of e that are looked at
 constexpr uint32_t kNoToken = 0xffffffffu;
 
 // Logits as integers in the same order; -0 is 0.
@@ -220,37 +220,37 @@ __device__ __forceinline__ uint32_t equal_draw(double t, double w, uint32_t n) {
     return steps >= double(n - 1) ? n - 1 : steps > 0.0 ? uint32_t(steps) : 0;
 }
 
-// ---- weights by bins of 1/64 of a power of e -------------------------------------------
+// ---- weights by bins of 1/128 of a power of e -------------------------------------------
 
 struct Powers {
-    double wholes[32], parts[kPerUnit];  // e^-i, e^(-i / 64)
+    double wholes[32], parts[kPerUnit];  // e^-i, e^(-i / 128)
 };
 
 struct Weights {
     const Powers &powers;  // in LDS
     double top, scale;     // the largest logit, bins of a unit of a logit
 
-    // Makes the powers, as products of e^(-2^b / 64) (to 6 * 2^-53); a barrier has to follow.
+    // Makes the powers, as products of e^(-2^b / 128) (to 7 * 2^-53); a barrier has to follow.
     static __device__ __forceinline__ void prepare(Powers &p) {
         const uint32_t i = threadIdx.x;
-        if (i >= 96) return;
-        const double of[11] = {0x1.f80feabfeefa5p-1, 0x1.f03f56a88b5d8p-1, 0x1.e0fabfbc702a4p-1, 0x1.c3d6a24ed8222p-1,
-                               0x1.8ebef9eac820bp-1, 0x1.368b2fc6f960ap-1, 0x1.78b56362cef38p-2, 0x1.152aaa3bf81ccp-3,
-                               0x1.2c155b8213cf4p-6, 0x1.5fc21041027adp-12, 0x1.e355bbaee85cbp-24};
+        if (i >= kPerUnit + 32) return;
+        const double of[12] = {0x1.fc03fd56aa225p-1, 0x1.f80feabfeefa5p-1, 0x1.f03f56a88b5d8p-1, 0x1.e0fabfbc702a4p-1,
+                               0x1.c3d6a24ed8222p-1, 0x1.8ebef9eac820bp-1, 0x1.368b2fc6f960ap-1, 0x1.78b56362cef38p-2,
+                               0x1.152aaa3bf81ccp-3, 0x1.2c155b8213cf4p-6, 0x1.5fc21041027adp-12, 0x1.e355bbaee85cbp-24};
         double w = 1.0;
 #pragma unroll
-        for (int b = 0; b < 6; ++b)
-            if (i >> b & 1) w *= i < kPerUnit ? of[b] : of[min(6 + b, 10)];
+        for (int b = 0; b < 7; ++b)
+            if (i >> b & 1) w *= i < kPerUnit ? of[b] : of[min(7 + b, 11)];
         (i < kPerUnit ? p.parts[i] : p.wholes[i - kPerUnit]) = w;
     }
     // Bins from the largest logit.
     __device__ __forceinline__ double place(float x) const { return (top - double(x)) * scale; }
     // The weight where a bin begins.
     __device__ __forceinline__ double begin_of(int bin) const { return powers.wholes[bin / kPerUnit] * powers.parts[bin % kPerUnit]; }
-    // e^(-r / 64) - 1 for r from 0 to 1: the sixth term of the series is under 2^-45.  r = 0 is
+    // e^(-r / 128) - 1 for r from 0 to 1: the fifth term of the series is under 2^-41.  r = 0 is
     // exact, and with it the sum of weights that equal the largest.
     static __device__ __forceinline__ double rest(double r) {
-        return r * fma(r, fma(r, fma(r, fma(r, -0x1p-30 / 120, 0x1p-24 / 24), -0x1p-18 / 6), 0x1p-12 / 2), -0x1p-6);
+        return r * fma(r, fma(r, fma(r, 0x1p-28 / 24, -0x1p-21 / 6), 0x1p-14 / 2), -0x1p-7);
     }
     __device__ __forceinline__ double of(float x) const {
         const double y = place(x), at = floor(y);
@@ -724,9 +724,9 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
 
 // The row's largest logit; then either few candidates (top_k bounds them by the
 // k-th largest of the threads' maxima, min_p by itself), which are gathered and
-// ranked, or bins of (max z - z) / T, 64 for each power of e.  A bin keeps its
+// ranked, or bins of (max z - z) / T, 128 for each power of e. A bin keeps its
 // tokens' count and the fixed-point sum of w / (w where it begins) - 1 in one LDS
-// word, exact to 2^-34 of a weight and the same in any order.  Where a border falls
+// word, exact to 2^-35 of a weight and the same in any order.  Where a border falls
 // into a bin, its tokens are gathered and ranked; if they are more than MOST, the
 // bin is divided by the bits of their logits until they are few enough or equal.
 enum Ask { kCount, kReachP, kLeast, kDraw, kAsks };
@@ -814,8 +814,13 @@ struct Bins {
                             s.list[b] = x;
                         }
                     }
-                    __syncthreads();
+                    // Pairs up to 64 apart are a wave's own: its LDS operations are in order.
+                    if (j > 64 || (j == 1 && k >= 128))
+                        __syncthreads();
+                    else
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 }
+            __syncthreads();
         }
         constexpr int E = MOST / THREADS;
         double w[E], sum = 0.0, total;
@@ -888,9 +893,7 @@ struct Bins {
     // Weights::rest in units of 2^-dev_bits, rounded by the addition of 1.5 * 2^52.
     __device__ __forceinline__ uint64_t term(double r) const {
         const auto units = [&](double v) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, v) + (uint64_t(dev_bits) << 52)); };
-        const double d = fma(r, fma(r, fma(r, fma(r, units(-0x1p-30 / 120), units(0x1p-24 / 24)), units(-0x1p-18 / 6)),
-                                    units(0x1p-12 / 2)),
-                             units(-0x1p-6));
+        const double d = fma(r, fma(r, fma(r, units(0x1p-28 / 24), units(-0x1p-21 / 6)), units(0x1p-14 / 2)), units(-0x1p-7));
         const double rounded = fma(r, d, 0x1.8p52);
         return __builtin_bit_cast(uint64_t, rounded) + ((uint64_t(1) << shift) - __builtin_bit_cast(uint64_t, 0x1.8p52));
     }
@@ -900,9 +903,9 @@ struct Bins {
         weight = begin * fma(double(dev), __builtin_bit_cast(double, uint64_t(1023 - dev_bits) << 52), double(tokens));
     }
     __device__ __forceinline__ void fill(uint32_t &all_c, double &all_w) {
-        // A bin's sum of `vocab` terms under 0.0156 stays in its field.
+        // A bin's sum of `vocab` terms under 0.0079 stays in its field.
         shift = 63 - (32 - __clz(int(vocab)));
-        dev_bits = min(36, 2 * shift - 58);
+        dev_bits = min(37, 2 * shift - 57);
         for (int i = tid; i < BINS; i += THREADS) s.bins[i] = 0;
         __syncthreads();
         const float from = least(kReach * kPerUnit);
@@ -1214,9 +1217,9 @@ void launch(const SampleArgs &a, hipStream_t stream) {
     if (a.vocab <= size_t(kShort))
         sample_short_kernel<T><<<rows, kShortThreads, 0, stream>>>(a);
     else if (a.vocab <= 8192)
-        sample_bins_kernel<T, 256, 2048, 1024><<<rows, 256, 0, stream>>>(a);
+        sample_bins_kernel<T, 512, 4096, 1024><<<rows, 512, 0, stream>>>(a);
     else if (sizeof(typename T::Raw) == 4 || a.vocab > size_t(kCodeMost))
-        sample_bins_kernel<T, 1024, 2048, 2048><<<rows, 1024, 0, stream>>>(a);
+        sample_bins_kernel<T, 1024, 4096, 2048><<<rows, 1024, 0, stream>>>(a);
     else if constexpr (sizeof(typename T::Raw) == 2)
         sample_codes_kernel<T><<<rows, kCodeThreads, 0, stream>>>(a);
 }
