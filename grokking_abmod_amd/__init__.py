@@ -33,7 +33,7 @@ EXPORTS = (
     "mg_token_logprobs_workspace", "mg_token_logprobs_noalloc", "mg_token_logprobs_backward_noalloc",
     "mg_token_logprobs", "mg_set_cache",
     "mg_sample_filtered_noalloc", "mg_rope_frequencies", "mg_rope_apply", "mg_rope_backward",
-    "mg_rms_norm", "mg_rms_norm_e4m3", "mg_rms_norm_backward_workspace", "mg_rms_norm_backward",
+    "mg_set_sampling", "mg_rms_norm", "mg_rms_norm_e4m3", "mg_rms_norm_backward_workspace", "mg_rms_norm_backward",
 )
 
 MG_F32, MG_F16, MG_BF16 = range(3)  # element types of the device operators
@@ -180,6 +180,7 @@ def lib():
                                   _u32p]),
         "mg_text_batch": (i, [_u32p, sz, _cfgp, i, sz, sz, u64, _u32p, _u32p]),
         "mg_set_cache": (i, [vp, i]),
+        "mg_set_sampling": (i, [vp, ctypes.c_uint32, f, f]),
         "mg_kv8_sizes": (i, [_kv8p, _szp, _szp]),
         "mg_kv8_append": (i, [i, _kv8p, i, sz, vp, _strides, vp, _strides, vp, vp, vp]),
         "mg_kv8_read": (i, [i, _kv8p, i, sz, sz, vp, _strides, vp, _strides, vp, vp]),
@@ -503,6 +504,10 @@ class MeshGpt:
     def set_cache(self, type):
         """mg_set_cache: MG_CACHE_F32 or MG_CACHE_E4M3; drops the current batch."""
         _check(lib().mg_set_cache(self._h, type))
+
+    def set_sampling(self, top_k=0, top_p=1.0, min_p=0.0):
+        """mg_set_sampling: filters of the tokens sampled from here on; the defaults filter nothing."""
+        _check(lib().mg_set_sampling(self._h, top_k, top_p, min_p))
         self._batch = 0
 
     def logits(self, tokens, sequence, last_only=False):

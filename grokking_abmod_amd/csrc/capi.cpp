@@ -211,6 +211,10 @@ int mg_set_parameters(mg_model *model, const float *values, size_t n) {
     });
 }
 
+int mg_set_sampling(mg_model *model, uint32_t top_k, float top_p, float min_p) {
+    return guarded([&] { model_of(model).set_sampling(top_k, top_p, min_p); });
+}
+
 int mg_set_cache(mg_model *model, int type) {
     return guarded([&] { model_of(model).set_cache(CacheType(type)); });
 }

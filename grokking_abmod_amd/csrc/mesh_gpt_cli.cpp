@@ -42,6 +42,8 @@ struct Options {
     std::string synthetic;
     size_t random_prompt = 0;
     bool cache8 = false;  // --cache e4m3
+    size_t top_k = 0;
+    float top_p = 1.0f, min_p = 0.0f;
     std::string prompt_file;
     std::string init = "reference";
     float init_sigma = 0.5f;
@@ -224,6 +226,9 @@ Options parse(int argc, char **argv) {
             if (type != "f32" && type != "e4m3") throw Error("unknown cache: " + type + "; use f32 or e4m3");
             o.cache8 = type == "e4m3";
         }
+        else if (flag == "--top-k") o.top_k = value<size_t>(it, end, flag);
+        else if (flag == "--top-p") o.top_p = value<float>(it, end, flag);
+        else if (flag == "--min-p") o.min_p = value<float>(it, end, flag);
         else if (flag == "--prompt-file") o.prompt_file = value<std::string>(it, end, flag);
         else if (flag == "--init") o.init = value<std::string>(it, end, flag);
         else if (flag == "--init-sigma") o.init_sigma = value<float>(it, end, flag);
@@ -276,6 +281,9 @@ const char *kHelp =
     "--seed N              Initialization/data/sampling seed (default: 7)\n"
     "--device N            HIP device ordinal (default: 0)\n"
     "--config NAME         generate: synthetic seeded model: tiny, symbolic, mid, long or high\n"
+    "--top-k N             generate: sample from the N most probable tokens (default: 0, all)\n"
+    "--top-p X             generate: from the fewest that reach X of the probability (default: 1, all)\n"
+    "--min-p X             generate: from those of X times the largest probability (default: 0, all)\n"
     "--cache NAME          generate: the KV cache, f32 or e4m3 (default: f32)\n"
     "--random-prompt LEN   With --config: LEN seeded uniform token ids as the prompt\n"
     "--prompt-file PATH    generate: read the prefix from PATH; with --batch N, N lines of\n"
@@ -918,6 +926,7 @@ int run(int argc, char **argv) {
         MeshGpt model(int(o.device), config, o.seed, o.batch);
         model.set_parameters(parameters.data(), parameters.size());
         if (o.cache8) model.set_cache(CacheType::E4M3);
+        model.set_sampling(uint32_t(std::min<size_t>(o.top_k, 0xffffffffu)), o.top_p, o.min_p);
         std::vector<std::string> texts;
         if (!o.prompt_file.empty() && prompt.empty()) texts = prompt_lines(o);
         if (prompt.empty() && !o.batch_set) {

@@ -157,6 +157,10 @@ struct MeshGpt::Impl {
     DevBuf k8, v8, ks8, vs8;
     // Sampler states and length right after the last prefill (rewind()).
     DevBuf drng_start;
+    // Filters of sampled tokens (set_sampling), and a step's settings and draws.
+    uint32_t top_k = 0;
+    float top_p = 1.0f, min_p = 0.0f;
+    DevBuf dfilter;
     // Sampler states a persistent decode launch writes (swapped with drng when
     // the launch completes).
     DevBuf drng_next;
@@ -1395,7 +1399,7 @@ struct MeshGpt::Impl {
     size_t allocated_device_bytes() const {
         size_t total = 0;
         for (const DevBuf *b : {&params, &codes, &E, &Et, &rope, &wdec, &Edec, &q0, &kc, &vc, &k8, &v8, &ks8, &vs8, &dx, &dx2, &dxn, &dq,
-                                &part, &dtokens, &dlen, &drng, &dlogits, &dflags, &drng_start, &drng_next, &dstage, &pxch, &pabort, &wx,
+                                &part, &dtokens, &dlen, &drng, &dlogits, &dflags, &drng_start, &drng_next, &dfilter, &dstage, &pxch, &pabort, &wx,
                                 &wxn, &wq, &wy, &wtok, &wlogits, &wk, &wv, &wsplit, &wlast, &tact, &tgrad, &tm, &tv, &tpart, &tin})
             total += b->bytes;
         return total;
@@ -1490,10 +1494,47 @@ struct MeshGpt::Impl {
         cached = 0;
         temperature = t;
         start_length = 0;
+        ensure_filter();
+    }
+
+    // Whether tokens are drawn through filters: then each step draws by sample_step, in
+    // one stream, on the per-phase kernels.
+    bool filtered() const { return temperature > 0.0f && (top_k > 0 || top_p < 1.0f || min_p > 0.0f); }
+    void ensure_filter() {
+        if (filtered() && batch_cap) dfilter.ensure(batch_cap * kern::kSampledBytes);
+    }
+    void set_sampling(uint32_t k, float p, float least) {
+        if (!(p > 0.0f && p <= 1.0f)) throw Error("top_p must be in (0, 1]");
+        if (!(least >= 0.0f && least <= 1.0f)) throw Error("min_p must be in [0, 1]");
+        if (k == top_k && p == top_p && least == min_p) return;
+        activate();
+        sync();
+        drop_graph();
+        const uint32_t was_k = top_k;
+        const float was_p = top_p, was_least = min_p;
+        top_k = k;
+        top_p = p;
+        min_p = least;
+        try {
+            ensure_filter();
+        } catch (...) {
+            top_k = was_k;
+            top_p = was_p;
+            min_p = was_least;
+            throw;
+        }
     }
 
     // The head and sampler for `n` sequence rows of xn (row i at i*row_mul+row_add).
     void head_and_sample(const float *xn, int row_mul, int row_add) {
+        if (filtered()) {
+            kern::head(shape, xn, int(batch), row_mul, row_add, Et.as<float>(), vpad, dlogits.as<float>(),
+                       head_rows(), stream);
+            kern::sample_step(dlogits.as<float>(), cfg.vocab_size, batch, temperature, top_k, top_p, min_p,
+                              drng.as<uint64_t>(), dfilter.p, dtokens.as<uint32_t>(), int(tcap), dlen.as<int>(),
+                              dflags.as<int>(), stream);
+            return;
+        }
         if (row_mul == 1 && row_add == 0 && kern::head_sample_lds_bytes(shape) <= lds_limit) {
             kern::head_sample(shape, xn, int(batch), Et.as<float>(), vpad, dlogits.as<float>(), temperature,
                               drng.as<uint64_t>(), dtokens.as<uint32_t>(), int(tcap), dlen.as<int>(),
@@ -1518,6 +1559,7 @@ struct MeshGpt::Impl {
     // kernel.  MG_DECODE_SLICES overrides the count (1 = one stream),
     // MG_DECODE_SLICE_MIN the sequences a slice needs.
     int decode_slices() const {
+        if (filtered()) return 1;
         const int want = std::min(env_int("MG_DECODE_SLICES", 2), kMaxSlices);
         if (kern::head_sample_lds_bytes(shape) > lds_limit) return 1;
         const size_t least = size_t(env_int("MG_DECODE_SLICE_MIN", length >= 2048 ? 4 : 32));
@@ -1652,7 +1694,7 @@ struct MeshGpt::Impl {
     }
 
     // Whether tokens can be generated from whole windows in one launch.
-    bool window_usable() const { return use_window && !cache8 && kern::window_supported(shape, cfg.context); }
+    bool window_usable() const { return use_window && !cache8 && !filtered() && kern::window_supported(shape, cfg.context); }
 
     // Whether they are, against the cached decode inside the context and a
     // prefill a token past it.  What the three take is estimated (us a token):
@@ -1761,7 +1803,7 @@ struct MeshGpt::Impl {
     }
 
     bool persistent_usable() const {
-        return persistent_ok && row_decode && !cache8 && kern::persistent_fits(shape, int(batch), device);
+        return persistent_ok && row_decode && !cache8 && !filtered() && kern::persistent_fits(shape, int(batch), device);
     }
 
     // Whether `steps` decode steps should run in the persistent kernel (the
@@ -1886,6 +1928,8 @@ void MeshGpt::set_cache(CacheType type) {
     if (type != CacheType::F32 && type != CacheType::E4M3) throw Error("unknown cache type code");
     impl_->set_cache(type == CacheType::E4M3);
 }
+
+void MeshGpt::set_sampling(uint32_t top_k, float top_p, float min_p) { impl_->set_sampling(top_k, top_p, min_p); }
 
 std::vector<float> MeshGpt::logits(const uint32_t *tokens, size_t n, size_t sequence, bool last_only) {
     impl_->cfg.validate_tokens(tokens, n, sequence);

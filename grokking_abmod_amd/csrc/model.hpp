@@ -34,6 +34,10 @@ class MeshGpt {
     // decodes from quantised keys and values on the per-phase kernels, prompts
     // attend in FP32.
     void set_cache(CacheType type);
+    // No counterpart in the reference.  Sampled tokens come from the first top_k in rank
+    // (0: all), of these from the shortest run that reaches top_p of their probability,
+    // of these from those of at least min_p times the largest; greedy ones stay.
+    void set_sampling(uint32_t top_k, float top_p, float min_p);
     // gpu.rs:1875-1887: logits of every row (or only each sequence's last row)
     std::vector<float> logits(const uint32_t *tokens, size_t n, size_t sequence, bool last_only = false);
     // The results of the calls of the same names, written to out, which holds

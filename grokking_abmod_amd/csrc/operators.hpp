@@ -133,6 +133,13 @@ struct SampleArgs {
     float *logprob;  // null: not wanted
 };
 void sample_filtered(const SampleArgs &a, Type type, hipStream_t stream);
+// A model's step: `batch` rows of F32 logits drawn with one set of filters, a number of
+// rng[r] each (advanced in place), the tokens appended at len[r].  scratch holds
+// kSampledBytes a row.  flags[0] becomes 1 where a row holds a non-finite logit.
+constexpr size_t kSampledBytes = 24;
+void sample_step(const float *logits, size_t vocab, size_t batch, float temperature, uint32_t top_k, float top_p,
+                 float min_p, uint64_t *rng, void *scratch, uint32_t *tokens, int token_stride, int *len, int *flags,
+                 hipStream_t stream);
 
 struct RopeSide {  // queries or keys
     const void *x;

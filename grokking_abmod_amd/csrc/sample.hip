@@ -16,10 +16,12 @@
 //   up to kShort logits: every token counts the tokens and weights before it;
 //   16-bit logits: a count for each of their 65536 values (sample_codes_kernel);
 //   else: bins of (max z - z) / T (sample_bins_kernel).
+#include <algorithm>
 #include <cfloat>
 
 #include "dpp.hpp"
 #include "operators.hpp"
+#include "sampler.hpp"
 #include "types.hpp"
 
 namespace meshgpt::kern {
@@ -1224,7 +1226,60 @@ void launch(const SampleArgs &a, hipStream_t stream) {
         sample_codes_kernel<T><<<rows, kCodeThreads, 0, stream>>>(a);
 }
 
+// ---- a model's step ---------------------------------------------------------------------
+
+// A step's scratch: temperatures, top_k, top_p, min_p, random numbers and tokens of `rows` rows.
+__global__ void sample_rows_kernel(uint32_t *scratch, size_t rows, float temperature, int top_k, float top_p, float min_p,
+                                   uint64_t *rng) {
+    const size_t r = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (r >= rows) return;
+    uint64_t state = rng[r];
+    scratch[r] = __builtin_bit_cast(uint32_t, temperature);
+    scratch[rows + r] = uint32_t(top_k);
+    scratch[2 * rows + r] = __builtin_bit_cast(uint32_t, top_p);
+    scratch[3 * rows + r] = __builtin_bit_cast(uint32_t, min_p);
+    scratch[4 * rows + r] = __builtin_bit_cast(uint32_t, rng_unit(state));
+    rng[r] = state;
+}
+
+// Appends a row's token, a wave a row; one with a logit that is not finite is flagged.
+__global__ void __launch_bounds__(64)
+sample_append_kernel(SampleArgs a, uint32_t *tokens, int token_stride, int *len, int *flags) {
+    const size_t r = blockIdx.x;
+    const float *const z = static_cast<const float *>(a.logits) + r * a.stride;
+    bool odd = false;
+    for (size_t i = threadIdx.x; i < a.vocab; i += 64) odd |= !(fabsf(z[i]) < INFINITY);
+    odd = __ballot(odd) != 0;
+    if (threadIdx.x) return;
+    const uint32_t token = a.tokens[r];
+    if (odd) atomicOr(flags, 1);
+    const int n = len[r];
+    tokens[r * size_t(token_stride) + n] = token < a.vocab ? token : 0;
+    len[r] = n + 1;
+}
+
 }  // namespace
+
+void sample_step(const float *logits, size_t vocab, size_t batch, float temperature, uint32_t top_k, float top_p,
+                 float min_p, uint64_t *rng, void *scratch, uint32_t *tokens, int token_stride, int *len, int *flags,
+                 hipStream_t stream) {
+    float *const f = static_cast<float *>(scratch);
+    SampleArgs a{};
+    a.logits = logits;
+    a.rows = batch;
+    a.vocab = a.stride = vocab;
+    a.temperatures = f;
+    a.top_k = reinterpret_cast<int *>(f + batch);
+    a.top_p = f + 2 * batch;
+    a.min_p = f + 3 * batch;
+    a.uniforms = f + 4 * batch;
+    a.tokens = reinterpret_cast<uint32_t *>(f + 5 * batch);
+    const int k = int(std::min<uint32_t>(top_k, 1u << 30));
+    sample_rows_kernel<<<dim3(unsigned((batch + 255) / 256)), 256, 0, stream>>>(static_cast<uint32_t *>(scratch), batch,
+                                                                                 temperature, k, top_p, min_p, rng);
+    launch<F32>(a, stream);
+    sample_append_kernel<<<dim3(unsigned(batch)), 64, 0, stream>>>(a, tokens, token_stride, len, flags);
+}
 
 void sample_filtered(const SampleArgs &a, Type type, hipStream_t stream) {
     switch (type) {

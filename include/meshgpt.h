@@ -213,6 +213,15 @@ int mg_last_call_ms(mg_model *model, float *ms);
  * return MG_UNSUPPORTED.  Head widths up to 256.  No reference counterpart. */
 enum { MG_CACHE_F32 = 0, MG_CACHE_E4M3 = 1 };
 int mg_set_cache(mg_model *model, int type);
+/* Filters of the tokens that a model samples at temperatures over 0, from the next
+ * one on: mg_sample_filtered_noalloc's with these settings for every row and the
+ * sampler's numbers (one of Random::unit() a token, as without filters).  top_k 0,
+ * top_p 1 and min_p 0 filter nothing and give the reference's sampler back; top_p lies
+ * in (0, 1], min_p in [0, 1].  Filtered tokens are drawn in the order of their
+ * probabilities, the reference's in that of the vocabulary, so the same number picks
+ * others.  Decode steps run on the per-phase kernels; mg_decode_traced returns
+ * MG_UNSUPPORTED.  No reference counterpart. */
+int mg_set_sampling(mg_model *model, uint32_t top_k, float top_p, float min_p);
 /* Current tokens per sequence (prompt + generated). */
 int mg_sequence_length(const mg_model *model, size_t *out);
 int mg_read_tokens(mg_model *model, uint32_t *out, size_t batch, size_t length);
