@@ -7,6 +7,7 @@ library; this module only marshals arrays.  Importing it fails loudly when the
 library has not been built: there is no fallback implementation.
 """
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -386,8 +387,11 @@ def rope_backward(rope, type, batch, count, heads, d_q_out, d_q_out_strides, d_q
                                   _three(d_k_strides), lengths, counts, positions, stream))
 
 
+_made_strides = functools.lru_cache(maxsize=256)(lambda strides: _strides(*strides))  # only read
+
+
 def _three(strides):
-    return None if strides is None else _strides(*strides)
+    return None if strides is None else _made_strides(tuple(strides))
 
 
 def rms_norm(type, rows, width, x, x_stride, residual, residual_stride, sum, sum_stride, weight, epsilon, out, out_stride,

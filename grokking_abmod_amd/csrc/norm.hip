@@ -7,8 +7,8 @@
 // with which the largest of them is at most 448.
 //   g = dy w;  dh = rstd (g - hat mean(g hat)) + dsum;  dw = sum of dy hat over rows, hat = h rstd.
 //
-// All of them read a row once: it stays in registers, 16 bytes a load, in one
-// wave for short rows and in 4 or 16 for longer ones.  Sums of a row are FP64,
+// All of them read a row once: it stays in registers, 16 bytes a load, in part of a
+// wave for short rows (heads) and in up to 8 for long ones.  Sums of a row are FP64,
 // which no FP32 value overflows; so is what decides a scale, where values next to
 // a power of two are met in any large batch.  The weight's gradient is summed in
 // registers over a team's rows, then over the teams in a fixed order.
@@ -24,7 +24,7 @@ template <class T>
 __device__ __forceinline__ uint4 load_group(const typename T::Raw *row, int g, int width) {
     const int have = width - g * T::kGroup;
     if (have >= T::kGroup) return get_any(reinterpret_cast<const char *>(row) + uint32_t(g) * 16u);  // 32 bits beside the row's address
-    return get_part<T>(row + g * T::kGroup, have);
+    return get_part<T>(row + g * T::kGroup, have, width >= T::kGroup);
 }
 template <class T>
 __device__ __forceinline__ void store_group(typename T::Raw *row, int g, int width, uint4 w) {
@@ -33,24 +33,21 @@ __device__ __forceinline__ void store_group(typename T::Raw *row, int g, int wid
     put_part<T>(row + g * T::kGroup, have, w);
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
-    return v;
-}
-
-// How a row is held: in a wave's registers, four rows a workgroup (BLOCK false), or in
-// those of a workgroup of whole waves.
-template <bool BLOCK>
+// How a row is held: in the registers of LANES lanes of a wave (16, 32 or 64), or (0) of a
+// workgroup of whole waves.
+template <int LANES>
 struct Team {
     int lane, lanes, of;  // this thread in its team, the team's threads, the team in its workgroup
     __device__ __forceinline__ Team()
-        : lane(BLOCK ? threadIdx.x : threadIdx.x % 64), lanes(BLOCK ? blockDim.x : 64),
-          of(BLOCK ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) {}
+        : lane(LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x), lanes(LANES ? LANES : blockDim.x),
+          of(LANES ? threadIdx.x / (LANES ? LANES : 1) : 0) {
+        if (LANES == 64) of = __builtin_amdgcn_readfirstlane(of);
+    }
     // The sum of its values, in all of its threads.
     __device__ __forceinline__ double sum(double v, double *room) const {
-        v = wave_sum64(v);
-        if constexpr (BLOCK) {
+#pragma unroll
+        for (int d = (LANES ? LANES : 64) / 2; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
+        if constexpr (LANES == 0) {
             __syncthreads();  // of the row before
             if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
             __syncthreads();
@@ -60,10 +57,8 @@ struct Team {
         return v;
     }
 };
-constexpr int kTeams = 4;  // waves of a workgroup that have a row each
+constexpr int kBlock = 256;  // threads of a workgroup with several rows
 constexpr int kWavesMost = 8;
-
-typedef uint32_t u32_any __attribute__((aligned(1)));
 
 // Four E4M3 codes.
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
@@ -71,15 +66,15 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
 }
 
-template <class T, bool BLOCK, int GROUPS, bool CODES>
-__global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_kernel(NormArgs a) {
+template <class T, int LANES, int GROUPS, bool CODES>
+__global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_kernel(NormArgs a) {
     using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
     __shared__ double room[kWavesMost];
-    const Team<BLOCK> team;
+    const Team<LANES> team;
     const int lane = team.lane, lanes = team.lanes, width = a.width;
-    const size_t row = BLOCK ? blockIdx.x : size_t(blockIdx.x) * kTeams + team.of;
-    if (row >= a.rows) return;  // a whole wave
+    const size_t row = LANES ? size_t(blockIdx.x) * (kBlock / (LANES ? LANES : 1)) + team.of : blockIdx.x;
+    if (row >= a.rows) return;  // whole teams, whose sums are their own
     const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs;
     const Raw *const weight = static_cast<const Raw *>(a.weight);
     uint4 h[GROUPS];
@@ -183,14 +178,15 @@ __global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_ke
 // the weight's gradient stay in registers, and so does the weight (KEEP), and the next
 // row's loads are under way while a row's mean is joined (AHEAD), where there is room.
 // 8192 x 4096 BF16 with a residual: 53 us (5 TB/s); a wave a row, without loads ahead, 114.
-template <class T, bool BLOCK, int GROUPS, bool AHEAD>
-__global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
+template <class T, int LANES, int GROUPS, bool AHEAD>
+__global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
     using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
     constexpr bool KEEP = GROUPS * G <= 16;  // more would not fit beside the rest
     __shared__ double room[kWavesMost];
-    __shared__ float joined[BLOCK ? 1 : 64 * GROUPS * G];
-    const Team<BLOCK> team;
+    constexpr int TEAMS = LANES ? kBlock / (LANES ? LANES : 1) : 1;
+    __shared__ float joined[LANES ? TEAMS * LANES * GROUPS * G : 1];
+    const Team<LANES> team;
     const int lane = team.lane, lanes = team.lanes, width = a.width;
     const Raw *const weight = static_cast<const Raw *>(a.weight);
     struct Groups {
@@ -200,12 +196,13 @@ __global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_ba
     const auto load = [&](size_t row, Groups &g) {
         const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs, *const dy = static_cast<const Raw *>(a.d_out) + row * a.dos,
                         *const ds = static_cast<const Raw *>(a.d_sum) + row * a.dss;
-        g.rstd = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(uint32_t, a.rstd[row])));
+        g.rstd = a.rstd[row];
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             g.h[i] = load_group<T>(x, lane + i * lanes, width);
             g.d[i] = load_group<T>(dy, lane + i * lanes, width);
             if (KEEP && a.d_sum) g.s[i] = load_group<T>(ds, lane + i * lanes, width);
+            if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);  // one group's addresses at a time
         }
     };
     const double share = 1.0 / double(width);
@@ -217,7 +214,7 @@ __global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_ba
 #pragma unroll
         for (int e = 0; e < G; ++e) dw[i][e] = 0.0f;
     }
-    size_t row = BLOCK ? blockIdx.x : size_t(blockIdx.x) * kTeams + team.of;
+    size_t row = size_t(blockIdx.x) * TEAMS + team.of;
     Groups now, next;
     if (row < a.rows) load(row, now);
     for (; row < a.rows; row += teams) {
@@ -265,21 +262,20 @@ __global__ void __launch_bounds__(BLOCK ? 64 * kWavesMost : 64 * kTeams) norm_ba
     }
     if (!a.part) return;
     float *const part = a.part + size_t(blockIdx.x) * width;
-    if constexpr (!BLOCK) {  // the waves one after the other, in one order
-        for (int t = 0; t < kTeams; ++t) {
-            if (team.of == t) {
+    if constexpr (LANES != 0) {  // the teams' sums, one after the other
 #pragma unroll
-                for (int i = 0; i < GROUPS; ++i)
+        for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-                    for (int e = 0; e < G; ++e) {
-                        float &at = joined[(i * G + e) * 64 + lane];
-                        if (t) dw[i][e] += at;
-                        at = dw[i][e];
-                    }
-            }
-            __syncthreads();
+            for (int e = 0; e < G; ++e) joined[((team.of * GROUPS + i) * G + e) * LANES + lane] = dw[i][e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < LANES * GROUPS * G; c += kBlock) {
+            float sum = joined[c];
+#pragma unroll
+            for (int t = 1; t < TEAMS; ++t) sum += joined[t * LANES * GROUPS * G + c];
+            const int at = (c % LANES + c / (LANES * G) * LANES) * G + c / LANES % G;
+            if (at < width) part[at] = sum;
         }
-        if (team.of != kTeams - 1) return;
+        return;
     }
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i)
@@ -308,57 +304,65 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const float *part, uint
     out[at] = float(sum);
 }
 
-// A row's 16-byte groups a lane, and its waves (0: a wave of a workgroup of kTeams).
+// How a row is cut: the lanes of a team (0: a workgroup, of so many threads), 16-byte
+// groups of a lane.
 struct Cut {
-    int groups, waves;
+    int lanes, groups, threads;
+    int teams() const { return lanes ? kBlock / lanes : 1; }
 };
 Cut cut_of(size_t width, int group) {
     const size_t n = (width + group - 1) / group;
-    if (n <= 64) return {1, 0};
-    if (n <= 128) return {2, 0};
+    for (int lanes : {16, 32, 64})
+        if (n <= size_t(lanes)) return {lanes, 1, kBlock};
+    if (n <= 128) return {64, 2, kBlock};
     for (int groups : {2, 4})
-        if (n <= size_t(64 * kWavesMost * groups)) return {groups, int((n + 64 * groups - 1) / (64 * groups))};
-    return {8, int((n + 64 * 8 - 1) / (64 * 8))};
+        if (n <= size_t(64 * kWavesMost * groups)) return {0, groups, 64 * int((n + 64 * groups - 1) / (64 * groups))};
+    return {0, 8, 64 * int((n + 64 * 8 - 1) / (64 * 8))};
 }
 
-// f(BLOCK, GROUPS) for a row's width.
+// f(LANES, GROUPS) for a row's width.
 template <class T, class F>
 void for_cut(const Cut &c, F &&f) {
     using std::integral_constant;
-    if (c.waves == 0)
-        return c.groups == 1 ? f(std::false_type(), integral_constant<int, 1>()) : f(std::false_type(), integral_constant<int, 2>());
-    if (c.groups == 2) return f(std::true_type(), integral_constant<int, 2>());
-    if (c.groups == 4) return f(std::true_type(), integral_constant<int, 4>());
-    if constexpr (T::kGroup == 4) f(std::true_type(), integral_constant<int, 8>());  // 16-bit rows end before
+    using One = integral_constant<int, 1>;
+    using Block = integral_constant<int, 0>;
+    switch (c.lanes) {
+        case 16: return f(integral_constant<int, 16>(), One());
+        case 32: return f(integral_constant<int, 32>(), One());
+        case 64:
+            return c.groups == 1 ? f(integral_constant<int, 64>(), One())
+                                 : f(integral_constant<int, 64>(), integral_constant<int, 2>());
+    }
+    if (c.groups == 2) return f(Block(), integral_constant<int, 2>());
+    if (c.groups == 4) return f(Block(), integral_constant<int, 4>());
+    if constexpr (T::kGroup == 4) f(Block(), integral_constant<int, 8>());  // 16-bit rows end before
 }
 
 template <class T>
 void norm_of(const NormArgs &a, hipStream_t stream) {
     const Cut c = cut_of(size_t(a.width), T::kGroup);
-    const int threads = c.waves ? 64 * c.waves : 64 * kTeams;
-    const dim3 grid(unsigned(c.waves ? a.rows : (a.rows + kTeams - 1) / kTeams));
-    for_cut<T>(c, [&](auto block, auto groups) {
+    const dim3 grid(unsigned((a.rows + c.teams() - 1) / c.teams()));
+    for_cut<T>(c, [&](auto lanes, auto groups) {
         if (a.codes)
-            norm_kernel<T, block.value, groups.value, true><<<grid, threads, 0, stream>>>(a);
+            norm_kernel<T, lanes.value, groups.value, true><<<grid, c.threads, 0, stream>>>(a);
         else
-            norm_kernel<T, block.value, groups.value, false><<<grid, threads, 0, stream>>>(a);
+            norm_kernel<T, lanes.value, groups.value, false><<<grid, c.threads, 0, stream>>>(a);
     });
 }
 
-uint32_t parts_of(size_t rows, int waves) {
-    const size_t teams = waves ? 1 : kTeams;
-    return uint32_t(std::min<size_t>((rows + teams - 1) / teams, 512));
+uint32_t parts_of(size_t rows, const Cut &c) {
+    return uint32_t(std::min<size_t>((rows + c.teams() - 1) / c.teams(), 512));
 }
 
 template <class T>
 void backward_of(const NormBackwardArgs &a, hipStream_t stream) {
     const Cut c = cut_of(size_t(a.width), T::kGroup);
-    const uint32_t parts = parts_of(a.rows, c.waves);
-    const int threads = c.waves ? 64 * c.waves : 64 * kTeams;
+    const uint32_t parts = parts_of(a.rows, c);
     if (parts)
-        for_cut<T>(c, [&](auto block, auto groups) {
-            norm_backward_kernel<T, block.value, groups.value, (groups.value * T::kGroup <= 16)>
-                <<<dim3(parts), threads, 0, stream>>>(a, parts * (c.waves ? 1 : kTeams));
+        for_cut<T>(c, [&](auto lanes, auto groups) {
+            constexpr bool AHEAD = groups.value * T::kGroup <= 16;
+            norm_backward_kernel<T, lanes.value, groups.value, AHEAD>
+                <<<dim3(parts), c.threads, 0, stream>>>(a, parts * uint32_t(c.teams()));
         });
     if (a.d_weight)
         norm_join_kernel<<<dim3(unsigned((a.width + 31) / 32)), 1024, 0, stream>>>(a.part, parts, a.width, a.d_weight);
@@ -367,7 +371,7 @@ void backward_of(const NormBackwardArgs &a, hipStream_t stream) {
 }  // namespace
 
 size_t norm_parts(size_t rows, size_t width) {
-    return std::max(parts_of(rows, cut_of(width, 4).waves), parts_of(rows, cut_of(width, 8).waves));
+    return std::max(parts_of(rows, cut_of(width, 4)), parts_of(rows, cut_of(width, 8)));
 }
 
 void rms_norm(const NormArgs &a, Type type, hipStream_t stream) {

@@ -36,8 +36,8 @@ __device__ __forceinline__ float2 turned(double t) {
 }
 
 template <class T>
-__device__ __forceinline__ uint4 load(const typename T::Raw *p, int have) {
-    return have >= T::kGroup ? get_any(p) : get_part<T>(p, have);
+__device__ __forceinline__ uint4 load(const typename T::Raw *p, int have, bool before) {
+    return have >= T::kGroup ? get_any(p) : get_part<T>(p, have, before);
 }
 template <class T, bool STREAM>
 __device__ __forceinline__ void store(typename T::Raw *p, int have, uint4 w) {
@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(kBlock) rope_kernel(RopeArgs a, int tile, int 
     };
     const auto fetch = [&](const Place &p, uint4 &x, uint4 &y) {
         if (p.t < 0) return;
-        x = load<T>(p.x, have);
-        if (!INTERLEAVED && turns) y = load<T>(p.x + half, have);
+        x = load<T>(p.x, have, at + have >= G);  // the head's own channels lie before
+        if (!INTERLEAVED && turns) y = load<T>(p.x + half, have, at + half + have >= G);
     };
     Place now = next();
     uint4 x{}, y{};

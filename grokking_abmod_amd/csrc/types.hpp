@@ -80,11 +80,20 @@ __device__ __forceinline__ void put_any(void *p, uint4 w) {
     *static_cast<u32x4_any *>(p) = __builtin_bit_cast(u32x4, w);
 }
 
-// The first `have` of a group's elements, the rest zero; and back.  (Loops: unrolled, the
+// The first `have` elements of a group, fewer than it holds, the rest zero; and back.
+// With `before`, a group's length of elements lies before p + have: one load that ends
+// there, moved down.  (Loops elsewhere, and stores by words: unrolled by elements, the
 // rare end of a row would take the registers of everything around it.)
 template <class T>
-__device__ __forceinline__ uint4 get_part(const typename T::Raw *p, int have) {
+__device__ __forceinline__ uint4 get_part(const typename T::Raw *p, int have, bool before) {
     constexpr int SIZE = sizeof(typename T::Raw);
+    if (before && have > 0) {
+        const uint4 w = get_any(p + have - T::kGroup);
+        const int bits = 8 * SIZE * (T::kGroup - have);  // 16 to 112
+        const uint64_t lo = uint64_t(w.y) << 32 | w.x, hi = uint64_t(w.w) << 32 | w.z;
+        const uint64_t down = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64), up = bits < 64 ? hi >> bits : 0;
+        return {uint32_t(down), uint32_t(down >> 32), uint32_t(up), uint32_t(up >> 32)};
+    }
     uint4 w{0, 0, 0, 0};
 #pragma unroll 1
     for (int e = 0; e < have; ++e) {
@@ -101,17 +110,21 @@ __device__ __forceinline__ uint4 get_part(const typename T::Raw *p, int have) {
     }
     return w;
 }
+typedef uint32_t u32_any __attribute__((aligned(1)));
 template <class T>
 __device__ __forceinline__ void put_part(typename T::Raw *p, int have, uint4 w) {
-    constexpr int SIZE = sizeof(typename T::Raw);
-#pragma unroll 1
-    for (int e = 0; e < have; ++e) {
-        const int word = e * SIZE / 4;
-        const uint32_t x = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
-        if constexpr (SIZE == 4)
-            p[e] = __builtin_bit_cast(float, x);
-        else
-            p[e] = __builtin_bit_cast(typename T::Raw, uint16_t(x >> (e % 2 * 16)));
+    if (have <= 0) return;
+    u32_any *const words = reinterpret_cast<u32_any *>(p);
+    if constexpr (sizeof(*p) == 4) {
+        words[0] = w.x;
+        if (have > 1) words[1] = w.y;
+        if (have > 2) words[2] = w.z;
+    } else {
+        if (have > 1) words[0] = w.x;
+        if (have > 3) words[1] = w.y;
+        if (have > 5) words[2] = w.z;
+        const uint32_t last = have < 2 ? w.x : have < 4 ? w.y : have < 6 ? w.z : w.w;
+        if (have % 2) p[have - 1] = __builtin_bit_cast(typename T::Raw, uint16_t(last));
     }
 }
 
