@@ -19,12 +19,21 @@
 namespace meshgpt::kern {
 namespace {
 
-// Group g of a row, zero behind its end.
+// Group g of a row: loaded, and then zero behind the row's end.  A group that the end cuts
+// is read by a load that ends there (a row of less than a group by its elements), and
+// trimmed once it is used, so that loads stay under way together.
 template <class T>
 __device__ __forceinline__ uint4 load_group(const typename T::Raw *row, int g, int width) {
-    const int have = width - g * T::kGroup;
-    if (have >= T::kGroup) return get_any(reinterpret_cast<const char *>(row) + uint32_t(g) * 16u);  // 32 bits beside the row's address
-    return get_part<T>(row + g * T::kGroup, have, width >= T::kGroup);
+    constexpr int G = T::kGroup;
+    if (width < G) return g == 0 ? get_part<T>(row, width) : uint4{0, 0, 0, 0};
+    return get_any(row + uint32_t(min(g * G, width - G)));
+}
+template <class T>
+__device__ __forceinline__ uint4 trim_group(uint4 w, int g, int width) {
+    constexpr int G = T::kGroup;
+    const int over = g * G - (width - G);
+    if (width >= G && __ballot(over > 0)) w = moved_down<T>(w, min(max(over, 0), G));
+    return w;
 }
 template <class T>
 __device__ __forceinline__ void store_group(typename T::Raw *row, int g, int width, uint4 w) {
@@ -33,10 +42,12 @@ __device__ __forceinline__ void store_group(typename T::Raw *row, int g, int wid
     put_part<T>(row + g * T::kGroup, have, w);
 }
 
-// How a row is held: in the registers of LANES lanes of a wave (16, 32 or 64), or (0) of a
-// workgroup of whole waves.
-template <int LANES>
+// How a row is held: in the registers of LANES lanes of a wave (16, 32 or 64), or of a
+// workgroup of whole waves: up to 8 (kBlockRow) or 16 (kWideRow), with half the registers.
+constexpr int kBlockRow = 0, kWideRow = -1;
+template <int LANES_>
 struct Team {
+    static constexpr int LANES = LANES_ > 0 ? LANES_ : 0;
     int lane, lanes, of;  // this thread in its team, the team's threads, the team in its workgroup
     __device__ __forceinline__ Team()
         : lane(LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x), lanes(LANES ? LANES : blockDim.x),
@@ -58,7 +69,9 @@ struct Team {
     }
 };
 constexpr int kBlock = 256;  // threads of a workgroup with several rows
-constexpr int kWavesMost = 8;
+constexpr int kWavesMost = 16;
+template <int LANES>
+constexpr int kThreads = LANES > 0 ? kBlock : LANES == kBlockRow ? 512 : 1024;  // at most
 
 // Four E4M3 codes.
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
@@ -67,13 +80,13 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
 }
 
 template <class T, int LANES, int GROUPS, bool CODES>
-__global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kThreads<LANES>) norm_kernel(NormArgs a) {
     using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
     __shared__ double room[kWavesMost];
     const Team<LANES> team;
     const int lane = team.lane, lanes = team.lanes, width = a.width;
-    const size_t row = LANES ? size_t(blockIdx.x) * (kBlock / (LANES ? LANES : 1)) + team.of : blockIdx.x;
+    const size_t row = LANES > 0 ? size_t(blockIdx.x) * (kBlock / (LANES > 0 ? LANES : 1)) + team.of : blockIdx.x;
     if (row >= a.rows) return;  // whole teams, whose sums are their own
     const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs;
     const Raw *const weight = static_cast<const Raw *>(a.weight);
@@ -88,12 +101,15 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_kernel(
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             float u[G], v[G];
-            T::unpack(h[i], u);
-            T::unpack(add[i], v);
+            T::unpack(trim_group<T>(h[i], lane + i * lanes, width), u);
+            T::unpack(trim_group<T>(add[i], lane + i * lanes, width), v);
 #pragma unroll
             for (int e = 0; e < G; ++e) u[e] += v[e];
             h[i] = T::pack(u);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) h[i] = trim_group<T>(h[i], lane + i * lanes, width);
     }
     double square = 0.0;
 #pragma unroll
@@ -119,7 +135,7 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_kernel(
             float u[G], w[G];
             T::unpack(h[i], u);
             if (weight) {
-                T::unpack(load_group<T>(weight, g, width), w);
+                T::unpack(trim_group<T>(load_group<T>(weight, g, width), g, width), w);
             } else {
 #pragma unroll
                 for (int e = 0; e < G; ++e) w[e] = 1.0f;
@@ -165,7 +181,7 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_kernel(
             for (int e = 0; e < G; ++e) u[e] = u[e] * pre * by;
             if (weight) {
                 float w[G];
-                T::unpack(load_group<T>(weight, g, width), w);
+                T::unpack(trim_group<T>(load_group<T>(weight, g, width), g, width), w);
 #pragma unroll
                 for (int e = 0; e < G; ++e) u[e] *= w[e];
             }
@@ -174,18 +190,21 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_kernel(
     }
 }
 
+// What the compiler knows of a group's contents ends here.
+__device__ __forceinline__ void forget(uint4 &w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
+
 // A team has every teams-th row, and its lanes the same channels of each: the sums of
-// the weight's gradient stay in registers, and so does the weight (KEEP), and the next
-// row's loads are under way while a row's mean is joined (AHEAD), where there is room.
+// the weight's gradient and the weight stay in registers, and the next row's loads are
+// under way while a row's mean is joined (AHEAD: where there is room).
 // 8192 x 4096 BF16 with a residual: 53 us (5 TB/s); a wave a row, without loads ahead, 114.
 template <class T, int LANES, int GROUPS, bool AHEAD>
-__global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
+__global__ void __launch_bounds__(kThreads<LANES>) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
     using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
-    constexpr bool KEEP = GROUPS * G <= 16;  // more would not fit beside the rest
+    constexpr bool TIGHT = LANES == kWideRow;  // one group at a time, for fewer registers
     __shared__ double room[kWavesMost];
-    constexpr int TEAMS = LANES ? kBlock / (LANES ? LANES : 1) : 1;
-    __shared__ float joined[LANES ? TEAMS * LANES * GROUPS * G : 1];
+    constexpr int TEAMS = LANES > 0 ? kBlock / (LANES > 0 ? LANES : 1) : 1;
+    __shared__ float joined[LANES > 0 ? TEAMS * LANES * GROUPS * G : 1];
     const Team<LANES> team;
     const int lane = team.lane, lanes = team.lanes, width = a.width;
     const Raw *const weight = static_cast<const Raw *>(a.weight);
@@ -201,8 +220,8 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backwar
         for (int i = 0; i < GROUPS; ++i) {
             g.h[i] = load_group<T>(x, lane + i * lanes, width);
             g.d[i] = load_group<T>(dy, lane + i * lanes, width);
-            if (KEEP && a.d_sum) g.s[i] = load_group<T>(ds, lane + i * lanes, width);
-            if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);  // one group's addresses at a time
+            if (a.d_sum) g.s[i] = load_group<T>(ds, lane + i * lanes, width);
+            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
     };
     const double share = 1.0 / double(width);
@@ -210,7 +229,7 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backwar
     float dw[GROUPS][G];
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
-        if (KEEP && weight) w[i] = load_group<T>(weight, lane + i * lanes, width);
+        if (weight) w[i] = trim_group<T>(load_group<T>(weight, lane + i * lanes, width), lane + i * lanes, width);
 #pragma unroll
         for (int e = 0; e < G; ++e) dw[i][e] = 0.0f;
     }
@@ -219,6 +238,12 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backwar
     if (row < a.rows) load(row, now);
     for (; row < a.rows; row += teams) {
         if (AHEAD && row + teams < a.rows) load(row + teams, next);
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            now.h[i] = trim_group<T>(now.h[i], lane + i * lanes, width);
+            now.d[i] = trim_group<T>(now.d[i], lane + i * lanes, width);
+            if (a.d_sum) now.s[i] = trim_group<T>(now.s[i], lane + i * lanes, width);
+        }
         // As in the forward pass, a rstd of rows over 1e30 is moved into FP32's range.
         const float pre = now.rstd < 0x1p-100f ? 0x1p-64f : 1.0f, by = now.rstd / pre;
         double dot = 0.0;
@@ -227,7 +252,7 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backwar
             float u[G], v[G], k[G], part = 0.0f;
             T::unpack(now.h[i], u);
             T::unpack(now.d[i], v);
-            if (weight) T::unpack(KEEP ? w[i] : load_group<T>(weight, lane + i * lanes, width), k);
+            if (weight) T::unpack(w[i], k);
 #pragma unroll
             for (int e = 0; e < G; ++e) {
                 const float hat = u[e] * pre * by;
@@ -235,25 +260,33 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backwar
                 part = fmaf(weight ? v[e] * k[e] : v[e], hat, part);
             }
             dot += double(part);
-            if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
         const float mean = float(team.sum(dot, room) * share);
+        if constexpr (TIGHT) {  // made anew below, not kept over the sum
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                forget(now.h[i]);
+                forget(now.d[i]);
+                forget(w[i]);
+            }
+        }
         Raw *const dx = static_cast<Raw *>(a.d_x) + row * a.dxs;
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             float u[G], v[G], k[G];
             T::unpack(now.h[i], u);
             T::unpack(now.d[i], v);
-            if (weight) T::unpack(KEEP ? w[i] : load_group<T>(weight, lane + i * lanes, width), k);
+            if (weight) T::unpack(w[i], k);
 #pragma unroll
             for (int e = 0; e < G; ++e) u[e] = now.rstd * fmaf(-(u[e] * pre * by), mean, weight ? v[e] * k[e] : v[e]);
             if (a.d_sum) {
-                T::unpack(KEEP ? now.s[i] : load_group<T>(static_cast<const Raw *>(a.d_sum) + row * a.dss, lane + i * lanes, width), v);
+                T::unpack(now.s[i], v);
 #pragma unroll
                 for (int e = 0; e < G; ++e) u[e] += v[e];
             }
             store_group<T>(dx, lane + i * lanes, width, T::pack(u));
-            if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (AHEAD)
             now = next;
@@ -262,7 +295,7 @@ __global__ void __launch_bounds__(LANES ? kBlock : 64 * kWavesMost) norm_backwar
     }
     if (!a.part) return;
     float *const part = a.part + size_t(blockIdx.x) * width;
-    if constexpr (LANES != 0) {  // the teams' sums, one after the other
+    if constexpr (LANES > 0) {  // the teams' sums, one after the other
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
@@ -304,20 +337,19 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const float *part, uint
     out[at] = float(sum);
 }
 
-// How a row is cut: the lanes of a team (0: a workgroup, of so many threads), 16-byte
-// groups of a lane.
+// How a row is cut: the lanes of a team (or kBlockRow, kWideRow), 16-byte groups of a
+// lane, threads of the workgroup.
 struct Cut {
     int lanes, groups, threads;
-    int teams() const { return lanes ? kBlock / lanes : 1; }
+    int teams() const { return lanes > 0 ? kBlock / lanes : 1; }
 };
 Cut cut_of(size_t width, int group) {
     const size_t n = (width + group - 1) / group;
     for (int lanes : {16, 32, 64})
         if (n <= size_t(lanes)) return {lanes, 1, kBlock};
     if (n <= 128) return {64, 2, kBlock};
-    for (int groups : {2, 4})
-        if (n <= size_t(64 * kWavesMost * groups)) return {0, groups, 64 * int((n + 64 * groups - 1) / (64 * groups))};
-    return {0, 8, 64 * int((n + 64 * 8 - 1) / (64 * 8))};
+    const auto of = [&](int lanes, int groups) { return Cut{lanes, groups, 64 * int((n + 64 * groups - 1) / (64 * groups))}; };
+    return n <= 1024 ? of(kBlockRow, 2) : n <= 2048 ? of(kWideRow, 2) : of(kWideRow, 4);
 }
 
 // f(LANES, GROUPS) for a row's width.
@@ -325,17 +357,15 @@ template <class T, class F>
 void for_cut(const Cut &c, F &&f) {
     using std::integral_constant;
     using One = integral_constant<int, 1>;
-    using Block = integral_constant<int, 0>;
+    using Two = integral_constant<int, 2>;
     switch (c.lanes) {
         case 16: return f(integral_constant<int, 16>(), One());
         case 32: return f(integral_constant<int, 32>(), One());
-        case 64:
-            return c.groups == 1 ? f(integral_constant<int, 64>(), One())
-                                 : f(integral_constant<int, 64>(), integral_constant<int, 2>());
+        case 64: return c.groups == 1 ? f(integral_constant<int, 64>(), One()) : f(integral_constant<int, 64>(), Two());
+        case kBlockRow: return f(integral_constant<int, kBlockRow>(), Two());
     }
-    if (c.groups == 2) return f(Block(), integral_constant<int, 2>());
-    if (c.groups == 4) return f(Block(), integral_constant<int, 4>());
-    if constexpr (T::kGroup == 4) f(Block(), integral_constant<int, 8>());  // 16-bit rows end before
+    if (c.groups == 2) return f(integral_constant<int, kWideRow>(), Two());
+    if constexpr (T::kGroup == 4) f(integral_constant<int, kWideRow>(), integral_constant<int, 4>());  // 16-bit rows end before
 }
 
 template <class T>
@@ -360,7 +390,7 @@ void backward_of(const NormBackwardArgs &a, hipStream_t stream) {
     const uint32_t parts = parts_of(a.rows, c);
     if (parts)
         for_cut<T>(c, [&](auto lanes, auto groups) {
-            constexpr bool AHEAD = groups.value * T::kGroup <= 16;
+            constexpr bool AHEAD = lanes.value != kWideRow;
             norm_backward_kernel<T, lanes.value, groups.value, AHEAD>
                 <<<dim3(parts), c.threads, 0, stream>>>(a, parts * uint32_t(c.teams()));
         });

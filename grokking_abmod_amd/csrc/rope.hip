@@ -35,10 +35,6 @@ __device__ __forceinline__ float2 turned(double t) {
     return {q == 1 || q == 2 ? -a : a, q >= 2 ? -b : b};
 }
 
-template <class T>
-__device__ __forceinline__ uint4 load(const typename T::Raw *p, int have, bool before) {
-    return have >= T::kGroup ? get_any(p) : get_part<T>(p, have, before);
-}
 template <class T, bool STREAM>
 __device__ __forceinline__ void store(typename T::Raw *p, int have, uint4 w) {
     if (have >= T::kGroup) return put_any<STREAM>(p, w);
@@ -100,10 +96,15 @@ __global__ void __launch_bounds__(kBlock) rope_kernel(RopeArgs a, int tile, int 
             return p;
         }
     };
+    // A group that an end cuts is read with other channels of the head, before it (and moved
+    // once it is used) or behind it; a head of less than a group by its elements.
+    const bool pairs = !INTERLEAVED && turns;
+    const int end = at + (pairs ? half : 0), back = a.width >= G ? max(0, end + G - a.width) : 0;
+    const int front = pairs ? (a.width >= G ? max(0, at + G - a.width) : 0) : back;
     const auto fetch = [&](const Place &p, uint4 &x, uint4 &y) {
         if (p.t < 0) return;
-        x = load<T>(p.x, have, at + have >= G);  // the head's own channels lie before
-        if (!INTERLEAVED && turns) y = load<T>(p.x + half, have, at + half + have >= G);
+        x = a.width >= G ? get_any(p.x - front) : get_part<T>(p.x, have);
+        if (pairs) y = a.width >= G ? get_any(p.x + half - back) : get_part<T>(p.x + half, have);
     };
     Place now = next();
     uint4 x{}, y{};
@@ -120,6 +121,8 @@ __global__ void __launch_bounds__(kBlock) rope_kernel(RopeArgs a, int tile, int 
         const Place then = next();
         uint4 x2{}, y2{};
         fetch(then, x2, y2);
+        if (front) x = moved_down<T>(x, front);
+        if (pairs && back) y = moved_down<T>(y, back);
         const float2 *const row = table + now.t * half;
         float p[G], q[G];
         T::unpack(x, p);
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(kBlock) rope_kernel(RopeArgs a, int tile, int 
                           words > 3 ? turned.w : x.w};
             }
             store<T, STREAM>(now.o, have, turned);
-        } else if (turns) {
+        } else if (pairs) {
             T::unpack(y, q);
 #pragma unroll
             for (int e = 0; e < G; ++e) {

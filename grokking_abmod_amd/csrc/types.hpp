@@ -80,20 +80,20 @@ __device__ __forceinline__ void put_any(void *p, uint4 w) {
     *static_cast<u32x4_any *>(p) = __builtin_bit_cast(u32x4, w);
 }
 
-// The first `have` elements of a group, fewer than it holds, the rest zero; and back.
-// With `before`, a group's length of elements lies before p + have: one load that ends
-// there, moved down.  (Loops elsewhere, and stores by words: unrolled by elements, the
-// rare end of a row would take the registers of everything around it.)
+// A group's elements from the n-th on, moved to its begin, and zeros (n from 0 to all).  A
+// row's end is read by a whole load that ends there, and moved.
 template <class T>
-__device__ __forceinline__ uint4 get_part(const typename T::Raw *p, int have, bool before) {
+__device__ __forceinline__ uint4 moved_down(uint4 w, int n) {
+    const uint32_t bits = 8 * sizeof(typename T::Raw) * uint32_t(n);
+    const uint64_t lo = uint64_t(w.y) << 32 | w.x, hi = uint64_t(w.w) << 32 | w.z;
+    const uint64_t low = bits < 64 ? lo >> (bits & 63) | (bits ? hi << (64 - bits & 63) : 0) : bits < 128 ? hi >> (bits & 63) : 0;
+    const uint64_t high = bits < 64 ? hi >> (bits & 63) : 0;
+    return {uint32_t(low), uint32_t(low >> 32), uint32_t(high), uint32_t(high >> 32)};
+}
+// The first `have` elements of a group, fewer than it holds, the rest zero; and back.
+template <class T>
+__device__ __forceinline__ uint4 get_part(const typename T::Raw *p, int have) {
     constexpr int SIZE = sizeof(typename T::Raw);
-    if (before && have > 0) {
-        const uint4 w = get_any(p + have - T::kGroup);
-        const int bits = 8 * SIZE * (T::kGroup - have);  // 16 to 112
-        const uint64_t lo = uint64_t(w.y) << 32 | w.x, hi = uint64_t(w.w) << 32 | w.z;
-        const uint64_t down = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64), up = bits < 64 ? hi >> bits : 0;
-        return {uint32_t(down), uint32_t(down >> 32), uint32_t(up), uint32_t(up >> 32)};
-    }
     uint4 w{0, 0, 0, 0};
 #pragma unroll 1
     for (int e = 0; e < have; ++e) {
