@@ -190,110 +190,116 @@ __global__ void __launch_bounds__(kThreads<LANES>) norm_kernel(NormArgs a) {
     }
 }
 
-// What the compiler knows of a group's contents ends here.
-__device__ __forceinline__ void forget(uint4 &w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
+// A row's part of a gradient in a team's registers, trimmed.
+template <class T, int GROUPS>
+struct Gradient {
+    static constexpr int G = T::kGroup;
+    uint4 h[GROUPS], d[GROUPS], s[GROUPS];
+    float rstd;
 
-// A team has every teams-th row, and its lanes the same channels of each: the sums of
-// the weight's gradient and the weight stay in registers, and the next row's loads are
-// under way while a row's mean is joined (AHEAD: where there is room).
-// 8192 x 4096 BF16 with a residual: 53 us (5 TB/s); a wave a row, without loads ahead, 114.
-template <class T, int LANES, int GROUPS, bool AHEAD>
+    __device__ __forceinline__ void load(const NormBackwardArgs &a, size_t row, int lane, int lanes) {
+        using Raw = typename T::Raw;
+        const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs, *const dy = static_cast<const Raw *>(a.d_out) + row * a.dos,
+                        *const ds = static_cast<const Raw *>(a.d_sum) + row * a.dss;
+        rstd = a.rstd[row];
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            h[i] = load_group<T>(x, lane + i * lanes, a.width);
+            d[i] = load_group<T>(dy, lane + i * lanes, a.width);
+            if (a.d_sum) s[i] = load_group<T>(ds, lane + i * lanes, a.width);
+        }
+    }
+    __device__ __forceinline__ void trim(const NormBackwardArgs &a, int lane, int lanes) {
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            h[i] = trim_group<T>(h[i], lane + i * lanes, a.width);
+            d[i] = trim_group<T>(d[i], lane + i * lanes, a.width);
+            if (a.d_sum) s[i] = trim_group<T>(s[i], lane + i * lanes, a.width);
+        }
+    }
+    // A rstd of rows over 1e30 is moved into FP32's range: hat = h * pre * by.
+    __device__ __forceinline__ float pre() const { return rstd < 0x1p-100f ? 0x1p-64f : 1.0f; }
+    // This lane's sum of g hat; each(i, e, dy, hat) on the way.
+    template <class F>
+    __device__ __forceinline__ double dot(bool weight, const uint4 (&w)[GROUPS], F &&each) const {
+        const float before = pre(), by = rstd / before;
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            float u[G], v[G], k[G], part = 0.0f;
+            T::unpack(h[i], u);
+            T::unpack(d[i], v);
+            if (weight) T::unpack(w[i], k);
+#pragma unroll
+            for (int e = 0; e < G; ++e) {
+                const float hat = u[e] * before * by;
+                each(i, e, v[e], hat);
+                part = fmaf(weight ? v[e] * k[e] : v[e], hat, part);
+            }
+            sum += double(part);
+        }
+        return sum;
+    }
+    __device__ __forceinline__ void store(const NormBackwardArgs &a, size_t row, int lane, int lanes, float mean,
+                                          const uint4 (&w)[GROUPS]) const {
+        const float before = pre(), by = rstd / before;
+        typename T::Raw *const dx = static_cast<typename T::Raw *>(a.d_x) + row * a.dxs;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            float u[G], v[G], k[G];
+            T::unpack(h[i], u);
+            T::unpack(d[i], v);
+            if (a.weight) T::unpack(w[i], k);
+#pragma unroll
+            for (int e = 0; e < G; ++e) u[e] = rstd * fmaf(-(u[e] * before * by), mean, a.weight ? v[e] * k[e] : v[e]);
+            if (a.d_sum) {
+                T::unpack(s[i], v);
+#pragma unroll
+                for (int e = 0; e < G; ++e) u[e] += v[e];
+            }
+            store_group<T>(dx, lane + i * lanes, a.width, T::pack(u));
+        }
+    }
+};
+template <class T, int GROUPS>
+__device__ __forceinline__ void load_weight(const NormBackwardArgs &a, int lane, int lanes, uint4 (&w)[GROUPS]) {
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+        const int g = lane + i * lanes;
+        if (a.weight) w[i] = trim_group<T>(load_group<T>(static_cast<const typename T::Raw *>(a.weight), g, a.width), g, a.width);
+    }
+}
+
+// Both gradients in one pass.  A team has every teams-th row, and its lanes the same
+// channels of each: the sums of the weight's gradient and the weight stay in registers,
+// and the next row's loads are under way while a row's mean is joined.
+// 8192 x 4096 BF16 with a residual: 49 us (5.5 TB/s); a wave a row, without loads ahead, 114.
+template <class T, int LANES, int GROUPS>
 __global__ void __launch_bounds__(kThreads<LANES>) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
-    using Raw = typename T::Raw;
     constexpr int G = T::kGroup;
-    constexpr bool TIGHT = LANES == kWideRow;  // one group at a time, for fewer registers
     __shared__ double room[kWavesMost];
     constexpr int TEAMS = LANES > 0 ? kBlock / (LANES > 0 ? LANES : 1) : 1;
     __shared__ float joined[LANES > 0 ? TEAMS * LANES * GROUPS * G : 1];
     const Team<LANES> team;
     const int lane = team.lane, lanes = team.lanes, width = a.width;
-    const Raw *const weight = static_cast<const Raw *>(a.weight);
-    struct Groups {
-        uint4 h[GROUPS], d[GROUPS], s[GROUPS];
-        float rstd;
-    };
-    const auto load = [&](size_t row, Groups &g) {
-        const Raw *const x = static_cast<const Raw *>(a.x) + row * a.xs, *const dy = static_cast<const Raw *>(a.d_out) + row * a.dos,
-                        *const ds = static_cast<const Raw *>(a.d_sum) + row * a.dss;
-        g.rstd = a.rstd[row];
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            g.h[i] = load_group<T>(x, lane + i * lanes, width);
-            g.d[i] = load_group<T>(dy, lane + i * lanes, width);
-            if (a.d_sum) g.s[i] = load_group<T>(ds, lane + i * lanes, width);
-            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
-        }
-    };
     const double share = 1.0 / double(width);
     uint4 w[GROUPS];
+    load_weight<T>(a, lane, lanes, w);
     float dw[GROUPS][G];
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
-        if (weight) w[i] = trim_group<T>(load_group<T>(weight, lane + i * lanes, width), lane + i * lanes, width);
+    for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
         for (int e = 0; e < G; ++e) dw[i][e] = 0.0f;
-    }
     size_t row = size_t(blockIdx.x) * TEAMS + team.of;
-    Groups now, next;
-    if (row < a.rows) load(row, now);
+    Gradient<T, GROUPS> now, next;
+    if (row < a.rows) now.load(a, row, lane, lanes);
     for (; row < a.rows; row += teams) {
-        if (AHEAD && row + teams < a.rows) load(row + teams, next);
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            now.h[i] = trim_group<T>(now.h[i], lane + i * lanes, width);
-            now.d[i] = trim_group<T>(now.d[i], lane + i * lanes, width);
-            if (a.d_sum) now.s[i] = trim_group<T>(now.s[i], lane + i * lanes, width);
-        }
-        // As in the forward pass, a rstd of rows over 1e30 is moved into FP32's range.
-        const float pre = now.rstd < 0x1p-100f ? 0x1p-64f : 1.0f, by = now.rstd / pre;
-        double dot = 0.0;
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            float u[G], v[G], k[G], part = 0.0f;
-            T::unpack(now.h[i], u);
-            T::unpack(now.d[i], v);
-            if (weight) T::unpack(w[i], k);
-#pragma unroll
-            for (int e = 0; e < G; ++e) {
-                const float hat = u[e] * pre * by;
-                dw[i][e] = fmaf(v[e], hat, dw[i][e]);
-                part = fmaf(weight ? v[e] * k[e] : v[e], hat, part);
-            }
-            dot += double(part);
-            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
-        }
-        const float mean = float(team.sum(dot, room) * share);
-        if constexpr (TIGHT) {  // made anew below, not kept over the sum
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                forget(now.h[i]);
-                forget(now.d[i]);
-                forget(w[i]);
-            }
-        }
-        Raw *const dx = static_cast<Raw *>(a.d_x) + row * a.dxs;
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            float u[G], v[G], k[G];
-            T::unpack(now.h[i], u);
-            T::unpack(now.d[i], v);
-            if (weight) T::unpack(w[i], k);
-#pragma unroll
-            for (int e = 0; e < G; ++e) u[e] = now.rstd * fmaf(-(u[e] * pre * by), mean, weight ? v[e] * k[e] : v[e]);
-            if (a.d_sum) {
-                T::unpack(now.s[i], v);
-#pragma unroll
-                for (int e = 0; e < G; ++e) u[e] += v[e];
-            }
-            store_group<T>(dx, lane + i * lanes, width, T::pack(u));
-            if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
-        }
-        if constexpr (AHEAD)
-            now = next;
-        else if (row + teams < a.rows)
-            load(row + teams, now);
+        if (row + teams < a.rows) next.load(a, row + teams, lane, lanes);
+        now.trim(a, lane, lanes);
+        const double dot = now.dot(a.weight, w, [&](int i, int e, float dy, float hat) { dw[i][e] = fmaf(dy, hat, dw[i][e]); });
+        now.store(a, row, lane, lanes, float(team.sum(dot, room) * share), w);
+        now = next;
     }
-    if (!a.part) return;
     float *const part = a.part + size_t(blockIdx.x) * width;
     if constexpr (LANES > 0) {  // the teams' sums, one after the other
 #pragma unroll
@@ -317,6 +323,86 @@ __global__ void __launch_bounds__(kThreads<LANES>) norm_backward_kernel(NormBack
             const int at = (lane + i * lanes) * G + e;
             if (at < width) part[at] = dw[i][e];
         }
+}
+
+// The weight's gradient alone, of SLAB groups of channels: a workgroup sums over every
+// parts-th of its rows, U at a time a thread, in a fixed order.
+template <class T, int SLAB, int U>
+__device__ __forceinline__ void sum_columns(const NormBackwardArgs &a, int slab, size_t part, size_t parts, float *out, float *room) {
+    using Raw = typename T::Raw;
+    constexpr int G = T::kGroup;
+    const int c = threadIdx.x % SLAB, of = threadIdx.x / SLAB, rows = blockDim.x / SLAB, g = slab * SLAB + c, width = a.width;
+    float sum[G];
+#pragma unroll
+    for (int e = 0; e < G; ++e) sum[e] = 0.0f;
+    if (g * G < width) {
+        const size_t step = parts * rows;
+        for (size_t first = part * rows + of; first < a.rows; first += U * step) {
+            uint4 h[U], d[U];
+            float rstd[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t row = first + u * step, in = row < a.rows ? row : first;
+                h[u] = load_group<T>(static_cast<const Raw *>(a.x) + in * a.xs, g, width);
+                d[u] = load_group<T>(static_cast<const Raw *>(a.d_out) + in * a.dos, g, width);
+                rstd[u] = a.rstd[in];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (first + u * step >= a.rows) continue;
+                const float pre = rstd[u] < 0x1p-100f ? 0x1p-64f : 1.0f, by = rstd[u] / pre;
+                float x[G], dy[G];
+                T::unpack(trim_group<T>(h[u], g, width), x);
+                T::unpack(trim_group<T>(d[u], g, width), dy);
+#pragma unroll
+                for (int e = 0; e < G; ++e) sum[e] = fmaf(dy[e], x[e] * pre * by, sum[e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < G; ++e) room[of * SLAB * G + c * G + e] = sum[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < SLAB * G; i += blockDim.x) {
+        const int at = slab * SLAB * G + i;
+        if (at >= width) break;
+        double all = 0.0;
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) all += double(room[r * SLAB * G + i]);
+        out[at] = float(all);
+    }
+}
+constexpr int kSlab = 64, kNarrow = 2;  // groups of channels of a workgroup: of many rows, of few
+template <class T>
+__global__ void __launch_bounds__(kBlock) norm_columns_kernel(NormBackwardArgs a, uint32_t slabs, uint32_t parts) {
+    __shared__ float room[kBlock * T::kGroup];
+    const uint32_t part = blockIdx.x / slabs;
+    sum_columns<T, kSlab, 4>(a, int(blockIdx.x - part * slabs), part, parts, a.part + size_t(part) * a.width, room);
+}
+
+// The rows' gradient alone, a row a team, in the first workgroups; in the others (few
+// rows) the weight's, which needs no row's mean.
+template <class T, int LANES, int GROUPS>
+__global__ void __launch_bounds__(kThreads<LANES>) norm_rows_kernel(NormBackwardArgs a, uint32_t row_blocks) {
+    constexpr int TEAMS = LANES > 0 ? kBlock / (LANES > 0 ? LANES : 1) : 1;
+    __shared__ union {
+        double sums[kWavesMost];
+        float columns[LANES == kWideRow ? 1 : kThreads<LANES> * T::kGroup];
+    } room;
+    if (blockIdx.x >= row_blocks) {
+        if constexpr (LANES != kWideRow) sum_columns<T, kNarrow, 8>(a, int(blockIdx.x - row_blocks), 0, 1, a.d_weight, room.columns);
+        return;
+    }
+    const Team<LANES> team;
+    const int lane = team.lane, lanes = team.lanes;
+    const size_t row = size_t(blockIdx.x) * TEAMS + team.of;
+    if (row >= a.rows) return;  // whole teams, whose sums are their own
+    Gradient<T, GROUPS> now;
+    uint4 w[GROUPS];
+    now.load(a, row, lane, lanes);
+    load_weight<T>(a, lane, lanes, w);
+    now.trim(a, lane, lanes);
+    const double dot = now.dot(a.weight, w, [](int, int, float, float) {});
+    now.store(a, row, lane, lanes, float(team.sum(dot, room.sums) / double(a.width)), w);
 }
 
 // Sums 32 channels over the parts, 32 threads each.
@@ -383,25 +469,54 @@ void norm_of(const NormArgs &a, hipStream_t stream) {
 uint32_t parts_of(size_t rows, const Cut &c) {
     return uint32_t(std::min<size_t>((rows + c.teams() - 1) / c.teams(), 512));
 }
+// Calls of few rows and elements take one launch, in which some workgroups read the rows
+// again for the weight's gradient: 1024 x 128 F32 took launches of 4.0 and 2.5 us, and takes
+// one of 5.9, and no workspace.
+bool few(size_t rows, size_t width) { return rows <= 1024 && rows * width <= size_t(1) << 18; }
 
 template <class T>
 void backward_of(const NormBackwardArgs &a, hipStream_t stream) {
     const Cut c = cut_of(size_t(a.width), T::kGroup);
-    const uint32_t parts = parts_of(a.rows, c);
-    if (parts)
-        for_cut<T>(c, [&](auto lanes, auto groups) {
-            constexpr bool AHEAD = lanes.value != kWideRow;
-            norm_backward_kernel<T, lanes.value, groups.value, AHEAD>
-                <<<dim3(parts), c.threads, 0, stream>>>(a, parts * uint32_t(c.teams()));
-        });
-    if (a.d_weight)
-        norm_join_kernel<<<dim3(unsigned((a.width + 31) / 32)), 1024, 0, stream>>>(a.part, parts, a.width, a.d_weight);
+    const uint32_t row_blocks = uint32_t((a.rows + c.teams() - 1) / c.teams());
+    const bool small = few(a.rows, size_t(a.width)) && c.lanes != kWideRow;
+    uint32_t parts = parts_of(a.rows, c);
+    for_cut<T>(c, [&](auto lanes, auto groups) {
+        const auto rows = [&](uint32_t first, uint32_t others) {
+            if (first + others) norm_rows_kernel<T, lanes.value, groups.value><<<dim3(first + others), c.threads, 0, stream>>>(a, first);
+        };
+        if (!a.d_weight) return rows(row_blocks, 0);
+        const int width = a.width, group = T::kGroup;
+        if (small) {
+            const uint32_t slabs = uint32_t((width + group * kNarrow - 1) / (group * kNarrow));
+            // What the rows' gradient replaces has to be read before.
+            const bool apart = a.d_x == a.x || a.d_x == a.d_out;
+            rows(apart ? 0 : row_blocks, slabs);
+            if (apart) rows(row_blocks, 0);
+            return;
+        }
+        if constexpr (lanes.value == kWideRow) {
+            // The registers do not hold the sums beside a row: 4000 x 15001 BF16 took 268 us so,
+            // and takes 194 with the rows read twice.
+            const uint32_t slabs = uint32_t((width + group * kSlab - 1) / (group * kSlab));
+            parts = std::min(parts, std::max(1u, 2048 / slabs));
+            if (parts) norm_columns_kernel<T><<<dim3(slabs * parts), kBlock, 0, stream>>>(a, slabs, parts);
+        } else if (parts) {
+            norm_backward_kernel<T, lanes.value, groups.value><<<dim3(parts), c.threads, 0, stream>>>(a, parts * uint32_t(c.teams()));
+        }
+        norm_join_kernel<<<dim3(unsigned((width + 31) / 32)), 1024, 0, stream>>>(a.part, parts, width, a.d_weight);
+        if constexpr (lanes.value == kWideRow) rows(row_blocks, 0);
+    });
 }
 
 }  // namespace
 
 size_t norm_parts(size_t rows, size_t width) {
-    return std::max(parts_of(rows, cut_of(width, 4)), parts_of(rows, cut_of(width, 8)));
+    size_t parts = 0;
+    for (int group : {4, 8}) {
+        const Cut c = cut_of(width, group);
+        if (!few(rows, width) || c.lanes == kWideRow) parts = std::max<size_t>(parts, parts_of(rows, c));
+    }
+    return parts;
 }
 
 void rms_norm(const NormArgs &a, Type type, hipStream_t stream) {

@@ -139,10 +139,10 @@ def test_norm_refusals(f):
 
 
 def test_norm_gradient_refusals():
-    need = G.rms_norm_backward_workspace(5, 64)
+    need = G.rms_norm_backward_workspace(5000, 64)
     assert need % (64 * 4) == 0 and need > 0
-    assert G.rms_norm_backward_workspace(0, 64) == 0
-    base = dict(type=G.MG_F32, rows=5, width=64, sum=256, sum_stride=64, weight=256, rstd=256, d_out=256, d_out_stride=64,
+    assert G.rms_norm_backward_workspace(0, 64) == G.rms_norm_backward_workspace(5, 64) == 0
+    base = dict(type=G.MG_F32, rows=5000, width=64, sum=256, sum_stride=64, weight=256, rstd=256, d_out=256, d_out_stride=64,
                 d_sum=256, d_sum_stride=64, d_x=256, d_x_stride=64, d_weight=256, workspace=256, workspace_bytes=need)
     call = lambda **kw: G.rms_norm_backward(**{**base, **kw})  # noqa: E731
     refused("element type", call, type=-1)
