@@ -12,10 +12,11 @@
 // tokens one is 1e-5 of the whole.  So weights are summed in 64 bits, in an
 // order that is the same in every call.
 //
-// A row has a workgroup, in one of three ways:
-//   up to kShort logits: every token counts the tokens and weights before it;
-//   16-bit logits: a count for each of their 65536 values (sample_codes_kernel);
-//   else: bins of (max z - z) / T (sample_bins_kernel).
+// A row has a workgroup, in one of three ways (`launch` has the sizes):
+//   up to 256 logits: every token counts the tokens and weights before it;
+//   many 16-bit logits: a count for each of their 65536 values (sample_codes_kernel);
+//   else: bins of (max z - z) / T (sample_bins_kernel), and where top_k or min_p leave few
+//   tokens before any weight is summed, these tokens alone.
 #include <algorithm>
 #include <cfloat>
 
@@ -27,8 +28,6 @@
 namespace meshgpt::kern {
 namespace {
 
-constexpr int kShort = 256;
-constexpr int kPerUnit = 128;      // bins of a factor e
 constexpr double kReach = 31.9;    // powers of e that are looked at
 constexpr uint32_t kNoToken = 0xffffffffu;
 
@@ -222,43 +221,55 @@ __device__ __forceinline__ uint32_t equal_draw(double t, double w, uint32_t n) {
     return steps >= double(n - 1) ? n - 1 : steps > 0.0 ? uint32_t(steps) : 0;
 }
 
-// ---- weights by bins of 1/128 of a power of e -------------------------------------------
+// ---- weights by bins of 1 / UNIT of a power of e ------------------------------------------
 
+template <int UNIT>
 struct Powers {
-    double wholes[32], parts[kPerUnit];  // e^-i, e^(-i / 128)
+    double wholes[32], parts[UNIT];  // e^-i, e^(-i / UNIT)
 };
 
+template <int UNIT>
 struct Weights {
-    const Powers &powers;  // in LDS
-    double top, scale;     // the largest logit, bins of a unit of a logit
+    const Powers<UNIT> &powers;  // in LDS
+    double top, scale;           // the largest logit, bins of a unit of a logit
 
     // Makes the powers, as products of e^(-2^b / 128) (to 7 * 2^-53); a barrier has to follow.
-    static __device__ __forceinline__ void prepare(Powers &p) {
+    static __device__ __forceinline__ void prepare(Powers<UNIT> &p) {
+        static_assert(UNIT == 32 || UNIT == 128, "units of the table");
+        constexpr int STEP = UNIT == 128 ? 0 : 2, BITS = UNIT == 128 ? 7 : 5;
         const uint32_t i = threadIdx.x;
-        if (i >= kPerUnit + 32) return;
+        if (i >= UNIT + 32) return;
         const double of[12] = {0x1.fc03fd56aa225p-1, 0x1.f80feabfeefa5p-1, 0x1.f03f56a88b5d8p-1, 0x1.e0fabfbc702a4p-1,
                                0x1.c3d6a24ed8222p-1, 0x1.8ebef9eac820bp-1, 0x1.368b2fc6f960ap-1, 0x1.78b56362cef38p-2,
                                0x1.152aaa3bf81ccp-3, 0x1.2c155b8213cf4p-6, 0x1.5fc21041027adp-12, 0x1.e355bbaee85cbp-24};
         double w = 1.0;
 #pragma unroll
-        for (int b = 0; b < 7; ++b)
-            if (i >> b & 1) w *= i < kPerUnit ? of[b] : of[min(7 + b, 11)];
-        (i < kPerUnit ? p.parts[i] : p.wholes[i - kPerUnit]) = w;
+        for (int b = 0; b < BITS; ++b)
+            if (i >> b & 1) w *= i < UNIT ? of[b + STEP] : of[min(7 + b, 11)];
+        (i < UNIT ? p.parts[i] : p.wholes[i - UNIT]) = w;
     }
     // Bins from the largest logit.
     __device__ __forceinline__ double place(float x) const { return (top - double(x)) * scale; }
     // The weight where a bin begins.
-    __device__ __forceinline__ double begin_of(int bin) const { return powers.wholes[bin / kPerUnit] * powers.parts[bin % kPerUnit]; }
-    // e^(-r / 128) - 1 for r from 0 to 1: the fifth term of the series is under 2^-41.  r = 0 is
-    // exact, and with it the sum of weights that equal the largest.
-    static __device__ __forceinline__ double rest(double r) {
-        return r * fma(r, fma(r, fma(r, 0x1p-28 / 24, -0x1p-21 / 6), 0x1p-14 / 2), -0x1p-7);
+    __device__ __forceinline__ double begin_of(int bin) const { return powers.wholes[bin / UNIT] * powers.parts[bin % UNIT]; }
+    // The series of e^(-r / UNIT) - 1 for r from 0 to 1, in units of `unit`, over r: what it
+    // leaves out is under 2^-39.  r = 0 is exact, and with it the sum of weights that equal
+    // the largest.
+    template <class Units>
+    static __device__ __forceinline__ double series(double r, Units &&units) {
+        constexpr double U = 1.0 / UNIT;
+        double v = UNIT == 128 ? units(U * U * U * U / 24)
+                               : fma(r, units(-U * U * U * U * U / 120), units(U * U * U * U / 24));
+        v = fma(r, v, units(-U * U * U / 6));
+        v = fma(r, v, units(U * U / 2));
+        return fma(r, v, units(-U));
     }
     __device__ __forceinline__ double of(float x) const {
         const double y = place(x), at = floor(y);
-        if (!(y < kReach * kPerUnit)) return 0.0;
+        if (!(y < kReach * UNIT)) return 0.0;
         const double begin = begin_of(int(at));
-        return fma(begin, rest(y - at), begin);
+        const double r = y - at;
+        return fma(begin, r * series(r, [](double v) { return v; }), begin);
     }
 };
 
@@ -267,24 +278,22 @@ struct Weights {
 // Four threads count the tokens before a token, a quarter of the row each, four to an
 // LDS read; then a thread has a place in the ranking, with the running sum of the weights
 // up to there.
-constexpr int kShortThreads = 4 * kShort;
-
-template <class T>
-__global__ void __launch_bounds__(kShortThreads) sample_short_kernel(SampleArgs a) {
+template <class T, int TOKENS>
+__global__ void __launch_bounds__(4 * TOKENS) sample_short_kernel(SampleArgs a) {
     using Raw = typename T::Raw;
-    constexpr int WAVES = kShort / 64;
-    __shared__ uint4 keys[kShort / 4];
-    __shared__ double weights[kShort], sums[kShort], room_d[kShortThreads / 64];
-    __shared__ uint32_t tokens[kShort], room_u[kShortThreads / 64], bads[WAVES];
+    constexpr int WAVES = TOKENS / 64, THREADS = 4 * TOKENS, UNIT = 32;
+    __shared__ uint4 keys[TOKENS / 4];
+    __shared__ double weights[TOKENS], sums[TOKENS], room_d[THREADS / 64];
+    __shared__ uint32_t tokens[TOKENS], room_u[THREADS / 64], bads[WAVES];
     __shared__ float tops[WAVES];
-    __shared__ Powers powers;
+    __shared__ Powers<UNIT> powers;
     const size_t row = blockIdx.x;
     const uint32_t tid = threadIdx.x, vocab = uint32_t(a.vocab);
     const Raw *const z = static_cast<const Raw *>(a.logits) + row * a.stride;
     const Settings set = settings_of(a, row);
     const uint32_t token = tid / 4, quarter = tid % 4;
     const float x = token < vocab ? T::to_float(z[token]) : -INFINITY;
-    if (tid < kShort) {
+    if (tid < TOKENS) {
         const float y = tid < vocab ? T::to_float(z[tid]) : -INFINITY;
         reinterpret_cast<uint32_t *>(keys)[tid] = order(y);
         weights[tid] = 0.0;
@@ -295,8 +304,8 @@ __global__ void __launch_bounds__(kShortThreads) sample_short_kernel(SampleArgs 
             bads[tid / 64] = wave_bad;
         }
     }
-    Weights::prepare(powers);
-    const double scale = set.greedy ? 1.0 : uniform(kPerUnit / set.temperature);
+    Weights<UNIT>::prepare(powers);
+    const double scale = set.greedy ? 1.0 : uniform(UNIT / set.temperature);
     __syncthreads();
     float top = -INFINITY;
     uint32_t bad = 0;
@@ -313,8 +322,8 @@ __global__ void __launch_bounds__(kShortThreads) sample_short_kernel(SampleArgs 
     const uint32_t key = order(x);
     uint32_t before = 0;
 #pragma unroll 4
-    for (uint32_t j = 0; j < kShort / 16; ++j) {
-        const uint32_t at = quarter * (kShort / 16) + (j + 4 * quarter) % (kShort / 16);
+    for (uint32_t j = 0; j < TOKENS / 16; ++j) {
+        const uint32_t at = quarter * (TOKENS / 16) + (j + 4 * quarter) % (TOKENS / 16);
         const uint4 k = keys[at];
         const int lower = int(token) - int(4 * at);  // so many of the four are lower tokens
         before += (k.x > key - (lower > 0)) + (k.y > key - (lower > 1)) + (k.z > key - (lower > 2)) + (k.w > key - (lower > 3));
@@ -326,17 +335,17 @@ __global__ void __launch_bounds__(kShortThreads) sample_short_kernel(SampleArgs 
         return;
     }
     if (quarter == 0 && token < vocab) {
-        weights[before] = Weights{powers, double(top), scale}.of(x);
+        weights[before] = Weights<UNIT>{powers, double(top), scale}.of(x);
         tokens[before] = token;
     }
     __syncthreads();
     // From here on a thread has a place in the ranking.
-    const double w = tid < kShort ? weights[tid] : 0.0;
+    const double w = tid < TOKENS ? weights[tid] : 0.0;
     double whole;
-    const double sum = block_scan<kShortThreads>(w, room_d, whole) + w;
-    if (tid < kShort) sums[tid] = sum;
+    const double sum = block_scan<THREADS>(w, room_d, whole) + w;
+    if (tid < TOKENS) sums[tid] = sum;
     __syncthreads();
-    const auto count = [&](bool is) { return block_total<kShortThreads>(uint32_t(is), room_u); };
+    const auto count = [&](bool is) { return block_total<THREADS>(uint32_t(is), room_u); };
     uint32_t left = count(w > 0.0);
     if (set.top_k) left = min(left, set.top_k);
     if (set.with_p) {
@@ -347,6 +356,510 @@ __global__ void __launch_bounds__(kShortThreads) sample_short_kernel(SampleArgs 
     whole = sums[left - 1];
     const uint32_t at = min(left - 1, count(tid < left && sum <= set.uniform * whole));
     if (tid == at) write(a, row, tokens[tid], float(log(w / whole)));
+}
+
+// ---- the general way -----------------------------------------------------------------
+
+// The row's largest logit; then either few candidates (top_k bounds them by the
+// k-th largest of the threads' maxima, min_p by itself), which are gathered and
+// ranked, or bins of (max z - z) / T, UNIT for each power of e. A bin keeps its
+// tokens' count and the fixed-point sum of w / (w where it begins) - 1 in one LDS
+// word, each term rounded to 2^-34 of a weight or better up to 2^17 tokens (2^-28 at
+// 2^20), so that it is the same in any order.  Where a border falls
+// into a bin, its tokens are gathered and ranked; if they are more than MOST, the
+// bin is divided by the bits of their logits until they are few enough or equal.
+enum Ask { kCount, kReachP, kLeast, kDraw, kAsks };
+
+template <class T, int THREADS, int UNIT, int MOST>
+struct Bins {
+    static constexpr int BINS = 32 * UNIT;
+    static constexpr int kEach = BINS / THREADS;
+    static_assert(BINS > kReach * UNIT && BINS % THREADS == 0 && MOST % THREADS == 0, "every place has a bin");
+    static constexpr int kCounted = THREADS / 4;  // up to so many are ranked by counting
+
+    struct Bin {
+        int at;
+        uint32_t taken, count;  // tokens before it and in it
+        double base, weight;    // weights before it and in it
+    };
+    struct Shared {
+        uint64_t bins[BINS], fine[THREADS], list[MOST];
+        double sums[MOST];
+        double before[THREADS];   // weights before a thread's bins
+        uint32_t taken[THREADS];  // and tokens
+        double room_d[THREADS / 64], base;
+        Bin found_by[THREADS / 64];
+        uint32_t room_u[THREADS / 64], n, lo, hi, found;
+        float room_f[THREADS / 64];
+        Powers<UNIT> powers;
+    };
+
+    const typename T::Raw *z;
+    uint32_t vocab;
+    Shared &s;
+    int tid;
+    float top;
+    double scale, until_min;  // bins of a unit of a logit, and to min_p
+    int dev_bits, shift;
+
+    __device__ __forceinline__ Bins(const typename T::Raw *z_, uint32_t vocab_, Shared &s_)
+        : z(z_), vocab(vocab_), s(s_), tid(threadIdx.x) {}
+
+    __device__ __forceinline__ Weights<UNIT> weights() const { return {s.powers, double(top), scale}; }
+    __device__ __forceinline__ double place(float x) const { return weights().place(x); }
+    __device__ __forceinline__ double weight_of(float x) const { return weights().of(x); }
+    __device__ __forceinline__ double begin_of(int bin) const { return weights().begin_of(bin); }
+    // A logit at or below every logit with place < `until`, and one at or above those with place >= `from`.
+    __device__ __forceinline__ float least(double until) const {
+        const double down = until / scale, x = double(top) - down - (fabs(double(top)) + down) * 0x1p-20;
+        return x > -double(FLT_MAX) ? float(x) : -FLT_MAX;
+    }
+    __device__ __forceinline__ float most(double from) const {
+        const double down = from / scale, x = double(top) - down + (fabs(double(top)) + down) * 0x1p-20;
+        return x < double(FLT_MAX) ? float(x) : FLT_MAX;
+    }
+
+    __device__ __forceinline__ void append(float x, uint32_t token) {
+        const uint32_t at = atomicAdd(&s.n, 1u);
+        if (at < uint32_t(MOST)) s.list[at] = uint64_t(order(x)) << 32 | uint32_t(~token);
+    }
+
+    // Ranks the first n of the list and makes their running sums.
+    __device__ __forceinline__ void rank(uint32_t n) {
+        if (n <= uint32_t(kCounted)) {  // four threads a token count those before it
+            const uint32_t i = tid / 4;
+            const uint64_t v = i < n ? s.list[i] : 0;
+            uint32_t before = 0;
+            if (i < n) {
+#pragma unroll 4
+                for (uint32_t j = tid % 4; j < n; j += 4) before += s.list[j] > v;
+            }
+            before += __shfl_xor(before, 1, 64);
+            before += __shfl_xor(before, 2, 64);
+            __syncthreads();
+            if (i < n && tid % 4 == 0) s.list[before] = v;
+            __syncthreads();
+        } else {
+            uint32_t size = 2 * kCounted;
+            while (size < n) size *= 2;
+            for (uint32_t i = n + tid; i < size; i += THREADS) s.list[i] = 0;
+            __syncthreads();
+            for (uint32_t k = 2; k <= size; k *= 2)
+                for (uint32_t j = k / 2; j > 0; j /= 2) {
+                    for (uint32_t i = tid; i < size / 2; i += THREADS) {
+                        const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
+                        const uint64_t x = s.list[a], y = s.list[b];
+                        if ((x < y) == ((a & k) == 0)) {
+                            s.list[a] = y;
+                            s.list[b] = x;
+                        }
+                    }
+                    // Pairs up to 64 apart are a wave's own: its LDS operations are in order.
+                    if (j > 64 || (j == 1 && k >= 128))
+                        __syncthreads();
+                    else
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                }
+            __syncthreads();
+        }
+        constexpr int E = MOST / THREADS;
+        double w[E], sum = 0.0, total;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t i = tid * E + e;
+            w[e] = i < n ? weight_of(unordered(uint32_t(s.list[i] >> 32))) : 0.0;
+            sum += w[e];
+        }
+        double run = block_scan<THREADS>(sum, s.room_d, total);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t i = tid * E + e;
+            run += w[e];
+            if (i < n) s.sums[i] = run;
+        }
+        __syncthreads();
+    }
+
+    // How many of the n ranked ones' running sums lie under t, or (up) do not exceed it.
+    __device__ __forceinline__ uint32_t below(uint32_t n, double t, bool up) {
+        uint32_t c = 0;
+        for (uint32_t i = tid; i < n; i += THREADS) c += up ? s.sums[i] <= t : s.sums[i] < t;
+        return block_total<THREADS>(c, s.room_u);
+    }
+
+    __device__ __forceinline__ void finish(const SampleArgs &a, size_t row, uint64_t v, double whole) {
+        if (tid == 0) write(a, row, ~uint32_t(v), float(log(weight_of(unordered(uint32_t(v >> 32))) / whole)));
+    }
+
+    // Draws from the n candidates of the list.
+    __device__ __forceinline__ void draw_few(const SampleArgs &a, size_t row, const Settings &set, uint32_t n) {
+        rank(n);
+        if (set.top_k) n = min(n, set.top_k);
+        if (set.with_p) n = min(n, below(n, set.top_p * s.sums[n - 1], false) + 1);
+        if (set.with_min) {
+            uint32_t c = 0;
+            for (uint32_t i = tid; i < n; i += THREADS)
+                c += weight_of(unordered(uint32_t(s.list[i] >> 32))) >= set.min_p;
+            n = max(1u, block_total<THREADS>(c, s.room_u));
+        }
+        const double whole = s.sums[n - 1];
+        finish(a, row, s.list[min(below(n, set.uniform * whole, true), n - 1)], whole);
+    }
+
+    // The bin of the k-th largest of the threads' maxima bounds the k-th largest logit
+    // from below; what lies past the last bin cannot be drawn.
+    __device__ __forceinline__ int bound_bin(float mine, uint32_t k) {
+        uint32_t *const counts = reinterpret_cast<uint32_t *>(s.bins);
+        for (int i = tid; i < BINS; i += THREADS) counts[i] = 0;
+        if (tid == 0) s.found = BINS - 1;
+        __syncthreads();
+        const double y = place(mine);
+        if (y < double(kReach * UNIT)) atomicAdd(&counts[int(y)], 1u);
+        __syncthreads();
+        uint32_t c[kEach], sum = 0, total;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum += c[e] = counts[tid * kEach + e];
+        uint32_t before = block_scan<THREADS>(sum, s.room_u, total);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (before < k && before + c[e] >= k) s.found = uint32_t(tid * kEach + e);
+            before += c[e];
+        }
+        __syncthreads();
+        return int(s.found);
+    }
+
+    // 1 for a token, and w / (w where the bin begins) - 1, r bins from there, in units of
+    // 2^-dev_bits, rounded by the addition of 1.5 * 2^52.
+    __device__ __forceinline__ uint64_t term(double r) const {
+        const double d = Weights<UNIT>::series(r, [&](double v) {
+            return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, v) + (uint64_t(dev_bits) << 52));
+        });
+        const double rounded = fma(r, d, 0x1.8p52);
+        return __builtin_bit_cast(uint64_t, rounded) + ((uint64_t(1) << shift) - __builtin_bit_cast(uint64_t, 0x1.8p52));
+    }
+    __device__ __forceinline__ void split(uint64_t h, double begin, uint32_t &tokens, double &weight) const {
+        const int64_t dev = int64_t(h << (64 - shift)) >> (64 - shift);
+        tokens = uint32_t((h - uint64_t(dev)) >> shift);
+        weight = begin * fma(double(dev), __builtin_bit_cast(double, uint64_t(1023 - dev_bits) << 52), double(tokens));
+    }
+    __device__ __forceinline__ void fill(uint32_t &all_c, double &all_w) {
+        // A bin's sum of `vocab` terms under 1 / UNIT stays in its field.
+        shift = 63 - (32 - __clz(int(vocab)));
+        dev_bits = min(37, 2 * shift - 64 + (31 - __builtin_clz(UNIT)));
+        for (int i = tid; i < BINS; i += THREADS) s.bins[i] = 0;
+        __syncthreads();
+        const float from = least(kReach * UNIT);
+        each_slowly<T, THREADS>(z, vocab, [&](float x) {
+            if (x < from) return;
+            const double y = place(x), at = floor(y);
+            if (y < kReach * UNIT)
+                atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(at)]),
+                          static_cast<unsigned long long>(term(y - at)));
+        });
+        __syncthreads();
+        double w = 0.0;
+        uint32_t c = 0;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            uint32_t tokens;
+            double weight;
+            split(s.bins[tid * kEach + e], begin_of(tid * kEach + e), tokens, weight);
+            w += weight;
+            c += tokens;
+        }
+        s.before[tid] = block_scan<THREADS>(w, s.room_d, all_w);
+        s.taken[tid] = block_scan<THREADS>(c, s.room_u, all_c);
+        __syncthreads();
+    }
+
+    // The first bin that `is` takes; there has to be one.
+    template <class Is>
+    __device__ __forceinline__ Bin find(Is &&is) {
+        Bin b{tid * kEach, s.taken[tid], 0, s.before[tid], 0.0};
+        bool mine = false;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (!mine) {
+                split(s.bins[b.at], begin_of(b.at), b.count, b.weight);
+                mine = is(b);
+            }
+            if (!mine) b = {b.at + 1, b.taken + b.count, 0, b.base + b.weight, 0.0};
+        }
+        const uint64_t those = __ballot(mine);
+        if (those == 0) {
+            if (tid % 64 == 0) s.found_by[tid / 64].at = BINS;
+        } else if (int(tid % 64) == __builtin_ctzll(those)) {
+            s.found_by[tid / 64] = b;
+        }
+        __syncthreads();
+        int w = 0;
+        while (w + 1 < THREADS / 64 && s.found_by[w].at == BINS) ++w;
+        b = s.found_by[w];
+        b.base = uniform(b.base);
+        b.weight = uniform(b.weight);
+        __syncthreads();
+        return b;
+    }
+
+    // The n-th token, from 0, whose logit has key k.
+    __device__ __forceinline__ uint32_t nth_of(uint32_t k, uint32_t n) {
+        const int lane = tid & 63;
+        const uint32_t share = (vocab + THREADS - 1) / THREADS * 64, from = min(vocab, (tid >> 6) * share),
+                       to = min(vocab, from + share);
+        uint32_t c = 0, total;
+        for (uint32_t i = from + lane; i < to; i += 64) c += order(T::to_float(z[i])) == k;
+        const uint32_t before = block_scan<THREADS>(c, s.room_u, total);
+        const uint32_t first = lane_value(before, 0), here = lane_value(before + c, 63) - first;
+        if (n >= first && n - first < here) {  // this wave has it
+            uint32_t left = n - first;
+            for (uint32_t i = from; i < to; i += 64) {
+                const bool is = i + lane < to && order(T::to_float(z[i + lane])) == k;
+                const uint64_t mask = __ballot(is);
+                const uint32_t step = uint32_t(__popcll(mask));
+                if (left < step) {
+                    if (is && uint32_t(__popcll(mask & ((uint64_t(1) << lane) - 1))) == left) s.found = i + lane;
+                    break;
+                }
+                left -= step;
+            }
+        }
+        __syncthreads();
+        return s.found;
+    }
+
+    // From the bins: one border after the other, then the token.
+    __device__ __forceinline__ void draw_bins(const SampleArgs &a, size_t row, const Settings &set) {
+        // What is left: the first `left` tokens, with the weight `whole`.
+        uint32_t left;
+        double whole;
+        fill(left, whole);
+        whole = uniform(whole);
+#pragma unroll 1
+        for (int ask = kCount; ask < kAsks; ++ask) {
+            // What depends on them alone is made where it is used, not kept in registers over the loop.
+            asm volatile("" : "+v"(tid), "+s"(z));
+            // The weight that is asked for, in all that is left or (kCount) its first tokens.
+            double t = 0.0;
+            if (ask == kCount) {
+                if (!set.top_k || set.top_k >= left) continue;
+                left = set.top_k;
+            } else if (ask == kReachP) {
+                if (!set.with_p) continue;
+                t = uniform(set.top_p * whole);
+            } else if (ask == kLeast) {
+                if (!set.with_min) continue;
+                // The bin of min_p, and its tokens from min_p on.
+                if (!(until_min < kReach * UNIT)) continue;
+                const int at = int(until_min);
+                const float from = least(double(at + 1)), to = most(double(at));
+                double w = 0.0;
+                uint32_t c = 0;
+                each_in<T, THREADS>(z, vocab, from, to, [&](float x, uint32_t) {
+                    const double o = place(x);
+                    if (o >= double(at) && o < double(at + 1)) {
+                        const double v = weight_of(x);
+                        if (v >= set.min_p) {
+                            w += v;
+                            ++c;
+                        }
+                    }
+                });
+                w = block_total<THREADS>(w, s.room_d);
+                c = block_total<THREADS>(c, s.room_u);
+                const Bin b = find([&](const Bin &o) { return o.at == at; });
+                if (b.taken + c < left) {
+                    left = b.taken + c;
+                    whole = uniform(b.base + w);
+                }
+                continue;
+            } else {
+                t = uniform(set.uniform * whole);
+            }
+            const Bin b = find([&](const Bin &o) {
+                return o.count && (o.taken + o.count >= left || (ask == kReachP ? o.base + o.weight >= t
+                                                                                : ask == kDraw && o.base + o.weight > t));
+            });
+            const uint32_t q = left - b.taken;  // tokens of the bin that are left, or more
+            // Inside the bin.
+            const double from = double(b.at), until = double(b.at + 1);
+            const float x_from = least(until), x_to = most(from);
+            double base = b.base;
+            uint32_t taken = 0, n = b.count;
+            uint32_t lo = 0, hi = 0;
+            bool ranked = n <= uint32_t(MOST);
+            if (ranked) {
+                if (tid == 0) s.n = 0;
+                __syncthreads();
+                each_in<T, THREADS>(z, vocab, x_from, x_to, [&](float x, uint32_t token) {
+                    const double y = place(x);
+                    if (y >= from && y < until) append(x, token);
+                });
+                __syncthreads();
+                n = min(s.n, uint32_t(MOST));
+            } else {
+                lo = 0xffffffffu;
+                each_in<T, THREADS>(z, vocab, x_from, x_to, [&](float x, uint32_t) {
+                    const double y = place(x);
+                    if (y >= from && y < until) {
+                        lo = min(lo, order(x));
+                        hi = max(hi, order(x));
+                    }
+                });
+                if (tid == 0) {
+                    s.lo = 0xffffffffu;
+                    s.hi = 0;
+                }
+                __syncthreads();
+                atomicMin(&s.lo, lo);
+                atomicMax(&s.hi, hi);
+                __syncthreads();
+                lo = s.lo;
+                hi = s.hi;
+                __syncthreads();
+            }
+            const double begin = begin_of(b.at);
+            while (!ranked && lo != hi) {
+                constexpr int kBits = 31 - __builtin_clz(THREADS);
+                const int step = max(0, 32 - __clz(int(hi - lo)) - kBits);  // (hi - lo) >> step < THREADS
+                s.fine[tid] = 0;
+                __syncthreads();
+                each_in<T, THREADS>(z, vocab, unordered(lo), unordered(hi), [&](float x, uint32_t) {
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&s.fine[(hi - order(x)) >> step]),
+                              static_cast<unsigned long long>(term(place(x) - from)));
+                });
+                if (tid == 0) {
+                    s.found = THREADS;
+                    s.n = 0;
+                }
+                __syncthreads();
+                uint32_t c, all_c;
+                double w, all_w;
+                split(s.fine[tid], begin, c, w);
+                const double before_w = base + block_scan<THREADS>(w, s.room_d, all_w);
+                const uint32_t before_c = taken + block_scan<THREADS>(c, s.room_u, all_c);
+                if (c) {
+                    atomicMax(&s.n, uint32_t(tid));
+                    if (before_c + c >= q || (ask == kReachP ? before_w + w >= t : ask == kDraw && before_w + w > t))
+                        atomicMin(&s.found, uint32_t(tid));
+                }
+                __syncthreads();
+                const uint32_t sub = s.found < uint32_t(THREADS) ? s.found : s.n;
+                __syncthreads();
+                if (sub == uint32_t(tid)) {
+                    s.base = before_w;
+                    s.lo = before_c;
+                    s.hi = c;
+                }
+                __syncthreads();
+                base = uniform(s.base);
+                taken = s.lo;
+                n = s.hi;
+                hi -= sub << step;
+                const uint32_t span = (uint32_t(1) << step) - 1;
+                if (hi - lo > span) lo = hi - span;
+                ranked = n <= uint32_t(MOST);
+                if (ranked) {
+                    if (tid == 0) s.n = 0;
+                    __syncthreads();
+                    each_in<T, THREADS>(z, vocab, unordered(lo), unordered(hi),
+                                        [&](float x, uint32_t token) { append(x, token); });
+                }
+                __syncthreads();
+            }
+            if (ranked) {
+                rank(n);
+                if (ask == kDraw) {
+                    finish(a, row, s.list[min(below(n, t - base, true), min(n, q - taken) - 1)], whole);
+                    return;
+                }
+                const uint32_t c = ask == kCount ? min(n, q - taken) : min(min(n, q - taken), below(n, t - base, false) + 1);
+                left = b.taken + taken + c;
+                whole = uniform(base + s.sums[c - 1]);
+                __syncthreads();
+            } else {  // equal logits, in the order of their tokens
+                const double w = weight_of(unordered(lo));
+                n = min(n, q - taken);
+                if (ask == kDraw) {
+                    const uint32_t token = nth_of(lo, equal_draw(t - base, w, n));
+                    if (tid == 0) write(a, row, token, float(log(w / whole)));
+                    return;
+                }
+                const uint32_t c = ask == kCount ? n : equal_reach(t - base, w, n);
+                left = b.taken + taken + c;
+                whole = uniform(base + double(c) * w);
+            }
+        }
+    }
+};
+
+// Rows of which few tokens are left before any weight is summed.
+__device__ __forceinline__ bool left_few(const Settings &set, int threads) {
+    return (set.top_k && set.top_k <= uint32_t(threads / 2)) || (set.with_min && !set.with_p);
+}
+
+template <class T, int THREADS, int UNIT, int MOST>
+__device__ __forceinline__ void sample_by_bins(const SampleArgs &a, size_t row, const Settings &set,
+                                               typename Bins<T, THREADS, UNIT, MOST>::Shared &s) {
+    using B = Bins<T, THREADS, UNIT, MOST>;
+    B b(static_cast<const typename T::Raw *>(a.logits) + row * a.stride, uint32_t(a.vocab), s);
+    b.until_min = uniform(set.with_min ? -log(set.min_p) * UNIT : 0.0);
+    Weights<UNIT>::prepare(s.powers);
+    float mine = -INFINITY;
+    bool bad = false;
+    each<T, THREADS>(b.z, b.vocab, [&](float x) {
+        mine = fmaxf(mine, x);
+        bad |= !(x < INFINITY);
+    });
+    const float wave_top = wave_largest(mine);
+    const bool wave_bad = __ballot(bad) != 0;
+    if (b.tid % 64 == 0) {
+        s.room_f[b.tid / 64] = wave_top;
+        s.room_u[b.tid / 64] = wave_bad;
+    }
+    if (b.tid == 0) {
+        s.n = 0;
+        s.found = kNoToken;
+    }
+    __syncthreads();
+    b.top = -INFINITY;
+    uint32_t any_bad = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        b.top = fmaxf(b.top, s.room_f[w]);
+        any_bad |= s.room_u[w];
+    }
+    b.top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(uint32_t, b.top)));
+    if (any_bad || b.top == -INFINITY || !set.valid) {
+        if (b.tid == 0) write(a, row, kNoToken, NAN);
+        return;
+    }
+    if (set.greedy) {
+        uint32_t first = kNoToken;
+        each_in<T, THREADS>(b.z, b.vocab, b.top, b.top, [&](float, uint32_t token) { first = min(first, token); });
+        if (first != kNoToken) atomicMin(&s.found, first);
+        __syncthreads();
+        if (b.tid == 0) write(a, row, s.found, 0.0f);
+        return;
+    }
+    b.scale = uniform(UNIT / set.temperature);
+    if (left_few(set, THREADS)) {
+        const bool by_k = set.top_k && set.top_k <= uint32_t(THREADS / 2);
+        const float from = by_k ? b.least(double(b.bound_bin(mine, set.top_k) + 1)) : b.least(b.until_min);
+        each_in<T, THREADS>(b.z, b.vocab, from, FLT_MAX, [&](float x, uint32_t token) { b.append(x, token); });
+        __syncthreads();
+        const uint32_t n = s.n;
+        if (n <= uint32_t(MOST)) return b.draw_few(a, row, set, n);
+        __syncthreads();
+    }
+    b.draw_bins(a, row, set);
+}
+
+template <class T, int THREADS, int UNIT, int MOST>
+__global__ void __launch_bounds__(THREADS) sample_bins_kernel(SampleArgs a) {
+    __shared__ typename Bins<T, THREADS, UNIT, MOST>::Shared s;
+    const size_t row = blockIdx.x;
+    sample_by_bins<T, THREADS, UNIT, MOST>(a, row, settings_of(a, row), s);
 }
 
 // ---- rows of 16 bits ------------------------------------------------------------------
@@ -363,12 +876,12 @@ __global__ void __launch_bounds__(kShortThreads) sample_short_kernel(SampleArgs 
 // and counted apart in a second pass.
 constexpr int kCodeThreads = 1024;
 constexpr int kCodeGroups = 16;  // of 8 logits a thread
-constexpr uint32_t kCodeMost = 131071;
+constexpr uint32_t kCodeLeast = 32769, kCodeMost = 131071;
 static_assert(kCodeMost < kCodeThreads * kCodeGroups * 8, "a row fits the registers");
 
 template <class T>
 struct Codes {
-    static constexpr int THREADS = kCodeThreads, WAVES = THREADS / 64, GROUPS = kCodeGroups;
+    static constexpr int kUnit = 128, THREADS = kCodeThreads, WAVES = THREADS / 64, GROUPS = kCodeGroups;
     static constexpr uint32_t kInf = std::is_same<T, F16>::value ? 0x7c00 : 0x7f80, kNegative = 0x8000 | kInf;
 
     struct Part {
@@ -379,7 +892,7 @@ struct Codes {
         uint32_t counts[32768 + THREADS];  // of a code and its negative; then of the code counted apart, a word a thread
         uint32_t in_segment[THREADS];
         double weights[THREADS];
-        Powers powers;
+        Powers<kUnit> powers;
         double room_d[WAVES];
         uint32_t room_u[WAVES];
         uint32_t bits[16];
@@ -389,7 +902,7 @@ struct Codes {
     Shared &s;
     uint32_t tid, lane, wave, each;
     uint32_t hot, hot_count;  // counted apart
-    Weights weights;
+    Weights<kUnit> weights;
 
     static __device__ __forceinline__ uint32_t code_at(uint32_t q) { return q < 0x8000 ? 0x7fff - q : q; }
     static __device__ __forceinline__ uint32_t segment_of(uint32_t code) { return (code < 0x8000 ? 0x7fff - code : code) / 64; }
@@ -491,8 +1004,16 @@ template <class T>
 __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a) {
     using C = Codes<T>;
     using Raw = typename T::Raw;
-    __shared__ typename C::Shared s;
+    using Few = typename Bins<T, kCodeThreads, 128, 2048>::Shared;
+    __shared__ union {
+        typename C::Shared codes;
+        Few bins;
+    } room;
     const size_t row = blockIdx.x;
+    const Settings set = settings_of(a, row);
+    // These want only the largest logit and the few next to it.
+    if (set.greedy || left_few(set, kCodeThreads)) return sample_by_bins<T, kCodeThreads, 128, 2048>(a, row, set, room.bins);
+    typename C::Shared &s = room.codes;
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64, vocab = uint32_t(a.vocab);
     const Raw *const z = static_cast<const Raw *>(a.logits) + row * a.stride;
     // A wave has `each` times 64 groups in a row, and a lane every 64th of them.
@@ -506,9 +1027,8 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
             w[j] |= group(j) < groups ? 0 : 0x7fff7fffu;  // NaN, which no token that is drawn is
         }
     const uint32_t last = tid < tail ? uint32_t(__builtin_bit_cast(uint16_t, z[groups * 8 + tid])) : 0;
-    const Settings set = settings_of(a, row);
-    Weights::prepare(s.powers);
-    C c{s, tid, lane, wave, each, 0, 0, {s.powers, 0.0, set.greedy ? 1.0 : uniform(kPerUnit / set.temperature)}};
+    Weights<C::kUnit>::prepare(s.powers);
+    C c{s, tid, lane, wave, each, 0, 0, {s.powers, 0.0, set.greedy ? 1.0 : uniform(C::kUnit / set.temperature)}};
     c.hot = sampled_code(c, w);
     uint32_t mine;  // tokens of a thread's segment, without those of -inf
 #pragma unroll 1
@@ -722,506 +1242,27 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
     write(a, row, token, float(log(share)));
 }
 
-// ---- the general way -----------------------------------------------------------------
-
-// The row's largest logit; then either few candidates (top_k bounds them by the
-// k-th largest of the threads' maxima, min_p by itself), which are gathered and
-// ranked, or bins of (max z - z) / T, 128 for each power of e. A bin keeps its
-// tokens' count and the fixed-point sum of w / (w where it begins) - 1 in one LDS
-// word, exact to 2^-35 of a weight and the same in any order.  Where a border falls
-// into a bin, its tokens are gathered and ranked; if they are more than MOST, the
-// bin is divided by the bits of their logits until they are few enough or equal.
-enum Ask { kCount, kReachP, kLeast, kDraw, kAsks };
-
-template <class T, int THREADS, int BINS, int MOST>
-struct Bins {
-    static constexpr int kEach = BINS / THREADS;
-    static_assert(BINS == 32 * kPerUnit && BINS > kReach * kPerUnit && BINS % THREADS == 0 && MOST % THREADS == 0, "every place has a bin");
-    static constexpr int kCounted = THREADS / 4;  // up to so many are ranked by counting
-
-    struct Bin {
-        int at;
-        uint32_t taken, count;  // tokens before it and in it
-        double base, weight;    // weights before it and in it
-    };
-    struct Shared {
-        uint64_t bins[BINS], fine[THREADS], list[MOST];
-        double sums[MOST];
-        double before[THREADS];   // weights before a thread's bins
-        uint32_t taken[THREADS];  // and tokens
-        double room_d[THREADS / 64], base;
-        Bin found_by[THREADS / 64];
-        uint32_t room_u[THREADS / 64], n, lo, hi, found;
-        float room_f[THREADS / 64];
-        Powers powers;
-    };
-
-    const typename T::Raw *z;
-    uint32_t vocab;
-    Shared &s;
-    int tid;
-    float top;
-    double scale, until_min;  // bins of a unit of a logit, and to min_p
-    int dev_bits, shift;
-
-    __device__ __forceinline__ Bins(const typename T::Raw *z_, uint32_t vocab_, Shared &s_)
-        : z(z_), vocab(vocab_), s(s_), tid(threadIdx.x) {}
-
-    __device__ __forceinline__ Weights weights() const { return {s.powers, double(top), scale}; }
-    __device__ __forceinline__ double place(float x) const { return weights().place(x); }
-    __device__ __forceinline__ double weight_of(float x) const { return weights().of(x); }
-    __device__ __forceinline__ double begin_of(int bin) const { return weights().begin_of(bin); }
-    // A logit at or below every logit with place < `until`, and one at or above those with place >= `from`.
-    __device__ __forceinline__ float least(double until) const {
-        const double down = until / scale, x = double(top) - down - (fabs(double(top)) + down) * 0x1p-20;
-        return x > -double(FLT_MAX) ? float(x) : -FLT_MAX;
-    }
-    __device__ __forceinline__ float most(double from) const {
-        const double down = from / scale, x = double(top) - down + (fabs(double(top)) + down) * 0x1p-20;
-        return x < double(FLT_MAX) ? float(x) : FLT_MAX;
-    }
-
-    __device__ __forceinline__ void append(float x, uint32_t token) {
-        const uint32_t at = atomicAdd(&s.n, 1u);
-        if (at < uint32_t(MOST)) s.list[at] = uint64_t(order(x)) << 32 | uint32_t(~token);
-    }
-
-    // Ranks the first n of the list and makes their running sums.
-    __device__ __forceinline__ void rank(uint32_t n) {
-        if (n <= uint32_t(kCounted)) {  // four threads a token count those before it
-            const uint32_t i = tid / 4;
-            const uint64_t v = i < n ? s.list[i] : 0;
-            uint32_t before = 0;
-            if (i < n) {
-#pragma unroll 4
-                for (uint32_t j = tid % 4; j < n; j += 4) before += s.list[j] > v;
-            }
-            before += __shfl_xor(before, 1, 64);
-            before += __shfl_xor(before, 2, 64);
-            __syncthreads();
-            if (i < n && tid % 4 == 0) s.list[before] = v;
-            __syncthreads();
-        } else {
-            uint32_t size = 2 * kCounted;
-            while (size < n) size *= 2;
-            for (uint32_t i = n + tid; i < size; i += THREADS) s.list[i] = 0;
-            __syncthreads();
-            for (uint32_t k = 2; k <= size; k *= 2)
-                for (uint32_t j = k / 2; j > 0; j /= 2) {
-                    for (uint32_t i = tid; i < size / 2; i += THREADS) {
-                        const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
-                        const uint64_t x = s.list[a], y = s.list[b];
-                        if ((x < y) == ((a & k) == 0)) {
-                            s.list[a] = y;
-                            s.list[b] = x;
-                        }
-                    }
-                    // Pairs up to 64 apart are a wave's own: its LDS operations are in order.
-                    if (j > 64 || (j == 1 && k >= 128))
-                        __syncthreads();
-                    else
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                }
-            __syncthreads();
-        }
-        constexpr int E = MOST / THREADS;
-        double w[E], sum = 0.0, total;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t i = tid * E + e;
-            w[e] = i < n ? weight_of(unordered(uint32_t(s.list[i] >> 32))) : 0.0;
-            sum += w[e];
-        }
-        double run = block_scan<THREADS>(sum, s.room_d, total);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t i = tid * E + e;
-            run += w[e];
-            if (i < n) s.sums[i] = run;
-        }
-        __syncthreads();
-    }
-
-    // How many of the n ranked ones' running sums lie under t, or (up) do not exceed it.
-    __device__ __forceinline__ uint32_t below(uint32_t n, double t, bool up) {
-        uint32_t c = 0;
-        for (uint32_t i = tid; i < n; i += THREADS) c += up ? s.sums[i] <= t : s.sums[i] < t;
-        return block_total<THREADS>(c, s.room_u);
-    }
-
-    __device__ __forceinline__ void finish(const SampleArgs &a, size_t row, uint64_t v, double whole) {
-        if (tid == 0) write(a, row, ~uint32_t(v), float(log(weight_of(unordered(uint32_t(v >> 32))) / whole)));
-    }
-
-    // Draws from the n candidates of the list.
-    __device__ __forceinline__ void draw_few(const SampleArgs &a, size_t row, const Settings &set, uint32_t n) {
-        rank(n);
-        if (set.top_k) n = min(n, set.top_k);
-        if (set.with_p) n = min(n, below(n, set.top_p * s.sums[n - 1], false) + 1);
-        if (set.with_min) {
-            uint32_t c = 0;
-            for (uint32_t i = tid; i < n; i += THREADS)
-                c += weight_of(unordered(uint32_t(s.list[i] >> 32))) >= set.min_p;
-            n = max(1u, block_total<THREADS>(c, s.room_u));
-        }
-        const double whole = s.sums[n - 1];
-        finish(a, row, s.list[min(below(n, set.uniform * whole, true), n - 1)], whole);
-    }
-
-    // The bin of the k-th largest of the threads' maxima bounds the k-th largest logit
-    // from below; what lies past the last bin cannot be drawn.
-    __device__ __forceinline__ int bound_bin(float mine, uint32_t k) {
-        uint32_t *const counts = reinterpret_cast<uint32_t *>(s.bins);
-        for (int i = tid; i < BINS; i += THREADS) counts[i] = 0;
-        if (tid == 0) s.found = BINS - 1;
-        __syncthreads();
-        const double y = place(mine);
-        if (y < double(kReach * kPerUnit)) atomicAdd(&counts[int(y)], 1u);
-        __syncthreads();
-        uint32_t c[kEach], sum = 0, total;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) sum += c[e] = counts[tid * kEach + e];
-        uint32_t before = block_scan<THREADS>(sum, s.room_u, total);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            if (before < k && before + c[e] >= k) s.found = uint32_t(tid * kEach + e);
-            before += c[e];
-        }
-        __syncthreads();
-        return int(s.found);
-    }
-
-    // 1 for a token, and w / (w where the bin begins) - 1, r bins from there: the series of
-    // Weights::rest in units of 2^-dev_bits, rounded by the addition of 1.5 * 2^52.
-    __device__ __forceinline__ uint64_t term(double r) const {
-        const auto units = [&](double v) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, v) + (uint64_t(dev_bits) << 52)); };
-        const double d = fma(r, fma(r, fma(r, units(0x1p-28 / 24), units(-0x1p-21 / 6)), units(0x1p-14 / 2)), units(-0x1p-7));
-        const double rounded = fma(r, d, 0x1.8p52);
-        return __builtin_bit_cast(uint64_t, rounded) + ((uint64_t(1) << shift) - __builtin_bit_cast(uint64_t, 0x1.8p52));
-    }
-    __device__ __forceinline__ void split(uint64_t h, double begin, uint32_t &tokens, double &weight) const {
-        const int64_t dev = int64_t(h << (64 - shift)) >> (64 - shift);
-        tokens = uint32_t((h - uint64_t(dev)) >> shift);
-        weight = begin * fma(double(dev), __builtin_bit_cast(double, uint64_t(1023 - dev_bits) << 52), double(tokens));
-    }
-    __device__ __forceinline__ void fill(uint32_t &all_c, double &all_w) {
-        // A bin's sum of `vocab` terms under 0.0079 stays in its field.
-        shift = 63 - (32 - __clz(int(vocab)));
-        dev_bits = min(37, 2 * shift - 57);
-        for (int i = tid; i < BINS; i += THREADS) s.bins[i] = 0;
-        __syncthreads();
-        const float from = least(kReach * kPerUnit);
-        each_slowly<T, THREADS>(z, vocab, [&](float x) {
-            if (x < from) return;
-            const double y = place(x), at = floor(y);
-            if (y < kReach * kPerUnit)
-                atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(at)]),
-                          static_cast<unsigned long long>(term(y - at)));
-        });
-        __syncthreads();
-        double w = 0.0;
-        uint32_t c = 0;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            uint32_t tokens;
-            double weight;
-            split(s.bins[tid * kEach + e], begin_of(tid * kEach + e), tokens, weight);
-            w += weight;
-            c += tokens;
-        }
-        s.before[tid] = block_scan<THREADS>(w, s.room_d, all_w);
-        s.taken[tid] = block_scan<THREADS>(c, s.room_u, all_c);
-        __syncthreads();
-    }
-
-    // The first bin that `is` takes; there has to be one.
-    template <class Is>
-    __device__ __forceinline__ Bin find(Is &&is) {
-        Bin b{tid * kEach, s.taken[tid], 0, s.before[tid], 0.0};
-        bool mine = false;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            if (!mine) {
-                split(s.bins[b.at], begin_of(b.at), b.count, b.weight);
-                mine = is(b);
-            }
-            if (!mine) b = {b.at + 1, b.taken + b.count, 0, b.base + b.weight, 0.0};
-        }
-        const uint64_t those = __ballot(mine);
-        if (those == 0) {
-            if (tid % 64 == 0) s.found_by[tid / 64].at = BINS;
-        } else if (int(tid % 64) == __builtin_ctzll(those)) {
-            s.found_by[tid / 64] = b;
-        }
-        __syncthreads();
-        int w = 0;
-        while (w + 1 < THREADS / 64 && s.found_by[w].at == BINS) ++w;
-        b = s.found_by[w];
-        b.base = uniform(b.base);
-        b.weight = uniform(b.weight);
-        __syncthreads();
-        return b;
-    }
-
-    // The n-th token, from 0, whose logit has key k.
-    __device__ __forceinline__ uint32_t nth_of(uint32_t k, uint32_t n) {
-        const int lane = tid & 63;
-        const uint32_t share = (vocab + THREADS - 1) / THREADS * 64, from = min(vocab, (tid >> 6) * share),
-                       to = min(vocab, from + share);
-        uint32_t c = 0, total;
-        for (uint32_t i = from + lane; i < to; i += 64) c += order(T::to_float(z[i])) == k;
-        const uint32_t before = block_scan<THREADS>(c, s.room_u, total);
-        const uint32_t first = lane_value(before, 0), here = lane_value(before + c, 63) - first;
-        if (n >= first && n - first < here) {  // this wave has it
-            uint32_t left = n - first;
-            for (uint32_t i = from; i < to; i += 64) {
-                const bool is = i + lane < to && order(T::to_float(z[i + lane])) == k;
-                const uint64_t mask = __ballot(is);
-                const uint32_t step = uint32_t(__popcll(mask));
-                if (left < step) {
-                    if (is && uint32_t(__popcll(mask & ((uint64_t(1) << lane) - 1))) == left) s.found = i + lane;
-                    break;
-                }
-                left -= step;
-            }
-        }
-        __syncthreads();
-        return s.found;
-    }
-
-    // From the bins: one border after the other, then the token.
-    __device__ __forceinline__ void draw_bins(const SampleArgs &a, size_t row, const Settings &set) {
-        // What is left: the first `left` tokens, with the weight `whole`.
-        uint32_t left;
-        double whole;
-        fill(left, whole);
-        whole = uniform(whole);
-#pragma unroll 1
-        for (int ask = kCount; ask < kAsks; ++ask) {
-            // What depends on them alone is made where it is used, not kept in registers over the loop.
-            asm volatile("" : "+v"(tid), "+s"(z));
-            // The weight that is asked for, in all that is left or (kCount) its first tokens.
-            double t = 0.0;
-            if (ask == kCount) {
-                if (!set.top_k || set.top_k >= left) continue;
-                left = set.top_k;
-            } else if (ask == kReachP) {
-                if (!set.with_p) continue;
-                t = uniform(set.top_p * whole);
-            } else if (ask == kLeast) {
-                if (!set.with_min) continue;
-                // The bin of min_p, and its tokens from min_p on.
-                if (!(until_min < kReach * kPerUnit)) continue;
-                const int at = int(until_min);
-                const float from = least(double(at + 1)), to = most(double(at));
-                double w = 0.0;
-                uint32_t c = 0;
-                each_in<T, THREADS>(z, vocab, from, to, [&](float x, uint32_t) {
-                    const double o = place(x);
-                    if (o >= double(at) && o < double(at + 1)) {
-                        const double v = weight_of(x);
-                        if (v >= set.min_p) {
-                            w += v;
-                            ++c;
-                        }
-                    }
-                });
-                w = block_total<THREADS>(w, s.room_d);
-                c = block_total<THREADS>(c, s.room_u);
-                const Bin b = find([&](const Bin &o) { return o.at == at; });
-                if (b.taken + c < left) {
-                    left = b.taken + c;
-                    whole = uniform(b.base + w);
-                }
-                continue;
-            } else {
-                t = uniform(set.uniform * whole);
-            }
-            const Bin b = find([&](const Bin &o) {
-                return o.count && (o.taken + o.count >= left || (ask == kReachP ? o.base + o.weight >= t
-                                                                                : ask == kDraw && o.base + o.weight > t));
-            });
-            const uint32_t q = left - b.taken;  // tokens of the bin that are left, or more
-            // Inside the bin.
-            const double from = double(b.at), until = double(b.at + 1);
-            const float x_from = least(until), x_to = most(from);
-            double base = b.base;
-            uint32_t taken = 0, n = b.count;
-            uint32_t lo = 0, hi = 0;
-            bool ranked = n <= uint32_t(MOST);
-            if (ranked) {
-                if (tid == 0) s.n = 0;
-                __syncthreads();
-                each_in<T, THREADS>(z, vocab, x_from, x_to, [&](float x, uint32_t token) {
-                    const double y = place(x);
-                    if (y >= from && y < until) append(x, token);
-                });
-                __syncthreads();
-                n = min(s.n, uint32_t(MOST));
-            } else {
-                lo = 0xffffffffu;
-                each_in<T, THREADS>(z, vocab, x_from, x_to, [&](float x, uint32_t) {
-                    const double y = place(x);
-                    if (y >= from && y < until) {
-                        lo = min(lo, order(x));
-                        hi = max(hi, order(x));
-                    }
-                });
-                if (tid == 0) {
-                    s.lo = 0xffffffffu;
-                    s.hi = 0;
-                }
-                __syncthreads();
-                atomicMin(&s.lo, lo);
-                atomicMax(&s.hi, hi);
-                __syncthreads();
-                lo = s.lo;
-                hi = s.hi;
-                __syncthreads();
-            }
-            const double begin = begin_of(b.at);
-            while (!ranked && lo != hi) {
-                constexpr int kBits = 31 - __builtin_clz(THREADS);
-                const int step = max(0, 32 - __clz(int(hi - lo)) - kBits);  // (hi - lo) >> step < THREADS
-                s.fine[tid] = 0;
-                __syncthreads();
-                each_in<T, THREADS>(z, vocab, unordered(lo), unordered(hi), [&](float x, uint32_t) {
-                    atomicAdd(reinterpret_cast<unsigned long long *>(&s.fine[(hi - order(x)) >> step]),
-                              static_cast<unsigned long long>(term(place(x) - from)));
-                });
-                if (tid == 0) {
-                    s.found = THREADS;
-                    s.n = 0;
-                }
-                __syncthreads();
-                uint32_t c, all_c;
-                double w, all_w;
-                split(s.fine[tid], begin, c, w);
-                const double before_w = base + block_scan<THREADS>(w, s.room_d, all_w);
-                const uint32_t before_c = taken + block_scan<THREADS>(c, s.room_u, all_c);
-                if (c) {
-                    atomicMax(&s.n, uint32_t(tid));
-                    if (before_c + c >= q || (ask == kReachP ? before_w + w >= t : ask == kDraw && before_w + w > t))
-                        atomicMin(&s.found, uint32_t(tid));
-                }
-                __syncthreads();
-                const uint32_t sub = s.found < uint32_t(THREADS) ? s.found : s.n;
-                __syncthreads();
-                if (sub == uint32_t(tid)) {
-                    s.base = before_w;
-                    s.lo = before_c;
-                    s.hi = c;
-                }
-                __syncthreads();
-                base = uniform(s.base);
-                taken = s.lo;
-                n = s.hi;
-                hi -= sub << step;
-                const uint32_t span = (uint32_t(1) << step) - 1;
-                if (hi - lo > span) lo = hi - span;
-                ranked = n <= uint32_t(MOST);
-                if (ranked) {
-                    if (tid == 0) s.n = 0;
-                    __syncthreads();
-                    each_in<T, THREADS>(z, vocab, unordered(lo), unordered(hi),
-                                        [&](float x, uint32_t token) { append(x, token); });
-                }
-                __syncthreads();
-            }
-            if (ranked) {
-                rank(n);
-                if (ask == kDraw) {
-                    finish(a, row, s.list[min(below(n, t - base, true), min(n, q - taken) - 1)], whole);
-                    return;
-                }
-                const uint32_t c = ask == kCount ? min(n, q - taken) : min(min(n, q - taken), below(n, t - base, false) + 1);
-                left = b.taken + taken + c;
-                whole = uniform(base + s.sums[c - 1]);
-                __syncthreads();
-            } else {  // equal logits, in the order of their tokens
-                const double w = weight_of(unordered(lo));
-                n = min(n, q - taken);
-                if (ask == kDraw) {
-                    const uint32_t token = nth_of(lo, equal_draw(t - base, w, n));
-                    if (tid == 0) write(a, row, token, float(log(w / whole)));
-                    return;
-                }
-                const uint32_t c = ask == kCount ? n : equal_reach(t - base, w, n);
-                left = b.taken + taken + c;
-                whole = uniform(base + double(c) * w);
-            }
-        }
-    }
-};
-
-template <class T, int THREADS, int BINS, int MOST>
-__global__ void __launch_bounds__(THREADS) sample_bins_kernel(SampleArgs a) {
-    using B = Bins<T, THREADS, BINS, MOST>;
-    __shared__ typename B::Shared s;
-    const size_t row = blockIdx.x;
-    B b(static_cast<const typename T::Raw *>(a.logits) + row * a.stride, uint32_t(a.vocab), s);
-    const Settings set = settings_of(a, row);
-    b.until_min = uniform(set.with_min ? -log(set.min_p) * kPerUnit : 0.0);
-    Weights::prepare(s.powers);
-    float mine = -INFINITY;
-    bool bad = false;
-    each<T, THREADS>(b.z, b.vocab, [&](float x) {
-        mine = fmaxf(mine, x);
-        bad |= !(x < INFINITY);
-    });
-    const float wave_top = wave_largest(mine);
-    const bool wave_bad = __ballot(bad) != 0;
-    if (b.tid % 64 == 0) {
-        s.room_f[b.tid / 64] = wave_top;
-        s.room_u[b.tid / 64] = wave_bad;
-    }
-    if (b.tid == 0) {
-        s.n = 0;
-        s.found = kNoToken;
-    }
-    __syncthreads();
-    b.top = -INFINITY;
-    uint32_t any_bad = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-        b.top = fmaxf(b.top, s.room_f[w]);
-        any_bad |= s.room_u[w];
-    }
-    b.top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(uint32_t, b.top)));
-    if (any_bad || b.top == -INFINITY || !set.valid) {
-        if (b.tid == 0) write(a, row, kNoToken, NAN);
-        return;
-    }
-    if (set.greedy) {
-        uint32_t first = kNoToken;
-        each_in<T, THREADS>(b.z, b.vocab, b.top, b.top, [&](float, uint32_t token) { first = min(first, token); });
-        if (first != kNoToken) atomicMin(&s.found, first);
-        __syncthreads();
-        if (b.tid == 0) write(a, row, s.found, 0.0f);
-        return;
-    }
-    b.scale = uniform(kPerUnit / set.temperature);
-    const bool by_k = set.top_k && set.top_k <= uint32_t(THREADS / 2);
-    if (by_k || (set.with_min && !set.with_p)) {
-        const float from = by_k ? b.least(double(b.bound_bin(mine, set.top_k) + 1)) : b.least(b.until_min);
-        each_in<T, THREADS>(b.z, b.vocab, from, FLT_MAX, [&](float x, uint32_t token) { b.append(x, token); });
-        __syncthreads();
-        const uint32_t n = s.n;
-        if (n <= uint32_t(MOST)) return b.draw_few(a, row, set, n);
-        __syncthreads();
-    }
-    b.draw_bins(a, row, set);
-}
-
+// What bounds short rows is the barriers and scans that a row takes, which wait less with
+// fewer waves; with bins of 1 / 32 each of 256 threads has four.  Measured, BF16 and top_p, in
+// us, with 256 threads and 512: 1024 rows of 300 19 and 43, of 4000 28 and 48, of 8000 38 and
+// 53, of 16000 54 and 58; 256 rows of 4000 16 and 19, of 8000 28 and 20.  With 512 and 1024:
+// 1024 rows of 30000 75 and 95, 256 of them 30 and 26.  Counting by value has a fixed part:
+// 256 rows of 16000 23 where 512 threads take 22, of 50000 29 where 1024 threads and bins
+// take 36, of 128000 42 and 78.
 template <class T>
 void launch(const SampleArgs &a, hipStream_t stream) {
     const dim3 rows(static_cast<unsigned>(a.rows));
-    if (a.vocab <= size_t(kShort))
-        sample_short_kernel<T><<<rows, kShortThreads, 0, stream>>>(a);
-    else if (a.vocab <= 8192)
-        sample_bins_kernel<T, 512, 4096, 1024><<<rows, 512, 0, stream>>>(a);
-    else if (sizeof(typename T::Raw) == 4 || a.vocab > size_t(kCodeMost))
-        sample_bins_kernel<T, 1024, 4096, 2048><<<rows, 1024, 0, stream>>>(a);
+    const bool many = a.rows > 512;  // workgroups share the CUs
+    if (a.vocab <= 64)
+        sample_short_kernel<T, 64><<<rows, 256, 0, stream>>>(a);
+    else if (a.vocab <= 256)
+        sample_short_kernel<T, 256><<<rows, 1024, 0, stream>>>(a);
+    else if (a.vocab <= (many ? 8192 : 4096))
+        sample_bins_kernel<T, 256, 32, 1024><<<rows, 256, 0, stream>>>(a);
+    else if (a.vocab <= (many ? 32768 : 16384))
+        sample_bins_kernel<T, 512, 128, 1024><<<rows, 512, 0, stream>>>(a);
+    else if (sizeof(typename T::Raw) == 4 || a.vocab < kCodeLeast || a.vocab > kCodeMost)
+        sample_bins_kernel<T, 1024, 128, 2048><<<rows, 1024, 0, stream>>>(a);
     else if constexpr (sizeof(typename T::Raw) == 2)
         sample_codes_kernel<T><<<rows, kCodeThreads, 0, stream>>>(a);
 }

@@ -13,7 +13,7 @@ void sample_filtered_noalloc(int device, Type type, const void *logits, size_t r
                              const float *temperatures, const int *top_k, const float *top_p, const float *min_p,
                              const float *uniforms, uint32_t *tokens, float *logprob, hipStream_t stream) {
     check_type(type);
-    require(vocab >= 1 && vocab <= size_t(1) << 24, "vocabulary must hold 1..2^24 tokens");
+    require(vocab >= 1 && vocab <= size_t(1) << 20, "vocabulary must hold 1..2^20 tokens");  // sums have 64 bits
     require(stride >= vocab, "the row stride must be at least the vocabulary");
     require(rows < size_t(1) << 22, "rows must stay below 2^22");  // of 1024 threads each, counted in 32 bits
     if (rows == 0) return;

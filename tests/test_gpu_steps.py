@@ -84,8 +84,68 @@ def test_tokens_are_those_of_the_formulas(kind, vocab):
             check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, stride=vocab + i % 3, **kw))
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("vocab", [32768, 32769, 65537, 131064, 131071, 131072])
+def test_long_rows_of_16_bits(kind, vocab):
+    rng = np.random.default_rng(vocab)
+    rows = 6
+    z = rng.normal(size=(rows, vocab)) * np.array([[0.01], [1.0], [2.0], [8.0], [1.0], [2.0]])
+    z[1, rng.random(vocab) < 0.7] = -np.inf
+    z[4, rng.random(vocab) < 0.9] = -65504.0  # a mask's value
+    z[5, rng.random(vocab) < 0.3] = -0.0
+    u = rng.random(rows, dtype=np.float32)
+    with L.Device() as dev:
+        for i, kw in enumerate(SETTINGS):
+            kw = {k: setting(rng, rows, v) for k, v in kw.items()}
+            check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, stride=vocab + i % 3, **kw))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("most", [3.0, 0.0, -0.5, -1000.0, -np.inf])
+@pytest.mark.parametrize("vocab", [100003, 131071])
+def test_one_value_in_most_of_a_long_row(kind, most, vocab):
+    """Seven of eight tokens; in the second row the eighth is each one whose place in
+    its group of eight is that of the group in eight groups."""
+    rng = np.random.default_rng(12)
+    z = np.full((4, vocab), most)
+    token = np.arange(vocab)
+    for r, others in enumerate((token % 8 == 0, token % 8 == token // 8 % 8, rng.random(vocab) < 0.125, token == 77)):
+        z[r, others] = rng.normal(size=others.sum())
+    u = np.array([0.1, 0.6, 0.99, 0.5], dtype=np.float32)
+    with L.Device() as dev:
+        for kw in (dict(), dict(top_p=np.full(4, 0.9)), dict(top_k=np.full(4, 60000), top_p=np.full(4, 0.7)),
+                   dict(top_k=np.full(4, 20)), dict(top_p=np.full(4, 0.95), min_p=np.full(4, 0.05))):
+            check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, **kw))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(512, 4099), (513, 270), (513, 4099), (513, 8192), (513, 8193), (520, 16400)])
+def test_many_rows(kind, rows, vocab):
+    rng = np.random.default_rng(vocab)
+    z = rng.normal(size=(rows, vocab)) * 2
+    u = rng.random(rows, dtype=np.float32)
+    kw = dict(top_k=rng.choice([0, 5, 90, 200, 1000], rows), top_p=rng.choice([0.3, 0.95, 1.0], rows),
+              min_p=rng.choice([0.0, 0.01], rows), temperature=rng.choice([0.0, 0.7, 1.0, 3.0], rows))
+    with L.Device() as dev:
+        check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, **kw))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_the_largest_vocabulary(kind):
+    rng = np.random.default_rng(13)
+    rows, vocab = 4, 1 << 20
+    z = rng.normal(size=(rows, vocab))
+    z[1], z[2, ::2] = 0.5, -0.25
+    z[2, 1::2] = -0.125
+    u = np.array([0.3, 0.7, 0.9, 1 - 2.0**-24], dtype=np.float32)
+    with L.Device() as dev:
+        for kw in (dict(), dict(top_p=np.full(rows, 0.8)), dict(top_k=np.full(rows, 50)), dict(top_k=np.full(rows, 400000)),
+                   dict(top_p=np.full(rows, 0.9), min_p=np.full(rows, 0.3))):
+            check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, **kw))
+
+
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("vocab", [900, 3001, 30011])
+@pytest.mark.parametrize("vocab", [900, 3001, 30011, 40003])
 def test_equal_logits_go_by_their_tokens(kind, vocab):
     rows = 9
     rng = np.random.default_rng(5)
@@ -106,22 +166,24 @@ def test_equal_logits_go_by_their_tokens(kind, vocab):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("spread", [1e-6, 1e-3, 0.02])
-def test_many_tokens_in_one_bin(kind, spread):
+@pytest.mark.parametrize("vocab", [3900, 25001, 40003])
+def test_many_tokens_in_one_bin(kind, spread, vocab):
     rng = np.random.default_rng(6)
-    rows, vocab = 8, 25001
+    rows = 8
     z = 3.0 + spread * rng.random((rows, vocab))
     z[4:, :100] = -40.0 + rng.random((4, 100))
     u = rng.random(rows, dtype=np.float32)
     u[:3] = 0.0, 1 - 2.0**-24, 0.5
     with L.Device() as dev:
-        for kw in (dict(), dict(top_k=rng.integers(2100, 24000, rows)), dict(top_p=rng.random(rows)),
-                   dict(top_k=rng.integers(2100, 24000, rows), top_p=rng.random(rows), min_p=np.full(rows, math.exp(-spread / 2))),
+        for kw in (dict(), dict(top_k=rng.integers(vocab // 10, vocab - 200, rows)), dict(top_p=rng.random(rows)),
+                   dict(top_k=rng.integers(vocab // 10, vocab - 200, rows), top_p=rng.random(rows), min_p=np.full(rows, math.exp(-spread / 2))),
                    dict(temperature=np.full(rows, 1e3), top_p=rng.random(rows))):
             check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, **kw))
 
 
-@pytest.mark.parametrize("vocab", [5, 700, 9000])
-def test_rows_and_settings_that_cannot_be(vocab):
+@pytest.mark.parametrize("vocab,kind", [(5, "f32"), (200, "f32"), (700, "f32"), (9000, "f32"), (9000, "bf16"), (40003, "f32"),
+                                        (40003, "f16"), (40003, "bf16")])
+def test_rows_and_settings_that_cannot_be(vocab, kind):
     rng = np.random.default_rng(7)
     rows = 16
     z = rng.normal(size=(rows, vocab))
@@ -139,7 +201,7 @@ def test_rows_and_settings_that_cannot_be(vocab):
     k = np.full(rows, 4)
     with L.Device() as dev:
         for kw in (dict(top_k=k, top_p=p, min_p=m), dict(top_p=p, min_p=m)):
-            got = sampled(dev, L.stored(z, "f32"), "f32", temperature=t, u=u, **kw)
+            got = sampled(dev, L.stored(z, kind), kind, temperature=t, u=u, **kw)
             check_drawn(got)
             assert [r for r in range(rows) if got[0][r] == S.NO_TOKEN] == [1, 2, 3, 6, 7, 8, 9, 10, 11, 12, 13, 15]
 

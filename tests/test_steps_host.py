@@ -25,8 +25,8 @@ def test_sampling_refusals():
                                                             uniforms=256, tokens=256), **kw})
     for code in (-1, 3):
         refused("element type", call, type=code)
-    refused("1..2\\^24 tokens", call, vocab=0)
-    refused("1..2\\^24 tokens", call, vocab=(1 << 24) + 1, stride=1 << 25)
+    refused("1..2\\^20 tokens", call, vocab=0)
+    refused("1..2\\^20 tokens", call, vocab=(1 << 20) + 1, stride=1 << 21)
     refused("row stride", call, stride=9)
     refused("rows must stay below", call, rows=1 << 22)
     for name in ("logits", "uniforms", "tokens"):
