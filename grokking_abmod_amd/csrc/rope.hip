@@ -165,15 +165,16 @@ template <class T>
 void launch(const RopeArgs &a, hipStream_t stream) {
     constexpr int G = T::kGroup;
     const int half = a.rotary / 2;
+    const bool interleaved = a.interleaved || a.rotary == 2;  // one pair is the same in both
     bool same = true;  // what stays is there already
     for (const RopeSide &s : a.side)
         if (s.heads)
             same = same && s.x == s.out && s.xs.s[0] == s.os.s[0] && s.xs.s[1] == s.os.s[1] && s.xs.s[2] == s.os.s[2];
-    const int turning = ((a.interleaved ? a.rotary : half) + G - 1) / G;
+    const int turning = ((interleaved ? a.rotary : half) + G - 1) / G;
     const int items = same            ? turning
-                      : a.interleaved ? (a.width + G - 1) / G
+                      : interleaved   ? (a.width + G - 1) / G
                                       : turning + (a.width - a.rotary + G - 1) / G;
-    if (items == 0) return;
+    if (items == 0) return;  // at most kBlock, for every width and rotary
     // Two or three heads a thread, where there are tokens enough for that: 32768 tokens of 40
     // heads of 128 BF16 took 128 us with 2 tokens a workgroup (2.5 heads), 142 with 1, 139
     // with 8 and 152 with 16; past the caches 121, with loads ahead 116 (5.8 TB/s).
@@ -182,9 +183,9 @@ void launch(const RopeArgs &a, hipStream_t stream) {
     const int tile = int(std::max<int64_t>(1, std::min<int64_t>({tokens / 1024, 5 * slots / (2 * heads), most})));
     const dim3 grid(unsigned((tokens + tile - 1) / tile));
     const bool past = double(tokens) * double(heads) * a.width * sizeof(typename T::Raw) > kCached;
-    if (a.interleaved && past)
+    if (interleaved && past)
         rope_kernel<T, true, true><<<grid, kBlock, 0, stream>>>(a, tile, items, slots);
-    else if (a.interleaved)
+    else if (interleaved)
         rope_kernel<T, true, false><<<grid, kBlock, 0, stream>>>(a, tile, items, slots);
     else if (past)
         rope_kernel<T, false, true><<<grid, kBlock, 0, stream>>>(a, tile, items, slots);

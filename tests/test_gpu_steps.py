@@ -288,6 +288,9 @@ ROPES = [
     ("bf16", 2, 17, 0, 3, 256, 130, False, "sthd", 0, None, None),
     ("f32", 1, 9, 2, 2, 1024, 1024, False, "sthd", 0, [1 << 20], None),
     ("f16", 1, 9, 2, 1, 1023, 1022, True, "sthd", 0, [50], None),
+    ("f32", 2, 3, 2, 1, 1024, 2, False, "sthd", 0, [50, 3], None),
+    ("f32", 1, 3, 2, 1, 1023, 2, False, "sthd", 1, [50], None),
+    ("f32", 1, 3, 1, 1, 1023, 10, False, "sthd", 0, [50], None),
     ("f32", 2, 4, 2, 1, 20, 0, False, "sthd", 0, [4, 4], [-1, 4]),
     ("bf16", 1, 1, 1, 1, 1, 0, True, "sthd", 0, [1], None),
     ("f32", 40, 70, 3, 2, 36, 36, True, "sthd", 0, [70 + 1000 * i for i in range(40)], None),
