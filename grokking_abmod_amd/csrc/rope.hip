@@ -9,7 +9,9 @@
 // position 10^6 an FP32 product is off by a thirtieth of a radian; sine and
 // cosine of what is left are FP32 series.  A workgroup makes them once for its
 // tokens, in LDS, and applies them to all heads, 16 bytes of each half a thread, with the
-// next head's loads under way.
+// next head's loads under way.  Every element is read and written once, and memory bounds
+// it: 32768 tokens of 40 heads of 128 BF16 115 us (5.8 TB/s), 16384 of 32 heads of 64 32
+// (4.2); 3003 of 16 heads of 80 F16 7 us, which its few workgroups' chains bound.
 #include <algorithm>
 
 #include "operators.hpp"

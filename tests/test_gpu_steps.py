@@ -206,6 +206,23 @@ def test_rows_and_settings_that_cannot_be(vocab, kind):
             assert [r for r in range(rows) if got[0][r] == S.NO_TOKEN] == [1, 2, 3, 6, 7, 8, 9, 10, 11, 12, 13, 15]
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("vocab", [3, 100, 1000, 5003, 20003, 40003])
+def test_rows_with_a_value_that_cannot_be(kind, vocab):
+    """NaN of either sign and +inf, in whole groups and behind them, with every way to draw."""
+    rng = np.random.default_rng(14)
+    places = [0, 1, vocab // 2, vocab - 2, vocab - 1]
+    z = rng.normal(size=(3 * len(places), vocab))
+    for i, at in enumerate(places):
+        z[3 * i, at], z[3 * i + 1, at], z[3 * i + 2, at] = np.nan, np.copysign(np.nan, -1.0), np.inf
+    rows = len(z)
+    with L.Device() as dev:
+        for kw in (dict(), dict(top_k=np.full(rows, 2)), dict(top_p=np.full(rows, 0.5)), dict(min_p=np.full(rows, 0.5)),
+                   dict(temperature=np.zeros(rows))):
+            tokens, logprob, _ = sampled(dev, L.stored(z, kind), kind, u=np.full(rows, 0.5), **kw)
+            assert np.all(tokens == S.NO_TOKEN) and np.all(np.isnan(logprob))
+
+
 def test_logits_and_temperatures_of_every_size():
     rng = np.random.default_rng(8)
     with L.Device() as dev:
