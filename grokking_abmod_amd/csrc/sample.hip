@@ -244,8 +244,10 @@ struct Weights {
                                0x1.152aaa3bf81ccp-3, 0x1.2c155b8213cf4p-6, 0x1.5fc21041027adp-12, 0x1.e355bbaee85cbp-24};
         double w = 1.0;
 #pragma unroll
-        for (int b = 0; b < BITS; ++b)
-            if (i >> b & 1) w *= i < UNIT ? of[b + STEP] : of[min(7 + b, 11)];
+        for (int b = 0; b < BITS; ++b) {  // constants, both of them: loads of one or the other would be a chain
+            const double part = of[b + STEP], whole = of[min(7 + b, 11)], factor = i < UNIT ? part : whole;
+            w *= i >> b & 1 ? factor : 1.0;
+        }
         (i < UNIT ? p.parts[i] : p.wholes[i - UNIT]) = w;
     }
     // Bins from the largest logit.
@@ -881,18 +883,22 @@ __global__ void __launch_bounds__(THREADS) sample_bins_kernel(SampleArgs a) {
 // and counted apart in a second pass.
 //
 // The counts fill a CU's LDS, so rows follow each other on it: 1000 rows of 128001 BF16
-// with top_p 168 to 172 us, 1.5 TB/s, four rows a CU of 42 us each: 12 for the row's loads,
-// 10 to count it by LDS atomics, 8 to sum and weigh the segments, 11 to find the borders
-// and the token.  1024 rows of 128000 take 163, and by bins, whose fill is FP64 work for each
-// logit, 261.
+// with top_p 163 us, 1.6 TB/s, four rows a CU of 41 us each: some 20 until the row is
+// there and counted as it comes, by LDS atomics (171 in all when counted afterwards), 8 to
+// sum and weigh the segments, 11 to find the borders and the token.  1024 rows of 128000
+// by bins, whose fill is FP64 work for each logit, take 261.
 constexpr int kCodeThreads = 1024;
 constexpr int kCodeGroups = 16;  // of 8 logits a thread
-constexpr uint32_t kCodeLeast = 32769, kCodeMost = 131071;
+constexpr uint32_t kCodeMost = 131071;
 static_assert(kCodeMost < kCodeThreads * kCodeGroups * 8, "a row fits the registers");
 
 template <class T>
 struct Codes {
     static constexpr int kUnit = 128, THREADS = kCodeThreads, WAVES = THREADS / 64, GROUPS = kCodeGroups;
+    // The shortest rows counted.  F16 has eight times the values at a logit's size, so more
+    // segments to weigh: counted and by bins, 1000 rows of 64000 take 167 and 142 us, of 96000
+    // 190 and 198 (BF16: of 50000 113 and 134 for 1024).
+    static constexpr uint32_t kLeast = std::is_same<T, F16>::value ? 81920 : 32769;
     static constexpr uint32_t kInf = std::is_same<T, F16>::value ? 0x7c00 : 0x7f80, kNegative = 0x8000 | kInf;
 
     struct Part {
@@ -986,8 +992,7 @@ __device__ __forceinline__ u32x4 group_of(const u32x4 (&w)[kCodeGroups], int at)
 
 // The code that most of a sample of the row has, if it has a quarter of a wave's.
 template <class C>
-__device__ __forceinline__ uint32_t sampled_code(C &c, const u32x4 (&w)[kCodeGroups]) {
-    const u32x4 g = group_of(w, int(c.wave % c.each));
+__device__ __forceinline__ uint32_t sampled_code(C &c, u32x4 g) {
     const uint32_t word = c.lane & 4 ? (c.lane & 2 ? g[3] : g[2]) : (c.lane & 2 ? g[1] : g[0]);
     const uint32_t code = word >> (c.lane % 2 * 16) & 0xffff;
     uint64_t rest = __ballot((code & 0x7fff) != 0x7fff);  // not what fills the last wave
@@ -1030,17 +1035,18 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
     // A wave has `each` times 64 groups in a row, and a lane every 64th of them.
     const uint32_t groups = vocab / 8, tail = vocab % 8, each = (groups + C::THREADS - 1) / C::THREADS;
     const auto group = [&](int g) { return (wave * each + uint32_t(g)) * 64 + lane; };
+    // All of them are loaded, those past `each` from one place: a load under a condition would
+    // make the wait for the first one a wait for all.
     u32x4 w[kCodeGroups];
 #pragma unroll
     for (int j = 0; j < kCodeGroups; ++j)
-        if (uint32_t(j) < each) {
-            w[j] = *reinterpret_cast<const u32x4_any *>(z + size_t(min(group(j), groups - 1)) * 8);
-            w[j] |= group(j) < groups ? 0 : 0x7fff7fffu;  // NaN, which no token that is drawn is
-        }
+        w[j] = *reinterpret_cast<const u32x4_any *>(z + size_t(uint32_t(j) < each ? min(group(j), groups - 1) : groups - 1) * 8);
     const uint32_t last = tid < tail ? uint32_t(__builtin_bit_cast(uint16_t, z[groups * 8 + tid])) : 0;
     Weights<C::kUnit>::prepare(s.powers);
     C c{s, tid, lane, wave, each, 0, 0, {s.powers, 0.0, set.greedy ? 1.0 : uniform(C::kUnit / set.temperature)}};
-    c.hot = sampled_code(c, w);
+    // Behind the row's groups there is NaN, which no token that is drawn is.
+    const auto filled = [&](int g) { return group(g) < groups ? w[g] : w[g] | 0x7fff7fffu; };
+    c.hot = sampled_code(c, filled(0));  // the others are counted as they come
     uint32_t mine;  // tokens of a thread's segment, without those of -inf
 #pragma unroll 1
     for (bool again = false;; again = true) {
@@ -1056,7 +1062,10 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         };
 #pragma unroll
         for (int j = 0; j < kCodeGroups; ++j) {
-            asm volatile("" : "+v"(w[j]));  // what is made of it is not kept from one pass for the other
+            if (uint32_t(j) < each) {
+                asm volatile("" : "+v"(w[j]));  // what is made of it is not kept from one pass for the other
+                w[j] = filled(j);
+            }
             if (uint32_t(j) < each && group(j) < groups) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) count(w[j][e / 2] >> (e % 2 * 16) & 0xffff);
@@ -1272,7 +1281,7 @@ void launch(const SampleArgs &a, hipStream_t stream) {
         sample_bins_kernel<T, 256, 32, 1024><<<rows, 256, 0, stream>>>(a);
     else if (a.vocab <= (many ? 32768 : 16384))
         sample_bins_kernel<T, 512, 128, 1024><<<rows, 512, 0, stream>>>(a);
-    else if (sizeof(typename T::Raw) == 4 || a.vocab < kCodeLeast || a.vocab > kCodeMost)
+    else if (sizeof(typename T::Raw) == 4 || a.vocab < Codes<T>::kLeast || a.vocab > kCodeMost)
         sample_bins_kernel<T, 1024, 128, 2048><<<rows, 1024, 0, stream>>>(a);
     else if constexpr (sizeof(typename T::Raw) == 2)
         sample_codes_kernel<T><<<rows, kCodeThreads, 0, stream>>>(a);
