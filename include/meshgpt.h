@@ -376,9 +376,9 @@ int mg_token_logprobs(int device, const float *logits, size_t rows, size_t vocab
  * always left.  A row gets the token 0xFFFFFFFF and a logprob of NaN where its
  * logits hold a NaN or +inf or are all -inf, its temperature is negative, NaN or
  * infinite, top_p or min_p is NaN, or its random number is not in [0, 1).  Sums are
- * exact to about 2^-34 of a weight (2^-28 beyond 2^17 tokens) and the same in every call;
- * tokens of less than e^-31.9 of the largest weight are not drawn.  logprob may be NULL.
- * Fewer than 2^22 rows, up to 2^20 tokens; no workspace. */
+ * exact to about 2^-34 of a weight (2^-28 beyond 2^17 tokens) and the same in every call
+ * of the same sizes; tokens of less than e^-31.9 of the largest weight are not drawn.
+ * logprob may be NULL.  Fewer than 2^22 rows, up to 2^20 tokens; no workspace. */
 int mg_sample_filtered_noalloc(int device, int type, const void *logits, size_t rows, size_t vocab, size_t stride,
                                const float *temperatures, const int32_t *top_k, const float *top_p, const float *min_p,
                                const float *uniforms, uint32_t *tokens, float *logprob, void *stream);
