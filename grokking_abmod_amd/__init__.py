@@ -508,11 +508,11 @@ class MeshGpt:
     def set_cache(self, type):
         """mg_set_cache: MG_CACHE_F32 or MG_CACHE_E4M3; drops the current batch."""
         _check(lib().mg_set_cache(self._h, type))
+        self._batch = 0
 
     def set_sampling(self, top_k=0, top_p=1.0, min_p=0.0):
         """mg_set_sampling: filters of the tokens sampled from here on; the defaults filter nothing."""
         _check(lib().mg_set_sampling(self._h, top_k, top_p, min_p))
-        self._batch = 0
 
     def logits(self, tokens, sequence, last_only=False):
         tokens = _u32(tokens).reshape(-1)
