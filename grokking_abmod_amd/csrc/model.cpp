@@ -1485,6 +1485,13 @@ struct MeshGpt::Impl {
         ensure_derived();
         ensure_decode(b, std::max(reserve, p));
         dstage.ensure(b * std::max(reserve, p) * 4);
+        try {
+            ensure_filter(t);
+        } catch (...) {  // the batch that was may have drawn from what is gone
+            batch = length = start_length = 0;
+            cached = kNoCache;
+            throw;
+        }
         upload(dstage.p, prompts, b * p * 4, "upload prompts");
         kern::start_rows(dstage.as<uint32_t>(), int(b), int(p), dtokens.as<uint32_t>(), tcap, dlen.as<int>(),
                          drng.as<uint64_t>(), seed, dflags.as<int>(), stream);
@@ -1494,14 +1501,15 @@ struct MeshGpt::Impl {
         cached = 0;
         temperature = t;
         start_length = 0;
-        ensure_filter();
     }
 
     // Whether tokens are drawn through filters: then each step draws by sample_step, in
     // one stream, on the per-phase kernels.
-    bool filtered() const { return temperature > 0.0f && (top_k > 0 || top_p < 1.0f || min_p > 0.0f); }
-    void ensure_filter() {
-        if (filtered() && batch_cap) dfilter.ensure(batch_cap * kern::kSampledBytes);
+    bool filtered() const { return filters(temperature); }
+    bool filters(float t) const { return t > 0.0f && (top_k > 0 || top_p < 1.0f || min_p > 0.0f); }
+    // The scratch of every step at temperature t.
+    void ensure_filter(float t) {
+        if (filters(t) && batch_cap) with_room([&] { dfilter.ensure(batch_cap * kern::kSampledBytes); });
     }
     void set_sampling(uint32_t k, float p, float least) {
         if (!(p > 0.0f && p <= 1.0f)) throw Error("top_p must be in (0, 1]");
@@ -1516,7 +1524,7 @@ struct MeshGpt::Impl {
         top_p = p;
         min_p = least;
         try {
-            ensure_filter();
+            ensure_filter(temperature);
         } catch (...) {
             top_k = was_k;
             top_p = was_p;

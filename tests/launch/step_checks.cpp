@@ -194,7 +194,35 @@ void filters_without_memory() {
     fake::on_launch = nullptr;
 }
 
+// A batch that finds no memory for its filters' scratch is not there: nothing decodes
+// from it, and no draw is launched without scratch.
+void batch_without_filter_memory() {
+    MeshGpt m(0, shape(), 7, 64);
+    const std::vector<uint32_t> prompts(64, 1);
+    auto begin = [&](float temperature) { m.prefill(prompts.data(), 64, 1, temperature, 7, 20); };
+    begin(0.0f);
+    m.set_sampling(3, 1.0f, 0.0f);  // a greedy batch needs none
+    size_t draws = 0;
+    bool scratch = true;
+    fake::on_launch = [&](const fake::Launch &l) {
+        if (l.kernel.find("sample_rows_kernel") == std::string::npos) return;
+        ++draws;
+        scratch = scratch && *static_cast<void **>(l.args[0]) != nullptr;
+    };
+    fake::memory = fake::used;
+    expect(status_of([&] { begin(0.7f); }) == kOutOfMemory, "no memory for the filters");
+    fake::memory = size_t(1) << 33;
+    const bool decoded = status_of([&] { m.decode(1); }) == 0;
+    expect(scratch, "no draw is launched without scratch");
+    expect(!decoded && m.sequence_length() == 0, "a refused batch does not decode");
+    begin(0.7f);
+    m.decode(1);
+    expect(draws > 0 && scratch, "it is drawn from where there is memory");
+    fake::on_launch = nullptr;
+}
+
 const std::map<std::string, void (*)()> kChecks = {
+    {"batch_without_filter_memory", batch_without_filter_memory},
     {"refused_launches", refused_launches},
     {"foreign_errors", foreign_errors},
     {"largest_calls", largest_calls},

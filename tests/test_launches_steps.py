@@ -32,3 +32,8 @@ def checks(tmp_path_factory):
 def test_launches(checks, name):
     run = subprocess.run([checks, name], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout == "ok\n", run.stdout + run.stderr
+
+
+def test_a_batch_without_memory_for_its_filters(checks):
+    run = subprocess.run([checks, "batch_without_filter_memory"], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout == "ok\n", run.stdout + run.stderr
