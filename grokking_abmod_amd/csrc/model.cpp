@@ -750,7 +750,7 @@ struct MeshGpt::Impl {
         dtokens.release();
         dtokens.ensure(batch_cap * tcap * 4);
         cached = kNoCache;
-        length = 0;
+        batch = length = start_length = 0;  // what there was is gone
         sync();
     }
 

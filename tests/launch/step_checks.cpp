@@ -221,7 +221,34 @@ void batch_without_filter_memory() {
     fake::on_launch = nullptr;
 }
 
+// A larger batch that is refused for want of memory, wherever it runs out, takes the
+// one before with it if that has lost its buffers: nothing decodes from new, empty ones.
+void larger_batch_without_memory() {
+    const std::vector<uint32_t> prompts(64 * 4, 1);
+    bool there = false;
+    size_t refused = 0;
+    for (size_t room = 0; !there; room += 4096) {
+        MeshGpt m(0, shape(), 7, 8);
+        m.prefill(prompts.data(), 8, 4, 0.0f, 7, 20);
+        std::vector<uint32_t> before(8 * 5), after(8 * 5);
+        m.read_tokens(before.data(), 8, 5);
+        fake::memory = fake::used + room;
+        const int status = status_of([&] { m.prefill(prompts.data(), 64, 4, 0.0f, 7, 20); });
+        fake::memory = size_t(1) << 33;
+        there = status == 0;
+        if (there) continue;
+        ++refused;
+        expect(status == kOutOfMemory, "a batch without memory is refused");
+        if (status_of([&] { m.decode(1); }) != 0) continue;
+        expect(m.sequence_length() == 6, "a batch goes on from where it was");
+        m.read_tokens(after.data(), 8, 5);
+        expect(before == after, "a batch goes on only with its tokens");
+    }
+    expect(refused > 0, "memory was short");
+}
+
 const std::map<std::string, void (*)()> kChecks = {
+    {"larger_batch_without_memory", larger_batch_without_memory},
     {"batch_without_filter_memory", batch_without_filter_memory},
     {"refused_launches", refused_launches},
     {"foreign_errors", foreign_errors},

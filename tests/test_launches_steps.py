@@ -37,3 +37,8 @@ def test_launches(checks, name):
 def test_a_batch_without_memory_for_its_filters(checks):
     run = subprocess.run([checks, "batch_without_filter_memory"], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout == "ok\n", run.stdout + run.stderr
+
+
+def test_a_larger_batch_without_memory(checks):
+    run = subprocess.run([checks, "larger_batch_without_memory"], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout == "ok\n", run.stdout + run.stderr
