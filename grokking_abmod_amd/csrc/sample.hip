@@ -201,8 +201,8 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs &a, size_t row)
     s.with_p = s.top_p < 1.0;
     s.with_min = s.min_p > 0.0;
     s.greedy = s.temperature == 0.0;
-    s.valid = s.temperature >= 0.0 && s.temperature <= double(FLT_MAX) && s.top_p == s.top_p && !(a.min_p && a.min_p[row] != a.min_p[row]) &&
-              (s.greedy || (s.uniform >= 0.0 && s.uniform < 1.0));
+    const bool settings = s.top_p == s.top_p && !(a.min_p && a.min_p[row] != a.min_p[row]) && s.uniform >= 0.0 && s.uniform < 1.0;
+    s.valid = s.greedy || (s.temperature > 0.0 && s.temperature <= double(FLT_MAX) && settings);
     return s;
 }
 

@@ -375,7 +375,8 @@ int mg_token_logprobs(int device, const float *logits, size_t rows, size_t vocab
  * top_p of 1 or more and a min_p of 0 or less filter nothing; the first token is
  * always left.  A row gets the token 0xFFFFFFFF and a logprob of NaN where its
  * logits hold a NaN or +inf or are all -inf, its temperature is negative, NaN or
- * infinite, top_p or min_p is NaN, or its random number is not in [0, 1).  Sums are
+ * infinite, or (not at temperature 0) top_p or min_p is NaN or its random number is
+ * not in [0, 1).  Sums are
  * exact to about 2^-34 of a weight (2^-28 beyond 2^17 tokens) and the same in every call
  * of the same sizes; tokens of less than e^-31.9 of the largest weight are not drawn.
  * logprob may be NULL.  Fewer than 2^22 rows, up to 2^20 tokens; no workspace. */
