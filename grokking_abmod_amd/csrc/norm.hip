@@ -77,6 +77,14 @@ constexpr int kWavesMost = 16;
 template <int LANES>
 constexpr int kThreads = LANES > 0 ? kBlock : LANES == kBlockRow ? 512 : 1024;  // at most
 
+// v in FP32 for a conversion to fewer bits: what FP32 does not hold of it sets the last
+// bit, so that a value next to the middle of two codes does not become it.
+__device__ __forceinline__ float for_rounding(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lost = uint32_t(b) & 0x1fffffffu;
+    return float(__builtin_bit_cast(double, (b & ~uint64_t(0x1fffffff)) | (lost ? 0x20000000u : 0u)));
+}
+
 // Four E4M3 codes.
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
     const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -161,7 +169,8 @@ __global__ void __launch_bounds__(kThreads<LANES>) norm_kernel(NormArgs a) {
             uint32_t c[G / 4];
 #pragma unroll
             for (int e = 0; e < G; e += 4)
-                c[e / 4] = encode4(float(y[e] * by), float(y[e + 1] * by), float(y[e + 2] * by), float(y[e + 3] * by));
+                c[e / 4] = encode4(for_rounding(y[e] * by), for_rounding(y[e + 1] * by), for_rounding(y[e + 2] * by),
+                                   for_rounding(y[e + 3] * by));
             if (at + G <= width) {
 #pragma unroll
                 for (int e = 0; e < G; e += 4) *reinterpret_cast<u32_any *>(codes + at + e) = c[e / 4];

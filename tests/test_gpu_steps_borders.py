@@ -26,3 +26,44 @@ def test_greedy_rows_look_at_no_filter_and_no_number(kind, vocab):
             tokens, logprob, _ = sampled(dev, z, kind, temperature=np.zeros(rows), u=rng.choice([math.nan, 2.0, 0.5], rows), **kw)
             assert np.array_equal(tokens, np.argmax(L.values(z, kind), 1))
             assert not logprob.any()
+
+
+def next_to_ties(rng, width):
+    """A row x and a weight with which values of the norm lie within 2^-24 of the middle of two
+    codes, on the side of the odd one: (x, w, y in 64 bits)."""
+    x = np.float32(rng.normal(size=width) + np.copysign(0.5, rng.normal(size=width)))
+    rstd = 1 / np.sqrt(np.mean(x.astype(np.longdouble) ** 2) + np.longdouble(np.float32(1e-5)))
+    # Each block of 32 begins with its largest, 400 codes' units of 2^-6; the others are codes of
+    # 8 to 15 units of 2^-2 .. 2^3 and a half.
+    code, power = rng.integers(8, 16, width), rng.integers(-2, 4, width)
+    tie = (code + 0.5) * 2.0**power
+    wanted = np.where(np.arange(width) % 32 == 0, 400.0, tie) * 2.0**-6 / (x * rstd)
+    w = wanted.astype(np.float32)
+    for i in np.flatnonzero(np.arange(width) % 32):
+        for step in range(-3, 4):  # the floats next to it
+            near = np.float32(w[i] + step * np.spacing(w[i]))
+            t = x[i].astype(np.longdouble) * near * rstd * 64
+            off = t / tie[i] - 1
+            if 2.0**-40 < abs(off) < 2.0**-26 and (off > 0) == (code[i] % 2 == 0):
+                w[i] = near
+                break
+    y = x.astype(np.longdouble) * w.astype(np.longdouble) * rstd
+    return x, w, y
+
+
+def test_codes_next_to_the_middle_of_two_are_the_nearest():
+    """They are rounded once: 2^-52 of a value, FP64's, is all that they may be off by."""
+    rng = np.random.default_rng(40)
+    apart = 0
+    with L.Device() as dev:
+        for width in (64, 1000, 5000):
+            x, w, y = next_to_ties(rng, width)
+            codes, scales = dev.alloc(width), dev.alloc((width + 31) // 32)
+            G.rms_norm_e4m3(G.MG_F32, 1, width, dev.put(x), width, None, 0, None, 0, dev.put(w), 1e-5, codes, width, scales,
+                            (width + 31) // 32)
+            e = dev.get(scales, (width + 31) // 32, np.uint8).astype(np.int64) - 127
+            t = (y * 2.0 ** -np.repeat(e, 32)[:width]).astype(np.float64)
+            nearest = L.e4m3(t)
+            assert np.array_equal(L.E4M3[dev.get(codes, width, np.uint8)], nearest)
+            apart += np.sum(L.e4m3(t.astype(np.float32).astype(np.float64)) != nearest)
+    assert apart > 100  # by way of FP32 so many would be others
