@@ -7,11 +7,13 @@
 // with which the largest of them is at most 448.
 //   g = dy w;  dh = rstd (g - hat mean(g hat)) + dsum;  dw = sum of dy hat over rows, hat = h rstd.
 //
-// All of them read a row once: it stays in registers, 16 bytes a load, in part of a
-// wave for short rows (heads) and in up to 16 for long ones.  Sums of a row are FP64,
-// which no FP32 value overflows; so is what decides a scale, where values next to
-// a power of two are met in any large batch.  The weight's gradient is summed in
-// registers over a team's rows, then over the teams in a fixed order.
+// All but the gradient of the widest rows read a row once: it stays in registers, 16 bytes
+// a load, in part of a wave for short rows (heads) and in up to 16 for long ones.  The norm's
+// sum of a row is FP64, which no FP32 value overflows; so is what decides a scale, where
+// values next to a power of two are met in any large batch.  The gradient's products, and
+// their sums over 16 bytes of a row, are FP32; a row's sum of those is FP64.  The weight's
+// gradient is summed over a team's rows, 64 of them in FP32 and such sums in FP64, then over
+// the teams in a fixed order.
 //
 // Memory bounds all of them at length: with a residual that is kept, 16384 x 4096 BF16 93 us
 // (5.8 TB/s), 4001 x 5120 F16 to codes 32 (4.5); 32 x 512 F32 3.1 us, a launch and a chain
@@ -283,16 +285,20 @@ __device__ __forceinline__ void load_weight(const NormBackwardArgs &a, int lane,
     }
 }
 
+// Rows of the weight's gradient that are summed in FP32; such sums are added up in FP64.
+constexpr int kRun = 64;
+
 // Both gradients in one pass.  A team has every teams-th row, and its lanes the same
 // channels of each: the sums of the weight's gradient and the weight stay in registers,
-// and the next row's loads are under way while a row's mean is joined.
+// and the next row's loads are under way while a row's mean is joined.  The sums of kRun
+// rows go to LDS, a place a thread and channel.
 // 8192 x 4096 BF16 with a residual: 49 us (5.5 TB/s); a wave a row, without loads ahead, 114.
 template <class T, int LANES, int GROUPS>
 __global__ void __launch_bounds__(kThreads<LANES>) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
     constexpr int G = T::kGroup;
     __shared__ double room[kWavesMost];
     constexpr int TEAMS = LANES > 0 ? kBlock / (LANES > 0 ? LANES : 1) : 1;
-    __shared__ float joined[LANES > 0 ? TEAMS * LANES * GROUPS * G : 1];
+    __shared__ double runs[GROUPS * G * kThreads<LANES>];
     const Team<LANES> team;
     const int lane = team.lane, lanes = team.lanes, width = a.width;
     const double share = 1.0 / double(width);
@@ -303,29 +309,44 @@ __global__ void __launch_bounds__(kThreads<LANES>) norm_backward_kernel(NormBack
     for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
         for (int e = 0; e < G; ++e) dw[i][e] = 0.0f;
+    // Channel i, e of this thread.  Teams of a wave are next to each other, so that its lanes meet no bank twice.
+    const auto place = [&](int i, int e) { return (i * G + e) * kThreads<LANES> + int(threadIdx.x); };
+    bool any = false;
+    const auto add_run = [&] {
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+            for (int e = 0; e < G; ++e) {
+                runs[place(i, e)] = (any ? runs[place(i, e)] : 0.0) + double(dw[i][e]);
+                dw[i][e] = 0.0f;
+            }
+        any = true;
+    };
     size_t row = size_t(blockIdx.x) * TEAMS + team.of;
     Gradient<T, GROUPS> now, next;
     if (row < a.rows) now.load(a, row, lane, lanes);
-    for (; row < a.rows; row += teams) {
+    for (int run = 0; row < a.rows; row += teams) {
         if (row + teams < a.rows) next.load(a, row + teams, lane, lanes);
         now.trim(a, lane, lanes);
         const double dot = now.dot(a.weight, w, [&](int i, int e, float dy, float hat) { dw[i][e] = fmaf(dy, hat, dw[i][e]); });
         now.store(a, row, lane, lanes, float(team.sum(dot, room) * share), w);
         now = next;
+        if (++run == kRun) {
+            add_run();
+            run = 0;
+        }
     }
     float *const part = a.part + size_t(blockIdx.x) * width;
     if constexpr (LANES > 0) {  // the teams' sums, one after the other
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i)
-#pragma unroll
-            for (int e = 0; e < G; ++e) joined[((team.of * GROUPS + i) * G + e) * LANES + lane] = dw[i][e];
+        add_run();
         __syncthreads();
         for (int c = threadIdx.x; c < LANES * GROUPS * G; c += kBlock) {
-            float sum = joined[c];
+            const double *const own = runs + c / LANES * kBlock + c % LANES;
+            double sum = own[0];
 #pragma unroll
-            for (int t = 1; t < TEAMS; ++t) sum += joined[t * LANES * GROUPS * G + c];
+            for (int t = 1; t < TEAMS; ++t) sum += own[t * LANES];
             const int at = (c % LANES + c / (LANES * G) * LANES) * G + c / LANES % G;
-            if (at < width) part[at] = sum;
+            if (at < width) part[at] = float(sum);
         }
         return;
     }
@@ -334,7 +355,7 @@ __global__ void __launch_bounds__(kThreads<LANES>) norm_backward_kernel(NormBack
 #pragma unroll
         for (int e = 0; e < G; ++e) {
             const int at = (lane + i * lanes) * G + e;
-            if (at < width) part[at] = dw[i][e];
+            if (at < width) part[at] = any ? float(runs[place(i, e)] + double(dw[i][e])) : dw[i][e];
         }
 }
 
@@ -482,6 +503,12 @@ void norm_of(const NormArgs &a, hipStream_t stream) {
 uint32_t parts_of(size_t rows, const Cut &c) {
     return uint32_t(std::min<size_t>((rows + c.teams() - 1) / c.teams(), 512));
 }
+// Of wide rows, for workgroups of norm_columns_kernel: eight a CU, and more where a thread
+// would have more than kRun rows.
+uint32_t wide_parts_of(size_t rows, size_t width, int group) {
+    const size_t slabs = (width + group * kSlab - 1) / (group * kSlab), run = size_t(kBlock / kSlab) * kRun;
+    return uint32_t(std::max(std::min(rows, std::min<size_t>(512, std::max<size_t>(1, 2048 / slabs))), (rows + run - 1) / run));
+}
 // Calls of few rows and elements take one launch, in which some workgroups read the rows
 // again for the weight's gradient: 1024 x 128 F32 took launches of 4.0 and 2.5 us, and takes
 // one of 5.9, and no workspace.
@@ -508,10 +535,10 @@ void backward_of(const NormBackwardArgs &a, hipStream_t stream) {
             return;
         }
         if constexpr (lanes.value == kWideRow) {
-            // The registers do not hold the sums beside a row: 4000 x 15001 BF16 took 268 us so,
-            // and takes 194 with the rows read twice.
+            // Registers do not hold the sums beside a row: 4000 x 15001 BF16 took 268 us so, and
+            // takes 170 with the rows read twice.  LDS would hold them, and has not been measured.
             const uint32_t slabs = uint32_t((width + group * kSlab - 1) / (group * kSlab));
-            parts = std::min(parts, std::max(1u, 2048 / slabs));
+            parts = wide_parts_of(a.rows, size_t(width), group);
             if (parts) norm_columns_kernel<T><<<dim3(slabs * parts), kBlock, 0, stream>>>(a, slabs, parts);
         } else if (parts) {
             norm_backward_kernel<T, lanes.value, groups.value><<<dim3(parts), c.threads, 0, stream>>>(a, parts * uint32_t(c.teams()));
@@ -527,7 +554,10 @@ size_t norm_parts(size_t rows, size_t width) {
     size_t parts = 0;
     for (int group : {4, 8}) {
         const Cut c = cut_of(width, group);
-        if (!few(rows, width) || c.lanes == kWideRow) parts = std::max<size_t>(parts, parts_of(rows, c));
+        if (c.lanes == kWideRow)
+            parts = std::max<size_t>(parts, wide_parts_of(rows, width, group));
+        else if (!few(rows, width))
+            parts = std::max<size_t>(parts, parts_of(rows, c));
     }
     return parts;
 }

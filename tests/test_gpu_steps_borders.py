@@ -67,3 +67,23 @@ def test_codes_next_to_the_middle_of_two_are_the_nearest():
             assert np.array_equal(L.E4M3[dev.get(codes, width, np.uint8)], nearest)
             apart += np.sum(L.e4m3(t.astype(np.float32).astype(np.float64)) != nearest)
     assert apart > 100  # by way of FP32 so many would be others
+
+
+@pytest.mark.parametrize("kind,width,rows", [("bf16", 8, (1 << 22) - 1), ("bf16", 1000, 2000000), ("f32", 516, 1500000),
+                                             ("f32", 4100, 700000), ("bf16", 16384, 400000)])
+def test_the_weights_gradient_of_many_rows(kind, width, rows):
+    """Rows of one value v, which are the gradient of the output too, and one rstd: the weight's
+    gradient is rows v^2 rstd.  FP32 sums of all rows of a workgroup would be off by 2^-18 or more."""
+    size = 4 if kind == "f32" else 2
+    v = float(L.values(np.frombuffer(b"\x3f" * size, dtype=L.STORED[kind]), kind)[0])
+    rstd = np.float32(1.2345678)
+    with L.Device() as dev:
+        at = dev.filled(rows * width * size, 0x3F)
+        room = G.rms_norm_backward_workspace(rows, width)
+        dw = dev.alloc(4 * width)
+        G.rms_norm_backward(L.CODES[kind], rows, width, at, width, None, dev.put(np.full(rows, rstd)), at, width, None, 0, at,
+                            width, dw, dev.alloc(room), room)
+        got = dev.get(dw, width, np.float32).astype(np.float64)
+    want = rows * v * v * float(rstd)
+    # Runs of up to 64 rows in FP32; hat, a part and the sum are rounded to it once each.
+    assert np.all(np.abs(got - want) <= (64 + 4) * 2.0**-24 * want)
