@@ -2,6 +2,7 @@
 // device of a call, alignments and the size of a launch.
 #pragma once
 
+#include <initializer_list>
 #include <string>
 
 #include "meshgpt_types.hpp"
@@ -62,6 +63,11 @@ inline int alignment(const void *k, const Strides &ks, const void *v, const Stri
 
 inline void check_aligned(const void *p, Type type, const char *message) {
     require(reinterpret_cast<uintptr_t>(p) % type_size(type) == 0, message);
+}
+
+// Of 32-bit values, null where there are none: scalar loads drop an address's last bits.
+inline void check_words(std::initializer_list<const void *> words, const char *message) {
+    for (const void *p : words) require(reinterpret_cast<uintptr_t>(p) % 4 == 0, message);
 }
 
 // A launch counts its threads, 256 a workgroup, in 32 bits.

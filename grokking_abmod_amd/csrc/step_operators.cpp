@@ -19,6 +19,8 @@ void sample_filtered_noalloc(int device, Type type, const void *logits, size_t r
     if (rows == 0) return;
     require(logits && uniforms && tokens, "logits, uniforms and tokens must not be null");
     check_aligned(logits, type, "logits must be aligned to their type");
+    check_words({temperatures, top_k, top_p, min_p, uniforms, tokens, logprob},
+                "settings, numbers, tokens and log probabilities must be aligned to 4 bytes");
     const OnDevice on(device);
     kern::SampleArgs a{};
     a.logits = logits;
@@ -86,6 +88,7 @@ void rope(int device, const Rope &r, Type type, size_t batch, size_t count, size
         for (const void *p : {k, static_cast<const void *>(k_out)})
             check_aligned(p, type, "keys must be aligned to their type");
     require(reinterpret_cast<uintptr_t>(r.frequencies) % 8 == 0, "frequencies must be aligned to 8 bytes");
+    check_words({lengths, counts, positions}, "lengths, counts and positions must be aligned to 4 bytes");
     const OnDevice on(device);
     kern::RopeArgs a{};
     a.side[0] = {q, q_out, qs, qos, int(heads)};
@@ -122,6 +125,7 @@ kern::NormArgs norm_args(Type type, size_t rows, size_t width, const void *x, si
     require(rows == 0 || x, "rows must not be null");
     for (const void *p : {x, residual, static_cast<const void *>(sum), weight})
         check_aligned(p, type, "rows and weight must be aligned to their type");
+    check_words({rstd}, "rstd must be aligned to 4 bytes");
     kern::NormArgs a{};
     a.x = x;
     a.residual = residual;
@@ -191,6 +195,7 @@ void rms_norm_backward(int device, Type type, size_t rows, size_t width, const v
     require(rows == 0 || (sum && rstd && d_out && d_x), "rows, rstd and the gradients must not be null");
     for (const void *p : {sum, weight, d_out, d_sum, static_cast<const void *>(d_x)})
         check_aligned(p, type, "rows, weight and gradients must be aligned to their type");
+    check_words({rstd, d_weight}, "rstd and the weight's gradient must be aligned to 4 bytes");
     require(need == 0 || (workspace && workspace_bytes >= need),
             "the workspace is too small: mg_rms_norm_backward_workspace gives its size");
     require(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "the workspace must be aligned to 4 bytes");

@@ -263,8 +263,8 @@ int mg_sample_logits_noalloc(int device, const float *logits, size_t rows, size_
  *
  * Each enqueues its work on `stream` (a hipStream_t of `device`; NULL is the
  * default stream) and returns without waiting, allocates nothing, and can be
- * captured into a HIP graph.  Pointers are device pointers; lengths, counts,
- * tokens and scratch are read and written by the enqueued work, so they have to
+ * captured into a HIP graph.  Pointers are device pointers, aligned to what they
+ * point to; lengths, counts, tokens and scratch are read and written by the enqueued work, so they have to
  * stay until it is done.  Calls that may overlap need workspaces of their own, as
  * do captured graphs that may.  The calling thread's current device is the same
  * on return as on entry. */
