@@ -917,7 +917,7 @@ struct Codes {
     };
 
     Shared &s;
-    uint32_t tid, lane, wave, each;
+    uint32_t tid, lane, wave;
     uint32_t hot, hot_count;  // counted apart
     Weights<kUnit> weights;
 
@@ -1043,7 +1043,7 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         w[j] = *reinterpret_cast<const u32x4_any *>(z + size_t(uint32_t(j) < each ? min(group(j), groups - 1) : groups - 1) * 8);
     const uint32_t last = tid < tail ? uint32_t(__builtin_bit_cast(uint16_t, z[groups * 8 + tid])) : 0;
     Weights<C::kUnit>::prepare(s.powers);
-    C c{s, tid, lane, wave, each, 0, 0, {s.powers, 0.0, set.greedy ? 1.0 : uniform(C::kUnit / set.temperature)}};
+    C c{s, tid, lane, wave, 0, 0, {s.powers, 0.0, uniform(C::kUnit / set.temperature)}};
     // Behind the row's groups there is NaN, which no token that is drawn is.
     const auto filled = [&](int g) { return group(g) < groups ? w[g] : w[g] | 0x7fff7fffu; };
     c.hot = sampled_code(c, filled(0));  // the others are counted as they come
@@ -1115,88 +1115,85 @@ __global__ void __launch_bounds__(kCodeThreads) sample_codes_kernel(SampleArgs a
         if (tid == 0) write(a, row, kNoToken, NAN);
         return;
     }
-    uint32_t code = C::code_at(begin.segment * 64 + lane), at = 0;
+    uint32_t code = C::code_at(begin.segment * 64 + lane);
     code = __builtin_amdgcn_readlane(code, __builtin_ctzll(__ballot(c.count_of(code) != 0)));
-    double share = 1.0;  // of the token that is drawn
-    if (!set.greedy) {
-        c.weights.top = uniform(double(C::value(code)));
-        // The segments' weights, a wave a segment; and what is over min_p.
-        double over = 0.0;
-        uint32_t over_count = 0;
-        uint64_t full = __ballot(s.in_segment[wave + C::WAVES * lane] != 0);
-        while (full) {  // two at a time: each is a chain
-            uint32_t segment[2];
+    c.weights.top = uniform(double(C::value(code)));
+    // The segments' weights, a wave a segment; and what is over min_p.
+    double over = 0.0;
+    uint32_t over_count = 0;
+    uint64_t full = __ballot(s.in_segment[wave + C::WAVES * lane] != 0);
+    while (full) {  // two at a time: each is a chain
+        uint32_t segment[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                segment[i] = full ? wave + C::WAVES * uint32_t(__builtin_ctzll(full)) : segment[0];
-                full &= full - 1;
-            }
-            const typename C::Value v[2] = {c.value_of(segment[0]), c.value_of(segment[1])};
-            double weight[2];
-            uint32_t count[2];
+        for (int i = 0; i < 2; ++i) {
+            segment[i] = full ? wave + C::WAVES * uint32_t(__builtin_ctzll(full)) : segment[0];
+            full &= full - 1;
+        }
+        const typename C::Value v[2] = {c.value_of(segment[0]), c.value_of(segment[1])};
+        double weight[2];
+        uint32_t count[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const double sum = double(v[i].count) * v[i].weight;
-                if (set.with_min && v[i].weight >= set.min_p && (i == 0 || segment[1] != segment[0])) {
-                    over += sum;
-                    over_count += v[i].count;
-                }
-                weight[i] = wave_total(sum);
-                count[i] = wave_total(v[i].count);
+        for (int i = 0; i < 2; ++i) {
+            const double sum = double(v[i].count) * v[i].weight;
+            if (set.with_min && v[i].weight >= set.min_p && (i == 0 || segment[1] != segment[0])) {
+                over += sum;
+                over_count += v[i].count;
             }
+            weight[i] = wave_total(sum);
+            count[i] = wave_total(v[i].count);
+        }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (lane == 0) {
-                    s.weights[segment[i]] = weight[i];
-                    s.in_segment[segment[i]] = count[i];
-                }
-        }
-        __syncthreads();
-        // What is left: the first `left` tokens, with the weight `whole`.
-        const double weight = s.weights[tid];
-        const uint32_t count = s.in_segment[tid];
-        double whole;
-        uint32_t left;
-        const double base = block_scan<C::THREADS>(weight, s.room_d, whole);
-        const uint32_t taken = block_scan<C::THREADS>(count, s.room_u, left);
-        whole = uniform(whole);
-        // The value at which the tokens reach `left`, or (p) the weights t, or exceed it.
-        const auto find = [&](double t, bool p, bool over_t) {
-            const typename C::Part part = c.first(base, taken, [&] {
-                return count && (taken + count >= left || (p && base + weight >= t) || (over_t && base + weight > t));
-            });
-            const typename C::Value v = c.value_in(part);
-            const double until = v.base + double(v.count) * v.weight;
-            const uint64_t any = __ballot(v.count != 0);
-            const uint64_t those = __ballot(v.count && (v.taken + v.count >= left || (p && until >= t) || (over_t && until > t)));
-            return C::lane_of(v, those ? __builtin_ctzll(those) : 63 - __builtin_clzll(any));
-        };
-        if (set.top_k && set.top_k < left) {
-            left = set.top_k;
-            const typename C::Value v = find(0.0, false, false);
-            whole = v.base + double(left - v.taken) * v.weight;
-        }
-        if (set.with_p) {
-            const double t = set.top_p * whole;
-            const typename C::Value v = find(t, true, false);
-            const uint32_t n = equal_reach(t - v.base, v.weight, min(v.count, left - v.taken));
-            left = v.taken + n;
-            whole = v.base + double(n) * v.weight;
-        }
-        if (set.with_min) {
-            over = block_total<C::THREADS>(over, s.room_d);
-            over_count = block_total<C::THREADS>(over_count, s.room_u);
-            if (over_count < left) {
-                left = over_count;
-                whole = over;
+        for (int i = 0; i < 2; ++i)
+            if (lane == 0) {
+                s.weights[segment[i]] = weight[i];
+                s.in_segment[segment[i]] = count[i];
             }
-        }
-        const double t = set.uniform * whole;
-        const typename C::Value v = find(t, false, true);
-        at = equal_draw(t - v.base, v.weight, min(v.count, left - v.taken));
-        code = v.code;
-        share = uniform(v.weight / whole);
     }
+    __syncthreads();
+    // What is left: the first `left` tokens, with the weight `whole`.
+    const double weight = s.weights[tid];
+    const uint32_t count = s.in_segment[tid];
+    double whole;
+    uint32_t left;
+    const double base = block_scan<C::THREADS>(weight, s.room_d, whole);
+    const uint32_t taken = block_scan<C::THREADS>(count, s.room_u, left);
+    whole = uniform(whole);
+    // The value at which the tokens reach `left`, or (p) the weights t, or exceed it.
+    const auto find = [&](double t, bool p, bool over_t) {
+        const typename C::Part part = c.first(base, taken, [&] {
+            return count && (taken + count >= left || (p && base + weight >= t) || (over_t && base + weight > t));
+        });
+        const typename C::Value v = c.value_in(part);
+        const double until = v.base + double(v.count) * v.weight;
+        const uint64_t any = __ballot(v.count != 0);
+        const uint64_t those = __ballot(v.count && (v.taken + v.count >= left || (p && until >= t) || (over_t && until > t)));
+        return C::lane_of(v, those ? __builtin_ctzll(those) : 63 - __builtin_clzll(any));
+    };
+    if (set.top_k && set.top_k < left) {
+        left = set.top_k;
+        const typename C::Value v = find(0.0, false, false);
+        whole = v.base + double(left - v.taken) * v.weight;
+    }
+    if (set.with_p) {
+        const double t = set.top_p * whole;
+        const typename C::Value v = find(t, true, false);
+        const uint32_t n = equal_reach(t - v.base, v.weight, min(v.count, left - v.taken));
+        left = v.taken + n;
+        whole = v.base + double(n) * v.weight;
+    }
+    if (set.with_min) {
+        over = block_total<C::THREADS>(over, s.room_d);
+        over_count = block_total<C::THREADS>(over_count, s.room_u);
+        if (over_count < left) {
+            left = over_count;
+            whole = over;
+        }
+    }
+    const double t = set.uniform * whole;
+    const typename C::Value v = find(t, false, true);
+    uint32_t at = equal_draw(t - v.base, v.weight, min(v.count, left - v.taken));
+    code = v.code;
+    const double share = uniform(v.weight / whole);  // of the token that is drawn
 
     // The at-th token of that code, from 0; the two zeros are equal.
     const bool zero = (code & 0x7fff) == 0;
