@@ -7,7 +7,7 @@ import pytest
 
 import grokking_abmod_amd as G
 import operators_lib as L
-from test_gpu_steps import KINDS, sampled
+from test_gpu_steps import KINDS, SETTINGS, check_drawn, sampled, setting
 
 pytestmark = pytest.mark.gpu
 
@@ -26,6 +26,37 @@ def test_greedy_rows_look_at_no_filter_and_no_number(kind, vocab):
             tokens, logprob, _ = sampled(dev, z, kind, temperature=np.zeros(rows), u=rng.choice([math.nan, 2.0, 0.5], rows), **kw)
             assert np.array_equal(tokens, np.argmax(L.values(z, kind), 1))
             assert not logprob.any()
+
+
+@pytest.mark.parametrize("vocab", [65, 256, 257, 4096, 8192, 16384, 16385, 32768])
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_at_which_the_way_to_draw_changes(kind, vocab):
+    """The longest and shortest rows of each way, also with a top_k of more than the threads that
+    have a logit (a group of 16 bytes each: 65 or 33 of 257)."""
+    rng = np.random.default_rng(vocab)
+    rows = 10
+    with L.Device() as dev:
+        for i, kw in enumerate(SETTINGS + [dict(top_k=[60, 100, 128, 129, 200]),
+                                           dict(top_k=[40, 90, 128], top_p=[0.9, 1.0], min_p=[0.0, 0.01])]):
+            z = rng.normal(size=(rows, vocab)) * rng.choice([0.01, 1.0, 2.0, 8.0], (rows, 1))
+            z[1::4, rng.random(vocab) < 0.7] = -np.inf
+            z[:, vocab // 2] = 0.25
+            u = rng.random(rows, dtype=np.float32)
+            u[0], u[-1] = 0.0, 1 - 2.0**-24
+            kw = {k: setting(rng, rows, v) for k, v in kw.items()}
+            check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, stride=vocab + i % 3, **kw))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,vocab", [(513, 256), (513, 257), (513, 32768), (513, 32769)])
+def test_many_rows_at_which_the_way_to_draw_changes(kind, rows, vocab):
+    rng = np.random.default_rng(vocab)
+    z = rng.normal(size=(rows, vocab)) * 2
+    u = rng.random(rows, dtype=np.float32)
+    kw = dict(top_k=rng.choice([0, 5, 90, 200, 1000], rows), top_p=rng.choice([0.3, 0.95, 1.0], rows),
+              min_p=rng.choice([0.0, 0.01], rows), temperature=rng.choice([0.0, 0.7, 1.0, 3.0], rows))
+    with L.Device() as dev:
+        check_drawn(sampled(dev, L.stored(z, kind), kind, u=u, **kw))
 
 
 def next_to_ties(rng, width):
