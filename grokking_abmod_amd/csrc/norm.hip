@@ -302,7 +302,7 @@ constexpr int kRun = 64;
 // channels of each: the sums of the weight's gradient and the weight stay in registers,
 // and the next row's loads are under way while a row's mean is joined.  The sums of kRun
 // rows go to LDS, a place a thread and channel.
-// 8192 x 4096 BF16 with a residual: 49 us (5.5 TB/s); a wave a row, without loads ahead, 114.
+// 8192 x 4096 BF16 with a residual: 51 us (5.3 TB/s); a wave a row, without loads ahead, 114.
 template <class T, int LANES, int GROUPS>
 __global__ void __launch_bounds__(kThreads<LANES>) norm_backward_kernel(NormBackwardArgs a, uint32_t teams) {
     constexpr int G = T::kGroup;
@@ -521,7 +521,7 @@ uint32_t wide_parts_of(size_t rows, size_t width, int group) {
 }
 // Calls of few rows and elements take one launch, in which some workgroups read the rows
 // again for the weight's gradient: 1024 x 128 F32 took launches of 4.0 and 2.5 us, and takes
-// one of 5.9, and no workspace.
+// one of 6.1, and no workspace.
 bool few(size_t rows, size_t width) { return rows <= 1024 && rows * width <= size_t(1) << 18; }
 
 template <class T>
@@ -546,7 +546,7 @@ void backward_of(const NormBackwardArgs &a, hipStream_t stream) {
         }
         if constexpr (lanes.value == kWideRow) {
             // Registers do not hold the sums beside a row: 4000 x 15001 BF16 took 268 us so, and
-            // takes 170 with the rows read twice.  LDS would hold them, and has not been measured.
+            // takes 173 with the rows read twice.  LDS would hold them, and has not been measured.
             const uint32_t slabs = uint32_t((width + group * kSlab - 1) / (group * kSlab));
             parts = wide_parts_of(a.rows, size_t(width), group);
             if (parts) norm_columns_kernel<T><<<dim3(slabs * parts), kBlock, 0, stream>>>(a, slabs, parts);

@@ -388,7 +388,8 @@ int mg_sample_filtered_noalloc(int device, int type, const void *logits, size_t 
  * 1024) turn in pairs, channels i and i + rotary / 2 (MG_ROPE_HALF) or 2 i and
  * 2 i + 1 (MG_ROPE_INTERLEAVED), by position times frequencies[i] radians, and are
  * multiplied by `magnitude`; the channels behind stay as they are.  frequencies holds
- * rotary / 2 doubles on the device, because an angle at a far position needs them. */
+ * rotary / 2 doubles on the device, because an angle at a far position needs them;
+ * angles are FP64, their sines and cosines FP32. */
 enum { MG_ROPE_HALF = 0, MG_ROPE_INTERLEAVED = 1 };
 typedef struct {
     uint32_t head_width, rotary, layout;
@@ -400,8 +401,9 @@ typedef struct {
  * MG_ROPE_BASE multiplies the base by factor^(rotary / (rotary - 2)), which divides
  * the last by factor and leaves the first; MG_ROPE_BANDS divides those that turn
  * less than `low` times over the original `context`, leaves those that turn more than
- * `high` times, and mixes in proportion to the turns between.  What a scaling does
- * not use is not looked at. */
+ * `high` times, and mixes in proportion to the turns between (not to a pair's index).
+ * What a scaling does not use is not looked at.  A magnitude that goes with a factor is
+ * the caller's to set. */
 enum { MG_ROPE_UNSCALED = 0, MG_ROPE_LINEAR = 1, MG_ROPE_BASE = 2, MG_ROPE_BANDS = 3 };
 int mg_rope_frequencies(size_t rotary, double base, int scaling, double factor, double context, double low, double high,
                         double *out);
