@@ -452,9 +452,9 @@ int mg_rms_norm_e4m3(int device, int type, size_t rows, size_t width, const void
  * well, and d_weight (`width` floats, or NULL: not wanted).  sum is what the forward
  * call normalised: its kept sum, or x where there was no residual.  d_x may be sum,
  * d_out or d_sum, with its stride.  Products are FP32, and infinite where they leave
- * its range.  d_weight is added up in one order, in FP64 but for runs of up to 64 rows,
- * and needs the workspace of mg_rms_norm_backward_workspace bytes, aligned to 4 (else
- * NULL, 0). */
+ * its range.  d_weight is added up in one order: runs of up to 64 rows in FP32, and
+ * these in FP64, by way of FP32 parts in the workspace of mg_rms_norm_backward_workspace
+ * bytes, aligned to 4 (NULL, 0 where that is 0 or d_weight is not wanted). */
 int mg_rms_norm_backward_workspace(size_t rows, size_t width, size_t *bytes);
 int mg_rms_norm_backward(int device, int type, size_t rows, size_t width, const void *sum, size_t sum_stride,
                          const void *weight, const float *rstd, const void *d_out, size_t d_out_stride,
